@@ -40,6 +40,9 @@ extern "C" {
 /* element types for state import/export */
 #define THRML_DTYPE_U8 0  /* 0/1 spins, or category index */
 #define THRML_DTYPE_F32 1 /* the reference's representation: 0.0/1.0, or category as float */
+/* further element types of the operators around a learned head */
+#define THRML_DTYPE_BF16 2
+#define THRML_DTYPE_F16 3
 
 typedef struct thrml_ctx thrml_ctx;     /* one HIP device + one stream */
 typedef struct thrml_prog thrml_prog;   /* compiled program (~ BlockSamplingProgram) */
@@ -462,6 +465,85 @@ int thrml_gumbel_argmax(thrml_ctx *ctx, const float *logits, const float *u, int
 int thrml_batch_gather(thrml_ctx *ctx, const float *weights, uint64_t n_weights,
                        const int32_t *indices, uint64_t batch, uint32_t n_indices,
                        const uint32_t *strides, uint32_t batch_stride, float *out);
+
+/* ---- operators around a learned head; no counterpart in the reference ------
+ * A learned head gives a row of q logits for each categorical variable that it
+ * predicts.  All pointers are device memory; rows lie `stride` elements apart
+ * (0: the same row for all) and start at any multiple of their element size.
+ * Calls queue their kernels on the context's stream, allocate nothing and do
+ * not wait, so that they may be captured into a graph.  `work` is device memory
+ * of at least the bytes that the _work function gives (16-byte aligned; NULL
+ * where it gives 0), used until the call's kernels have ended.
+ *
+ * thrml_logits: rows of logits with what acts on them, in this order, each step
+ * in f32.  Parts whose pointer is NULL are left out.
+ *   history      categories of the row so far, the first lengths[row] of
+ *                history_len (NULL: all), the first prompt_lengths[row] of these
+ *                (NULL: none) a prompt; entries outside 0 .. q-1 do not count
+ *   repetition   a category that occurs in the history: z / repetition for
+ *                z > 0, else z * repetition
+ *   frequency    less frequency times its occurrences after the prompt
+ *   presence     less presence if it occurs after the prompt
+ *   bias         plus bias_values at bias_ids (entries outside 0 .. q-1 do not
+ *                count, several for one category are added in their order)
+ *   temperature  divided by it where it is > 0
+ *   mask         -inf, whatever the logit, where bit c % 32 of word c / 32 of the
+ *                row's mask is clear (mask_stride 0: one mask for all rows) */
+typedef struct {
+  const void *logits;
+  int32_t dtype; /* THRML_DTYPE_F32, _BF16 or _F16 */
+  uint32_t q;
+  uint64_t rows;
+  int64_t logits_stride;
+  const int32_t *history;
+  int64_t history_stride;
+  uint32_t history_len;
+  const int32_t *lengths;
+  const int32_t *prompt_lengths;
+  const float *repetition;
+  const float *presence;
+  const float *frequency;
+  const int32_t *bias_ids;
+  const float *bias_values;
+  int64_t bias_stride;
+  uint32_t n_bias;
+  const float *temperature;
+  const uint32_t *mask;
+  int64_t mask_stride;
+} thrml_logits;
+/* out[row][c] of the processed logits, rounded once to out_dtype; out may be the
+ * logits themselves (same type and stride). */
+int thrml_process_logits(thrml_ctx *ctx, const thrml_logits *in, void *out, int out_dtype,
+                         int64_t out_stride);
+/* A category for each row from the processed logits x: the first argmax of
+ * x - log(-log(u[row][c])) over the allowed categories, the scores in 64 bits
+ * (u: uniforms in [0, 1); a category with u = 0 is taken only where there is no
+ * other), or of x where u is NULL or the row's temperature is not above 0.
+ * logprob[row] = x - log sum exp x at that category.  A row without a
+ * distribution (nothing allowed, or a NaN or +inf among the allowed logits)
+ * gets index -1 and logprob NaN. */
+uint64_t thrml_sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q);
+int thrml_sample_logits(thrml_ctx *ctx, const thrml_logits *in, const float *u, int64_t u_stride,
+                        int32_t *index, float *logprob, void *work, uint64_t work_bytes);
+/* Distillation from a teacher's k top candidates: with p = softmax of
+ * teacher[row][i] / tau over the row's entries (those whose ids lie in 0 .. q-1;
+ * an id named twice has both probabilities),
+ *   loss[row] = tau^2 sum_i p_i (log p_i - log softmax(logits / tau)[ids_i])
+ *   grad[row][c] = d(weight[row] loss[row]) / d logits[row][c], in the logits' type
+ * (weight NULL: the loss alone).  A row without an entry has loss and gradient 0. */
+uint64_t thrml_distill_work(thrml_ctx *ctx, uint64_t rows, uint32_t q, uint32_t k);
+int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint64_t rows, uint32_t q,
+                  int64_t logits_stride, const int32_t *ids, int64_t ids_stride, const float *teacher,
+                  int64_t teacher_stride, uint32_t k, float tau, const float *weight, float *loss,
+                  void *grad, int64_t grad_stride, void *work, uint64_t work_bytes);
+/* y[row][c] = (sum_j a[row][j] w[c][j]) s[row] w_scale[c] + bias[c] with s[row] =
+ * max_j |x[row][j]| / 127 and a = x / s rounded to integers (ties to even; the
+ * quotient in f32), the sum exact in integers, the rest in f32, rounded once to
+ * out_dtype.  bias may be NULL.  A row of x with an infinity or a NaN gives NaN. */
+uint64_t thrml_linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
+int thrml_linear_i8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
+                    const int8_t *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,
+                    void *y, int out_dtype, int64_t y_stride, void *work, uint64_t work_bytes);
 
 /* ---- self-check; no counterpart in the reference ---------------------------
  * Worst-case errors of the hardware-math fast paths of the sweep kernels,

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "dev_util.hpp"
+#include "head.hpp"
 #include "internal.hpp"
 #include "thrml_math.hpp"
 #include "thrml_rng.hpp"
@@ -2070,6 +2071,165 @@ extern "C" int thrml_batch_gather(thrml_ctx *ctx, const float *weights, uint64_t
   st.batch_stride = batch_stride;
   THRML_HIP(hipSetDevice(ctx->device));
   return launch_batch_gather(ctx, weights, n_weights, indices, batch, n_indices, st, out);
+}
+
+// ---------------------------------------------------------------------------
+// Operators around a learned head
+namespace {
+
+uint32_t head_type_size(int dtype) {
+  return dtype == THRML_DTYPE_F32 ? 4u : dtype == THRML_DTYPE_BF16 || dtype == THRML_DTYPE_F16 ? 2u : 0u;
+}
+
+// rows of n values of `size` bytes at p: null pointers, alignment, strides
+int check_rows(const char *name, const void *p, uint32_t size, uint64_t rows, uint64_t n, int64_t stride, bool out) {
+  if (rows == 0 || n == 0) return THRML_OK;
+  if (!p) return fail(THRML_EINVAL, std::string(name) + " is NULL");
+  if (reinterpret_cast<uintptr_t>(p) % size)
+    return fail(THRML_EINVAL, std::string(name) + " is not aligned to its element type");
+  if (rows > 1 && (stride < 0 || (out && (uint64_t)stride < n)))
+    return fail(THRML_EINVAL, std::string(name) + ": stride " + std::to_string(stride) +
+                                  (out ? " makes rows overlap" : " is negative"));
+  return THRML_OK;
+}
+
+int check_vector(const char *name, const void *p) {
+  if (reinterpret_cast<uintptr_t>(p) % 4)
+    return fail(THRML_EINVAL, std::string(name) + " is not aligned to its element type");
+  return THRML_OK;
+}
+
+int check_work(const void *work, uint64_t have, uint64_t need) {
+  if (have < need || (need && !work))
+    return fail(THRML_EINVAL, "work holds " + std::to_string(work ? have : 0) + " bytes, " + std::to_string(need) +
+                                  " are needed");
+  if (need && reinterpret_cast<uintptr_t>(work) % 16) return fail(THRML_EINVAL, "work is not aligned to 16 bytes");
+  return THRML_OK;
+}
+
+constexpr uint32_t HEAD_MAX_Q = 1u << 30;   // categories; indices and paddings stay below 2^31
+constexpr uint64_t HEAD_MAX_ROWS = 1u << 30;
+
+int check_sizes(uint64_t rows, uint32_t q) {
+  if (q == 0) return fail(THRML_EINVAL, "q must be positive");
+  if (q > HEAD_MAX_Q) return fail(THRML_EUNSUPPORTED, "at most 2^30 categories");
+  if (rows > HEAD_MAX_ROWS) return fail(THRML_EUNSUPPORTED, "at most 2^30 rows");
+  return THRML_OK;
+}
+
+int logit_rows(const thrml_logits *in, LogitRows *a) {
+  if (int rc = check_sizes(in->rows, in->q)) return rc;
+  const uint32_t size = head_type_size(in->dtype);
+  if (!size) return fail(THRML_EINVAL, "logits must be f32, bf16 or f16");
+  if (int rc = check_rows("logits", in->logits, size, in->rows, in->q, in->logits_stride, false)) return rc;
+  if (in->history_len > HEAD_MAX_HISTORY) return fail(THRML_EUNSUPPORTED, "histories of at most 2^29 - 1 entries");
+  if (int rc = check_rows("history", in->history, 4, in->rows, in->history_len, in->history_stride, false)) return rc;
+  if (int rc = check_rows("bias_ids", in->bias_ids, 4, in->rows, in->n_bias, in->bias_stride, false)) return rc;
+  if (int rc = check_rows("bias_values", in->bias_values, 4, in->rows, in->n_bias, in->bias_stride, false)) return rc;
+  if (in->mask)
+    if (int rc = check_rows("mask", in->mask, 4, in->rows, (in->q + 31u) / 32u, in->mask_stride, in->mask_stride != 0))
+      return rc;
+  const std::pair<const char *, const void *> vec[] = {
+      {"lengths", in->lengths},   {"prompt_lengths", in->prompt_lengths}, {"repetition", in->repetition},
+      {"presence", in->presence}, {"frequency", in->frequency},           {"temperature", in->temperature}};
+  for (const auto &v : vec)
+    if (int rc = check_vector(v.first, v.second)) return rc;
+  *a = LogitRows{in->logits,     in->logits_stride, in->rows,           in->q,          in->history_len ? in->history : nullptr,
+                 in->history_stride, in->history_len, in->lengths,       in->prompt_lengths, in->repetition,
+                 in->presence,   in->frequency,     in->bias_ids,       in->bias_values, in->bias_stride,
+                 in->n_bias,     in->temperature,   in->mask,           in->mask_stride};
+  return THRML_OK;
+}
+
+}  // namespace
+
+extern "C" int thrml_process_logits(thrml_ctx *ctx, const thrml_logits *in, void *out, int out_dtype,
+                                    int64_t out_stride) {
+  if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
+  LogitRows a;
+  if (int rc = logit_rows(in, &a)) return rc;
+  const uint32_t size = head_type_size(out_dtype);
+  if (!size) return fail(THRML_EINVAL, "the output must be f32, bf16 or f16");
+  if (int rc = check_rows("out", out, size, a.rows, a.q, out_stride, true)) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  return launch_process_logits(ctx, a, in->dtype, out, out_dtype, out_stride);
+}
+
+extern "C" uint64_t thrml_sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q) {
+  return ctx && rows && q && rows <= HEAD_MAX_ROWS && q <= HEAD_MAX_Q ? sample_logits_work(ctx, rows, q) : 0;
+}
+
+extern "C" int thrml_sample_logits(thrml_ctx *ctx, const thrml_logits *in, const float *u, int64_t u_stride,
+                                   int32_t *index, float *logprob, void *work, uint64_t work_bytes) {
+  if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
+  LogitRows a;
+  if (int rc = logit_rows(in, &a)) return rc;
+  if (u)
+    if (int rc = check_rows("u", u, 4, a.rows, a.q, u_stride, false)) return rc;
+  if (int rc = check_rows("index", index, 4, a.rows, 1, 1, true)) return rc;
+  if (int rc = check_rows("logprob", logprob, 4, a.rows, 1, 1, true)) return rc;
+  if (int rc = check_work(work, work_bytes, thrml_sample_logits_work(ctx, a.rows, a.q))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  return launch_sample_logits(ctx, a, in->dtype, u, u_stride, index, logprob, work);
+}
+
+extern "C" uint64_t thrml_distill_work(thrml_ctx *ctx, uint64_t rows, uint32_t q, uint32_t k) {
+  return ctx && rows && q && rows <= HEAD_MAX_ROWS && q <= HEAD_MAX_Q && k <= DISTILL_MAX_K ? distill_work(ctx, rows, q) : 0;
+}
+
+extern "C" int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint64_t rows, uint32_t q,
+                             int64_t logits_stride, const int32_t *ids, int64_t ids_stride, const float *teacher,
+                             int64_t teacher_stride, uint32_t k, float tau, const float *weight, float *loss,
+                             void *grad, int64_t grad_stride, void *work, uint64_t work_bytes) {
+  if (!ctx) return fail(THRML_EINVAL, "NULL argument");
+  if (int rc = check_sizes(rows, q)) return rc;
+  const uint32_t size = head_type_size(dtype);
+  if (!size) return fail(THRML_EINVAL, "logits must be f32, bf16 or f16");
+  if (k > DISTILL_MAX_K)
+    return fail(THRML_EUNSUPPORTED, "at most " + std::to_string(DISTILL_MAX_K) + " candidates per row");
+  if (!(tau > 0.0f) || !std::isfinite(tau)) return fail(THRML_EINVAL, "tau must be positive and finite");
+  if (int rc = check_rows("logits", logits, size, rows, q, logits_stride, false)) return rc;
+  if (int rc = check_rows("ids", ids, 4, rows, k, ids_stride, false)) return rc;
+  if (int rc = check_rows("teacher", teacher, 4, rows, k, teacher_stride, false)) return rc;
+  if (int rc = check_vector("weight", weight)) return rc;
+  if (int rc = check_rows("loss", loss, 4, rows, 1, 1, true)) return rc;
+  if (weight) {
+    if (int rc = check_rows("grad", grad, size, rows, q, grad_stride, true)) return rc;
+    if (grad && grad == logits) return fail(THRML_EINVAL, "grad must not be the logits");
+  }
+  if (int rc = check_work(work, work_bytes, thrml_distill_work(ctx, rows, q, k))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  const DistillArgs a{logits, logits_stride, rows, q, k, ids, teacher, ids_stride, teacher_stride, tau, weight, loss,
+                      grad, grad_stride};
+  return launch_distill(ctx, a, dtype, work);
+}
+
+extern "C" uint64_t thrml_linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q) {
+  return ctx && rows && k && q && rows <= HEAD_MAX_ROWS && q <= HEAD_MAX_Q && k <= LINEAR_MAX_K
+             ? linear_i8_work(ctx, rows, k, q)
+             : 0;
+}
+
+extern "C" int thrml_linear_i8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
+                               const int8_t *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,
+                               void *y, int out_dtype, int64_t y_stride, void *work, uint64_t work_bytes) {
+  if (!ctx) return fail(THRML_EINVAL, "NULL argument");
+  if (int rc = check_sizes(rows, q)) return rc;
+  if (k == 0) return fail(THRML_EINVAL, "k must be positive");
+  if (k > LINEAR_MAX_K) return fail(THRML_EUNSUPPORTED, "k is at most 131072 (the 32-bit sum)");
+  const uint32_t size = head_type_size(dtype), out_size = head_type_size(out_dtype);
+  if (!size) return fail(THRML_EINVAL, "x must be f32, bf16 or f16");
+  if (!out_size) return fail(THRML_EINVAL, "the output must be f32, bf16 or f16");
+  if (int rc = check_rows("x", x, size, rows, k, x_stride, false)) return rc;
+  if (int rc = check_rows("w", w, 1, q, k, w_stride, false)) return rc;
+  if (rows && !w_scale) return fail(THRML_EINVAL, "w_scale is NULL");
+  if (int rc = check_vector("w_scale", w_scale)) return rc;
+  if (int rc = check_vector("bias", bias)) return rc;
+  if (int rc = check_rows("y", y, out_size, rows, q, y_stride, true)) return rc;
+  if (int rc = check_work(work, work_bytes, thrml_linear_i8_work(ctx, rows, k, q))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  const LinearArgs a{x, x_stride, rows, k, q, w, w_stride, w_scale, bias, y, y_stride};
+  return launch_linear_i8(ctx, a, dtype, out_dtype, work);
 }
 
 extern "C" int thrml_fast_math_check(thrml_ctx *ctx, float *out) {

@@ -1,0 +1,164 @@
+// head.hpp -- operators around a learned head over q categories: the launchers,
+// and the device helpers that their kernels share.  Rows of bf16, f16 or f32
+// values may start at any multiple of their element size: a lane loads 8
+// neighbouring values as 16-byte pieces at the element's own alignment (global
+// loads and stores need no more on gfx950).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "internal.hpp"
+
+namespace thrml {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// thrml_logits with its pointers typed; a row's parameters that are NULL leave
+// their step out.
+struct LogitRows {
+  const void *z;
+  int64_t z_stride;
+  uint64_t rows;
+  uint32_t q;
+  const int32_t *history;
+  int64_t history_stride;
+  uint32_t history_len;
+  const int32_t *lengths, *prompt_lengths;
+  const float *repetition, *presence, *frequency;
+  const int32_t *bias_ids;
+  const float *bias_values;
+  int64_t bias_stride;
+  uint32_t n_bias;
+  const float *temperature;
+  const uint32_t *mask;
+  int64_t mask_stride;  // 0: one mask for all rows
+};
+
+struct DistillArgs {
+  const void *z;
+  int64_t z_stride;
+  uint64_t rows;
+  uint32_t q, k;
+  const int32_t *ids;
+  const float *teacher;
+  int64_t ids_stride, teacher_stride;
+  float tau;
+  const float *weight;  // null: the loss alone
+  float *loss;
+  void *grad;
+  int64_t grad_stride;
+};
+
+struct LinearArgs {
+  const void *x;
+  int64_t x_stride;
+  uint64_t rows;
+  uint32_t k, q;
+  const int8_t *w;
+  int64_t w_stride;
+  const float *w_scale, *bias;
+  void *y;
+  int64_t y_stride;
+};
+
+constexpr uint32_t HEAD_MAX_HISTORY = (1u << 29) - 1;  // the counter bits of a table word
+constexpr uint32_t DISTILL_MAX_K = 4096;               // candidates kept in LDS
+constexpr uint32_t LINEAR_MAX_K = 131072;              // 127 * 128 * k stays below 2^31
+
+int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *out, int out_dtype,
+                          int64_t out_stride);
+uint64_t sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q);
+int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const float *u, int64_t u_stride,
+                         int32_t *index, float *logprob, void *work);
+uint64_t distill_work(thrml_ctx *ctx, uint64_t rows, uint32_t q);
+int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work);
+uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
+int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work);
+
+// ---------------------------------------------------------------------------
+// Device helpers
+template <class T>
+struct Raw8 {  // 8 values as they lie in memory
+  static constexpr int W = (int)sizeof(T) * 2;
+  uint32_t w[W];
+};
+
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+template <class T>
+struct Vec4 {
+  typedef std::conditional_t<sizeof(T) == 2, u32x4_a2, u32x4_a4> type;
+};
+
+template <class T>
+__device__ __forceinline__ void load8(const T *p, Raw8<T> &r) {
+  const typename Vec4<T>::type *v = reinterpret_cast<const typename Vec4<T>::type *>(p);
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::W / 4; ++i) {
+    const typename Vec4<T>::type t = v[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.w[4 * i + j] = t[j];
+  }
+}
+
+// p[0 .. n-1] and zeros for the rest, n < 8
+template <class T>
+__device__ __forceinline__ void load8_part(const T *p, uint32_t n, Raw8<T> &r) {
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::W; ++i) r.w[i] = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    if (j < n) {
+      if constexpr (sizeof(T) == 4)
+        r.w[j] = __builtin_bit_cast(uint32_t, p[j]);
+      else
+        r.w[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[j]) << (16u * (j & 1u));
+    }
+}
+
+template <class T>
+__device__ __forceinline__ float value(const Raw8<T> &r, int j) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(float, r.w[j]);
+  else if constexpr (__is_same(T, bf16_t))
+    return __builtin_bit_cast(float, (j & 1) ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+  else
+    return (float)__builtin_bit_cast(f16_t, (uint16_t)(r.w[j / 2] >> (16 * (j & 1))));
+}
+
+// The first n (at most 8) of v to p, rounded to nearest, ties to even.
+template <class T>
+__device__ __forceinline__ void store8(T *p, uint32_t n, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
+  if (n >= 8) {
+    uint32_t w[Raw8<T>::W];
+    __builtin_memcpy(w, t, sizeof(w));
+    typename Vec4<T>::type *o = reinterpret_cast<typename Vec4<T>::type *>(p);
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::W / 4; ++i) {
+      typename Vec4<T>::type x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = w[4 * i + j];
+      o[i] = x;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (j < n) p[j] = t[j];
+  }
+}
+
+// f(the element type of dtype); an unknown dtype is the caller's to refuse
+template <class F>
+int with_type(int dtype, F &&f) {
+  if (dtype == THRML_DTYPE_BF16) return f(bf16_t{});
+  if (dtype == THRML_DTYPE_F16) return f(f16_t{});
+  return f(float{});
+}
+
+}  // namespace thrml

@@ -44,6 +44,7 @@ __all__ = [
     "IsingTrainingSpec", "estimate_kl_grad", "ising_energy", "potts_energy", "energy",
     "MomentAccumulatorObserver", "make_nearest_neighbor_lattice",
     "greedy_coloring", "coloring_to_blocks", "erdos_renyi", "double_grid", "param_normal", "bf16_round",
+    "process_logits", "sample_logits", "distill_loss", "distill_grad", "linear_i8",
 ]
 
 
@@ -1076,3 +1077,7 @@ def param_normal(seed, n, mean, std):
     check(load().thrml_param_normal(int(seed), int(n), float(mean), float(std),
                                     ptr(out, ctypes.c_float)))
     return out
+
+
+# the operators around a learned head
+from .head import distill_grad, distill_loss, linear_i8, process_logits, sample_logits  # noqa: E402

@@ -16,6 +16,8 @@ THRML_ENOMEM = -3
 THRML_EUNSUPPORTED = -4
 DTYPE_U8 = 0
 DTYPE_F32 = 1
+DTYPE_BF16 = 2
+DTYPE_F16 = 3
 
 KIND_NAMES = {0: "lattice", 1: "csr", 2: "potts", 3: "dense", 4: "discrete"}
 
@@ -137,6 +139,31 @@ class Schedule(ctypes.Structure):
     ]
 
 
+class Logits(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("q", ctypes.c_uint32),
+        ("rows", ctypes.c_uint64),
+        ("logits_stride", ctypes.c_int64),
+        ("history", ctypes.c_void_p),
+        ("history_stride", ctypes.c_int64),
+        ("history_len", ctypes.c_uint32),
+        ("lengths", ctypes.c_void_p),
+        ("prompt_lengths", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_stride", ctypes.c_int64),
+        ("n_bias", ctypes.c_uint32),
+        ("temperature", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+    ]
+
+
 # int observe(void *user, uint64_t iteration, thrml_state *st, void *hip_stream)
 OBSERVE_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p,
                               ctypes.c_void_p)
@@ -240,6 +267,24 @@ SIGNATURES = [
     ("thrml_batch_gather", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64,
       ctypes.c_uint32, c_u32p, ctypes.c_uint32, ctypes.c_void_p]),
+    ("thrml_process_logits", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.POINTER(Logits), ctypes.c_void_p, ctypes.c_int, ctypes.c_int64]),
+    ("thrml_sample_logits_work", ctypes.c_uint64, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32]),
+    ("thrml_sample_logits", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.POINTER(Logits), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64]),
+    ("thrml_distill_work", ctypes.c_uint64,
+     [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32]),
+    ("thrml_distill", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int64,
+      ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, ctypes.c_float,
+      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_uint64]),
+    ("thrml_linear_i8_work", ctypes.c_uint64,
+     [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32]),
+    ("thrml_linear_i8", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int64,
+      ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+      ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_uint64]),
     ("thrml_fast_math_check", ctypes.c_int, [ctypes.c_void_p, c_f32p]),
     ("thrml_fast_math_status", ctypes.c_int,
      [ctypes.c_void_p, c_f32p, ctypes.POINTER(ctypes.c_int)]),
