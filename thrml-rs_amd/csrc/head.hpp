@@ -153,6 +153,25 @@ __device__ __forceinline__ void store8(T *p, uint32_t n, const float (&v)[8]) {
   }
 }
 
+// The first n (at most 4) of v to p.
+template <class T>
+__device__ __forceinline__ void store4(T *p, uint32_t n, const float (&v)[4]) {
+  T t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = (T)v[j];
+  if (n >= 4) {
+    typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<u32x4_a4 *>(p) = __builtin_bit_cast(u32x4_a4, t);
+    else
+      *reinterpret_cast<u32x2_a2 *>(p) = __builtin_bit_cast(u32x2_a2, t);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      if (j < n) p[j] = t[j];
+  }
+}
+
 // f(the element type of dtype); an unknown dtype is the caller's to refuse
 template <class F>
 int with_type(int dtype, F &&f) {

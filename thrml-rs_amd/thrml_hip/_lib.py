@@ -139,7 +139,7 @@ class Schedule(ctypes.Structure):
     ]
 
 
-class Logits(ctypes.Structure):
+class Logits(ctypes.Structure):  # calls also take the same bytes, packed
     _fields_ = [
         ("logits", ctypes.c_void_p),
         ("dtype", ctypes.c_int32),
@@ -268,10 +268,10 @@ SIGNATURES = [
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64,
       ctypes.c_uint32, c_u32p, ctypes.c_uint32, ctypes.c_void_p]),
     ("thrml_process_logits", ctypes.c_int,
-     [ctypes.c_void_p, ctypes.POINTER(Logits), ctypes.c_void_p, ctypes.c_int, ctypes.c_int64]),
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64]),
     ("thrml_sample_logits_work", ctypes.c_uint64, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32]),
     ("thrml_sample_logits", ctypes.c_int,
-     [ctypes.c_void_p, ctypes.POINTER(Logits), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64]),
     ("thrml_distill_work", ctypes.c_uint64,
      [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32]),

@@ -12,142 +12,140 @@ that is another stream than torch's current one, the kernels wait for what torch
 has queued there, and what torch queues there afterwards waits for them.  Calls
 may be captured into a graph.
 """
-import ctypes
+import struct
 
 from . import _lib
 from ._lib import ThrmlError, check, load
+
+torch = None  # the module, from the first call on (the package works without it)
+_TYPES = {}
+_FLOATS = _INT32 = _FLOAT32 = _INT8 = _WORDS = ()
+_PACK = struct.Struct("@PiIQqPqIPPPPPPPqIPPq").pack  # thrml_logits
+
+
+def _setup():
+    global torch, _FLOATS, _INT32, _FLOAT32, _INT8, _WORDS
+    import torch
+
+    _TYPES.update({torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16})
+    _FLOATS, _INT32, _FLOAT32, _INT8 = tuple(_TYPES), (torch.int32,), (torch.float32,), (torch.int8,)
+    _WORDS = (torch.int32, torch.uint32)
 
 
 def _refuse(msg):
     raise ThrmlError(_lib.THRML_EINVAL, msg)
 
 
-def _types():
-    import torch
-
-    return {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-
-
-class _Call:
-    """The tensors of one call: checks them, and orders the device's stream with
-    torch's current one around the launches."""
-
-    def __init__(self, device):
-        import torch
-
-        self.torch = torch
-        self.device = device
-        self.types = _types()
-        self.where = []  # (name, tensor), to be on the device
-
-    def floats(self, name, t):
-        if not isinstance(t, self.torch.Tensor) or t.dtype not in self.types:
-            _refuse(f"{name} must be a float32, bfloat16 or float16 tensor")
-        return t
-
-    def matrix(self, name, t, dtypes=None, rows=None, cols=None):
-        """A [rows, cols] tensor whose rows are contiguous."""
-        if dtypes is None:
-            self.floats(name, t)
-        elif not isinstance(t, self.torch.Tensor) or t.dtype not in dtypes:
-            _refuse(f"{name} must be a {' or '.join(str(d)[6:] for d in dtypes)} tensor")
-        if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-            _refuse(f"{name} must have shape [{'rows' if rows is None else rows}, "
-                    f"{'n' if cols is None else cols}], got {list(t.shape)}")
-        self.where.append((name, t))
-        return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
-
-    def vector(self, name, t, n, dtype):
-        if t is None:
-            return None
-        if not isinstance(t, self.torch.Tensor) or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
-            _refuse(f"{name} must be a {str(dtype)[6:]} tensor of shape [{n}]")
-        self.where.append((name, t))
-        return t.contiguous()
-
-    def dtype(self, name, d):
-        if d not in self.types:
-            _refuse(f"{name} must be float32, bfloat16 or float16")
-        return self.types[d]
-
-    def out(self, name, t, rows, q, dtype, like):
-        if t is None:
-            return self.torch.empty(rows, q, dtype=dtype, device=like.device)
-        if not isinstance(t, self.torch.Tensor) or t.dtype != dtype or tuple(t.shape) != (rows, q) or (
-                t.stride(1) != 1 and q > 1):
-            _refuse(f"{name} must be a {str(dtype)[6:]} tensor of shape [{rows}, {q}] with contiguous rows")
-        self.where.append((name, t))
-        return t
-
-    def work(self, n, like):
-        return self.torch.empty(n, dtype=self.torch.uint8, device=like.device) if n else None
-
-    def on_device(self):
-        for name, t in self.where:
-            if t.device.type != "cuda" or t.device.index != self.device.ordinal:
-                _refuse(f"{name} is on {t.device}, the device is cuda:{self.device.ordinal}")
-
-    def run(self, fn, *args):
-        torch = self.torch
-        mine = self.device.stream or 0
-        current = torch.cuda.current_stream(self.device.ordinal)
-        if current.cuda_stream == mine:
-            check(fn(self.device.handle, *args))
-            return
-        stream = torch.cuda.ExternalStream(mine, device=self.device.ordinal)
-        stream.wait_stream(current)
-        check(fn(self.device.handle, *args))
-        current.wait_stream(stream)
+# The checks read few attributes of a tensor: a call's time on the host is what small
+# calls cost (each attribute is about 0.1 us).
+def _matrix(name, t, dtypes, rows=None, cols=None):
+    """t, a [rows, cols] tensor, with contiguous rows."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        _refuse(f"{name} must be a {' or '.join(str(d)[6:] for d in dtypes)} tensor")
+    s = t.shape
+    if len(s) != 2 or (rows is not None and s[0] != rows) or (cols is not None and s[1] != cols):
+        _refuse(f"{name} must have shape [{'rows' if rows is None else rows}, "
+                f"{'n' if cols is None else cols}], got {list(s)}")
+    return t if t.stride(1) == 1 or s[1] <= 1 else t.contiguous()
 
 
-def _stride(t):
-    return t.stride(0) if t is not None and t.shape[0] > 1 else (t.shape[1] if t is not None else 0)
+def _vector(name, t, n, dtypes):
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.shape != (n,):
+        _refuse(f"{name} must be a {str(dtypes[0])[6:]} tensor of shape [{n}]")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
+def _type(name, d):
+    if d not in _TYPES:
+        _refuse(f"{name} must be float32, bfloat16 or float16")
+    return _TYPES[d]
 
 
-def _rows(call, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
+def _out(name, t, rows, q, dtype):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows, q) or (t.stride(1) != 1 and q > 1):
+        _refuse(f"{name} must be a {str(dtype)[6:]} tensor of shape [{rows}, {q}] with contiguous rows")
+    return t
+
+
+def _on_device(device, names, tensors):
+    for t in tensors:
+        if t is not None and t.get_device() != device.ordinal:
+            name = next(n for n, x in zip(names, tensors) if x is t)
+            _refuse(f"{name} is on {t.device}, the device is cuda:{device.ordinal}")
+
+
+def _run(device, fn, *args):
+    """fn on the device's stream, ordered with torch's current one."""
+    mine = device.stream or 0
+    current = torch.cuda.current_stream(device.ordinal)
+    if current.cuda_stream == mine:
+        check(fn(device.handle, *args))
+        return
+    stream = torch.cuda.ExternalStream(mine, device=device.ordinal)
+    stream.wait_stream(current)
+    check(fn(device.handle, *args))
+    current.wait_stream(stream)
+
+
+_ROW_NAMES = ("logits", "history", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "bias_ids",
+              "bias_values", "temperature", "mask")
+
+
+def _rows(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
           temperature, mask):
-    """(the C descriptor, the tensors that it points into)"""
-    torch = call.torch
-    logits = call.matrix("logits", logits)
-    rows, q = logits.shape
+    """(the C descriptor, the tensors that it points into, rows, q)"""
+    if torch is None:
+        _setup()
+    z = _matrix("logits", logits, _FLOATS)
+    rows, q = z.shape
     if q == 0:
         _refuse("logits must have at least one category")
-    i32, f32 = (torch.int32,), (torch.float32,)
-    if history is None:
-        for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths), ("repetition", repetition),
-                        ("presence", presence), ("frequency", frequency)):
+    hp = hs = hn = lp = pp = rp = np_ = fp = bp = vp = bs = bn = tp = mp = ms = 0
+    if history is not None:
+        history = _matrix("history", history, _INT32, rows)
+        hp, hs, hn = history.data_ptr(), history.stride(0), history.shape[1]
+        if lengths is not None:
+            lengths = _vector("lengths", lengths, rows, _INT32)
+            lp = lengths.data_ptr()
+        if prompt_lengths is not None:
+            prompt_lengths = _vector("prompt_lengths", prompt_lengths, rows, _INT32)
+            pp = prompt_lengths.data_ptr()
+        if repetition is not None:
+            repetition = _vector("repetition", repetition, rows, _FLOAT32)
+            rp = repetition.data_ptr()
+        if presence is not None:
+            presence = _vector("presence", presence, rows, _FLOAT32)
+            np_ = presence.data_ptr()
+        if frequency is not None:
+            frequency = _vector("frequency", frequency, rows, _FLOAT32)
+            fp = frequency.data_ptr()
+    else:
+        for name, t in zip(_ROW_NAMES[2:7], (lengths, prompt_lengths, repetition, presence, frequency)):
             if t is not None:
                 _refuse(f"{name} needs a history")
-    else:
-        history = call.matrix("history", history, i32, rows)
-    if (bias_ids is None) != (bias_values is None):
+    if bias_ids is not None and bias_values is not None:
+        bias_ids = _matrix("bias_ids", bias_ids, _INT32, rows)
+        bn = bias_ids.shape[1]
+        bias_values = _matrix("bias_values", bias_values, _FLOAT32, rows, bn)
+        bs = bias_ids.stride(0)
+        if rows > 1 and bs != bias_values.stride(0):
+            bias_ids, bias_values, bs = bias_ids.contiguous(), bias_values.contiguous(), bn
+        bp, vp = bias_ids.data_ptr(), bias_values.data_ptr()
+    elif bias_ids is not None or bias_values is not None:
         _refuse("bias_ids and bias_values go together")
-    if bias_ids is not None:
-        bias_ids = call.matrix("bias_ids", bias_ids, i32, rows)
-        n = bias_ids.shape[1]
-        bias_values = call.matrix("bias_values", bias_values, f32, rows, n)
-        if rows > 1 and bias_ids.stride(0) != bias_values.stride(0):
-            bias_ids, bias_values = bias_ids.contiguous(), bias_values.contiguous()
+    if temperature is not None:
+        temperature = _vector("temperature", temperature, rows, _FLOAT32)
+        tp = temperature.data_ptr()
     if mask is not None:
-        words = (q + 31) // 32
-        mask = call.matrix("mask", mask, (torch.int32, getattr(torch, "uint32", torch.int32)), None, words)
-        if mask.shape[0] not in (1, rows):
-            _refuse(f"mask must have 1 or {rows} rows, got {mask.shape[0]}")
-    vec = {name: call.vector(name, t, rows, dtype) for name, t, dtype in (
-        ("lengths", lengths, torch.int32), ("prompt_lengths", prompt_lengths, torch.int32),
-        ("repetition", repetition, torch.float32), ("presence", presence, torch.float32),
-        ("frequency", frequency, torch.float32), ("temperature", temperature, torch.float32))}
-    d = _lib.Logits(
-        _ptr(logits), call.types[logits.dtype], q, rows, _stride(logits), _ptr(history), _stride(history),
-        history.shape[1] if history is not None else 0, _ptr(vec["lengths"]), _ptr(vec["prompt_lengths"]),
-        _ptr(vec["repetition"]), _ptr(vec["presence"]), _ptr(vec["frequency"]), _ptr(bias_ids), _ptr(bias_values),
-        _stride(bias_ids), bias_ids.shape[1] if bias_ids is not None else 0, _ptr(vec["temperature"]), _ptr(mask),
-        _stride(mask) if mask is not None and mask.shape[0] > 1 else 0)
-    return d, logits, (logits, history, bias_ids, bias_values, mask, vec)
+        mask = _matrix("mask", mask, _WORDS, None, (q + 31) // 32)
+        n = mask.shape[0]
+        if n != 1 and n != rows:
+            _refuse(f"mask must have 1 or {rows} rows, got {n}")
+        mp, ms = mask.data_ptr(), mask.stride(0) if n > 1 else 0
+    d = _PACK(z.data_ptr(), _TYPES[z.dtype], q, rows, z.stride(0) if rows > 1 else q, hp, hs, hn, lp, pp, rp, np_, fp,
+              bp, vp, bs, bn, tp, mp, ms)
+    return d, (z, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
+               temperature, mask), rows, q
 
 
 def process_logits(device, logits, *, history=None, lengths=None, prompt_lengths=None, repetition=None,
@@ -171,16 +169,19 @@ def process_logits(device, logits, *, history=None, lengths=None, prompt_lengths
           c // 32 is clear, whatever the logit
 
     out: a tensor for the result; it may be the logits themselves."""
-    call = _Call(device)
-    d, z, keep = _rows(call, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids,
-                       bias_values, temperature, mask)
-    dt = call.dtype("out_dtype", out_dtype or z.dtype)
-    if out is logits and z is not logits:
-        _refuse("out may be the logits only where their rows are contiguous")
-    out = call.out("out", out, d.rows, d.q, out_dtype or z.dtype, z)
-    call.on_device()
-    call.run(load().thrml_process_logits, ctypes.byref(d), out.data_ptr(), dt, _stride(out))
-    del keep
+    d, keep, rows, q = _rows(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids,
+                             bias_values, temperature, mask)
+    z = keep[0]
+    dtype = out_dtype or z.dtype
+    code = _type("out_dtype", dtype)
+    if out is not None:
+        if out is logits and z is not logits:
+            _refuse("out may be the logits only where their rows are contiguous")
+        _out("out", out, rows, q, dtype)
+    _on_device(device, _ROW_NAMES + ("out",), keep + (out,))
+    if out is None:
+        out = torch.empty((rows, q), dtype=dtype, device=z.device)
+    _run(device, load().thrml_process_logits, d, out.data_ptr(), code, out.stride(0) if rows > 1 else q)
     return out
 
 
@@ -193,45 +194,51 @@ def sample_logits(device, logits, u=None, *, history=None, lengths=None, prompt_
     The same inputs give the same category.  logprob is x less log sum exp x.  A
     row without a distribution (nothing allowed; a NaN or +inf among the allowed
     logits) gets index -1 and logprob NaN."""
-    call = _Call(device)
-    torch = call.torch
-    d, z, keep = _rows(call, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids,
-                       bias_values, temperature, mask)
+    d, keep, rows, q = _rows(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids,
+                             bias_values, temperature, mask)
     if u is not None:
-        u = call.matrix("u", u, (torch.float32,), d.rows, d.q)
-    call.on_device()
-    index = torch.empty(d.rows, dtype=torch.int32, device=z.device)
-    logprob = torch.empty(d.rows, dtype=torch.float32, device=z.device)
+        u = _matrix("u", u, _FLOAT32, rows, q)
+    _on_device(device, _ROW_NAMES + ("u",), keep + (u,))
+    where = keep[0].device
+    index = torch.empty(rows, dtype=torch.int32, device=where)
+    logprob = torch.empty(rows, dtype=torch.float32, device=where)
     lib = load()
-    n = lib.thrml_sample_logits_work(device.handle, d.rows, d.q)
-    work = call.work(n, z)
-    call.run(lib.thrml_sample_logits, ctypes.byref(d), _ptr(u), _stride(u), index.data_ptr(), logprob.data_ptr(),
-             _ptr(work), n)
-    del keep
+    n = lib.thrml_sample_logits_work(device.handle, rows, q)
+    work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    _run(device, lib.thrml_sample_logits, d, u.data_ptr() if u is not None else 0,
+         u.stride(0) if u is not None and rows > 1 else q, index.data_ptr(), logprob.data_ptr(),
+         work.data_ptr() if n else 0, n)
     return index, logprob
 
 
-def _distill(device, logits, ids, teacher, weight, tau, out):
-    call = _Call(device)
-    torch = call.torch
-    z = call.matrix("logits", logits)
+def _distill(device, logits, ids, teacher, weight, tau, grad):
+    """weight None: the loss alone; grad: a tensor for the gradient, or None"""
+    if torch is None:
+        _setup()
+    z = _matrix("logits", logits, _FLOATS)
     rows, q = z.shape
     if q == 0:
         _refuse("logits must have at least one category")
-    ids = call.matrix("ids", ids, (torch.int32,), rows)
-    teacher = call.matrix("teacher", teacher, (torch.float32,), rows, ids.shape[1])
-    grad = None
+    ids = _matrix("ids", ids, _INT32, rows)
+    k = ids.shape[1]
+    teacher = _matrix("teacher", teacher, _FLOAT32, rows, k)
     if weight is not None:
-        weight = call.vector("weight", weight, rows, torch.float32)
-        grad = call.out("out", out, rows, q, z.dtype, z)
-    call.on_device()
-    loss = torch.empty(rows, dtype=torch.float32, device=z.device)
+        weight = _vector("weight", weight, rows, _FLOAT32)
+        if grad is not None:
+            _out("out", grad, rows, q, z.dtype)
+    _on_device(device, ("logits", "ids", "teacher", "weight", "out"), (z, ids, teacher, weight, grad))
+    where = z.device
+    loss = torch.empty(rows, dtype=torch.float32, device=where)
+    if weight is not None and grad is None:
+        grad = torch.empty((rows, q), dtype=z.dtype, device=where)
     lib = load()
-    n = lib.thrml_distill_work(device.handle, rows, q, ids.shape[1])
-    work = call.work(n, z)
-    call.run(lib.thrml_distill, _ptr(z), call.types[z.dtype], rows, q, _stride(z), _ptr(ids), _stride(ids),
-             _ptr(teacher), _stride(teacher), ids.shape[1], float(tau), _ptr(weight), _ptr(loss), _ptr(grad),
-             _stride(grad), _ptr(work), n)
+    n = lib.thrml_distill_work(device.handle, rows, q, k)
+    work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    wp, gp, gs = (weight.data_ptr(), grad.data_ptr(), grad.stride(0) if rows > 1 else q) if weight is not None else (
+        0, 0, q)
+    _run(device, lib.thrml_distill, z.data_ptr(), _TYPES[z.dtype], rows, q, z.stride(0) if rows > 1 else q,
+         ids.data_ptr(), ids.stride(0) if rows > 1 else k, teacher.data_ptr(), teacher.stride(0) if rows > 1 else k, k,
+         float(tau), wp, loss.data_ptr(), gp, gs, work.data_ptr() if n else 0, n)
     return loss, grad
 
 
@@ -262,24 +269,28 @@ def linear_i8(device, x, w, w_scale, bias=None, out_dtype=None):
     = x / s rounded to integers (ties to even).  The sum is exact in integers, the
     rest is in f32.  A row of x with an infinity or a NaN gives NaN.  k is at most
     131072."""
-    call = _Call(device)
-    torch = call.torch
-    x = call.matrix("x", x)
+    if torch is None:
+        _setup()
+    x = _matrix("x", x, _FLOATS)
     rows, k = x.shape
-    w = call.matrix("w", w, (torch.int8,), None, k)
+    w = _matrix("w", w, _INT8, None, k)
     q = w.shape[0]
     if k == 0 or q == 0:
         _refuse("w must have at least one row and column")
-    w_scale = call.vector("w_scale", w_scale, q, torch.float32)
     if w_scale is None:
         _refuse("w_scale is needed")
-    bias = call.vector("bias", bias, q, torch.float32)
-    dt = call.dtype("out_dtype", out_dtype or x.dtype)
-    call.on_device()
-    y = torch.empty(rows, q, dtype=out_dtype or x.dtype, device=x.device)
+    w_scale = _vector("w_scale", w_scale, q, _FLOAT32)
+    if bias is not None:
+        bias = _vector("bias", bias, q, _FLOAT32)
+    dtype = out_dtype or x.dtype
+    code = _type("out_dtype", dtype)
+    _on_device(device, ("x", "w", "w_scale", "bias"), (x, w, w_scale, bias))
+    where = x.device
+    y = torch.empty((rows, q), dtype=dtype, device=where)
     lib = load()
     n = lib.thrml_linear_i8_work(device.handle, rows, k, q)
-    work = call.work(n, x)
-    call.run(lib.thrml_linear_i8, _ptr(x), call.types[x.dtype], rows, k, _stride(x), _ptr(w), q, _stride(w),
-             _ptr(w_scale), _ptr(bias), _ptr(y), dt, _stride(y), _ptr(work), n)
+    work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    _run(device, lib.thrml_linear_i8, x.data_ptr(), _TYPES[x.dtype], rows, k, x.stride(0) if rows > 1 else k,
+         w.data_ptr(), q, w.stride(0) if q > 1 else k, w_scale.data_ptr(), bias.data_ptr() if bias is not None else 0,
+         y.data_ptr(), code, q, work.data_ptr() if n else 0, n)
     return y
