@@ -6,16 +6,22 @@ namespace thrml {
 
 static inline uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+// a launch of f with that much LDS of its own choice
+static int lds_limit(const void *f, size_t bytes) {
+  if (bytes > 65536) THRML_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return THRML_OK;
+}
+
 // ---------------------------------------------------------------------------
-// What a row's history and biases say of the categories c0 .. c0 + n - 1: a word
-// for each category in LDS,
+// What a row's history and biases say of a chunk of categories: a word for each in LDS,
 //   bit 31   the category occurs in the prompt part of the history
-//   bit 30   it has a bias (its value in the second table)
+//   bit 30   it has a bias, which a small hash table holds under its place in the
+//            chunk (the sum of its entries, in list order)
 //   bits 0-28  how often it was drawn after the prompt
-// and, where rows have biases, the sum of its bias entries, in list order.  A
-// workgroup scans the row's whole history (it is short beside the row, and all
-// workgroups of a row share it in L2) and keeps what falls into its categories.
+// A workgroup scans the row's whole history for each chunk: it is short beside the
+// row, its first entries stay in registers, and the rest lies in L2.
 constexpr uint32_t T_PROMPT = 1u << 31, T_BIAS = 1u << 30, T_COUNT = (1u << 29) - 1u;
+constexpr uint32_t NO_KEY = 0xffffffffu;
 
 struct RowParams {
   float theta, presence, frequency, t;
@@ -35,49 +41,136 @@ __device__ __forceinline__ RowParams row_params(const LogitRows &a, uint64_t row
   return p;
 }
 
-// tab: n words, then n floats where there are biases.  All threads of the
-// workgroup call it; it ends with a barrier.
-__device__ __forceinline__ void build_table(const LogitRows &a, const RowParams &p, uint64_t row, uint32_t c0,
-                                            uint32_t n, uint32_t *tab, float *btab) {
-  const uint32_t tid = threadIdx.x, nt = blockDim.x;
-  for (uint32_t i = tid; i < n; i += nt) tab[i] = 0;
+// The table's place in LDS: `chunk` words, then `hash` keys and values.
+struct Table {
+  uint32_t *tab, *keys;
+  float *vals;
+  uint32_t chunk, hash;
+};
+
+// Slots of the hash table for n biases: at least twice as many as a chunk can have.
+static uint32_t hash_slots(uint32_t n_bias, uint32_t chunk) {
+  if (!n_bias) return 0;
+  uint32_t h = 64;
+  while (h < 2 * std::min(n_bias, chunk)) h *= 2;
+  return h;
+}
+static size_t table_bytes(const LogitRows &a, uint32_t chunk) {
+  return a.history || a.n_bias ? (size_t)chunk * 4 + (size_t)hash_slots(a.n_bias, chunk) * 8 : 0;
+}
+
+__device__ __forceinline__ uint32_t hash_at(uint32_t d, uint32_t hash) { return (d * 2654435761u >> 12) & (hash - 1u); }
+
+__device__ __forceinline__ float bias_of(const Table &t, uint32_t d) {
+  uint32_t h = hash_at(d, t.hash);
+  while (t.keys[h] != d) h = (h + 1u) & (t.hash - 1u);  // it is there
+  return t.vals[h];
+}
+
+// The row's first 8 BLOCK history entries, 4 neighbouring ones at a time (behind the
+// end: -1, which no chunk holds).
+constexpr int KEPT = 2;
+template <int BLOCK>
+struct History {
+  int32_t id[KEPT][4];
+  __device__ __forceinline__ void load(const int32_t *h, uint32_t len) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) get(h, len, (uint32_t)k * BLOCK * 4u + threadIdx.x * 4u, id[k]);
+  }
+  static __device__ __forceinline__ void get(const int32_t *h, uint32_t len, uint32_t i, int32_t (&v)[4]) {
+    typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (i + 4u <= len) {
+      const i32x4_a4 x = *reinterpret_cast<const i32x4_a4 *>(h + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x[j];
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) v[j] = i + j < len ? h[i + j] : -1;
+    }
+  }
+};
+
+__device__ __forceinline__ void table_clear(const Table &t, uint32_t block) {
+  for (uint32_t i = threadIdx.x * 4u; i < t.chunk; i += block * 4u)
+    *reinterpret_cast<uint4 *>(t.tab + i) = make_uint4(0, 0, 0, 0);
+}
+
+// Fills the (cleared) table for categories c0 .. c0 + chunk - 1.  The workgroup calls
+// it together; it begins and ends with a barrier.
+template <int BLOCK>
+__device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &p, const History<BLOCK> &hist,
+                                           uint64_t row, uint32_t c0, const Table &t) {
+  const uint32_t tid = threadIdx.x;
   __syncthreads();
-  if (a.history) {
-    const int32_t *h = a.history + (int64_t)row * a.history_stride;
-    for (uint32_t i = tid; i < p.len; i += nt) {
-      const uint32_t d = (uint32_t)h[i] - c0;
-      if (d < n) {
-        if (i < p.prompt)
-          atomicOr(&tab[d], T_PROMPT);
+  if (t.hash) {
+    for (uint32_t i = tid; i < t.hash; i += BLOCK) t.keys[i] = NO_KEY;
+    __syncthreads();
+  }
+  auto note = [&](uint32_t i, const int32_t (&v)[4]) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t d = (uint32_t)v[j] - c0;
+      if (d < t.chunk) {
+        if (i + j < p.prompt)
+          atomicOr(&t.tab[d], T_PROMPT);
         else
-          atomicAdd(&tab[d], 1u);
+          atomicAdd(&t.tab[d], 1u);
       }
+    }
+  };
+  if (p.len) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if ((uint32_t)k * BLOCK * 4u < p.len) note((uint32_t)k * BLOCK * 4u + tid * 4u, hist.id[k]);
+    const int32_t *h = a.history + (int64_t)row * a.history_stride;
+    for (uint32_t i = KEPT * BLOCK * 4u + tid * 4u; i < p.len; i += 2u * BLOCK * 4u) {
+      int32_t v[2][4];
+      History<BLOCK>::get(h, p.len, i, v[0]);
+      History<BLOCK>::get(h, p.len, i + BLOCK * 4u, v[1]);
+      note(i, v[0]);
+      note(i + BLOCK * 4u, v[1]);
     }
   }
   if (a.n_bias) {
     const int32_t *ids = a.bias_ids + (int64_t)row * a.bias_stride;
     const float *vals = a.bias_values + (int64_t)row * a.bias_stride;
     int again = 0;
-    for (uint32_t i = tid; i < a.n_bias; i += nt) {
+    for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
       const uint32_t d = (uint32_t)ids[i] - c0;
-      if (d < n) {
-        if (atomicOr(&tab[d], T_BIAS) & T_BIAS) again = 1;
-        btab[d] = vals[i];
+      const float v = vals[i];
+      if (d < t.chunk && d < a.q - c0) {
+        uint32_t h = hash_at(d, t.hash);
+        for (;;) {  // (at most half of the slots are ever taken)
+          const uint32_t old = atomicCAS(&t.keys[h], NO_KEY, d);
+          if (old == NO_KEY) {
+            atomicOr(&t.tab[d], T_BIAS);
+            t.vals[h] = v;
+            break;
+          }
+          if (old == d) {
+            again = 1;
+            break;
+          }
+          h = (h + 1u) & (t.hash - 1u);
+        }
       }
     }
     // a category named more than once: its entries are added in list order by
     // the thread of the first one
     if (__syncthreads_or(again)) {
-      for (uint32_t i = tid; i < a.n_bias; i += nt) {
+      for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
         const int32_t id = ids[i];
-        if ((uint32_t)id - c0 >= n) continue;
+        const uint32_t d = (uint32_t)id - c0;
+        if (d >= t.chunk || d >= a.q - c0) continue;
         bool first = true;
         for (uint32_t j = 0; j < i && first; ++j) first = ids[j] != id;
         if (!first) continue;
         float s = vals[i];
         for (uint32_t j = i + 1; j < a.n_bias; ++j)
           if (ids[j] == id) s += vals[j];
-        btab[(uint32_t)id - c0] = s;
+        uint32_t h = hash_at(d, t.hash);
+        while (t.keys[h] != d) h = (h + 1u) & (t.hash - 1u);
+        t.vals[h] = s;
       }
     }
   }
@@ -96,79 +189,110 @@ __device__ __forceinline__ float penalised(float z, uint32_t w, float bias, cons
   return z;
 }
 
-// y[j] = the 8 logits from c0 + d on with penalties and biases
+// y[j] = the 8 logits at place d of the chunk with penalties and biases; their table
+// words are cleared for the next chunk
 template <class T>
-__device__ __forceinline__ void row_values(const Raw8<T> &r, const uint32_t *tab, const float *btab, uint32_t d,
+__device__ __forceinline__ void row_values(const Raw8<T> &r, bool table, const Table &t, uint32_t d,
                                            const RowParams &p, float (&y)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) y[j] = value(r, j);
-  if (tab) {
-    const uint4 t0 = *reinterpret_cast<const uint4 *>(tab + d), t1 = *reinterpret_cast<const uint4 *>(tab + d + 4);
-    const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+  if (table) {
+    uint4 *w4 = reinterpret_cast<uint4 *>(t.tab + d);
+    const uint4 t0 = w4[0], t1 = w4[1];
     if ((t0.x | t0.y | t0.z | t0.w | t1.x | t1.y | t1.z | t1.w) != 0u) {
+      const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (w[j]) y[j] = penalised(y[j], w[j], (w[j] & T_BIAS) ? btab[d + j] : 0.0f, p);
+        if (w[j]) y[j] = penalised(y[j], w[j], (w[j] & T_BIAS) ? bias_of(t, d + j) : 0.0f, p);
+      w4[0] = w4[1] = make_uint4(0, 0, 0, 0);
     }
   }
 }
 
+// Eight logits at place d of n.
+template <class T>
+__device__ __forceinline__ void load_place(const T *z, uint32_t d, uint32_t n, Raw8<T> &r) {
+  if (d + 8u <= n)
+    load8(z + d, r);
+  else
+    load8_part(z + d, d < n ? n - d : 0u, r);
+}
+
 // ---------------------------------------------------------------------------
-// Processing: a workgroup writes `chunk` categories of one row.
-template <class TI, class TO>
-__global__ __launch_bounds__(256) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
-                                                      uint32_t chunk, uint32_t n_chunks, uint64_t n_tasks) {
+// Processing: a workgroup writes P_BLOCK * 8 V categories of one row.  Their logits
+// are on their way while it fills its table.
+constexpr int P_BLOCK = 512;
+
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(P_BLOCK) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
+                                                          uint32_t n_chunks, uint64_t n_tasks, uint32_t hash) {
   extern __shared__ uint32_t lds[];
+  constexpr uint32_t CHUNK = P_BLOCK * 8 * V;
   const bool table = a.history || a.n_bias;
-  float *btab = reinterpret_cast<float *>(lds + chunk);
+  const Table tab{lds, lds + CHUNK, reinterpret_cast<float *>(lds + CHUNK + hash), CHUNK, hash};
+  if (table) table_clear(tab, P_BLOCK);
   for (uint64_t task = blockIdx.x; task < n_tasks; task += gridDim.x) {
     const uint64_t row = task / n_chunks;
-    const uint32_t c0 = (uint32_t)(task % n_chunks) * chunk;
-    const uint32_t n = min(chunk, a.q - c0);
-    const RowParams p = row_params(a, row);
-    if (table) build_table(a, p, row, c0, (n + 7u) & ~7u, lds, btab);
+    const uint32_t c0 = (uint32_t)(task % n_chunks) * CHUNK;
+    const uint32_t n = min(CHUNK, a.q - c0);
     const TI *z = reinterpret_cast<const TI *>(a.z) + (int64_t)row * a.z_stride + c0;
     TO *o = out + (int64_t)row * out_stride + c0;
     const uint8_t *mask =
         a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) + c0 / 8u : nullptr;
-    for (uint32_t d = threadIdx.x * 8u; d < n; d += 256u * 8u) {
-      Raw8<TI> r;
-      if (d + 8u <= n)
-        load8(z + d, r);
-      else
-        load8_part(z + d, n - d, r);
+    Raw8<TI> r[V];
+    uint32_t m[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint32_t d = ((uint32_t)v * P_BLOCK + threadIdx.x) * 8u;
+      load_place(z, d, n, r[v]);
+      m[v] = mask && d < n ? mask[d / 8u] : 255u;
+    }
+    const RowParams p = row_params(a, row);
+    if (table) {
+      History<P_BLOCK> hist;
+      if (p.len) hist.load(a.history + (int64_t)row * a.history_stride, p.len);
+      table_fill(a, p, hist, row, c0, tab);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint32_t d = ((uint32_t)v * P_BLOCK + threadIdx.x) * 8u;
+      if (d >= n) break;
       float y[8];
-      row_values(r, table ? lds : nullptr, btab, d, p, y);
+      row_values(r[v], table, tab, d, p, y);
       if (p.t > 0.0f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = y[j] / p.t;
       }
       if (mask) {
-        const uint32_t m = mask[d / 8u];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (m >> j & 1u) ? y[j] : -INFINITY;
+        for (int j = 0; j < 8; ++j) y[j] = (m[v] >> j & 1u) ? y[j] : -INFINITY;
       }
       store8(o + d, n - d, y);
     }
-    if (table) __syncthreads();  // the next task builds its own
+    // (the last chunk's words behind the row's end belong to no one)
+    if (table && gridDim.x < n_tasks) {
+      __syncthreads();
+      table_clear(tab, P_BLOCK);
+    }
   }
 }
 
 int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *out, int out_dtype,
                           int64_t out_stride) {
   if (a.rows == 0) return THRML_OK;
-  uint32_t chunk = 8192;
-  while (chunk > 2048 && a.rows * cdiv(a.q, chunk) < 4ull * ctx->cu_count) chunk /= 2;
-  const uint32_t nc = cdiv(a.q, chunk);
+  // two groups of 8 per lane where that leaves enough workgroups (and LDS)
+  const bool two = a.rows * cdiv(a.q, P_BLOCK * 16) >= 4ull * ctx->cu_count && a.n_bias <= 1024;
+  const uint32_t chunk = P_BLOCK * (two ? 16 : 8), nc = cdiv(a.q, chunk);
   const uint64_t tasks = a.rows * nc;
-  const uint32_t grid = (uint32_t)std::min<uint64_t>(tasks, 1u << 20);
-  const size_t lds = (a.n_bias ? 2 : a.history ? 1 : 0) * (size_t)chunk * 4;
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(tasks, 1u << 20), hash = hash_slots(a.n_bias, chunk);
   return with_type(dtype, [&](auto ti) {
     return with_type(out_dtype, [&](auto to) -> int {
       typedef decltype(ti) TI;
       typedef decltype(to) TO;
-      hipLaunchKernelGGL((process_kernel<TI, TO>), dim3(grid), dim3(256), lds, ctx->stream, a,
-                         reinterpret_cast<TO *>(out), out_stride, chunk, nc, tasks);
+      auto *f = two ? &process_kernel<TI, TO, 2> : &process_kernel<TI, TO, 1>;
+      if (int rc = lds_limit(reinterpret_cast<const void *>(f), table_bytes(a, chunk))) return rc;
+      hipLaunchKernelGGL(f, dim3(grid), dim3(P_BLOCK), table_bytes(a, chunk), ctx->stream, a,
+                         reinterpret_cast<TO *>(out), out_stride, nc, tasks, hash);
       THRML_HIP(hipGetLastError());
       return THRML_OK;
     });
@@ -226,18 +350,38 @@ __device__ __forceinline__ void part_write(const SamplePart &s, uint64_t row, in
   logprob[row] = ok ? (s.x - s.m) - logf(s.sum) : __builtin_nanf("");
 }
 
-constexpr int S_BLOCK = 512;
+// A workgroup takes a segment of a row in chunks of BLOCK * 8 V categories; the next
+// chunk's logits and uniforms are on their way while it works on one.
+template <class T, int V>
+struct SampleChunk {
+  Raw8<T> z[V];
+  Raw8<float> u[V];
+  uint32_t live[V];
+};
 
-template <class T>
-__global__ __launch_bounds__(S_BLOCK) void sample_kernel(LogitRows a, const float *__restrict__ u,
-                                                         int64_t u_stride, uint32_t seg, uint32_t n_seg,
-                                                         uint32_t chunk, SamplePart *__restrict__ parts,
-                                                         int32_t *__restrict__ index,
-                                                         float *__restrict__ logprob) {
+template <class T, int BLOCK, int V>
+__device__ __forceinline__ void sample_load(const T *z, const float *u, const uint8_t *mask, uint32_t c0, uint32_t n,
+                                            SampleChunk<T, V> &k) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const uint32_t d = ((uint32_t)v * BLOCK + threadIdx.x) * 8u;
+    load_place(z + c0, d, n, k.z[v]);
+    if (u) load_place(u + c0, d, n, k.u[v]);
+    const uint32_t in = d >= n ? 0u : d + 8u <= n ? 255u : (1u << (n - d)) - 1u;
+    k.live[v] = mask && in ? mask[(c0 + d) / 8u] & in : in;
+  }
+}
+
+template <class T, int BLOCK, int V>
+__global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const float *__restrict__ u, int64_t u_stride,
+                                                       uint32_t seg, uint32_t n_seg, uint32_t hash,
+                                                       SamplePart *__restrict__ parts, int32_t *__restrict__ index,
+                                                       float *__restrict__ logprob) {
   extern __shared__ uint32_t lds[];
-  __shared__ SamplePart wave_part[S_BLOCK / 64];
+  __shared__ SamplePart wave_part[BLOCK / 64];
+  constexpr uint32_t CHUNK = BLOCK * 8 * V;
   const bool table = a.history || a.n_bias;
-  float *btab = reinterpret_cast<float *>(lds + chunk);
+  const Table tab{lds, lds + CHUNK, reinterpret_cast<float *>(lds + CHUNK + hash), CHUNK, hash};
   const uint64_t n_tasks = a.rows * n_seg;
   for (uint64_t task = blockIdx.x; task < n_tasks; task += gridDim.x) {
     const uint64_t row = task / n_seg;
@@ -248,28 +392,24 @@ __global__ __launch_bounds__(S_BLOCK) void sample_kernel(LogitRows a, const floa
     const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
     const float *ur = noisy ? u + (int64_t)row * u_stride : nullptr;
     const uint8_t *mask = a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) : nullptr;
+    SampleChunk<T, V> next{};
+    sample_load<T, BLOCK, V>(z, ur, mask, s0, min(CHUNK, s1 - s0), next);
+    History<BLOCK> hist;
+    if (table) {
+      if (p.len) hist.load(a.history + (int64_t)row * a.history_stride, p.len);
+      table_clear(tab, BLOCK);
+    }
     SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
     float thr = -INFINITY;  // of the wave
-    for (uint32_t c0 = s0; c0 < s1; c0 += chunk) {
-      const uint32_t n = min(chunk, s1 - c0);
-      if (table) build_table(a, p, row, c0, (n + 7u) & ~7u, lds, btab);
-      // whole waves stay in the loop: the threshold is the wave's
-      for (uint32_t d0 = (threadIdx.x & ~63u) * 8u; d0 < n; d0 += S_BLOCK * 8u) {
-        const uint32_t d = d0 + (threadIdx.x & 63u) * 8u, c = c0 + d;
-        float x[8], y[8] = {}, v[8];
-        Raw8<T> r{};
-        Raw8<float> ru{};
-        uint32_t live = 0;
-        if (d + 8u <= n) {
-          load8(z + c, r);
-          if (noisy) load8(ur + c, ru);
-          live = mask ? mask[c / 8u] : 255u;
-        } else if (d < n) {
-          load8_part(z + c, n - d, r);
-          if (noisy) load8_part(ur + c, n - d, ru);
-          live = (mask ? mask[c / 8u] : 255u) & ((1u << (n - d)) - 1u);
-        }
-        if (live) row_values(r, table ? lds : nullptr, btab, d, p, y);
+    for (uint32_t c0 = s0; c0 < s1; c0 += CHUNK) {
+      const SampleChunk<T, V> k = next;
+      if (table) table_fill(a, p, hist, row, c0, tab);
+      if (c0 + CHUNK < s1) sample_load<T, BLOCK, V>(z, ur, mask, c0 + CHUNK, min(CHUNK, s1 - c0 - CHUNK), next);
+#pragma unroll
+      for (int g = 0; g < V; ++g) {
+        const uint32_t d = ((uint32_t)g * BLOCK + threadIdx.x) * 8u, live = k.live[g];
+        float x[8], y[8], v[8];
+        row_values(k.z[g], table, tab, d, p, y);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? y[j] * rt : -INFINITY;
         float m = s.m;
@@ -285,24 +425,37 @@ __global__ __launch_bounds__(S_BLOCK) void sample_kernel(LogitRows a, const floa
         for (int j = 0; j < 8; ++j) {
           v[j] = x[j];
           if (noisy) {
-            const float l = __builtin_amdgcn_logf(fmaxf(__builtin_bit_cast(float, ru.w[j]), 0x1p-126f));
+            const float l = __builtin_amdgcn_logf(fmaxf(__builtin_bit_cast(float, k.u[g].w[j]), 0x1p-126f));
             v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
           }
           top = fmaxf(top, v[j]);
         }
         if (__any(top > thr)) {
+          const bool exact = !(noisy || scaled);
+          // the wave's best v bounds what is worth an exact score; those of u
+          // below 2^-126 are too high for that
+          float b = top;
+          if (noisy) {
+            b = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              b = fmaxf(b, __builtin_bit_cast(float, k.u[g].w[j]) >= 0x1p-126f ? v[j] : -INFINITY);
+          }
+#pragma unroll
+          for (int w = 32; w > 0; w >>= 1) b = fmaxf(b, __shfl_xor(b, w));
+          const float low = exact ? b : b - (S_MARGIN + fabsf(b) * S_REL);
           uint32_t todo = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) todo |= (v[j] > thr ? 1u : 0u) << j;
+          for (int j = 0; j < 8; ++j) todo |= (v[j] > thr && !(v[j] < low) ? 1u : 0u) << j;
           while (todo) {
             const int j = __builtin_ctz(todo);
             todo &= todo - 1u;
             float yj = y[0];
-            uint32_t uj = ru.w[0];
+            uint32_t uj = k.u[g].w[0];
 #pragma unroll
             for (int i = 1; i < 8; ++i) {
               yj = i == j ? y[i] : yj;
-              uj = i == j ? ru.w[i] : uj;
+              uj = i == j ? k.u[g].w[i] : uj;
             }
             const float xj = scaled ? yj / p.t : yj;
             double e = xj;
@@ -313,23 +466,22 @@ __global__ __launch_bounds__(S_BLOCK) void sample_kernel(LogitRows a, const floa
             if (e > s.best) {
               s.best = e;
               s.x = xj;
-              s.arg = (int32_t)(c + j);
+              s.arg = (int32_t)(c0 + d + j);
             }
           }
-          float b = (float)s.best;
+          b = (float)s.best;
 #pragma unroll
-          for (int k = 32; k > 0; k >>= 1) b = fmaxf(b, __shfl_xor(b, k));
-          thr = noisy || scaled ? b - (S_MARGIN + fabsf(b) * S_REL) : b;
+          for (int w = 32; w > 0; w >>= 1) b = fmaxf(b, __shfl_xor(b, w));
+          thr = exact ? b : b - (S_MARGIN + fabsf(b) * S_REL);
         }
       }
-      if (table) __syncthreads();
     }
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) part_merge(s, part_xor(s, k));
     if ((threadIdx.x & 63u) == 0) wave_part[threadIdx.x / 64u] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < S_BLOCK / 64; ++w) part_merge(s, wave_part[w]);
+      for (int w = 1; w < BLOCK / 64; ++w) part_merge(s, wave_part[w]);
       if (n_seg > 1)
         parts[task] = s;
       else
@@ -352,40 +504,54 @@ __global__ __launch_bounds__(64) void sample_join_kernel(const SamplePart *__res
   }
 }
 
-// Segments of a row: enough workgroups for the device, none shorter than a pass of a workgroup.
-static void sample_split(thrml_ctx *ctx, uint64_t rows, uint32_t q, uint32_t *seg, uint32_t *n_seg) {
-  constexpr uint32_t unit = S_BLOCK * 8;
+// How a call is laid out: a workgroup of 1024 per row where there are about as many
+// rows as compute units (two rows at a time would leave half of them idle at the
+// end), of 512 for more rows, and segments of rows, joined by a second kernel, for
+// few.
+struct SamplePlan {
+  bool wide;  // 1024 threads
+  uint32_t chunk, seg, n_seg;
+};
+static SamplePlan sample_plan(thrml_ctx *ctx, uint64_t rows, uint32_t q) {
+  SamplePlan p;
+  p.wide = rows < 2ull * ctx->cu_count && rows * 2 > (uint64_t)ctx->cu_count && q > 8192;
+  p.chunk = p.wide ? 8192 : 4096;
   uint32_t n = 1;
-  while (rows * n * 2 <= 2ull * ctx->cu_count && cdiv(q, n * 2) >= unit) n *= 2;
-  *seg = cdiv(cdiv(q, n), unit) * unit;
-  *n_seg = cdiv(q, *seg);
+  if (!p.wide)
+    while (rows * n * 2 <= 2ull * ctx->cu_count && cdiv(q, n * 2) >= p.chunk) n *= 2;
+  p.seg = cdiv(cdiv(q, n), p.chunk) * p.chunk;
+  p.n_seg = cdiv(q, p.seg);
+  return p;
 }
 
 uint64_t sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q) {
-  uint32_t seg, n;
-  sample_split(ctx, rows, q, &seg, &n);
-  return n > 1 ? rows * n * sizeof(SamplePart) : 0;
+  const SamplePlan p = sample_plan(ctx, rows, q);
+  return p.n_seg > 1 ? rows * p.n_seg * sizeof(SamplePart) : 0;
 }
 
 int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const float *u, int64_t u_stride,
                          int32_t *index, float *logprob, void *work) {
   if (a.rows == 0) return THRML_OK;
-  uint32_t seg, n_seg;
-  sample_split(ctx, a.rows, a.q, &seg, &n_seg);
-  const uint32_t chunk = 4096;
-  const size_t lds = (a.n_bias ? 2 : a.history ? 1 : 0) * (size_t)chunk * 4;
-  const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows * n_seg, 1u << 20);
+  SamplePlan p = sample_plan(ctx, a.rows, a.q);
+  if (p.wide && a.n_bias > 2048) {  // (the table's place in LDS)
+    p.wide = false;
+    p.chunk = 4096;
+  }
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows * p.n_seg, 1u << 20);
   SamplePart *parts = reinterpret_cast<SamplePart *>(work);
   const int rc = with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
-    hipLaunchKernelGGL((sample_kernel<T>), dim3(grid), dim3(S_BLOCK), lds, ctx->stream, a, u, u_stride, seg, n_seg,
-                       chunk, parts, index, logprob);
+    auto *f = p.wide ? &sample_kernel<T, 1024, 1> : &sample_kernel<T, 512, 1>;
+    const size_t lds = table_bytes(a, p.chunk);
+    if (int rc = lds_limit(reinterpret_cast<const void *>(f), lds)) return rc;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(p.wide ? 1024 : 512), lds, ctx->stream, a, u, u_stride, p.seg, p.n_seg,
+                       hash_slots(a.n_bias, p.chunk), parts, index, logprob);
     THRML_HIP(hipGetLastError());
     return THRML_OK;
   });
-  if (rc || n_seg == 1) return rc;
+  if (rc || p.n_seg == 1) return rc;
   hipLaunchKernelGGL(sample_join_kernel, dim3((uint32_t)std::min<uint64_t>(a.rows, 1u << 20)), dim3(64), 0, ctx->stream,
-                     parts, a.rows, n_seg, index, logprob);
+                     parts, a.rows, p.n_seg, index, logprob);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
 }
