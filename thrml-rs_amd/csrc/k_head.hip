@@ -67,15 +67,27 @@ __device__ __forceinline__ float bias_of(const Table &t, uint32_t d) {
   return t.vals[h];
 }
 
-// The row's first 8 BLOCK history entries, 4 neighbouring ones at a time (behind the
-// end: -1, which no chunk holds).
-constexpr int KEPT = 2;
+// What a lane keeps of its row's lists: of the first 4096 history entries, 4
+// neighbouring ones at a time (the row's length is applied at their use, so that
+// these loads wait for nothing; behind the history's end: -1, which no chunk holds),
+// and of the first BLOCK biases.
 template <int BLOCK>
-struct History {
-  int32_t id[KEPT][4];
-  __device__ __forceinline__ void load(const int32_t *h, uint32_t len) {
+struct RowLists {
+  static constexpr int KEPT = BLOCK == 1024 ? 1 : 2;
+  int32_t id[KEPT][4], bias_id;
+  float bias;
+  __device__ __forceinline__ void load(const LogitRows &a, uint64_t row) {
+    if (a.history) {
+      const int32_t *h = a.history + (int64_t)row * a.history_stride;
 #pragma unroll
-    for (int k = 0; k < KEPT; ++k) get(h, len, (uint32_t)k * BLOCK * 4u + threadIdx.x * 4u, id[k]);
+      for (int k = 0; k < KEPT; ++k) get(h, a.history_len, (uint32_t)k * BLOCK * 4u + threadIdx.x * 4u, id[k]);
+    }
+    bias_id = -1;
+    bias = 0.0f;
+    if (threadIdx.x < a.n_bias) {
+      bias_id = a.bias_ids[(int64_t)row * a.bias_stride + threadIdx.x];
+      bias = a.bias_values[(int64_t)row * a.bias_stride + threadIdx.x];
+    }
   }
   static __device__ __forceinline__ void get(const int32_t *h, uint32_t len, uint32_t i, int32_t (&v)[4]) {
     typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -98,8 +110,9 @@ __device__ __forceinline__ void table_clear(const Table &t, uint32_t block) {
 // Fills the (cleared) table for categories c0 .. c0 + chunk - 1.  The workgroup calls
 // it together; it begins and ends with a barrier.
 template <int BLOCK>
-__device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &p, const History<BLOCK> &hist,
+__device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
                                            uint64_t row, uint32_t c0, const Table &t) {
+  constexpr int KEPT = RowLists<BLOCK>::KEPT;
   const uint32_t tid = threadIdx.x;
   __syncthreads();
   if (t.hash) {
@@ -110,7 +123,7 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
       const uint32_t d = (uint32_t)v[j] - c0;
-      if (d < t.chunk) {
+      if (d < t.chunk && i + j < p.len) {
         if (i + j < p.prompt)
           atomicOr(&t.tab[d], T_PROMPT);
         else
@@ -121,12 +134,12 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
   if (p.len) {
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
-      if ((uint32_t)k * BLOCK * 4u < p.len) note((uint32_t)k * BLOCK * 4u + tid * 4u, hist.id[k]);
+      if ((uint32_t)k * BLOCK * 4u < p.len) note((uint32_t)k * BLOCK * 4u + tid * 4u, lists.id[k]);
     const int32_t *h = a.history + (int64_t)row * a.history_stride;
     for (uint32_t i = KEPT * BLOCK * 4u + tid * 4u; i < p.len; i += 2u * BLOCK * 4u) {
       int32_t v[2][4];
-      History<BLOCK>::get(h, p.len, i, v[0]);
-      History<BLOCK>::get(h, p.len, i + BLOCK * 4u, v[1]);
+      RowLists<BLOCK>::get(h, p.len, i, v[0]);
+      RowLists<BLOCK>::get(h, p.len, i + BLOCK * 4u, v[1]);
       note(i, v[0]);
       note(i + BLOCK * 4u, v[1]);
     }
@@ -136,8 +149,8 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
     const float *vals = a.bias_values + (int64_t)row * a.bias_stride;
     int again = 0;
     for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
-      const uint32_t d = (uint32_t)ids[i] - c0;
-      const float v = vals[i];
+      const uint32_t d = (uint32_t)(i == tid ? lists.bias_id : ids[i]) - c0;
+      const float v = i == tid ? lists.bias : vals[i];
       if (d < t.chunk && d < a.q - c0) {
         uint32_t h = hash_at(d, t.hash);
         for (;;) {  // (at most half of the slots are ever taken)
@@ -218,6 +231,29 @@ __device__ __forceinline__ void load_place(const T *z, uint32_t d, uint32_t n, R
     load8_part(z + d, d < n ? n - d : 0u, r);
 }
 
+// The same with -inf behind the n.
+template <class T>
+__device__ __forceinline__ void load_place_low(const T *z, uint32_t d, uint32_t n, Raw8<T> &r) {
+  load_place(z, d, n, r);
+  if (d + 8u > n) {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (d + j >= n) {
+        if constexpr (sizeof(T) == 4)
+          r.w[j] = 0xff800000u;
+        else
+          r.w[j / 2] |= (__is_same(T, bf16_t) ? 0xff80u : 0xfc00u) << (16u * (j & 1u));
+      }
+  }
+}
+
+// Values computed from r so far are not kept for later uses of r.
+template <class T>
+__device__ __forceinline__ void hide(Raw8<T> &r) {
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::W; ++i) asm volatile("" : "+v"(r.w[i]));
+}
+
 // ---------------------------------------------------------------------------
 // Processing: a workgroup writes P_BLOCK * 8 V categories of one row.  Their logits
 // are on their way while it fills its table.
@@ -247,11 +283,11 @@ __global__ __launch_bounds__(P_BLOCK) void process_kernel(LogitRows a, TO *__res
       load_place(z, d, n, r[v]);
       m[v] = mask && d < n ? mask[d / 8u] : 255u;
     }
+    RowLists<P_BLOCK> lists;
+    if (table) lists.load(a, row);
     const RowParams p = row_params(a, row);
     if (table) {
-      History<P_BLOCK> hist;
-      if (p.len) hist.load(a.history + (int64_t)row * a.history_stride, p.len);
-      table_fill(a, p, hist, row, c0, tab);
+      table_fill(a, p, lists, row, c0, tab);
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -394,16 +430,16 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
     const uint8_t *mask = a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) : nullptr;
     SampleChunk<T, V> next{};
     sample_load<T, BLOCK, V>(z, ur, mask, s0, min(CHUNK, s1 - s0), next);
-    History<BLOCK> hist;
+    RowLists<BLOCK> lists;
     if (table) {
-      if (p.len) hist.load(a.history + (int64_t)row * a.history_stride, p.len);
+      lists.load(a, row);
       table_clear(tab, BLOCK);
     }
     SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
     float thr = -INFINITY;  // of the wave
     for (uint32_t c0 = s0; c0 < s1; c0 += CHUNK) {
       const SampleChunk<T, V> k = next;
-      if (table) table_fill(a, p, hist, row, c0, tab);
+      if (table) table_fill(a, p, lists, row, c0, tab);
       if (c0 + CHUNK < s1) sample_load<T, BLOCK, V>(z, ur, mask, c0 + CHUNK, min(CHUNK, s1 - c0 - CHUNK), next);
 #pragma unroll
       for (int g = 0; g < V; ++g) {
@@ -557,31 +593,20 @@ int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const fl
 }
 
 // ---------------------------------------------------------------------------
-// Distillation from a teacher's top k candidates.  With z = logits / tau, lse =
-// log sum exp z, p = softmax(teacher / tau) over the row's entries,
-//   loss = tau^2 sum_i p_i (log p_i - z[id_i] + lse)
+// Distillation from a teacher's top k candidates.  With z = logits / tau, p =
+// softmax(teacher / tau) over the row's entries,
+//   loss = tau^2 sum_i p_i (log p_i - log softmax(z)[id_i])
 //   d(weight loss)/d logits = weight tau (softmax(z) - p)
-// Two passes over a row: the running maximum and sum, then the gradient.
-constexpr int D_BLOCK = 512;
-
-template <class Op>
-__device__ __forceinline__ float block_reduce(float v, float *buf, Op op) {
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) v = op(v, __shfl_xor(v, k));
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) buf[threadIdx.x / 64u] = v;
-  __syncthreads();
-  float r = buf[0];
-  for (uint32_t w = 1; w < blockDim.x / 64u; ++w) r = op(r, buf[w]);
-  return r;
-}
-struct MaxOp {
-  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-struct AddOp {
-  __device__ float operator()(float a, float b) const { return a + b; }
-};
-
+// log softmax(z) = (z - m) - log(sum exp(z - m)) keeps its two parts apart, so that
+// logits of any size lose nothing.
+//
+// A workgroup takes a row.  Its first wave does the teacher's part, with the
+// candidates in LDS, while the row's logits load; the other waves need its result
+// only behind the barrier that joins the maxima and sums.  The gradient is written
+// without p first, and at the candidates' places once more behind a barrier.
+//
+// Where the row fits the workgroup's registers, the gradient reads it there: one
+// read and one write of memory.
 // e^x: the hardware's 2^x of the rounded product, times what the rounding left
 // out (the relative error stays at 2 in 10^7 for x down to -100, 2 in 10^6 without)
 __device__ __forceinline__ float exp_wide(float x) {
@@ -591,96 +616,233 @@ __device__ __forceinline__ float exp_wide(float x) {
   return p == -INFINITY ? 0.0f : __builtin_fmaf(r, e * 0.693147182f, r);
 }
 
+// The scaled logit's exponential against the row's sum, for the gradient.  16-bit
+// gradients take the hardware's 2^x as it is (2 in 10^6 off where their own step is
+// 5 in 10^4 or more).
 template <class T>
-__global__ __launch_bounds__(D_BLOCK) void distill_kernel(DistillArgs a) {
+__device__ __forceinline__ float softmax_of(float z, float m, float rtau, float ls) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(__builtin_fmaf(z - m, rtau * LOG2E, -(ls * LOG2E)));
+  return exp_wide(__builtin_fmaf(z - m, rtau, -ls));
+}
+
+// The teacher's candidates of a row in LDS: ids (-1: does not count), probabilities,
+// log p, the logits at the ids, and a hash table that finds ids named twice.
+struct Candidates {
+  int32_t *ids;
+  float *p, *logp, *z;
+  int32_t *keys;
+  uint32_t k, hash;
+  bool some, again;  // of the first wave: there is an entry; an id comes twice
+};
+static uint32_t candidate_slots(uint32_t k) {
+  uint32_t h = 64;
+  while (h < 2 * k) h *= 2;
+  return h;
+}
+static size_t candidate_bytes(uint32_t k) { return (size_t)k * 16 + (size_t)candidate_slots(k) * 4; }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+  return v;
+}
+
+// By the first wave alone: its LDS accesses are in order.
+template <class T>
+__device__ __forceinline__ void teacher_part(const DistillArgs &a, uint64_t row, const T *z, Candidates &c) {
+  const uint32_t l = threadIdx.x;
+  const int32_t *id_row = a.ids + (int64_t)row * a.ids_stride;
+  const float *t_row = a.teacher + (int64_t)row * a.teacher_stride;
+  for (uint32_t i = l; i < c.hash; i += 64u) c.keys[i] = -1;
+  float tm = -INFINITY;
+  for (uint32_t i = l; i < c.k; i += 64u) {
+    int32_t id = id_row[i];
+    float t = t_row[i] / a.tau;
+    if ((uint32_t)id >= a.q) {
+      id = -1;
+      t = -INFINITY;
+    }
+    c.ids[i] = id;
+    c.logp[i] = t;
+    c.z[i] = id >= 0 ? (float)z[id] : 0.0f;
+    tm = fmaxf(tm, t);
+  }
+  tm = wave_max(tm);
+  if (!(tm > -INFINITY)) tm = 0.0f;
+  float ts = 0.0f;
+  bool again = false;
+  for (uint32_t i = l; i < c.k; i += 64u) {
+    const float e = expf(c.logp[i] - tm);
+    c.p[i] = e;
+    ts += e;
+    const int32_t id = c.ids[i];
+    if (id >= 0) {
+      uint32_t h = hash_at((uint32_t)id, c.hash);
+      for (;;) {  // (at most half of the slots are ever taken)
+        const int32_t old = atomicCAS(&c.keys[h], -1, id);
+        again = again || old == id;
+        if (old == -1 || old == id) break;
+        h = (h + 1u) & (c.hash - 1u);
+      }
+    }
+  }
+  ts = wave_sum(ts);
+  const float lts = logf(ts), rts = 1.0f / ts;
+  for (uint32_t i = l; i < c.k; i += 64u) {
+    c.logp[i] = (c.logp[i] - tm) - lts;
+    c.p[i] *= rts;
+  }
+  c.some = !(ts == 0.0f);
+  c.again = __any(again);
+}
+
+// By the first wave: the loss, from the row's maximum (a logit) and log sum.
+__device__ __forceinline__ void teacher_loss(const DistillArgs &a, uint64_t row, const Candidates &c, float m,
+                                             float ls, float rtau) {
+  float l = 0.0f;
+  for (uint32_t i = threadIdx.x; i < c.k; i += 64u) {
+    const float p = c.p[i];
+    if (c.ids[i] >= 0 && p != 0.0f) l += p * (c.logp[i] - ((c.z[i] - m) * rtau - ls));
+  }
+  l = wave_sum(l);
+  if (threadIdx.x == 0) a.loss[row] = c.some ? a.tau * a.tau * l : 0.0f;
+}
+
+// The gradient at the candidates' places, by the whole workgroup: an id that comes
+// more than once has the sum of its probabilities, in the order of the list.
+template <class T>
+__device__ __forceinline__ void candidate_grads(const Candidates &c, bool again, T *g, float f, float m, float ls,
+                                                float rtau) {
+  for (uint32_t i = threadIdx.x; i < c.k; i += blockDim.x) {
+    const int32_t id = c.ids[i];
+    if (id < 0) continue;
+    float p = c.p[i];
+    if (again) {
+      bool first = true;
+      for (uint32_t j = 0; j < i && first; ++j) first = c.ids[j] != id;
+      if (!first) continue;
+      for (uint32_t j = i + 1; j < c.k; ++j)
+        if (c.ids[j] == id) p += c.p[j];
+    }
+    g[id] = (T)(f * (softmax_of<T>(c.z[i], m, rtau, ls) - p));
+  }
+}
+
+// Maximum and sum of exponentials of z rtau, of lanes and waves.
+struct MaxSum {
+  float m, s;
+};
+__device__ __forceinline__ MaxSum max_sum_merge(MaxSum a, MaxSum b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + b.s * __builtin_amdgcn_exp2f((b.m - m) * c)};
+}
+template <int BLOCK>
+__device__ __forceinline__ MaxSum max_sum_block(MaxSum v, float c, MaxSum *buf) {
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) v = max_sum_merge(v, {__shfl_xor(v.m, k), __shfl_xor(v.s, k)}, c);
+  if ((threadIdx.x & 63u) == 0) buf[threadIdx.x / 64u] = v;
+  __syncthreads();
+  v = buf[0];
+#pragma unroll
+  for (int w = 1; w < BLOCK / 64; ++w) v = max_sum_merge(v, buf[w], c);
+  return v;
+}
+
+// GROUPS > 0: the row, of at most BLOCK * 8 GROUPS logits, stays in registers;
+// 0: it is read twice.
+template <class T, int BLOCK, int GROUPS>
+__global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillArgs a, uint32_t hash) {
   extern __shared__ uint32_t lds[];
-  __shared__ float buf[D_BLOCK / 64];
-  int32_t *ids = reinterpret_cast<int32_t *>(lds);
-  float *pr = reinterpret_cast<float *>(lds + a.k);
-  const float rtau = 1.0f / a.tau;
+  __shared__ MaxSum buf[BLOCK / 64];
+  __shared__ uint32_t flags;  // 1: there is an entry, 2: an id comes twice
+  Candidates c;
+  c.ids = reinterpret_cast<int32_t *>(lds);
+  c.p = reinterpret_cast<float *>(lds) + a.k;
+  c.logp = c.p + a.k;
+  c.z = c.logp + a.k;
+  c.keys = reinterpret_cast<int32_t *>(c.z + a.k);
+  c.k = a.k;
+  c.hash = hash;
+  const float rtau = 1.0f / a.tau, l2 = rtau * LOG2E;
+  constexpr int G = GROUPS ? GROUPS : 1;
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
-    float m = -__FLT_MAX__, sum = 0.0f;
-    for (uint32_t c = threadIdx.x * 8u; c < a.q; c += D_BLOCK * 8u) {
-      Raw8<T> r;
-      float x[8];
-      const uint32_t n = a.q - c;
-      if (n >= 8u)
-        load8(z + c, r);
-      else
-        load8_part(z + c, n, r);
-      float mn = m, t = 0.0f;
+    Raw8<T> r[G];
+    if constexpr (GROUPS > 0) {
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        x[j] = j < n ? value(r, j) * rtau : -INFINITY;
-        mn = fmaxf(mn, x[j]);
+      for (int g = 0; g < G; ++g)
+        if ((uint32_t)g * BLOCK * 8u < a.q) load_place_low(z, ((uint32_t)g * BLOCK + threadIdx.x) * 8u, a.q, r[g]);
+    }
+    if (threadIdx.x < 64u) {
+      teacher_part(a, row, z, c);
+      if (threadIdx.x == 0) flags = (c.some ? 1u : 0u) | (c.again ? 2u : 0u);
+    }
+    MaxSum t{-__FLT_MAX__, 0.0f};
+    if constexpr (GROUPS > 0) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if ((uint32_t)g * BLOCK * 8u < a.q) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t.m = fmaxf(t.m, value(r[g], j));
+          hide(r[g]);
+        }
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if ((uint32_t)g * BLOCK * 8u < a.q) {
+          float s = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((value(r[g], j) - t.m) * l2);
+          t.s += s;
+          hide(r[g]);
+        }
+    } else {
+      for (uint32_t d = threadIdx.x * 8u; d < a.q; d += BLOCK * 8u) {
+        load_place_low(z, d, a.q, r[0]);
+        float x[8], m = t.m, s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = value(r[0], j);
+          m = fmaxf(m, x[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * l2);
+        t.s = t.s * __builtin_amdgcn_exp2f((t.m - m) * l2) + s;
+        t.m = m;
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t += __builtin_amdgcn_exp2f((x[j] - mn) * LOG2E);
-      sum = sum * __builtin_amdgcn_exp2f((m - mn) * LOG2E) + t;
-      m = mn;
     }
-    const float top = block_reduce(m, buf, MaxOp());
-    sum = block_reduce(sum * __builtin_amdgcn_exp2f((m - top) * LOG2E), buf, AddOp());
-    // log softmax(z) = (z - top) - ls: the two parts stay apart, so that logits of
-    // any size lose nothing
-    const float ls = logf(sum);
-    // the teacher's entries; those out of range do not count
-    const int32_t *id_row = a.ids + (int64_t)row * a.ids_stride;
-    const float *t_row = a.teacher + (int64_t)row * a.teacher_stride;
-    float tm = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < a.k; i += D_BLOCK) {
-      const int32_t id = id_row[i];
-      const bool ok = (uint32_t)id < a.q;
-      const float t = ok ? t_row[i] / a.tau : -INFINITY;
-      ids[i] = ok ? id : -1;
-      pr[i] = t;
-      tm = fmaxf(tm, t);
-    }
-    tm = block_reduce(tm, buf, MaxOp());
-    if (!(tm > -INFINITY)) tm = 0.0f;
-    float ts = 0.0f;
-    for (uint32_t i = threadIdx.x; i < a.k; i += D_BLOCK) ts += expf(pr[i] - tm);
-    ts = block_reduce(ts, buf, AddOp());
-    const float lts = logf(ts), rts = 1.0f / ts;
-    float l = 0.0f;
-    for (uint32_t i = threadIdx.x; i < a.k; i += D_BLOCK) {
-      const float lp = (pr[i] - tm) - lts;
-      const float p = expf(pr[i] - tm) * rts;
-      if (p != 0.0f && ids[i] >= 0) l += p * (lp - (((float)z[ids[i]] * rtau - top) - ls));
-      pr[i] = p;
-    }
-    l = block_reduce(l, buf, AddOp());
-    const bool none = ts == 0.0f;  // no entry
-    if (threadIdx.x == 0) a.loss[row] = none ? 0.0f : a.tau * a.tau * l;
+    t = max_sum_block<BLOCK>(t, l2, buf);
+    const float ls = logf(t.s);
+    if (threadIdx.x < 64u) teacher_loss(a, row, c, t.m, ls, rtau);
     if (a.weight) {
+      const uint32_t fl = flags;
+      const bool some = fl & 1u;
       const float f = a.tau * a.weight[row];
-      T *g = reinterpret_cast<T *>(a.grad) + (int64_t)row * a.grad_stride;
-      for (uint32_t c = threadIdx.x * 8u; c < a.q; c += D_BLOCK * 8u) {
-        Raw8<T> r;
+      T *o = reinterpret_cast<T *>(a.grad) + (int64_t)row * a.grad_stride;
+      auto write = [&](uint32_t d, const Raw8<T> &v) {
         float x[8];
-        const uint32_t n = a.q - c;
-        if (n >= 8u)
-          load8(z + c, r);
-        else
-          load8_part(z + c, n, r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = none ? 0.0f : f * exp_wide((value(r, j) * rtau - top) - ls);
-        store8(g + c, n, x);
+        for (int j = 0; j < 8; ++j) x[j] = some ? f * softmax_of<T>(value(v, j), t.m, rtau, ls) : 0.0f;
+        store8(o + d, a.q - d, x);
+      };
+      if constexpr (GROUPS > 0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t d = ((uint32_t)g * BLOCK + threadIdx.x) * 8u;
+          if (d < a.q) write(d, r[g]);
+        }
+      } else {
+        for (uint32_t d = threadIdx.x * 8u; d < a.q; d += BLOCK * 8u) {
+          load_place(z, d, a.q, r[0]);
+          write(d, r[0]);
+        }
       }
       __syncthreads();
-      if (!none)
-        for (uint32_t i = threadIdx.x; i < a.k; i += D_BLOCK) {
-          const int32_t id = ids[i];
-          if (id < 0) continue;
-          bool first = true;
-          for (uint32_t j = 0; j < i && first; ++j) first = ids[j] != id;
-          if (!first) continue;
-          float p = pr[i];
-          for (uint32_t j = i + 1; j < a.k; ++j)
-            if (ids[j] == id) p += pr[j];
-          g[id] = (T)(f * (exp_wide(((float)z[id] * rtau - top) - ls) - p));
-        }
+      if (some) candidate_grads(c, fl & 2u, o, f, t.m, ls, rtau);
     }
     __syncthreads();
   }
@@ -693,7 +855,17 @@ int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *) {
   const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows, 1u << 20);
   return with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
-    hipLaunchKernelGGL((distill_kernel<T>), dim3(grid), dim3(D_BLOCK), (size_t)a.k * 8, ctx->stream, a);
+    // 64 registers of logits a lane
+    constexpr int G = sizeof(T) == 2 ? 16 : 8;
+    auto *f = &distill_kernel<T, 512, 0>;
+    uint32_t block = 512;
+    if (a.weight && a.q <= 1024 * 8 * G) {
+      block = a.q <= 256 * 8 * G ? 256 : a.q <= 512 * 8 * G ? 512 : 1024;
+      f = block == 256 ? &distill_kernel<T, 256, G> : block == 512 ? &distill_kernel<T, 512, G> : &distill_kernel<T, 1024, G>;
+    }
+    const size_t lds = candidate_bytes(a.k);
+    if (int rc = lds_limit(reinterpret_cast<const void *>(f), lds)) return rc;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(block), lds, ctx->stream, a, candidate_slots(a.k));
     THRML_HIP(hipGetLastError());
     return THRML_OK;
   });
