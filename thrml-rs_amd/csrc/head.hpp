@@ -104,18 +104,28 @@ __device__ __forceinline__ void load8(const T *p, Raw8<T> &r) {
   }
 }
 
-// p[0 .. n-1] and zeros for the rest, n < 8
+// n where it is used: its comparisons are made there and not kept in registers from
+// far before
+__device__ __forceinline__ uint32_t here(uint32_t n) {
+  asm volatile("" : "+v"(n));
+  return n;
+}
+
+// p[0 .. n-1], and the bits `fill` for the rest, n < 8
 template <class T>
-__device__ __forceinline__ void load8_part(const T *p, uint32_t n, Raw8<T> &r) {
+__device__ __forceinline__ void load8_part(const T *p, uint32_t n_, Raw8<T> &r, uint32_t fill = 0) {
+  const uint32_t n = here(n_);
 #pragma unroll
-  for (int i = 0; i < Raw8<T>::W; ++i) r.w[i] = 0;
+  for (int i = 0; i < Raw8<T>::W; ++i) r.w[i] = sizeof(T) == 4 ? fill : fill | fill << 16;
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j)
     if (j < n) {
-      if constexpr (sizeof(T) == 4)
+      if constexpr (sizeof(T) == 4) {
         r.w[j] = __builtin_bit_cast(uint32_t, p[j]);
-      else
-        r.w[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[j]) << (16u * (j & 1u));
+      } else {
+        const uint32_t b = __builtin_bit_cast(uint16_t, p[j]);
+        r.w[j / 2] = (j & 1u) ? (r.w[j / 2] & 0xffffu) | b << 16 : (r.w[j / 2] & 0xffff0000u) | b;
+      }
     }
 }
 
@@ -129,46 +139,67 @@ __device__ __forceinline__ float value(const Raw8<T> &r, int j) {
     return (float)__builtin_bit_cast(f16_t, (uint16_t)(r.w[j / 2] >> (16 * (j & 1))));
 }
 
-// The first n (at most 8) of v to p, rounded to nearest, ties to even.
+// N values rounded to nearest, ties to even, as they lie in memory
+template <class T, int N>
+struct Rounded {
+  uint32_t w[N * (int)sizeof(T) / 4];
+};
+template <class T, int N>
+__device__ __forceinline__ Rounded<T, N> rounded(const float (&v)[N]) {
+  Rounded<T, N> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.w[j] = __builtin_bit_cast(uint32_t, v[j]);
+  } else {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef float fpair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const fpair f = {v[j], v[j + 1]};
+      r.w[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, pair));
+    }
+  }
+  return r;
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_part(T *p, uint32_t n_, const Rounded<T, N> &r) {
+  const uint32_t n = here(n_);
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j)
+    if (j < n) {
+      if constexpr (sizeof(T) == 4)
+        p[j] = __builtin_bit_cast(T, r.w[j]);
+      else
+        p[j] = __builtin_bit_cast(T, (uint16_t)(r.w[j / 2] >> (16u * (j & 1u))));
+    }
+}
+
+// The first n (at most 8) of v to p.
 template <class T>
 __device__ __forceinline__ void store8(T *p, uint32_t n, const float (&v)[8]) {
-  T t[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
+  const Rounded<T, 8> r = rounded<T>(v);
   if (n >= 8) {
-    uint32_t w[Raw8<T>::W];
-    __builtin_memcpy(w, t, sizeof(w));
     typename Vec4<T>::type *o = reinterpret_cast<typename Vec4<T>::type *>(p);
 #pragma unroll
-    for (int i = 0; i < Raw8<T>::W / 4; ++i) {
-      typename Vec4<T>::type x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = w[4 * i + j];
-      o[i] = x;
-    }
+    for (int i = 0; i < Raw8<T>::W / 4; ++i) o[i] = typename Vec4<T>::type{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
   } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (j < n) p[j] = t[j];
+    store_part<T, 8>(p, n, r);
   }
 }
 
 // The first n (at most 4) of v to p.
 template <class T>
 __device__ __forceinline__ void store4(T *p, uint32_t n, const float (&v)[4]) {
-  T t[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) t[j] = (T)v[j];
+  const Rounded<T, 4> r = rounded<T>(v);
   if (n >= 4) {
     typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
     if constexpr (sizeof(T) == 4)
-      *reinterpret_cast<u32x4_a4 *>(p) = __builtin_bit_cast(u32x4_a4, t);
+      *reinterpret_cast<u32x4_a4 *>(p) = u32x4_a4{r.w[0], r.w[1], r.w[2], r.w[3]};
     else
-      *reinterpret_cast<u32x2_a2 *>(p) = __builtin_bit_cast(u32x2_a2, t);
+      *reinterpret_cast<u32x2_a2 *>(p) = u32x2_a2{r.w[0], r.w[1]};
   } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-      if (j < n) p[j] = t[j];
+    store_part<T, 4>(p, n, r);
   }
 }
 

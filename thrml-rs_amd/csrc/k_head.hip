@@ -190,16 +190,64 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
   __syncthreads();
 }
 
-// A logit with its row's penalties and its bias, each step rounded to f32.
-__device__ __forceinline__ float penalised(float z, uint32_t w, float bias, const RowParams &p) {
-  const uint32_t n = w & T_COUNT;
-  if (n || (w & T_PROMPT)) z = z > 0.0f ? z / p.theta : z * p.theta;
-  if (n) {
-    z = z - p.frequency * (float)n;
-    z = z - p.presence;
+// a / b for many a: q = a r with r = 1 / b rounded, and one step of the remainder,
+// which an fma gives exactly, leave the correctly rounded quotient (Markstein 1990)
+// as long as nothing under- or overflows: b within 2^-20 .. 2^20, |a| within 2^-70 ..
+// 2^100.  3 operations instead of the 10 of a full division.
+struct Divisor {
+  float b, r;
+  bool plain;
+  __device__ __forceinline__ explicit Divisor(float b_) : b(b_), r(1.0f / b_), plain(b_ >= 0x1p-20f && b_ <= 0x1p20f) {}
+  __device__ __forceinline__ float fast(float a) const {
+    const float q = a * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
   }
-  if (w & T_BIAS) z = z + bias;
-  return z;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float min3_abs(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// all of a fit Divisor::fast (a NaN may pass: it divides to NaN either way)
+__device__ __forceinline__ bool divides_fast(const float (&a)[8]) {
+  float hi = 0.0f, lo = 1.0f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    hi = max3_abs(hi, a[j], a[j + 1]);
+    lo = min3_abs(lo, a[j], a[j + 1]);
+  }
+  return hi <= 0x1p100f && lo >= 0x1p-70f;
+}
+
+// a / b for what Divisor::fast does not take, one after the other (side by side they
+// would take the registers of all other work)
+__device__ __forceinline__ void divide_each(float (&a)[8], float b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a[j] = a[j] / b;
+    if (j < 7) asm volatile("" : "+v"(a[j]), "+v"(a[j + 1]));
+  }
+}
+
+// z with its row's penalties, each step rounded to f32; q: z / theta
+__device__ __forceinline__ float penalised(float z, float q, uint32_t w, const RowParams &p) {
+  const uint32_t n = w & T_COUNT;
+  const float fn = (float)n;
+  float y = z > 0.0f ? q : z * p.theta;
+  y = (w & ~T_BIAS) ? y : z;
+  const float less = (y - p.frequency * fn) - p.presence;
+  return n ? less : y;
 }
 
 // y[j] = the 8 logits at place d of the chunk with penalties and biases; their table
@@ -214,38 +262,40 @@ __device__ __forceinline__ void row_values(const Raw8<T> &r, bool table, const T
     const uint4 t0 = w4[0], t1 = w4[1];
     if ((t0.x | t0.y | t0.z | t0.w | t1.x | t1.y | t1.z | t1.w) != 0u) {
       const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+      const Divisor theta(p.theta);
+      if (theta.plain && divides_fast(y)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (w[j]) y[j] = penalised(y[j], w[j], (w[j] & T_BIAS) ? bias_of(t, d + j) : 0.0f, p);
+        for (int j = 0; j < 8; ++j)
+          if (w[j]) y[j] = penalised(y[j], theta.fast(y[j]), w[j], p);
+      } else {
+        float q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = y[j];
+        divide_each(q, p.theta);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (w[j]) y[j] = penalised(y[j], q[j], w[j], p);
+      }
+      if (((w[0] | w[1] | w[2] | w[3] | w[4] | w[5] | w[6] | w[7]) & T_BIAS) != 0u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (w[j] & T_BIAS) y[j] = y[j] + bias_of(t, d + j);
+      }
       w4[0] = w4[1] = make_uint4(0, 0, 0, 0);
     }
   }
 }
 
-// Eight logits at place d of n.
+// Eight logits at place d of n; what lies behind them has the bits `fill`.
 template <class T>
-__device__ __forceinline__ void load_place(const T *z, uint32_t d, uint32_t n, Raw8<T> &r) {
+__device__ __forceinline__ void load_place(const T *z, uint32_t d, uint32_t n, Raw8<T> &r, uint32_t fill = 0) {
   if (d + 8u <= n)
     load8(z + d, r);
   else
-    load8_part(z + d, d < n ? n - d : 0u, r);
+    load8_part(z + d, d < n ? n - d : 0u, r, fill);
 }
-
-// The same with -inf behind the n.
 template <class T>
-__device__ __forceinline__ void load_place_low(const T *z, uint32_t d, uint32_t n, Raw8<T> &r) {
-  load_place(z, d, n, r);
-  if (d + 8u > n) {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (d + j >= n) {
-        if constexpr (sizeof(T) == 4)
-          r.w[j] = 0xff800000u;
-        else
-          r.w[j / 2] |= (__is_same(T, bf16_t) ? 0xff80u : 0xfc00u) << (16u * (j & 1u));
-      }
-  }
-}
+constexpr uint32_t LOWEST = sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16_t) ? 0xff80u : 0xfc00u;  // -inf
 
 // Values computed from r so far are not kept for later uses of r.
 template <class T>
@@ -260,7 +310,7 @@ __device__ __forceinline__ void hide(Raw8<T> &r) {
 constexpr int P_BLOCK = 512;
 
 template <class TI, class TO, int V>
-__global__ __launch_bounds__(P_BLOCK) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
+__global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
                                                           uint32_t n_chunks, uint64_t n_tasks, uint32_t hash) {
   extern __shared__ uint32_t lds[];
   constexpr uint32_t CHUNK = P_BLOCK * 8 * V;
@@ -286,9 +336,8 @@ __global__ __launch_bounds__(P_BLOCK) void process_kernel(LogitRows a, TO *__res
     RowLists<P_BLOCK> lists;
     if (table) lists.load(a, row);
     const RowParams p = row_params(a, row);
-    if (table) {
-      table_fill(a, p, lists, row, c0, tab);
-    }
+    const Divisor t(p.t);
+    if (table) table_fill(a, p, lists, row, c0, tab);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t d = ((uint32_t)v * P_BLOCK + threadIdx.x) * 8u;
@@ -296,8 +345,12 @@ __global__ __launch_bounds__(P_BLOCK) void process_kernel(LogitRows a, TO *__res
       float y[8];
       row_values(r[v], table, tab, d, p, y);
       if (p.t > 0.0f) {
+        if (t.plain && divides_fast(y)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = y[j] / p.t;
+          for (int j = 0; j < 8; ++j) y[j] = t.fast(y[j]);
+        } else {
+          divide_each(y, p.t);
+        }
       }
       if (mask) {
 #pragma unroll
@@ -447,25 +500,33 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         float x[8], y[8], v[8];
         row_values(k.z[g], table, tab, d, p, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? y[j] * rt : -INFINITY;
+        for (int j = 0; j < 8; ++j) x[j] = y[j] * rt;
+        if (__any(live != 255u)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
+        }
         float m = s.m;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, x[j]);
+        for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
         s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * LOG2E) + sum;
         s.m = m;
-        float top = -INFINITY;
+        if (noisy) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = x[j];
-          if (noisy) {
-            const float l = __builtin_amdgcn_logf(fmaxf(__builtin_bit_cast(float, k.u[g].w[j]), 0x1p-126f));
+          for (int j = 0; j < 8; ++j) {
+            const float l = __builtin_amdgcn_logf(
+                __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, k.u[g].w[j]), 0x1p-126f, INFINITY));
             v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
           }
-          top = fmaxf(top, v[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = x[j];
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) top = max3(top, v[j], v[j + 1]);
         if (__any(top > thr)) {
           const bool exact = !(noisy || scaled);
           // the wave's best v bounds what is worth an exact score; those of u
@@ -776,7 +837,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
     if constexpr (GROUPS > 0) {
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        if ((uint32_t)g * BLOCK * 8u < a.q) load_place_low(z, ((uint32_t)g * BLOCK + threadIdx.x) * 8u, a.q, r[g]);
+        if ((uint32_t)g * BLOCK * 8u < a.q) load_place(z, ((uint32_t)g * BLOCK + threadIdx.x) * 8u, a.q, r[g], LOWEST<T>);
     }
     if (threadIdx.x < 64u) {
       teacher_part(a, row, z, c);
@@ -788,7 +849,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
       for (int g = 0; g < G; ++g)
         if ((uint32_t)g * BLOCK * 8u < a.q) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) t.m = fmaxf(t.m, value(r[g], j));
+          for (int j = 0; j < 8; j += 2) t.m = max3(t.m, value(r[g], j), value(r[g], j + 1));
           hide(r[g]);
         }
 #pragma unroll
@@ -802,13 +863,12 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
         }
     } else {
       for (uint32_t d = threadIdx.x * 8u; d < a.q; d += BLOCK * 8u) {
-        load_place_low(z, d, a.q, r[0]);
+        load_place(z, d, a.q, r[0], LOWEST<T>);
         float x[8], m = t.m, s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = value(r[0], j);
-          m = fmaxf(m, x[j]);
-        }
+        for (int j = 0; j < 8; ++j) x[j] = value(r[0], j);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * l2);
         t.s = t.s * __builtin_amdgcn_exp2f((t.m - m) * l2) + s;
@@ -825,8 +885,13 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
       T *o = reinterpret_cast<T *>(a.grad) + (int64_t)row * a.grad_stride;
       auto write = [&](uint32_t d, const Raw8<T> &v) {
         float x[8];
+        if (some) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = some ? f * softmax_of<T>(value(v, j), t.m, rtau, ls) : 0.0f;
+          for (int j = 0; j < 8; ++j) x[j] = f * softmax_of<T>(value(v, j), t.m, rtau, ls);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+        }
         store8(o + d, a.q - d, x);
       };
       if constexpr (GROUPS > 0) {
