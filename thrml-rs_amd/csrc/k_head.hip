@@ -61,10 +61,41 @@ static size_t table_bytes(const LogitRows &a, uint32_t chunk) {
 
 __device__ __forceinline__ uint32_t hash_at(uint32_t d, uint32_t hash) { return (d * 2654435761u >> 12) & (hash - 1u); }
 
-__device__ __forceinline__ float bias_of(const Table &t, uint32_t d) {
-  uint32_t h = hash_at(d, t.hash);
-  while (t.keys[h] != d) h = (h + 1u) & (t.hash - 1u);  // it is there
-  return t.vals[h];
+// The biases' hash table: a value for each place; bias_put is false where the place
+// has one already.
+__device__ __forceinline__ bool bias_put(uint32_t *keys, float *vals, uint32_t hash, uint32_t d, float v) {
+  uint32_t h = hash_at(d, hash);
+  for (;;) {  // (at most half of the slots are ever taken)
+    const uint32_t old = atomicCAS(&keys[h], NO_KEY, d);
+    if (old == NO_KEY) vals[h] = v;
+    if (old == NO_KEY || old == d) return old != d;
+    h = (h + 1u) & (hash - 1u);
+  }
+}
+__device__ __forceinline__ uint32_t bias_slot(const uint32_t *keys, uint32_t hash, uint32_t d) {
+  uint32_t h = hash_at(d, hash);
+  while (keys[h] != d) h = (h + 1u) & (hash - 1u);  // it is there
+  return h;
+}
+__device__ __forceinline__ float bias_of(const uint32_t *keys, const float *vals, uint32_t hash, uint32_t d) {
+  return vals[bias_slot(keys, hash, d)];
+}
+// Where a category is named more than once, its entries are added in list order by the
+// thread of the first one.
+__device__ __forceinline__ void bias_sums(const LogitRows &a, const int32_t *ids, const float *vals, uint32_t c0,
+                                          uint32_t n, const uint32_t *keys, float *sums, uint32_t hash,
+                                          uint32_t block) {
+  for (uint32_t i = threadIdx.x; i < a.n_bias; i += block) {
+    const int32_t id = ids[i];
+    if ((uint32_t)id - c0 >= n) continue;
+    bool first = true;
+    for (uint32_t j = 0; j < i && first; ++j) first = ids[j] != id;
+    if (!first) continue;
+    float s = vals[i];
+    for (uint32_t j = i + 1; j < a.n_bias; ++j)
+      if (ids[j] == id) s += vals[j];
+    sums[bias_slot(keys, hash, (uint32_t)id - c0)] = s;
+  }
 }
 
 // What a lane keeps of its row's lists: of the first 4096 history entries, 4
@@ -148,44 +179,15 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
     const int32_t *ids = a.bias_ids + (int64_t)row * a.bias_stride;
     const float *vals = a.bias_values + (int64_t)row * a.bias_stride;
     int again = 0;
+    const uint32_t n = min(t.chunk, a.q - c0);
     for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
       const uint32_t d = (uint32_t)(i == tid ? lists.bias_id : ids[i]) - c0;
-      const float v = i == tid ? lists.bias : vals[i];
-      if (d < t.chunk && d < a.q - c0) {
-        uint32_t h = hash_at(d, t.hash);
-        for (;;) {  // (at most half of the slots are ever taken)
-          const uint32_t old = atomicCAS(&t.keys[h], NO_KEY, d);
-          if (old == NO_KEY) {
-            atomicOr(&t.tab[d], T_BIAS);
-            t.vals[h] = v;
-            break;
-          }
-          if (old == d) {
-            again = 1;
-            break;
-          }
-          h = (h + 1u) & (t.hash - 1u);
-        }
+      if (d < n) {
+        atomicOr(&t.tab[d], T_BIAS);
+        again |= bias_put(t.keys, t.vals, t.hash, d, i == tid ? lists.bias : vals[i]) ? 0 : 1;
       }
     }
-    // a category named more than once: its entries are added in list order by
-    // the thread of the first one
-    if (__syncthreads_or(again)) {
-      for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
-        const int32_t id = ids[i];
-        const uint32_t d = (uint32_t)id - c0;
-        if (d >= t.chunk || d >= a.q - c0) continue;
-        bool first = true;
-        for (uint32_t j = 0; j < i && first; ++j) first = ids[j] != id;
-        if (!first) continue;
-        float s = vals[i];
-        for (uint32_t j = i + 1; j < a.n_bias; ++j)
-          if (ids[j] == id) s += vals[j];
-        uint32_t h = hash_at(d, t.hash);
-        while (t.keys[h] != d) h = (h + 1u) & (t.hash - 1u);
-        t.vals[h] = s;
-      }
-    }
+    if (__syncthreads_or(again)) bias_sums(a, ids, vals, c0, n, t.keys, t.vals, t.hash, BLOCK);
   }
   __syncthreads();
 }
@@ -279,7 +281,7 @@ __device__ __forceinline__ void row_values(const Raw8<T> &r, bool table, const T
       if (((w[0] | w[1] | w[2] | w[3] | w[4] | w[5] | w[6] | w[7]) & T_BIAS) != 0u) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (w[j] & T_BIAS) y[j] = y[j] + bias_of(t, d + j);
+          if (w[j] & T_BIAS) y[j] = y[j] + bias_of(t.keys, t.vals, t.hash, d + j);
       }
       w4[0] = w4[1] = make_uint4(0, 0, 0, 0);
     }
@@ -394,16 +396,29 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
 // row, and its log-probability is x - m - log(sum exp(x - m)), all in one pass
 // over the row: the running maximum and sum of a softmax per lane, and the pick.
 //
-// The pick is exact in 64 bits at f32 cost.  v, the score from hardware
-// logarithms and x from a reciprocal of the temperature, is within S_MARGIN +
-// |v| S_REL of the score in 64 bits; only a lane whose v exceeds its wave's best
-// exact score less that margin computes the score in 64 bits (from x as the
-// steps in f32 give it), a few times per wave and row.  A score of u below 2^-126 is
-// that of 2^-126 in v, which is no less than its own.  An allowed category
-// whose own score is -inf (u = 0) is taken only where there is no other, a
-// masked one never.
+// The pick is exact in 64 bits at f32 cost.  v, the score from hardware logarithms and
+// x from a reciprocal of the temperature, is within S_MARGIN + |v| S_REL of the score in
+// 64 bits.  A lane keeps its best group of 8 by v and the best v of its other groups;
+// at the end of a part of the row the workgroup's best v, less that margin twice over, says
+// which lanes look at their group again (or, if their second is that close, at all
+// their groups) and compute the score in 64 bits, from x as the steps in f32 give it.
+// That is mostly one lane, once.  v of a u below 2^-126 is that of 2^-126, no less than
+// its own: where one comes into play, the row is done again without a bound.  An
+// allowed category whose own score is -inf (u = 0) is taken only where there is no
+// other, a masked one never.
 constexpr float S_MARGIN = 1e-4f, S_REL = 0x1p-18f;
 constexpr float LOG2E = 1.44269504f;
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+  return v;
+}
 
 struct SamplePart {
   double best;
@@ -439,150 +454,360 @@ __device__ __forceinline__ void part_write(const SamplePart &s, uint64_t row, in
   logprob[row] = ok ? (s.x - s.m) - logf(s.sum) : __builtin_nanf("");
 }
 
-// A workgroup takes a segment of a row in chunks of BLOCK * 8 V categories; the next
-// chunk's logits and uniforms are on their way while it works on one.
-template <class T, int V>
-struct SampleChunk {
-  Raw8<T> z[V];
-  Raw8<float> u[V];
-  uint32_t live[V];
+// What the lists name is few beside the row and goes apart: a hash table in LDS holds
+// the words (T_PROMPT, T_BIAS, count) of the categories named in a part of the row,
+// a bitmap says which these are.  The pass over the part leaves them out, and lanes
+// score them eight slots at a time.  So the lists are scanned once for a part, as
+// large as LDS allows, and the waves go over it without a barrier.
+struct Named {
+  uint32_t *keys, *words, *flags, *bias_keys;
+  float *bias_vals;
+  uint32_t slots, hash;  // of the table, of the biases' table
 };
+constexpr uint32_t PART_MAX = 131072;  // categories that a bitmap of 16 KB holds
 
-template <class T, int BLOCK, int V>
-__device__ __forceinline__ void sample_load(const T *z, const float *u, const uint8_t *mask, uint32_t c0, uint32_t n,
-                                            SampleChunk<T, V> &k) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const uint32_t d = ((uint32_t)v * BLOCK + threadIdx.x) * 8u;
-    load_place(z + c0, d, n, k.z[v]);
-    if (u) load_place(u + c0, d, n, k.u[v]);
-    const uint32_t in = d >= n ? 0u : d + 8u <= n ? 255u : (1u << (n - d)) - 1u;
-    k.live[v] = mask && in ? mask[(c0 + d) / 8u] & in : in;
+struct NamedPlan {
+  uint32_t part, slots, hash;
+  size_t bytes;
+};
+// The largest part (a multiple of unit, at least unit) whose tables take `limit` bytes.
+static NamedPlan named_plan(const LogitRows &a, uint32_t seg, uint32_t unit, size_t limit) {
+  NamedPlan p{std::min(seg, PART_MAX), 0, 0, 0};
+  if (!a.history && !a.n_bias) {
+    p.part = seg;
+    return p;
+  }
+  for (;;) {
+    const uint64_t n = std::min<uint64_t>((uint64_t)a.history_len * (a.history ? 1 : 0) + a.n_bias, p.part);
+    p.slots = 512;  // at most three quarters are taken
+    while ((uint64_t)p.slots * 3 < n * 4) p.slots *= 2;
+    p.hash = hash_slots(a.n_bias, p.part);
+    p.bytes = (size_t)p.slots * 8 + p.part / 8 + (size_t)p.hash * 8;
+    if (p.bytes <= limit || p.part <= unit) return p;
+    p.part = std::max(unit, p.part / 2 / unit * unit);
   }
 }
 
-template <class T, int BLOCK, int V>
+__device__ __forceinline__ uint32_t named_slot(const Named &t, uint32_t d, bool *fresh) {
+  uint32_t h = hash_at(d, t.slots);
+  for (;;) {
+    const uint32_t old = atomicCAS(&t.keys[h], NO_KEY, d);
+    *fresh = old == NO_KEY;
+    if (old == NO_KEY || old == d) return h;
+    h = (h + 1u) & (t.slots - 1u);
+  }
+}
+
+// Fills the tables for the n categories from c0 on; begins and ends with a barrier.
+template <int BLOCK>
+__device__ __forceinline__ void named_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
+                                           uint64_t row, uint32_t c0, uint32_t n, const Named &t) {
+  constexpr int KEPT = RowLists<BLOCK>::KEPT;
+  const uint32_t tid = threadIdx.x;
+  __syncthreads();
+  for (uint32_t i = tid; i < t.slots; i += BLOCK) {
+    t.keys[i] = NO_KEY;
+    t.words[i] = 0;
+  }
+  for (uint32_t i = tid; i < (n + 31u) / 32u; i += BLOCK) t.flags[i] = 0;
+  for (uint32_t i = tid; i < t.hash; i += BLOCK) t.bias_keys[i] = NO_KEY;
+  __syncthreads();
+  auto name = [&](uint32_t d) {
+    bool fresh;
+    const uint32_t h = named_slot(t, d, &fresh);
+    if (fresh) atomicOr(&t.flags[d / 32u], 1u << (d % 32u));
+    return h;
+  };
+  auto note = [&](uint32_t i, const int32_t (&v)[4]) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t d = (uint32_t)v[j] - c0;
+      if (i + j < p.len && d < n) {
+        const uint32_t h = name(d);
+        if (i + j < p.prompt)
+          atomicOr(&t.words[h], T_PROMPT);
+        else
+          atomicAdd(&t.words[h], 1u);
+      }
+    }
+  };
+  if (a.history) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if ((uint32_t)k * BLOCK * 4u < p.len) note((uint32_t)k * BLOCK * 4u + tid * 4u, lists.id[k]);
+    const int32_t *h = a.history + (int64_t)row * a.history_stride;
+    for (uint32_t i = KEPT * BLOCK * 4u + tid * 4u; i < p.len; i += BLOCK * 4u) {
+      int32_t v[4];
+      RowLists<BLOCK>::get(h, p.len, i, v);
+      note(i, v);
+    }
+  }
+  if (a.n_bias) {
+    const int32_t *ids = a.bias_ids + (int64_t)row * a.bias_stride;
+    const float *vals = a.bias_values + (int64_t)row * a.bias_stride;
+    int again = 0;
+    for (uint32_t i = tid; i < a.n_bias; i += BLOCK) {
+      const uint32_t d = (uint32_t)(i == tid ? lists.bias_id : ids[i]) - c0;
+      if (d < n) {
+        atomicOr(&t.words[name(d)], T_BIAS);
+        again |= bias_put(t.bias_keys, t.bias_vals, t.hash, d, i == tid ? lists.bias : vals[i]) ? 0 : 1;
+      }
+    }
+    if (__syncthreads_or(again)) bias_sums(a, ids, vals, c0, n, t.bias_keys, t.bias_vals, t.hash, BLOCK);
+  }
+  __syncthreads();
+}
+
+// One row's state in a lane.
+struct Sampler {
+  SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
+  // of a part's groups: the best v, the place of its group, the best v of the others
+  float first, second;
+  uint32_t at;
+  float t, rt;
+  bool scaled, noisy, odd = false;
+
+  __device__ __forceinline__ void begin(const RowParams &p, const float *u, const float *temperature) {
+    t = p.t;
+    scaled = p.t > 0.0f;
+    noisy = u && (scaled || !temperature);
+    rt = scaled ? 1.0f / p.t : 1.0f;
+  }
+
+  // What v has to reach where the best is b.  Greedy rows without a temperature have
+  // x exactly, and of equal ones the lowest category counts.
+  __device__ __forceinline__ float bound(float b) const {
+    return noisy || scaled ? b - (S_MARGIN + fabsf(b) * S_REL) : b;
+  }
+
+  // v of eight logits with penalties and biases; -inf where the bit in live is clear
+  __device__ __forceinline__ void scores(const float (&y)[8], const uint32_t (&u)[8], uint32_t live, float (&x)[8],
+                                         float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = y[j] * rt;
+    if (__any(live != 255u)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
+    }
+    if (noisy) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float l =
+            __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(__builtin_bit_cast(float, u[j]), 0x1p-126f, INFINITY));
+        v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = x[j];
+    }
+  }
+
+  __device__ __forceinline__ void add(const float (&x)[8]) {
+    float m = s.m;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
+    s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * LOG2E) + sum;
+    s.m = m;
+  }
+
+  // Eight logits from place d on.
+  __device__ __forceinline__ void take(const float (&y)[8], const uint32_t (&u)[8], uint32_t live, uint32_t d) {
+    float x[8], v[8];
+    scores(y, u, live, x, v);
+    add(x);
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) top = max3(top, v[j], v[j + 1]);
+    second = __builtin_amdgcn_fmed3f(second, first, top);
+    at = top > first ? d : at;
+    first = fmaxf(first, top);
+  }
+
+  // The scores in 64 bits of those of eight logits that `todo` names; id(j): category.
+  template <class Id>
+  __device__ __forceinline__ void settle(const float (&y)[8], const uint32_t (&u)[8], const float (&v)[8],
+                                         uint32_t todo, Id id) {
+    while (todo) {
+      const int j = __builtin_ctz(todo);
+      todo &= todo - 1u;
+      float yj = y[0], vj = v[0];
+      uint32_t uj = u[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        yj = i == j ? y[i] : yj;
+        uj = i == j ? u[i] : uj;
+        vj = i == j ? v[i] : vj;
+      }
+      const float xj = scaled ? yj / t : yj;
+      double e = xj;
+      if (noisy) {
+        e = xj - log(-log((double)__builtin_bit_cast(float, uj)));
+        // (v of a u below 2^-126 is too high, and so are bounds that come from it)
+        odd = odd || __builtin_bit_cast(float, uj) < 0x1p-126f;
+        e = e == -INFINITY && xj > -INFINITY ? -__DBL_MAX__ : e;
+      }
+      const int32_t c = id(j);
+      if (e > s.best || (e == s.best && c < s.arg)) {
+        s.best = e;
+        s.x = xj;
+        s.arg = c;
+      }
+    }
+  }
+
+  static __device__ __forceinline__ uint32_t reach(const float (&v)[8], const float (&x)[8], float cut) {
+    uint32_t todo = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) todo |= (x[j] > -INFINITY && !(v[j] < cut) ? 1u : 0u) << j;
+    return todo;
+  }
+};
+
+// A lane's next 8 logits and uniforms.
+template <class T>
+struct SampleGroup {
+  Raw8<T> z;
+  Raw8<float> u;
+  uint32_t live;
+  __device__ __forceinline__ void load(const T *z_, const float *u_, const uint8_t *mask, uint32_t c, uint32_t end) {
+    load_place(z_, c, end, z);
+    if (u_) load_place(u_, c, end, u);
+    const uint32_t in = c >= end ? 0u : c + 8u <= end ? 255u : (1u << (end - c)) - 1u;
+    live = mask && in ? mask[c / 8u] & in : in;
+  }
+};
+
+template <class T, int BLOCK>
 __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const float *__restrict__ u, int64_t u_stride,
-                                                       uint32_t seg, uint32_t n_seg, uint32_t hash,
-                                                       SamplePart *__restrict__ parts, int32_t *__restrict__ index,
-                                                       float *__restrict__ logprob) {
+                                                          uint32_t seg, uint32_t n_seg, NamedPlan plan,
+                                                          SamplePart *__restrict__ parts, int32_t *__restrict__ index,
+                                                          float *__restrict__ logprob) {
   extern __shared__ uint32_t lds[];
   __shared__ SamplePart wave_part[BLOCK / 64];
-  constexpr uint32_t CHUNK = BLOCK * 8 * V;
+  __shared__ float wave_best[BLOCK / 64];
   const bool table = a.history || a.n_bias;
-  const Table tab{lds, lds + CHUNK, reinterpret_cast<float *>(lds + CHUNK + hash), CHUNK, hash};
+  const Named named{lds, lds + plan.slots, lds + 2 * plan.slots, lds + 2 * plan.slots + plan.part / 32u,
+                    reinterpret_cast<float *>(lds + 2 * plan.slots + plan.part / 32u + plan.hash), plan.slots, plan.hash};
+  const uint8_t *flags = reinterpret_cast<const uint8_t *>(named.flags);
   const uint64_t n_tasks = a.rows * n_seg;
   for (uint64_t task = blockIdx.x; task < n_tasks; task += gridDim.x) {
     const uint64_t row = task / n_seg;
     const uint32_t s0 = (uint32_t)(task % n_seg) * seg, s1 = min(s0 + seg, a.q);
-    const RowParams p = row_params(a, row);
-    const bool scaled = p.t > 0.0f, noisy = u && (scaled || !a.temperature);
-    const float rt = scaled ? 1.0f / p.t : 1.0f;
-    const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
-    const float *ur = noisy ? u + (int64_t)row * u_stride : nullptr;
-    const uint8_t *mask = a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) : nullptr;
-    SampleChunk<T, V> next{};
-    sample_load<T, BLOCK, V>(z, ur, mask, s0, min(CHUNK, s1 - s0), next);
     RowLists<BLOCK> lists;
-    if (table) {
-      lists.load(a, row);
-      table_clear(tab, BLOCK);
-    }
-    SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
-    float thr = -INFINITY;  // of the wave
-    for (uint32_t c0 = s0; c0 < s1; c0 += CHUNK) {
-      const SampleChunk<T, V> k = next;
-      if (table) table_fill(a, p, lists, row, c0, tab);
-      if (c0 + CHUNK < s1) sample_load<T, BLOCK, V>(z, ur, mask, c0 + CHUNK, min(CHUNK, s1 - c0 - CHUNK), next);
+    if (table) lists.load(a, row);
+    const RowParams p = row_params(a, row);
+    Sampler s;
+    s.begin(p, u, a.temperature);
+    const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
+    const float *ur = s.noisy ? u + (int64_t)row * u_stride : nullptr;
+    const uint8_t *mask = a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) : nullptr;
+    for (bool bounded = true;; bounded = false) {
+      SampleGroup<T> next{};
+      next.load(z, ur, mask, s0 + threadIdx.x * 8u, s1);
+      for (uint32_t c0 = s0; c0 < s1; c0 += plan.part) {
+        const uint32_t end = min(c0 + plan.part, s1);
+        if (table) named_fill(a, p, lists, row, c0, end - c0, named);
+        auto group = [&](const SampleGroup<T> &k, uint32_t d, float (&y)[8]) {
 #pragma unroll
-      for (int g = 0; g < V; ++g) {
-        const uint32_t d = ((uint32_t)g * BLOCK + threadIdx.x) * 8u, live = k.live[g];
-        float x[8], y[8], v[8];
-        row_values(k.z[g], table, tab, d, p, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = y[j] * rt;
-        if (__any(live != 255u)) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
+          for (int j = 0; j < 8; ++j) y[j] = value(k.z, j);
+          return table && d < end ? k.live & ~(uint32_t)flags[(d - c0) / 8u] : k.live;
+        };
+        s.first = s.second = -INFINITY;
+        s.at = c0;
+        for (uint32_t d0 = c0 + (threadIdx.x & ~63u) * 8u; d0 < end; d0 += BLOCK * 8u) {
+          const uint32_t d = d0 + (threadIdx.x & 63u) * 8u;
+          const SampleGroup<T> k = next;
+          // the next one: in this part, or this wave's first in the next part
+          const uint32_t ahead = d0 + BLOCK * 8u < end ? d0 + BLOCK * 8u : end + (threadIdx.x & ~63u) * 8u;
+          if (ahead < s1) next.load(z, ur, mask, ahead + (threadIdx.x & 63u) * 8u, s1);
+          float y[8];
+          const uint32_t live = group(k, d, y);
+          s.take(y, k.u.w, live, d);
         }
-        float m = s.m;
+        const float w = wave_max(s.first);
+        if ((threadIdx.x & 63u) == 0) wave_best[threadIdx.x / 64u] = w;
+        __syncthreads();
+        float cut = -INFINITY;
+        if (bounded) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
-        s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * LOG2E) + sum;
-        s.m = m;
-        if (noisy) {
+          for (int i = 0; i < BLOCK / 64; ++i) cut = fmaxf(cut, wave_best[i]);
+          cut = s.bound(cut);
+        }
+        if (!(s.first < cut) && (s.first > -INFINITY || !bounded)) {
+          const bool all = !(s.second < cut);
+          for (uint32_t d = all ? c0 + threadIdx.x * 8u : s.at; d < end; d += all ? BLOCK * 8u : end) {
+            SampleGroup<T> k{};
+            k.load(z, ur, mask, d, s1);
+            float y[8], x[8], v[8];
+            const uint32_t live = group(k, d, y);
+            s.scores(y, k.u.w, live, x, v);
+            s.settle(y, k.u.w, v, Sampler::reach(v, x, cut), [&](int j) { return (int32_t)(d + j); });
+          }
+        }
+        // the named ones
+        for (uint32_t b = 0; b < plan.slots; b += BLOCK * 8u) {
+          float y[8], x[8], v[8];
+          uint32_t c[8], n[8], r[8], live = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float l = __builtin_amdgcn_logf(
-                __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, k.u[g].w[j]), 0x1p-126f, INFINITY));
-            v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
+            const uint32_t i = b + (uint32_t)j * BLOCK + threadIdx.x, key = i < plan.slots ? named.keys[i] : NO_KEY;
+            c[j] = key == NO_KEY ? c0 : c0 + key;
+            n[j] = key == NO_KEY ? 0u : named.words[i];
+            if (key != NO_KEY) live |= 1u << j;
           }
-        } else {
+          if (!__any(live != 0u)) continue;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = x[j];
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) top = max3(top, v[j], v[j + 1]);
-        if (__any(top > thr)) {
-          const bool exact = !(noisy || scaled);
-          // the wave's best v bounds what is worth an exact score; those of u
-          // below 2^-126 are too high for that
-          float b = top;
-          if (noisy) {
-            b = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              b = fmaxf(b, __builtin_bit_cast(float, k.u[g].w[j]) >= 0x1p-126f ? v[j] : -INFINITY);
-          }
-#pragma unroll
-          for (int w = 32; w > 0; w >>= 1) b = fmaxf(b, __shfl_xor(b, w));
-          const float low = exact ? b : b - (S_MARGIN + fabsf(b) * S_REL);
-          uint32_t todo = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) todo |= (v[j] > thr && !(v[j] < low) ? 1u : 0u) << j;
-          while (todo) {
-            const int j = __builtin_ctz(todo);
-            todo &= todo - 1u;
-            float yj = y[0];
-            uint32_t uj = k.u[g].w[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) {
-              yj = i == j ? y[i] : yj;
-              uj = i == j ? k.u[g].w[i] : uj;
-            }
-            const float xj = scaled ? yj / p.t : yj;
-            double e = xj;
-            if (noisy) {
-              e = xj - log(-log((double)__builtin_bit_cast(float, uj)));
-              e = e == -INFINITY && xj > -INFINITY ? -__DBL_MAX__ : e;
-            }
-            if (e > s.best) {
-              s.best = e;
-              s.x = xj;
-              s.arg = (int32_t)(c0 + d + j);
+          for (int j = 0; j < 8; ++j) {
+            y[j] = 0.0f;
+            r[j] = 0;
+            if (live >> j & 1u) {
+              y[j] = (float)z[c[j]];
+              if (ur) r[j] = __builtin_bit_cast(uint32_t, ur[c[j]]);
+              if (mask && !(mask[c[j] / 8u] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
             }
           }
-          b = (float)s.best;
+          float q[8];
 #pragma unroll
-          for (int w = 32; w > 0; w >>= 1) b = fmaxf(b, __shfl_xor(b, w));
-          thr = exact ? b : b - (S_MARGIN + fabsf(b) * S_REL);
+          for (int j = 0; j < 8; ++j) q[j] = y[j];
+          divide_each(q, p.theta);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            y[j] = penalised(y[j], q[j], n[j], p);
+            if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
+          }
+          s.scores(y, r, live, x, v);
+          s.add(x);
+          // (no bound but the other categories': few of these reach it)
+          s.settle(y, r, v, Sampler::reach(v, x, cut), [&](int j) {
+            uint32_t cj = c[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) cj = i == j ? c[i] : cj;
+            return (int32_t)cj;
+          });
         }
       }
+      if (!__syncthreads_or(bounded && s.odd)) break;
+      const Sampler again = s;
+      s = Sampler{};
+      s.t = again.t;
+      s.rt = again.rt;
+      s.scaled = again.scaled;
+      s.noisy = again.noisy;
     }
+    SamplePart o = s.s;
 #pragma unroll
-    for (int k = 32; k > 0; k >>= 1) part_merge(s, part_xor(s, k));
-    if ((threadIdx.x & 63u) == 0) wave_part[threadIdx.x / 64u] = s;
+    for (int k = 32; k > 0; k >>= 1) part_merge(o, part_xor(o, k));
+    if ((threadIdx.x & 63u) == 0) wave_part[threadIdx.x / 64u] = o;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < BLOCK / 64; ++w) part_merge(s, wave_part[w]);
+      for (int w = 1; w < BLOCK / 64; ++w) part_merge(o, wave_part[w]);
       if (n_seg > 1)
-        parts[task] = s;
+        parts[task] = o;
       else
-        part_write(s, row, index, logprob);
+        part_write(o, row, index, logprob);
     }
     __syncthreads();
   }
@@ -607,16 +832,16 @@ __global__ __launch_bounds__(64) void sample_join_kernel(const SamplePart *__res
 // few.
 struct SamplePlan {
   bool wide;  // 1024 threads
-  uint32_t chunk, seg, n_seg;
+  uint32_t seg, n_seg;
 };
 static SamplePlan sample_plan(thrml_ctx *ctx, uint64_t rows, uint32_t q) {
   SamplePlan p;
   p.wide = rows < 2ull * ctx->cu_count && rows * 2 > (uint64_t)ctx->cu_count && q > 8192;
-  p.chunk = p.wide ? 8192 : 4096;
+  const uint32_t pass = p.wide ? 8192 : 4096;  // categories that a workgroup takes at a time
   uint32_t n = 1;
   if (!p.wide)
-    while (rows * n * 2 <= 2ull * ctx->cu_count && cdiv(q, n * 2) >= p.chunk) n *= 2;
-  p.seg = cdiv(cdiv(q, n), p.chunk) * p.chunk;
+    while (rows * n * 2 <= 2ull * ctx->cu_count && cdiv(q, n * 2) >= pass) n *= 2;
+  p.seg = cdiv(cdiv(q, n), pass) * pass;
   p.n_seg = cdiv(q, p.seg);
   return p;
 }
@@ -629,20 +854,19 @@ uint64_t sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q) {
 int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const float *u, int64_t u_stride,
                          int32_t *index, float *logprob, void *work) {
   if (a.rows == 0) return THRML_OK;
-  SamplePlan p = sample_plan(ctx, a.rows, a.q);
-  if (p.wide && a.n_bias > 2048) {  // (the table's place in LDS)
-    p.wide = false;
-    p.chunk = 4096;
-  }
+  const SamplePlan p = sample_plan(ctx, a.rows, a.q);
+  // two workgroups of 512 in a compute unit's LDS, or one of 1024
+  NamedPlan named = named_plan(a, p.seg, 8192, 150 << 10);
+  const bool wide = p.wide && named.bytes <= 150 << 10;
+  if (!wide) named = named_plan(a, p.seg, 4096, 76 << 10);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows * p.n_seg, 1u << 20);
   SamplePart *parts = reinterpret_cast<SamplePart *>(work);
   const int rc = with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
-    auto *f = p.wide ? &sample_kernel<T, 1024, 1> : &sample_kernel<T, 512, 1>;
-    const size_t lds = table_bytes(a, p.chunk);
-    if (int rc = lds_limit(reinterpret_cast<const void *>(f), lds)) return rc;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(p.wide ? 1024 : 512), lds, ctx->stream, a, u, u_stride, p.seg, p.n_seg,
-                       hash_slots(a.n_bias, p.chunk), parts, index, logprob);
+    auto *f = wide ? &sample_kernel<T, 1024> : &sample_kernel<T, 512>;
+    if (int rc = lds_limit(reinterpret_cast<const void *>(f), named.bytes)) return rc;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(wide ? 1024 : 512), named.bytes, ctx->stream, a, u, u_stride, p.seg, p.n_seg,
+                       named, parts, index, logprob);
     THRML_HIP(hipGetLastError());
     return THRML_OK;
   });
@@ -701,17 +925,6 @@ static uint32_t candidate_slots(uint32_t k) {
   return h;
 }
 static size_t candidate_bytes(uint32_t k) { return (size_t)k * 16 + (size_t)candidate_slots(k) * 4; }
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
-  return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
-  return v;
-}
 
 // By the first wave alone: its LDS accesses are in order.
 template <class T>
