@@ -234,11 +234,12 @@ __device__ __forceinline__ bool divides_fast(const float (&a)[8]) {
 
 // a / b for what Divisor::fast does not take, one after the other (side by side they
 // would take the registers of all other work)
-__device__ __forceinline__ void divide_each(float (&a)[8], float b) {
+template <int N>
+__device__ __forceinline__ void divide_each(float (&a)[N], float b) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < N; ++j) {
     a[j] = a[j] / b;
-    if (j < 7) asm volatile("" : "+v"(a[j]), "+v"(a[j + 1]));
+    if (j < N - 1) asm volatile("" : "+v"(a[j]), "+v"(a[j + 1]));
   }
 }
 
@@ -397,15 +398,15 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
 // over the row: the running maximum and sum of a softmax per lane, and the pick.
 //
 // The pick is exact in 64 bits at f32 cost.  v, the score from hardware logarithms and
-// x from a reciprocal of the temperature, is within S_MARGIN + |v| S_REL of the score in
-// 64 bits.  A lane keeps its best group of 8 by v and the best v of its other groups;
-// at the end of a part of the row the workgroup's best v, less that margin twice over, says
-// which lanes look at their group again (or, if their second is that close, at all
-// their groups) and compute the score in 64 bits, from x as the steps in f32 give it.
-// That is mostly one lane, once.  v of a u below 2^-126 is that of 2^-126, no less than
-// its own: where one comes into play, the row is done again without a bound.  An
-// allowed category whose own score is -inf (u = 0) is taken only where there is no
-// other, a masked one never.
+// x from a reciprocal of the temperature, is within S_MARGIN / 2 + |v| S_REL / 2 of the
+// score in 64 bits; picks are compared by v where that decides and in 64 bits, from x as
+// the steps in f32 give it, where it does not.  A lane keeps its best group of 8 by v
+// and the best v of its other groups; at the end of a part of the row the workgroup's
+// best v less the margin says which lanes look at their group again (or, if their
+// second is that close, at all their groups): mostly one.  v of a u below 2^-126 is that
+// of 2^-126, no less than its own: where one comes into play, the row is done again
+// without a bound.  An allowed category whose own score is -inf (u = 0) is taken only
+// where there is no other, a masked one never.
 constexpr float S_MARGIN = 1e-4f, S_REL = 0x1p-18f;
 constexpr float LOG2E = 1.44269504f;
 
@@ -421,30 +422,52 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 struct SamplePart {
-  double best;
-  float m, sum, x;
-  int32_t arg;
+  float m, sum;   // running maximum and sum of exponentials
+  float v, x, u;  // of the pick: its score in 32 bits, logit and uniform (-1: the logit is the score)
+  int32_t arg;    // -1: none yet
 };
+constexpr float U_MIN = 0x1p-126f;
+
+__device__ __forceinline__ double exact_score(float x, float u) {
+  if (u < 0.0f) return x;
+  const double e = x - log(-log((double)u));
+  return e == -INFINITY && x > -INFINITY ? -__DBL_MAX__ : e;
+}
+// b's pick comes before a's: by v where that decides, else in 64 bits.
+__device__ __forceinline__ bool beats(const SamplePart &b, const SamplePart &a) {
+  if (b.arg < 0 || a.arg < 0) return b.arg >= 0;
+  const float margin = 2.0f * S_MARGIN + (fabsf(a.v) + fabsf(b.v)) * S_REL, d = b.v - a.v;
+  if (d > margin && b.u >= U_MIN) return true;
+  if (d < -margin && a.u >= U_MIN) return false;
+  const double ea = exact_score(a.x, a.u), eb = exact_score(b.x, b.u);
+  return eb > ea || (eb == ea && b.arg < a.arg);
+}
 
 __device__ __forceinline__ void part_merge(SamplePart &a, const SamplePart &b) {
   const float m = fmaxf(a.m, b.m);
   a.sum = a.sum * __builtin_amdgcn_exp2f((a.m - m) * LOG2E) + b.sum * __builtin_amdgcn_exp2f((b.m - m) * LOG2E);
   a.m = m;
-  if (b.best > a.best || (b.best == a.best && (uint32_t)b.arg < (uint32_t)a.arg)) {
-    a.best = b.best;
-    a.arg = b.arg;
+  if (beats(b, a)) {
+    a.v = b.v;
     a.x = b.x;
+    a.u = b.u;
+    a.arg = b.arg;
   }
 }
 
-__device__ __forceinline__ SamplePart part_xor(const SamplePart &a, int s) {
-  SamplePart b;
-  b.best = __shfl_xor(a.best, s);
-  b.m = __shfl_xor(a.m, s);
-  b.sum = __shfl_xor(a.sum, s);
-  b.x = __shfl_xor(a.x, s);
-  b.arg = __shfl_xor(a.arg, s);
-  return b;
+// of all lanes of a wave, in lane 0 (a loop, so that there is one merge to compile)
+__device__ __forceinline__ void part_join_wave(SamplePart &a) {
+#pragma unroll 1
+  for (int s = 32; s > 0; s >>= 1) {
+    SamplePart b;
+    b.m = __shfl_xor(a.m, s);
+    b.sum = __shfl_xor(a.sum, s);
+    b.v = __shfl_xor(a.v, s);
+    b.x = __shfl_xor(a.x, s);
+    b.u = __shfl_xor(a.u, s);
+    b.arg = __shfl_xor(a.arg, s);
+    part_merge(a, b);
+  }
 }
 
 __device__ __forceinline__ void part_write(const SamplePart &s, uint64_t row, int32_t *index, float *logprob) {
@@ -560,7 +583,7 @@ __device__ __forceinline__ void named_fill(const LogitRows &a, const RowParams &
 
 // One row's state in a lane.
 struct Sampler {
-  SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
+  SamplePart s{-__FLT_MAX__, 0.0f, -INFINITY, 0.0f, -1.0f, -1};
   // of a part's groups: the best v, the place of its group, the best v of the others
   float first, second;
   uint32_t at;
@@ -580,35 +603,37 @@ struct Sampler {
     return noisy || scaled ? b - (S_MARGIN + fabsf(b) * S_REL) : b;
   }
 
-  // v of eight logits with penalties and biases; -inf where the bit in live is clear
-  __device__ __forceinline__ void scores(const float (&y)[8], const uint32_t (&u)[8], uint32_t live, float (&x)[8],
-                                         float (&v)[8]) const {
+  // v of N logits with penalties and biases; -inf where the bit in live is clear
+  template <int N>
+  __device__ __forceinline__ void scores(const float (&y)[N], const uint32_t (&u)[N], uint32_t live, float (&x)[N],
+                                         float (&v)[N]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = y[j] * rt;
-    if (__any(live != 255u)) {
+    for (int j = 0; j < N; ++j) x[j] = y[j] * rt;
+    if (__any(live != (1u << N) - 1u)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
+      for (int j = 0; j < N; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
     }
     if (noisy) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < N; ++j) {
         const float l =
-            __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(__builtin_bit_cast(float, u[j]), 0x1p-126f, INFINITY));
+            __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(__builtin_bit_cast(float, u[j]), U_MIN, INFINITY));
         v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = x[j];
+      for (int j = 0; j < N; ++j) v[j] = x[j];
     }
   }
 
-  __device__ __forceinline__ void add(const float (&x)[8]) {
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N]) {
     float m = s.m;
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
+    for (int j = 0; j < N; j += 2) m = max3(m, x[j], x[j + 1]);
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
+    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
     s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * LOG2E) + sum;
     s.m = m;
   }
@@ -626,9 +651,9 @@ struct Sampler {
     first = fmaxf(first, top);
   }
 
-  // The scores in 64 bits of those of eight logits that `todo` names; id(j): category.
-  template <class Id>
-  __device__ __forceinline__ void settle(const float (&y)[8], const uint32_t (&u)[8], const float (&v)[8],
+  // Those of N logits that `todo` names against the lane's pick; id(j): category.
+  template <int N, class Id>
+  __device__ __forceinline__ void settle(const float (&y)[N], const uint32_t (&u)[N], const float (&v)[N],
                                          uint32_t todo, Id id) {
     while (todo) {
       const int j = __builtin_ctz(todo);
@@ -636,32 +661,32 @@ struct Sampler {
       float yj = y[0], vj = v[0];
       uint32_t uj = u[0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) {
+      for (int i = 1; i < N; ++i) {
         yj = i == j ? y[i] : yj;
         uj = i == j ? u[i] : uj;
         vj = i == j ? v[i] : vj;
       }
-      const float xj = scaled ? yj / t : yj;
-      double e = xj;
-      if (noisy) {
-        e = xj - log(-log((double)__builtin_bit_cast(float, uj)));
-        // (v of a u below 2^-126 is too high, and so are bounds that come from it)
-        odd = odd || __builtin_bit_cast(float, uj) < 0x1p-126f;
-        e = e == -INFINITY && xj > -INFINITY ? -__DBL_MAX__ : e;
-      }
-      const int32_t c = id(j);
-      if (e > s.best || (e == s.best && c < s.arg)) {
-        s.best = e;
-        s.x = xj;
-        s.arg = c;
+      SamplePart b;
+      b.v = vj;
+      b.x = scaled ? yj / t : yj;
+      b.u = noisy ? __builtin_bit_cast(float, uj) : -1.0f;
+      b.arg = id(j);
+      // (v of a u below 2^-126 is too high, and so are bounds that come from it)
+      odd = odd || (noisy && b.u < U_MIN);
+      if (beats(b, s)) {
+        s.v = b.v;
+        s.x = b.x;
+        s.u = b.u;
+        s.arg = b.arg;
       }
     }
   }
 
-  static __device__ __forceinline__ uint32_t reach(const float (&v)[8], const float (&x)[8], float cut) {
+  template <int N>
+  static __device__ __forceinline__ uint32_t reach(const float (&v)[N], const float (&x)[N], float cut) {
     uint32_t todo = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) todo |= (x[j] > -INFINITY && !(v[j] < cut) ? 1u : 0u) << j;
+    for (int j = 0; j < N; ++j) todo |= (x[j] > -INFINITY && !(v[j] < cut) ? 1u : 0u) << j;
     return todo;
   }
 };
@@ -748,11 +773,12 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
           }
         }
         // the named ones
-        for (uint32_t b = 0; b < plan.slots; b += BLOCK * 8u) {
-          float y[8], x[8], v[8];
-          uint32_t c[8], n[8], r[8], live = 0;
+        constexpr int N = 4;
+        for (uint32_t b = 0; b < plan.slots; b += BLOCK * N) {
+          float y[N], x[N], v[N];
+          uint32_t c[N], n[N], r[N], live = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < N; ++j) {
             const uint32_t i = b + (uint32_t)j * BLOCK + threadIdx.x, key = i < plan.slots ? named.keys[i] : NO_KEY;
             c[j] = key == NO_KEY ? c0 : c0 + key;
             n[j] = key == NO_KEY ? 0u : named.words[i];
@@ -760,7 +786,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
           }
           if (!__any(live != 0u)) continue;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < N; ++j) {
             y[j] = 0.0f;
             r[j] = 0;
             if (live >> j & 1u) {
@@ -769,12 +795,12 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
               if (mask && !(mask[c[j] / 8u] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
             }
           }
-          float q[8];
+          float q[N];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) q[j] = y[j];
+          for (int j = 0; j < N; ++j) q[j] = y[j];
           divide_each(q, p.theta);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < N; ++j) {
             y[j] = penalised(y[j], q[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
@@ -784,7 +810,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
           s.settle(y, r, v, Sampler::reach(v, x, cut), [&](int j) {
             uint32_t cj = c[0];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) cj = i == j ? c[i] : cj;
+            for (int i = 1; i < N; ++i) cj = i == j ? c[i] : cj;
             return (int32_t)cj;
           });
         }
@@ -798,11 +824,11 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
       s.noisy = again.noisy;
     }
     SamplePart o = s.s;
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) part_merge(o, part_xor(o, k));
+    part_join_wave(o);
     if ((threadIdx.x & 63u) == 0) wave_part[threadIdx.x / 64u] = o;
     __syncthreads();
     if (threadIdx.x == 0) {
+#pragma unroll 1
       for (int w = 1; w < BLOCK / 64; ++w) part_merge(o, wave_part[w]);
       if (n_seg > 1)
         parts[task] = o;
@@ -818,10 +844,9 @@ __global__ __launch_bounds__(64) void sample_join_kernel(const SamplePart *__res
                                                          uint32_t n_seg, int32_t *__restrict__ index,
                                                          float *__restrict__ logprob) {
   for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    SamplePart s{-INFINITY, -__FLT_MAX__, 0.0f, 0.0f, -1};
+    SamplePart s{-__FLT_MAX__, 0.0f, -INFINITY, 0.0f, -1.0f, -1};
     for (uint32_t i = threadIdx.x; i < n_seg; i += 64u) part_merge(s, parts[row * n_seg + i]);
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) part_merge(s, part_xor(s, k));
+    part_join_wave(s);
     if (threadIdx.x == 0) part_write(s, row, index, logprob);
   }
 }
