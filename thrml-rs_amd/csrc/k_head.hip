@@ -192,20 +192,6 @@ __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &
   __syncthreads();
 }
 
-// a / b for many a: q = a r with r = 1 / b rounded, and one step of the remainder,
-// which an fma gives exactly, leave the correctly rounded quotient (Markstein 1990)
-// as long as nothing under- or overflows: b within 2^-20 .. 2^20, |a| within 2^-70 ..
-// 2^100.  3 operations instead of the 10 of a full division.
-struct Divisor {
-  float b, r;
-  bool plain;
-  __device__ __forceinline__ explicit Divisor(float b_) : b(b_), r(1.0f / b_), plain(b_ >= 0x1p-20f && b_ <= 0x1p20f) {}
-  __device__ __forceinline__ float fast(float a) const {
-    const float q = a * r;
-    return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
-  }
-};
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

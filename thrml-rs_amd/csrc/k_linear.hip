@@ -24,101 +24,199 @@ uint64_t linear_i8_work(thrml_ctx *, uint64_t rows, uint32_t k, uint32_t) {
   return scales_bytes(rows) + rows * padded_k(k);
 }
 
-// A workgroup quantises one row.
+// x / d, rounded to integers; |x| is at most 127 d, so that only d decides whether
+// Divisor::fast is exact (a quotient below 2^-50 may be off and rounds to 0 either way).
+__device__ __forceinline__ uint32_t integers4(const float *v, const Divisor &d) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w |= ((uint32_t)(int)rintf(d.plain ? d.fast(v[j]) : v[j] / d.b) & 255u) << (8 * j);
+  return w;
+}
+template <class T>
+__device__ __forceinline__ uint2 integers8(const Raw8<T> &r, const Divisor &d) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = value(r, j);
+  return make_uint2(integers4(v, d), integers4(v + 4, d));
+}
+// a row's largest magnitude and whether it has an infinity or NaN
+struct Peak {
+  float m = 0.0f;
+  int bad = 0;
+  template <class T>
+  __device__ __forceinline__ void take(const Raw8<T> &r) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = fabsf(value(r, j));
+      bad |= !(v < INFINITY);
+      m = fmaxf(m, v);
+    }
+  }
+  __device__ __forceinline__ void join_wave() {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+    bad = __any(bad);
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void load_x(const T *xr, uint32_t c, uint32_t k, Raw8<T> &r) {
+  if (c + 8u <= k)
+    load8(xr + c, r);
+  else
+    load8_part(xr + c, c < k ? k - c : 0u, r);
+}
+
+// A workgroup quantises one row; one of at most 8192 values stays in registers between
+// its maximum and its integers.
 template <class T>
 __global__ __launch_bounds__(256) void quantise_kernel(const T *__restrict__ x, int64_t x_stride, uint64_t rows,
                                                        uint32_t k, uint32_t kp, float *__restrict__ scale,
                                                        int8_t *__restrict__ xq) {
-  __shared__ float buf[4];
+  __shared__ float peak[4];
+  __shared__ int bads[4];
+  constexpr int KEPT = 4;
   for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T *xr = x + (int64_t)row * x_stride;
-    float m = 0.0f;
-    int bad = 0;
-    for (uint32_t c = threadIdx.x * 8u; c < k; c += 2048u) {
-      Raw8<T> r;
-      if (c + 8u <= k)
-        load8(xr + c, r);
-      else
-        load8_part(xr + c, k - c, r);
+    Raw8<T> r[KEPT];
+    Peak p;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = fabsf(value(r, j));
-        bad |= !(v < INFINITY);
-        m = fmaxf(m, v);
-      }
+    for (int g = 0; g < KEPT; ++g)
+      if ((uint32_t)g * 2048u < kp) load_x(xr, (uint32_t)g * 2048u + threadIdx.x * 8u, k, r[g]);
+#pragma unroll
+    for (int g = 0; g < KEPT; ++g)
+      if ((uint32_t)g * 2048u < kp) p.take(r[g]);
+    for (uint32_t c = KEPT * 2048u + threadIdx.x * 8u; c < k; c += 2048u) {
+      Raw8<T> t;
+      load_x(xr, c, k, t);
+      p.take(t);
     }
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-    if ((threadIdx.x & 63u) == 0) buf[threadIdx.x / 64u] = m;
-    bad = __syncthreads_or(bad);
-    m = fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
-    const float s = m / 127.0f, d = s > 0.0f ? s : 1.0f;
+    p.join_wave();
+    if ((threadIdx.x & 63u) == 0) {
+      peak[threadIdx.x / 64u] = p.m;
+      bads[threadIdx.x / 64u] = p.bad;
+    }
+    __syncthreads();
+    const float m = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
+    const int bad = bads[0] | bads[1] | bads[2] | bads[3];
+    const float s = m / 127.0f;
+    const Divisor d(s > 0.0f ? s : 1.0f);
     if (threadIdx.x == 0) scale[row] = bad ? __builtin_nanf("") : s;
     int8_t *o = xq + row * kp;
-    for (uint32_t c = threadIdx.x * 8u; c < kp; c += 2048u) {
-      Raw8<T> r;
-      if (c + 8u <= k)
-        load8(xr + c, r);
-      else
-        load8_part(xr + c, c < k ? k - c : 0u, r);
-      uint32_t w[2] = {0, 0};
+    auto put = [&](uint32_t c, const Raw8<T> &t) {
+      if (c < kp) *reinterpret_cast<uint2 *>(o + c) = bad ? make_uint2(0, 0) : integers8(t, d);
+    };
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int v = bad ? 0 : (int)rintf(value(r, j) / d);
-        w[j / 4] |= ((uint32_t)v & 255u) << (8 * (j & 3));
-      }
-      *reinterpret_cast<uint2 *>(o + c) = make_uint2(w[0], w[1]);
+    for (int g = 0; g < KEPT; ++g)
+      if ((uint32_t)g * 2048u < kp) put((uint32_t)g * 2048u + threadIdx.x * 8u, r[g]);
+    for (uint32_t c = KEPT * 2048u + threadIdx.x * 8u; c < kp; c += 2048u) {
+      Raw8<T> t;
+      load_x(xr, c, k, t);
+      put(c, t);
     }
     __syncthreads();
   }
 }
 
-// 16 weights from column c0 on; zeros behind k
-__device__ __forceinline__ i32x4 load_w16(const int8_t *wr, uint32_t c0, uint32_t k) {
-  if (c0 + 16u <= k) return *reinterpret_cast<const i32x4_a1 *>(wr + c0);
+// 16 weights of a row from column c0 on, any weights behind k (x is zero there): as
+// they lie in memory up to `end`, the end of the last row's weights, which is all that
+// may be read
+__device__ __forceinline__ i32x4 load_w16(const int8_t *wr, uint32_t c0, uint32_t k, const int8_t *end) {
+  if (wr + c0 + 16u <= end) return *reinterpret_cast<const i32x4_a1 *>(wr + c0);
   i32x4 r = {0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 16; ++j)
     if (c0 + j < k) r[j / 4] |= (int32_t)((uint32_t)(uint8_t)wr[c0 + j] << (8 * (j & 3)));
   return r;
 }
+__device__ __forceinline__ const int8_t *weights_end(const LinearArgs &a) {
+  return a.w + (int64_t)(a.q - 1u) * a.w_stride + a.k;
+}
 
 // ---------------------------------------------------------------------------
-// Few rows: the weights are read once and that is what it costs.  A workgroup takes
-// 16 CT output channels and all rows (16 RT of them at most); its four waves take
-// every fourth 64-column step of k, so that together they read 256 neighbouring
-// bytes of each weight row, straight into the operand registers of
-// v_mfma_i32_16x16x64_i8 (lane l: row l % 16, columns 16 (l / 16) .. + 15), and
-// their sums, exact integers, meet in LDS.
+// Few rows, or few channels: the weights are read once and that, or the chain of
+// loads, is what it costs.  A workgroup takes 16 CT output channels and 16 RT rows; its
+// four waves take every fourth 64-column step of k, so that together they read 256
+// neighbouring bytes of each weight row, straight into the operand registers of
+// v_mfma_i32_16x16x64_i8 (lane l: row l % 16, columns 16 (l / 16) .. + 15), U steps at
+// a time, and their sums, exact integers, meet in LDS.
+//
+// OWN (one row of at most 8192 values): each workgroup quantises the row itself, into
+// LDS, while its first weights load.
 constexpr uint32_t LF_WAVES = 4;
-constexpr uint32_t FEW_ROWS = 64;
+constexpr uint32_t OWN_GROUPS = 4;  // of 8 values a lane
 
-template <class TO, int CT, int RT>
-__global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a, const float *__restrict__ scale,
-                                                                   const int8_t *__restrict__ xq, uint32_t kp) {
+template <class T, class TO, int CT, int RT, bool OWN>
+__global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a, const float *__restrict__ scale_,
+                                                                   const int8_t *__restrict__ xq_, uint32_t kp) {
   __shared__ i32x4 part[LF_WAVES][CT * RT][64];
+  __shared__ float own_peak[LF_WAVES];
+  __shared__ int own_bad[LF_WAVES];
+  extern __shared__ __attribute__((aligned(16))) int8_t own_x[];
   const uint32_t l = threadIdx.x & 63u, wave = threadIdx.x / 64u, lo = l & 15u, hi = l >> 4;
+  const uint32_t r0 = blockIdx.y * 16u * RT, steps = kp / 64u;
+  const int8_t *end = weights_end(a);
+  constexpr int U = CT * RT <= 2 ? 8 : 4;
+  const int8_t *xr[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const uint32_t row = min(r0 + 16u * j + lo, (uint32_t)a.rows - 1u);
+    xr[j] = OWN ? own_x : xq_ + (uint64_t)row * kp;
+  }
+  bool quantised = !OWN;
+  float own_scale = 0.0f;
   for (uint32_t c0 = blockIdx.x * 16u * CT; c0 < a.q; c0 += gridDim.x * 16u * CT) {
-    const int8_t *wr[CT], *xr[RT];
+    const int8_t *wr[CT];
 #pragma unroll
     for (int i = 0; i < CT; ++i) wr[i] = a.w + (int64_t)min(c0 + 16u * i + lo, a.q - 1u) * a.w_stride;
-#pragma unroll
-    for (int j = 0; j < RT; ++j) xr[j] = xq + (uint64_t)min(16u * j + lo, (uint32_t)a.rows - 1u) * kp;
     i32x4 acc[CT][RT] = {};
-    // steps that lie within the weight rows, U at a time so that their loads are in
-    // flight together
-    constexpr int U = CT * RT <= 2 ? 8 : 4;
-    const uint32_t whole = a.k / 64u, steps = kp / 64u;
-    uint32_t s = wave;
-    for (; s + LF_WAVES * (U - 1) < whole; s += LF_WAVES * U) {
+    for (uint32_t s = wave; s < steps || !quantised; s += LF_WAVES * U) {
       i32x4 w[U][CT], x[U][RT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t k0 = (s + LF_WAVES * u) * 64u + hi * 16u;
 #pragma unroll
-        for (int i = 0; i < CT; ++i) w[u][i] = *reinterpret_cast<const i32x4_a1 *>(wr[i] + k0);
+        for (int i = 0; i < CT; ++i)
+          w[u][i] = s + LF_WAVES * u < steps ? load_w16(wr[i], k0, a.k, end) : i32x4{0, 0, 0, 0};
+        if (!OWN) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j) x[u][j] = *reinterpret_cast<const i32x4 *>(xr[j] + k0);
+          for (int j = 0; j < RT; ++j)
+            x[u][j] = s + LF_WAVES * u < steps ? *reinterpret_cast<const i32x4 *>(xr[j] + k0) : i32x4{0, 0, 0, 0};
+        }
+      }
+      if constexpr (OWN) {
+        if (!quantised) {
+          Raw8<T> r[OWN_GROUPS];
+          Peak p;
+#pragma unroll
+          for (uint32_t g = 0; g < OWN_GROUPS; ++g)
+            if (g * 2048u < kp) load_x(reinterpret_cast<const T *>(a.x), g * 2048u + threadIdx.x * 8u, a.k, r[g]);
+#pragma unroll
+          for (uint32_t g = 0; g < OWN_GROUPS; ++g)
+            if (g * 2048u < kp) p.take(r[g]);
+          p.join_wave();
+          if (l == 0) {
+            own_peak[wave] = p.m;
+            own_bad[wave] = p.bad;
+          }
+          __syncthreads();
+          p.m = fmaxf(fmaxf(own_peak[0], own_peak[1]), fmaxf(own_peak[2], own_peak[3]));
+          p.bad = own_bad[0] | own_bad[1] | own_bad[2] | own_bad[3];
+          own_scale = p.bad ? __builtin_nanf("") : p.m / 127.0f;
+          const Divisor d(own_scale > 0.0f ? own_scale : 1.0f);
+#pragma unroll
+          for (uint32_t g = 0; g < OWN_GROUPS; ++g) {
+            const uint32_t c = g * 2048u + threadIdx.x * 8u;
+            if (c < kp) *reinterpret_cast<uint2 *>(own_x + c) = p.bad ? make_uint2(0, 0) : integers8(r[g], d);
+          }
+          quantised = true;
+          __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < RT; ++j)
+            x[u][j] = *reinterpret_cast<const i32x4 *>(xr[j] + (s + LF_WAVES * u < steps ? (s + LF_WAVES * u) * 64u + hi * 16u : 0u));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -126,18 +224,6 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
         for (int i = 0; i < CT; ++i)
 #pragma unroll
           for (int j = 0; j < RT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], x[u][j], acc[i][j], 0, 0, 0);
-    }
-    for (; s < steps; s += LF_WAVES) {
-      const uint32_t k0 = s * 64u + hi * 16u;
-      i32x4 w[CT];
-#pragma unroll
-      for (int i = 0; i < CT; ++i) w[i] = load_w16(wr[i], k0, a.k);
-#pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        const i32x4 x = *reinterpret_cast<const i32x4 *>(xr[j] + k0);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x, acc[i][j], 0, 0, 0);
-      }
     }
 #pragma unroll
     for (int t = 0; t < CT * RT; ++t) part[wave][t][l] = acc[t / RT][t % RT];
@@ -147,9 +233,9 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
       i32x4 v = part[0][t][l];
 #pragma unroll
       for (uint32_t o = 1; o < LF_WAVES; ++o) v += part[o][t][l];
-      const uint32_t row = 16u * (t % RT) + lo, c = c0 + 16u * (t / RT) + 4u * hi;
+      const uint32_t row = r0 + 16u * (t % RT) + lo, c = c0 + 16u * (t / RT) + 4u * hi;
       if (row < a.rows && c < a.q) {
-        const float sx = scale[row];
+        const float sx = OWN ? own_scale : scale_[row];
         float f[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
@@ -298,6 +384,7 @@ __global__ __launch_bounds__(S::THREADS) void linear_tile_kernel(LinearArgs a, c
     wait_loads_barrier<0>();
   } else {
     i32x4 reg[PIECES];
+    const int8_t *end = weights_end(a);
     auto load = [&](uint32_t s) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
@@ -305,7 +392,7 @@ __global__ __launch_bounds__(S::THREADS) void linear_tile_kernel(LinearArgs a, c
         if (is_x(p))
           reg[p] = *reinterpret_cast<const i32x4 *>(src[p] + k);
         else
-          reg[p] = load_w16(src[p], k, a.k);
+          reg[p] = load_w16(src[p], k, a.k, end);
       }
     };
     auto put = [&](uint32_t s) {
@@ -386,10 +473,11 @@ static int launch_tiles(thrml_ctx *ctx, const LinearArgs &a, const float *scale,
   return THRML_OK;
 }
 
-template <class TO, int CT, int RT>
+template <class T, class TO, int CT, int RT, bool OWN>
 static int launch_few(thrml_ctx *ctx, const LinearArgs &a, const float *scale, const int8_t *xq, uint32_t kp) {
-  hipLaunchKernelGGL((linear_few_kernel<TO, CT, RT>), dim3(std::min(cdiv(a.q, 16 * CT), 1u << 20)), dim3(64 * LF_WAVES), 0, ctx->stream, a,
-                     scale, xq, kp);
+  const dim3 grid(std::min(cdiv(a.q, 16 * CT), 1u << 20), cdiv(a.rows, 16 * RT));
+  hipLaunchKernelGGL((linear_few_kernel<T, TO, CT, RT, OWN>), grid, dim3(64 * LF_WAVES), OWN ? kp : 0, ctx->stream,
+                     a, scale, xq, kp);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
 }
@@ -399,6 +487,12 @@ int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dty
   const uint32_t kp = padded_k(a.k);
   float *scale = reinterpret_cast<float *>(work);
   int8_t *xq = reinterpret_cast<int8_t *>(work) + scales_bytes(a.rows);
+  if (a.rows == 1 && kp <= OWN_GROUPS * 2048)
+    return with_type(dtype, [&](auto ti) {
+      return with_type(out_dtype, [&](auto to) {
+        return launch_few<decltype(ti), decltype(to), 1, 1, true>(ctx, a, scale, xq, kp);
+      });
+    });
   int rc = with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
     hipLaunchKernelGGL((quantise_kernel<T>), dim3((uint32_t)std::min<uint64_t>(a.rows, 1u << 20)), dim3(256), 0,
@@ -409,10 +503,24 @@ int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dty
   if (rc) return rc;
   return with_type(out_dtype, [&](auto t) -> int {
     typedef decltype(t) TO;
-    if (a.rows <= 16) return launch_few<TO, 1, 1>(ctx, a, scale, xq, kp);
-    if (a.rows <= 32) return launch_few<TO, 2, 2>(ctx, a, scale, xq, kp);
-    if (a.rows <= 48) return launch_few<TO, 2, 3>(ctx, a, scale, xq, kp);
-    if (a.rows <= FEW_ROWS) return launch_few<TO, 2, 4>(ctx, a, scale, xq, kp);
+#ifdef LINEAR_CONFIG
+    if (const char *e = getenv("LINEAR_CONFIG")) switch (atoi(e)) {
+      case 1: return launch_few<float, TO, 1, 1, false>(ctx, a, scale, xq, kp);
+      case 2: return launch_few<float, TO, 2, 2, false>(ctx, a, scale, xq, kp);
+      case 3: return launch_few<float, TO, 2, 3, false>(ctx, a, scale, xq, kp);
+      case 4: return launch_few<float, TO, 2, 4, false>(ctx, a, scale, xq, kp);
+      case 5: return launch_tiles<TileShape<1, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 6: return launch_tiles<TileShape<2, 2, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 7: return launch_tiles<TileShape<4, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
+      case 8: return launch_tiles<TileShape<2, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 9: return launch_tiles<TileShape<2, 4, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 10: return launch_tiles<TileShape<2, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
+    }
+#endif
+    if (a.rows <= 16) return launch_few<float, TO, 1, 1, false>(ctx, a, scale, xq, kp);
+    if (a.rows <= 32) return launch_few<float, TO, 2, 2, false>(ctx, a, scale, xq, kp);
+    if (a.rows <= 48) return launch_few<float, TO, 2, 3, false>(ctx, a, scale, xq, kp);
+    if (a.rows <= 64) return launch_few<float, TO, 2, 4, false>(ctx, a, scale, xq, kp);
     const uint64_t cu = ctx->cu_count;
     if ((uint64_t)cdiv(a.rows, 256) * cdiv(a.q, 256) >= cu)
       return launch_tiles<TileShape<4, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
