@@ -134,55 +134,43 @@ __device__ __forceinline__ const int8_t *weights_end(const LinearArgs &a) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows, or few channels: the weights are read once and that, or the chain of
-// loads, is what it costs.  A workgroup takes 16 CT output channels and 16 RT rows; its
-// four waves take every fourth 64-column step of k, so that together they read 256
-// neighbouring bytes of each weight row, straight into the operand registers of
-// v_mfma_i32_16x16x64_i8 (lane l: row l % 16, columns 16 (l / 16) .. + 15), U steps at
-// a time, and their sums, exact integers, meet in LDS.
+// Little work: the chain of loads is what it costs.  A workgroup takes 16 output
+// channels and 16 rows; its four waves take turns in 64-column steps of k, straight
+// from memory into the operand registers of v_mfma_i32_16x16x64_i8 (lane l: row l % 16,
+// columns 16 (l / 16) .. + 15), U steps at a time, and their sums, exact integers, meet
+// in LDS.  (More waves, or 32 x 32 tiles, were no faster where this kernel is taken; where
+// there is much to read, its 64 neighbouring bytes a row at a time reach 4 TB/s
+// against 6 through LDS.)
 //
 // OWN (one row of at most 8192 values): each workgroup quantises the row itself, into
-// LDS, while its first weights load.
+// LDS, while its first weights load: one launch for a call.
 constexpr uint32_t LF_WAVES = 4;
 constexpr uint32_t OWN_GROUPS = 4;  // of 8 values a lane
 
-template <class T, class TO, int CT, int RT, bool OWN>
+template <class T, class TO, bool OWN>
 __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a, const float *__restrict__ scale_,
                                                                    const int8_t *__restrict__ xq_, uint32_t kp) {
-  __shared__ i32x4 part[LF_WAVES][CT * RT][64];
+  __shared__ i32x4 part[LF_WAVES][64];
   __shared__ float own_peak[LF_WAVES];
   __shared__ int own_bad[LF_WAVES];
   extern __shared__ __attribute__((aligned(16))) int8_t own_x[];
   const uint32_t l = threadIdx.x & 63u, wave = threadIdx.x / 64u, lo = l & 15u, hi = l >> 4;
-  const uint32_t r0 = blockIdx.y * 16u * RT, steps = kp / 64u;
+  const uint32_t r0 = blockIdx.y * 16u, steps = kp / 64u, row = min(r0 + lo, (uint32_t)a.rows - 1u);
   const int8_t *end = weights_end(a);
-  constexpr int U = CT * RT <= 2 ? 8 : 4;
-  const int8_t *xr[RT];
-#pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const uint32_t row = min(r0 + 16u * j + lo, (uint32_t)a.rows - 1u);
-    xr[j] = OWN ? own_x : xq_ + (uint64_t)row * kp;
-  }
+  constexpr int U = 8;
+  const int8_t *xr = OWN ? own_x : xq_ + (uint64_t)row * kp;
   bool quantised = !OWN;
   float own_scale = 0.0f;
-  for (uint32_t c0 = blockIdx.x * 16u * CT; c0 < a.q; c0 += gridDim.x * 16u * CT) {
-    const int8_t *wr[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) wr[i] = a.w + (int64_t)min(c0 + 16u * i + lo, a.q - 1u) * a.w_stride;
-    i32x4 acc[CT][RT] = {};
+  for (uint32_t c0 = blockIdx.x * 16u; c0 < a.q; c0 += gridDim.x * 16u) {
+    const int8_t *wr = a.w + (int64_t)min(c0 + lo, a.q - 1u) * a.w_stride;
+    i32x4 acc = {};
     for (uint32_t s = wave; s < steps || !quantised; s += LF_WAVES * U) {
-      i32x4 w[U][CT], x[U][RT];
+      i32x4 w[U], x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint32_t k0 = (s + LF_WAVES * u) * 64u + hi * 16u;
-#pragma unroll
-        for (int i = 0; i < CT; ++i)
-          w[u][i] = s + LF_WAVES * u < steps ? load_w16(wr[i], k0, a.k, end) : i32x4{0, 0, 0, 0};
-        if (!OWN) {
-#pragma unroll
-          for (int j = 0; j < RT; ++j)
-            x[u][j] = s + LF_WAVES * u < steps ? *reinterpret_cast<const i32x4 *>(xr[j] + k0) : i32x4{0, 0, 0, 0};
-        }
+        const uint32_t st = s + LF_WAVES * u, k0 = st * 64u + hi * 16u;
+        w[u] = st < steps ? load_w16(wr, k0, a.k, end) : i32x4{0, 0, 0, 0};
+        if (!OWN) x[u] = st < steps ? *reinterpret_cast<const i32x4 *>(xr + k0) : i32x4{0, 0, 0, 0};
       }
       if constexpr (OWN) {
         if (!quantised) {
@@ -213,39 +201,31 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
           __syncthreads();
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < RT; ++j)
-            x[u][j] = *reinterpret_cast<const i32x4 *>(xr[j] + (s + LF_WAVES * u < steps ? (s + LF_WAVES * u) * 64u + hi * 16u : 0u));
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < CT; ++i)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], x[u][j], acc[i][j], 0, 0, 0);
-    }
-#pragma unroll
-    for (int t = 0; t < CT * RT; ++t) part[wave][t][l] = acc[t / RT][t % RT];
-    __syncthreads();
-#pragma unroll 1
-    for (uint32_t t = wave; t < CT * RT; t += LF_WAVES) {
-      i32x4 v = part[0][t][l];
-#pragma unroll
-      for (uint32_t o = 1; o < LF_WAVES; ++o) v += part[o][t][l];
-      const uint32_t row = r0 + 16u * (t % RT) + lo, c = c0 + 16u * (t / RT) + 4u * hi;
-      if (row < a.rows && c < a.q) {
-        const float sx = OWN ? own_scale : scale_[row];
-        float f[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          // (the sum times a weight's scale first: a row's scale may be near the ends of f32)
-          const uint32_t ci = min(c + i, a.q - 1u);
-          f[i] = (float)v[i] * a.w_scale[ci] * sx;
-          if (a.bias) f[i] = f[i] + a.bias[ci];
+        for (int u = 0; u < U; ++u) {
+          const uint32_t st = s + LF_WAVES * u;
+          x[u] = *reinterpret_cast<const i32x4 *>(xr + (st < steps ? st * 64u + hi * 16u : 0u));
         }
-        store4(reinterpret_cast<TO *>(a.y) + (int64_t)row * a.y_stride + c, a.q - c, f);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u], acc, 0, 0, 0);
+    }
+    part[wave][l] = acc;
+    __syncthreads();
+    const uint32_t c = c0 + 4u * hi;
+    if (wave == 0 && r0 + lo < a.rows && c < a.q) {
+      i32x4 v = part[0][l];
+#pragma unroll
+      for (uint32_t o = 1; o < LF_WAVES; ++o) v += part[o][l];
+      const float sx = OWN ? own_scale : scale_[row];
+      float f[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        // (the sum times a weight's scale first: a row's scale may be near the ends of f32)
+        const uint32_t ci = min(c + i, a.q - 1u);
+        f[i] = (float)v[i] * a.w_scale[ci] * sx;
+        if (a.bias) f[i] = f[i] + a.bias[ci];
+      }
+      store4(reinterpret_cast<TO *>(a.y) + (int64_t)row * a.y_stride + c, a.q - c, f);
     }
     __syncthreads();  // the sums of the next channels
   }
@@ -286,6 +266,7 @@ struct TileShape {
   static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int STAGE = (BM + BN) * 64;           // bytes
   static constexpr int PIECES = STAGE / 16 / THREADS;    // 16-byte pieces of a stage per lane
+  static_assert(PIECES * 16 * THREADS == STAGE, "a stage is whole pieces of every lane");
 };
 
 template <class S, class TO, bool DIRECT>
@@ -383,16 +364,14 @@ __global__ __launch_bounds__(S::THREADS) void linear_tile_kernel(LinearArgs a, c
     }
     wait_loads_barrier<0>();
   } else {
+    // (two stages ahead, in twice the registers, was no faster)
     i32x4 reg[PIECES];
     const int8_t *end = weights_end(a);
     auto load = [&](uint32_t s) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
         const uint32_t k = s * 64u + col[p];
-        if (is_x(p))
-          reg[p] = *reinterpret_cast<const i32x4 *>(src[p] + k);
-        else
-          reg[p] = load_w16(src[p], k, a.k, end);
+        reg[p] = is_x(p) ? *reinterpret_cast<const i32x4 *>(src[p] + k) : load_w16(src[p], k, a.k, end);
       }
     };
     auto put = [&](uint32_t s) {
@@ -473,11 +452,11 @@ static int launch_tiles(thrml_ctx *ctx, const LinearArgs &a, const float *scale,
   return THRML_OK;
 }
 
-template <class T, class TO, int CT, int RT, bool OWN>
+template <class T, class TO, bool OWN>
 static int launch_few(thrml_ctx *ctx, const LinearArgs &a, const float *scale, const int8_t *xq, uint32_t kp) {
-  const dim3 grid(std::min(cdiv(a.q, 16 * CT), 1u << 20), cdiv(a.rows, 16 * RT));
-  hipLaunchKernelGGL((linear_few_kernel<T, TO, CT, RT, OWN>), grid, dim3(64 * LF_WAVES), OWN ? kp : 0, ctx->stream,
-                     a, scale, xq, kp);
+  const dim3 grid(std::min(cdiv(a.q, 16), 1u << 20), cdiv(a.rows, 16));
+  hipLaunchKernelGGL((linear_few_kernel<T, TO, OWN>), grid, dim3(64 * LF_WAVES), OWN ? kp : 0, ctx->stream, a, scale, xq,
+                     kp);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
 }
@@ -487,11 +466,12 @@ int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dty
   const uint32_t kp = padded_k(a.k);
   float *scale = reinterpret_cast<float *>(work);
   int8_t *xq = reinterpret_cast<int8_t *>(work) + scales_bytes(a.rows);
+  // one row: one launch (4096 x 32768, weights from memory: 33 us against 36 with the
+  // quantisation's own launch and tiles)
   if (a.rows == 1 && kp <= OWN_GROUPS * 2048)
     return with_type(dtype, [&](auto ti) {
-      return with_type(out_dtype, [&](auto to) {
-        return launch_few<decltype(ti), decltype(to), 1, 1, true>(ctx, a, scale, xq, kp);
-      });
+      return with_type(out_dtype,
+                       [&](auto to) { return launch_few<decltype(ti), decltype(to), true>(ctx, a, scale, xq, kp); });
     });
   int rc = with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
@@ -503,30 +483,38 @@ int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dty
   if (rc) return rc;
   return with_type(out_dtype, [&](auto t) -> int {
     typedef decltype(t) TO;
-#ifdef LINEAR_CONFIG
-    if (const char *e = getenv("LINEAR_CONFIG")) switch (atoi(e)) {
-      case 1: return launch_few<float, TO, 1, 1, false>(ctx, a, scale, xq, kp);
-      case 2: return launch_few<float, TO, 2, 2, false>(ctx, a, scale, xq, kp);
-      case 3: return launch_few<float, TO, 2, 3, false>(ctx, a, scale, xq, kp);
-      case 4: return launch_few<float, TO, 2, 4, false>(ctx, a, scale, xq, kp);
-      case 5: return launch_tiles<TileShape<1, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
-      case 6: return launch_tiles<TileShape<2, 2, 2, 2>, TO>(ctx, a, scale, xq, kp);
-      case 7: return launch_tiles<TileShape<4, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
-      case 8: return launch_tiles<TileShape<2, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
-      case 9: return launch_tiles<TileShape<2, 4, 2, 2>, TO>(ctx, a, scale, xq, kp);
-      case 10: return launch_tiles<TileShape<2, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
+    // The kind of tile by an estimate of each one's time: steps of k, and about 6 more
+    // for beginning and end, at its time for a step, which is that of a tile alone on a
+    // compute unit or, where a unit has several, their number times that of one of many.
+    // In us a step, measured (alone / of many): 16 x 16 without LDS 0.078 / 0.063, 64 x 64
+    // 0.195 / 0.164, 64 x 128 0.21 / 0.25, 128 x 256 0.45 / 0.67, 256 x 256 0.69 / 1.13.
+    // The kind taken and the next best of calls (us, quantisation included):
+    //    65 x 1000 x 700     16 x 16: 8      64 x 64: 14     512 x 4096 x 4096   64 x 128: 25    64 x 64: 27
+    //   128 x 8192 x 512     16 x 16: 16     64 x 64: 29    2000 x 8192 x 4096  128 x 256: 93  256 x 256: 112
+    //     4 x 2048 x 40000   64 x 64: 19     16 x 16: 21    4096 x 1000 x 65536 256 x 256: 512 128 x 256: 585
+    struct Kind {
+      uint32_t bm, bn;
+      float alone, many;
+    };
+    static constexpr Kind kinds[] = {
+        {16, 16, 0.078f, 0.063f}, {64, 64, 0.195f, 0.164f}, {64, 128, 0.21f, 0.25f}, {128, 256, 0.45f, 0.67f}, {256, 256, 0.69f, 1.13f}};
+    int best = 0;
+    double best_t = 0.0;
+    for (int i = 0; i < 5; ++i) {
+      const uint64_t tiles = (uint64_t)cdiv(a.rows, kinds[i].bm) * cdiv(a.q, kinds[i].bn);
+      const double t = std::max<double>(kinds[i].alone, (double)kinds[i].many * (double)cdiv(tiles, ctx->cu_count));
+      if (i == 0 || t < best_t) {
+        best = i;
+        best_t = t;
+      }
     }
-#endif
-    if (a.rows <= 16) return launch_few<float, TO, 1, 1, false>(ctx, a, scale, xq, kp);
-    if (a.rows <= 32) return launch_few<float, TO, 2, 2, false>(ctx, a, scale, xq, kp);
-    if (a.rows <= 48) return launch_few<float, TO, 2, 3, false>(ctx, a, scale, xq, kp);
-    if (a.rows <= 64) return launch_few<float, TO, 2, 4, false>(ctx, a, scale, xq, kp);
-    const uint64_t cu = ctx->cu_count;
-    if ((uint64_t)cdiv(a.rows, 256) * cdiv(a.q, 256) >= cu)
-      return launch_tiles<TileShape<4, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
-    if ((uint64_t)cdiv(a.rows, 128) * cdiv(a.q, 128) >= cu)
-      return launch_tiles<TileShape<2, 2, 2, 2>, TO>(ctx, a, scale, xq, kp);
-    return launch_tiles<TileShape<1, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
+    switch (best) {
+      case 0: return launch_few<float, TO, false>(ctx, a, scale, xq, kp);
+      case 1: return launch_tiles<TileShape<1, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 2: return launch_tiles<TileShape<1, 2, 2, 2>, TO>(ctx, a, scale, xq, kp);
+      case 3: return launch_tiles<TileShape<2, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
+      default: return launch_tiles<TileShape<4, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
+    }
   });
 }
 
