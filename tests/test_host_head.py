@@ -69,8 +69,8 @@ REFUSED = [
     (_linear(k=0), "k must be positive"), (_linear(k=131073), "at most 131072"), (_linear(q=0), "q must be positive"),
     (_linear(dtype=0), "x must be"), (_linear(od=7), "output must be"), (_linear(x=None), "x is NULL"),
     (_linear(w=None), "w is NULL"), (_linear(sc=None), "w_scale is NULL"), (_linear(y=None), "y is NULL"),
-    (_linear(ys=39), "rows overlap"), (_linear(ws=-70), "w: stride -70"), (_linear(work=None), "work holds 0 bytes"),
-    (_linear(n=100), "bytes"), (_linear(b=P + 2), "bias is not aligned"),
+    (_linear(ys=39), "rows overlap"), (_linear(ws=-70), "w: stride -70"), (_linear(rows=99, work=None), "work holds 0 bytes"),
+    (_linear(rows=99, n=100), "bytes"), (_linear(b=P + 2), "bias is not aligned"),
 ]
 
 

@@ -14,16 +14,13 @@ static inline uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b -
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef int32_t i32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 
 // Workspace: the scales of the rows, then their integers in rows of kp (k rounded
 // up to 64, zeros behind k).
 static inline uint32_t padded_k(uint32_t k) { return (k + 63u) & ~63u; }
 static inline uint64_t scales_bytes(uint64_t rows) { return (rows * 4 + 255) & ~(uint64_t)255; }
-uint64_t linear_i8_work(thrml_ctx *, uint64_t rows, uint32_t k, uint32_t) {
-  return scales_bytes(rows) + rows * padded_k(k);
-}
-
 // x / d, rounded to integers; |x| is at most 127 d, so that only d decides whether
 // Divisor::fast is exact (a quotient below 2^-50 may be off and rounds to 0 either way).
 __device__ __forceinline__ uint32_t integers4(const float *v, const Divisor &d) {
@@ -119,16 +116,44 @@ __global__ __launch_bounds__(256) void quantise_kernel(const T *__restrict__ x, 
 }
 
 // 16 weights of a row from column c0 on, any weights behind k (x is zero there): as
-// they lie in memory up to `end`, the end of the last row's weights, which is all that
-// may be read
-__device__ __forceinline__ i32x4 load_w16(const int8_t *wr, uint32_t c0, uint32_t k, const int8_t *end) {
-  if (wr + c0 + 16u <= end) return *reinterpret_cast<const i32x4_a1 *>(wr + c0);
-  i32x4 r = {0, 0, 0, 0};
+// they lie in memory up to `end`, the end of the last row's weights.
+//
+// ODD: rows that do not start at multiples of 4, for a wave that waits for its loads.
+// A 16-byte load from such an address takes longer (27 x 7806 x 64: 18.7 us against 9.7 at
+// k = 7808), so the words that hold them are loaded, 5 where they start within one, and
+// shifted at their use (13 us).  Tiles through LDS take such loads as they are (1245 x 2834
+// x 1467: 28 us, 39 by words).
+template <bool ODD>
+struct Weights16 {
+  i32x4 w = {0, 0, 0, 0};
+  int32_t next = 0;
+  uint32_t shift = 0;
+  __device__ __forceinline__ void load(const int8_t *wr, uint32_t c0, uint32_t k, const int8_t *end) {
+    const int8_t *p = wr + c0;
+    shift = ODD ? (uint32_t)(uintptr_t)p & 3u : 0u;
+    if (p + (ODD ? 20 : 16) <= end) {
+      if (ODD) {
+        const i32x4_a4 *v = reinterpret_cast<const i32x4_a4 *>(p - shift);
+        w = *v;
+        next = reinterpret_cast<const int32_t *>(v)[shift ? 4 : 0];
+      } else {
+        w = *reinterpret_cast<const i32x4_a1 *>(p);
+      }
+    } else {
+      w = i32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (c0 + j < k) r[j / 4] |= (int32_t)((uint32_t)(uint8_t)wr[c0 + j] << (8 * (j & 3)));
-  return r;
-}
+      for (int j = 0; j < 16; ++j)
+        if (c0 + j < k) w[j / 4] |= (int32_t)((uint32_t)(uint8_t)p[j] << (8 * (j & 3)));
+      shift = 0;
+      next = 0;
+    }
+  }
+  __device__ __forceinline__ i32x4 get() const {
+    if (!ODD) return w;
+    return i32x4{(int32_t)__builtin_amdgcn_alignbyte(w[1], w[0], shift), (int32_t)__builtin_amdgcn_alignbyte(w[2], w[1], shift),
+                 (int32_t)__builtin_amdgcn_alignbyte(w[3], w[2], shift), (int32_t)__builtin_amdgcn_alignbyte(next, w[3], shift)};
+  }
+};
 __device__ __forceinline__ const int8_t *weights_end(const LinearArgs &a) {
   return a.w + (int64_t)(a.q - 1u) * a.w_stride + a.k;
 }
@@ -142,37 +167,73 @@ __device__ __forceinline__ const int8_t *weights_end(const LinearArgs &a) {
 // there is much to read, its 64 neighbouring bytes a row at a time reach 4 TB/s
 // against 6 through LDS.)
 //
-// OWN (one row of at most 8192 values): each workgroup quantises the row itself, into
-// LDS, while its first weights load: one launch for a call.
+// OWN (at most 16 rows of at most 8192 values together): each workgroup quantises the
+// rows itself, into LDS, while its first weights load: one launch for a call.  1: one
+// row, by all waves, from registers; 2: a wave takes every fourth row.
 constexpr uint32_t LF_WAVES = 4;
-constexpr uint32_t OWN_GROUPS = 4;  // of 8 values a lane
+constexpr uint32_t OWN_GROUPS = 4;  // of 8 values a lane, for one row
+constexpr uint32_t OWN_VALUES = OWN_GROUPS * 8 * 64 * LF_WAVES;
+// (more than one row and many channels: tiles read the weights faster; 4 x 2048 x 40000
+// takes 20 us with them, 25 so)
+static bool own_rows(const thrml_ctx *ctx, uint64_t rows, uint32_t kp, uint32_t q) {
+  return rows <= 16 && rows * kp <= OWN_VALUES && (rows == 1 || q <= 64u * (uint32_t)ctx->cu_count);
+}
 
-template <class T, class TO, bool OWN>
+template <class T, class TO, int OWN, bool ODD>
 __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a, const float *__restrict__ scale_,
                                                                    const int8_t *__restrict__ xq_, uint32_t kp) {
   __shared__ i32x4 part[LF_WAVES][64];
   __shared__ float own_peak[LF_WAVES];
   __shared__ int own_bad[LF_WAVES];
+  __shared__ float own_scales[16];
   extern __shared__ __attribute__((aligned(16))) int8_t own_x[];
   const uint32_t l = threadIdx.x & 63u, wave = threadIdx.x / 64u, lo = l & 15u, hi = l >> 4;
   const uint32_t r0 = blockIdx.y * 16u, steps = kp / 64u, row = min(r0 + lo, (uint32_t)a.rows - 1u);
   const int8_t *end = weights_end(a);
   constexpr int U = 8;
-  const int8_t *xr = OWN ? own_x : xq_ + (uint64_t)row * kp;
+  const int8_t *xr = OWN ? own_x + row * kp : xq_ + (uint64_t)row * kp;
   bool quantised = !OWN;
   float own_scale = 0.0f;
   for (uint32_t c0 = blockIdx.x * 16u; c0 < a.q; c0 += gridDim.x * 16u) {
     const int8_t *wr = a.w + (int64_t)min(c0 + lo, a.q - 1u) * a.w_stride;
     i32x4 acc = {};
     for (uint32_t s = wave; s < steps || !quantised; s += LF_WAVES * U) {
-      i32x4 w[U], x[U];
+      Weights16<ODD> w[U];
+      i32x4 x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t st = s + LF_WAVES * u, k0 = st * 64u + hi * 16u;
-        w[u] = st < steps ? load_w16(wr, k0, a.k, end) : i32x4{0, 0, 0, 0};
+        if (st < steps)
+          w[u].load(wr, k0, a.k, end);
+        else
+          w[u] = Weights16<ODD>{};
         if (!OWN) x[u] = st < steps ? *reinterpret_cast<const i32x4 *>(xr + k0) : i32x4{0, 0, 0, 0};
       }
-      if constexpr (OWN) {
+      if constexpr (OWN == 2) {
+        if (!quantised) {
+          for (uint32_t i = wave; i < (uint32_t)a.rows; i += LF_WAVES) {
+            const T *x_row = reinterpret_cast<const T *>(a.x) + (int64_t)i * a.x_stride;
+            Peak p;
+            for (uint32_t c = l * 8u; c < a.k; c += 512u) {
+              Raw8<T> r;
+              load_x(x_row, c, a.k, r);
+              p.take(r);
+            }
+            p.join_wave();
+            const float sx = p.m / 127.0f;
+            const Divisor d(sx > 0.0f ? sx : 1.0f);
+            if (l == 0) own_scales[i] = p.bad ? __builtin_nanf("") : sx;
+            for (uint32_t c = l * 8u; c < kp; c += 512u) {
+              Raw8<T> r;
+              load_x(x_row, c, a.k, r);
+              *reinterpret_cast<uint2 *>(own_x + i * kp + c) = p.bad ? make_uint2(0, 0) : integers8(r, d);
+            }
+          }
+          quantised = true;
+          __syncthreads();
+        }
+      }
+      if constexpr (OWN == 1) {
         if (!quantised) {
           Raw8<T> r[OWN_GROUPS];
           Peak p;
@@ -200,14 +261,16 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
           quantised = true;
           __syncthreads();
         }
+      }
+      if constexpr (OWN != 0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint32_t st = s + LF_WAVES * u;
-          x[u] = *reinterpret_cast<const i32x4 *>(xr + (st < steps ? st * 64u + hi * 16u : 0u));
+          x[u] = st < steps ? *reinterpret_cast<const i32x4 *>(xr + st * 64u + hi * 16u) : i32x4{0, 0, 0, 0};
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u], acc, 0, 0, 0);
+      for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u].get(), x[u], acc, 0, 0, 0);
     }
     part[wave][l] = acc;
     __syncthreads();
@@ -216,7 +279,7 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
       i32x4 v = part[0][l];
 #pragma unroll
       for (uint32_t o = 1; o < LF_WAVES; ++o) v += part[o][l];
-      const float sx = OWN ? own_scale : scale_[row];
+      const float sx = OWN == 1 ? own_scale : OWN == 2 ? own_scales[row] : scale_[row];
       float f[4];
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
@@ -365,19 +428,22 @@ __global__ __launch_bounds__(S::THREADS) void linear_tile_kernel(LinearArgs a, c
     wait_loads_barrier<0>();
   } else {
     // (two stages ahead, in twice the registers, was no faster)
-    i32x4 reg[PIECES];
+    Weights16<false> reg[PIECES];
     const int8_t *end = weights_end(a);
     auto load = [&](uint32_t s) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
         const uint32_t k = s * 64u + col[p];
-        reg[p] = is_x(p) ? *reinterpret_cast<const i32x4 *>(src[p] + k) : load_w16(src[p], k, a.k, end);
+        if (is_x(p))
+          reg[p].w = *reinterpret_cast<const i32x4 *>(src[p] + k);
+        else
+          reg[p].load(src[p], k, a.k, end);
       }
     };
     auto put = [&](uint32_t s) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
-        *reinterpret_cast<i32x4 *>(lds + (s & 1u) * S::STAGE + ((uint32_t)p * S::THREADS + tid) * 16u) = reg[p];
+        *reinterpret_cast<i32x4 *>(lds + (s & 1u) * S::STAGE + ((uint32_t)p * S::THREADS + tid) * 16u) = reg[p].get();
     };
     load(0);
     put(0);
@@ -438,10 +504,15 @@ __global__ __launch_bounds__(S::THREADS) void linear_tile_kernel(LinearArgs a, c
   }
 }
 
+// weight rows at multiples of n bytes
+static bool weights_at(const LinearArgs &a, uint32_t n) {
+  return (a.q == 1 || a.w_stride % n == 0) && reinterpret_cast<uintptr_t>(a.w) % n == 0;
+}
+
 template <class S, class TO>
 static int launch_tiles(thrml_ctx *ctx, const LinearArgs &a, const float *scale, const int8_t *xq, uint32_t kp) {
   const uint32_t tm = cdiv(a.rows, S::BM), tn = cdiv(a.q, S::BN);
-  const bool direct = a.w_stride % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && a.k % 16u == 0;
+  const bool direct = weights_at(a, 16) && a.k % 16u == 0;
   const size_t turn = (size_t)S::WAVES * 32 * 32 * S::TN * 4;
   const size_t lds = std::max<size_t>((direct ? 4 : 2) * (size_t)S::STAGE, turn);
   auto *f = direct ? &linear_tile_kernel<S, TO, true> : &linear_tile_kernel<S, TO, false>;
@@ -452,27 +523,33 @@ static int launch_tiles(thrml_ctx *ctx, const LinearArgs &a, const float *scale,
   return THRML_OK;
 }
 
-template <class T, class TO, bool OWN>
+template <class T, class TO, int OWN>
 static int launch_few(thrml_ctx *ctx, const LinearArgs &a, const float *scale, const int8_t *xq, uint32_t kp) {
   const dim3 grid(std::min(cdiv(a.q, 16), 1u << 20), cdiv(a.rows, 16));
-  hipLaunchKernelGGL((linear_few_kernel<T, TO, OWN>), grid, dim3(64 * LF_WAVES), OWN ? kp : 0, ctx->stream, a, scale, xq,
-                     kp);
+  auto *f = weights_at(a, 4) ? &linear_few_kernel<T, TO, OWN, false> : &linear_few_kernel<T, TO, OWN, true>;
+  hipLaunchKernelGGL(f, grid, dim3(64 * LF_WAVES), OWN ? a.rows * kp : 0, ctx->stream, a, scale, xq, kp);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
+}
+
+uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q) {
+  return own_rows(ctx, rows, padded_k(k), q) ? 0 : scales_bytes(rows) + rows * padded_k(k);
 }
 
 int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work) {
   if (a.rows == 0) return THRML_OK;
   const uint32_t kp = padded_k(a.k);
+  // one launch (1 x 4096 x 32768, weights from memory: 33 us against 36 with the
+  // quantisation's own launch and tiles)
+  if (own_rows(ctx, a.rows, kp, a.q))
+    return with_type(dtype, [&](auto ti) {
+      return with_type(out_dtype, [&](auto to) {
+        return a.rows == 1 ? launch_few<decltype(ti), decltype(to), 1>(ctx, a, nullptr, nullptr, kp)
+                           : launch_few<decltype(ti), decltype(to), 2>(ctx, a, nullptr, nullptr, kp);
+      });
+    });
   float *scale = reinterpret_cast<float *>(work);
   int8_t *xq = reinterpret_cast<int8_t *>(work) + scales_bytes(a.rows);
-  // one row: one launch (4096 x 32768, weights from memory: 33 us against 36 with the
-  // quantisation's own launch and tiles)
-  if (a.rows == 1 && kp <= OWN_GROUPS * 2048)
-    return with_type(dtype, [&](auto ti) {
-      return with_type(out_dtype,
-                       [&](auto to) { return launch_few<decltype(ti), decltype(to), true>(ctx, a, scale, xq, kp); });
-    });
   int rc = with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
     hipLaunchKernelGGL((quantise_kernel<T>), dim3((uint32_t)std::min<uint64_t>(a.rows, 1u << 20)), dim3(256), 0,
@@ -509,7 +586,7 @@ int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dty
       }
     }
     switch (best) {
-      case 0: return launch_few<float, TO, false>(ctx, a, scale, xq, kp);
+      case 0: return launch_few<float, TO, 0>(ctx, a, scale, xq, kp);
       case 1: return launch_tiles<TileShape<1, 1, 2, 2>, TO>(ctx, a, scale, xq, kp);
       case 2: return launch_tiles<TileShape<1, 2, 2, 2>, TO>(ctx, a, scale, xq, kp);
       case 3: return launch_tiles<TileShape<2, 2, 2, 4>, TO>(ctx, a, scale, xq, kp);
