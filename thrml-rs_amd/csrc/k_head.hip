@@ -358,8 +358,10 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
 int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *out, int out_dtype,
                           int64_t out_stride) {
   if (a.rows == 0) return THRML_OK;
-  // two groups of 8 per lane where that leaves enough workgroups (and LDS)
-  const bool two = a.rows * cdiv(a.q, P_BLOCK * 16) >= 4ull * ctx->cu_count && a.n_bias <= 1024;
+  // two groups of 8 per lane where that leaves two workgroups for each compute unit, and
+  // LDS for many biases (48 x 131071: 18 us, 23 with one; four spill registers: 512 x
+  // 65536 101 us against 87)
+  const bool two = a.rows * cdiv(a.q, P_BLOCK * 16) >= 2ull * ctx->cu_count && a.n_bias <= 1024;
   const uint32_t chunk = P_BLOCK * (two ? 16 : 8), nc = cdiv(a.q, chunk);
   const uint64_t tasks = a.rows * nc;
   const uint32_t grid = (uint32_t)std::min<uint64_t>(tasks, 1u << 20), hash = hash_slots(a.n_bias, chunk);
