@@ -359,8 +359,8 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
                           int64_t out_stride) {
   if (a.rows == 0) return THRML_OK;
   // two groups of 8 per lane where that leaves two workgroups for each compute unit, and
-  // LDS for many biases (48 x 131071: 18 us, 23 with one; four spill registers: 512 x
-  // 65536 101 us against 87)
+  // LDS for many biases (48 x 131071: 18 us, 23 with one group; four groups, which spill
+  // registers, take 101 us at 512 x 65536 where two take 87)
   const bool two = a.rows * cdiv(a.q, P_BLOCK * 16) >= 2ull * ctx->cu_count && a.n_bias <= 1024;
   const uint32_t chunk = P_BLOCK * (two ? 16 : 8), nc = cdiv(a.q, chunk);
   const uint64_t tasks = a.rows * nc;
