@@ -308,7 +308,13 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
 // LDS, three ahead, with explicit waits; one barrier a stage, between the two
 // halves of the one before, where the matrix unit has work queued.  Otherwise the
 // pieces go through registers, one stage ahead.
-__device__ __forceinline__ uint32_t tile_swz(uint32_t r) { return ((r >> 1) ^ (r >> 3)) & 3u; }
+//
+// A 16-byte LDS read takes 16 lanes at a time, four quads of lanes: 0, 3, 5, 6 of a half
+// wave, then 1, 2, 4, 7; four rows of 64 bytes fill the banks, so that the rows r, r + 12,
+// r + 20, r + 24 that meet have to differ in their permutation (by bits 1 and 2 of r
+// instead, two and two met: 99 of 210 thousand LDS cycles per compute unit at 4096 x 4096
+// x 16384).
+__device__ __forceinline__ uint32_t tile_swz(uint32_t r) { return (r >> 3) & 3u; }
 
 // lane l's 16 bytes from g to LDS address lds + 16 l (lds wave-uniform); counted by
 // the explicit waits alone
