@@ -205,15 +205,17 @@ __device__ __forceinline__ void store4(T *p, uint32_t n, const float (&v)[4]) {
 
 // a / b for many a: q = a r with r = 1 / b rounded, and one step of the remainder,
 // which an fma gives exactly, leave the correctly rounded quotient (Markstein 1990)
-// as long as nothing under- or overflows: b within 2^-20 .. 2^20, |a| within 2^-70 ..
-// 2^100.  3 operations instead of the 10 of a full division.
+// for |b| within 2^-100 .. 2^100 and |a| from 2^-100 on, but for one within a step of
+// overflow; infinities, zeros and NaN divide as they should for every b that is not
+// subnormal.  5 operations instead of the 10 of a full division, in line.
 struct Divisor {
-  float b, r;
-  bool plain;
-  __device__ __forceinline__ explicit Divisor(float b_) : b(b_), r(1.0f / b_), plain(b_ >= 0x1p-20f && b_ <= 0x1p20f) {}
+  float b, r, m;  // m: b, or 1 for an infinite one
+  bool plain;     // b is within 2^-100 .. 2^100
+  __device__ __forceinline__ explicit Divisor(float b_)
+      : b(b_), r(1.0f / b_), m(__builtin_isinf(b_) ? 1.0f : b_), plain(b_ >= 0x1p-100f && b_ <= 0x1p100f) {}
   __device__ __forceinline__ float fast(float a) const {
     const float q = a * r;
-    return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
+    return __builtin_isinf(q) ? q : __builtin_fmaf(__builtin_fmaf(-q, m, a), r, q);
   }
 };
 

@@ -24,13 +24,13 @@ constexpr uint32_t T_PROMPT = 1u << 31, T_BIAS = 1u << 30, T_COUNT = (1u << 29) 
 constexpr uint32_t NO_KEY = 0xffffffffu;
 
 struct RowParams {
-  float theta, presence, frequency, t;
+  Divisor theta;
+  float presence, frequency, t;
   uint32_t len, prompt;
 };
 
 __device__ __forceinline__ RowParams row_params(const LogitRows &a, uint64_t row) {
-  RowParams p;
-  p.theta = a.repetition ? a.repetition[row] : 1.0f;
+  RowParams p{Divisor(a.repetition ? a.repetition[row] : 1.0f)};
   p.presence = a.presence ? a.presence[row] : 0.0f;
   p.frequency = a.frequency ? a.frequency[row] : 0.0f;
   p.t = a.temperature ? a.temperature[row] : 0.0f;
@@ -197,43 +197,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-__device__ __forceinline__ float min3_abs(float a, float b, float c) {
-  float r;
-  asm("v_min3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-// all of a fit Divisor::fast (a NaN may pass: it divides to NaN either way)
-__device__ __forceinline__ bool divides_fast(const float (&a)[8]) {
-  float hi = 0.0f, lo = 1.0f;
-#pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    hi = max3_abs(hi, a[j], a[j + 1]);
-    lo = min3_abs(lo, a[j], a[j + 1]);
-  }
-  return hi <= 0x1p100f && lo >= 0x1p-70f;
-}
-
-// a / b for what Divisor::fast does not take, one after the other (side by side they
-// would take the registers of all other work)
-template <int N>
-__device__ __forceinline__ void divide_each(float (&a)[N], float b) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    a[j] = a[j] / b;
-    if (j < N - 1) asm volatile("" : "+v"(a[j]), "+v"(a[j + 1]));
-  }
-}
-
-// z with its row's penalties, each step rounded to f32; q: z / theta
-__device__ __forceinline__ float penalised(float z, float q, uint32_t w, const RowParams &p) {
+// z with its row's penalties, each step rounded to f32 (w = 0: none)
+__device__ __forceinline__ float penalised(float z, uint32_t w, const RowParams &p) {
   const uint32_t n = w & T_COUNT;
   const float fn = (float)n;
-  float y = z > 0.0f ? q : z * p.theta;
+  float y = z > 0.0f ? p.theta.fast(z) : z * p.theta.b;
   y = (w & ~T_BIAS) ? y : z;
   const float less = (y - p.frequency * fn) - p.presence;
   return n ? less : y;
@@ -251,20 +219,8 @@ __device__ __forceinline__ void row_values(const Raw8<T> &r, bool table, const T
     const uint4 t0 = w4[0], t1 = w4[1];
     if ((t0.x | t0.y | t0.z | t0.w | t1.x | t1.y | t1.z | t1.w) != 0u) {
       const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
-      const Divisor theta(p.theta);
-      if (theta.plain && divides_fast(y)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (w[j]) y[j] = penalised(y[j], theta.fast(y[j]), w[j], p);
-      } else {
-        float q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = y[j];
-        divide_each(q, p.theta);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (w[j]) y[j] = penalised(y[j], q[j], w[j], p);
-      }
+      for (int j = 0; j < 8; ++j) y[j] = penalised(y[j], w[j], p);
       if (((w[0] | w[1] | w[2] | w[3] | w[4] | w[5] | w[6] | w[7]) & T_BIAS) != 0u) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -334,12 +290,8 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
       float y[8];
       row_values(r[v], table, tab, d, p, y);
       if (p.t > 0.0f) {
-        if (t.plain && divides_fast(y)) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = t.fast(y[j]);
-        } else {
-          divide_each(y, p.t);
-        }
+        for (int j = 0; j < 8; ++j) y[j] = t.fast(y[j]);
       }
       if (mask) {
 #pragma unroll
@@ -783,13 +735,9 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
               if (mask && !(mask[c[j] / 8u] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
             }
           }
-          float q[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) q[j] = y[j];
-          divide_each(q, p.theta);
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            y[j] = penalised(y[j], q[j], n[j], p);
+            y[j] = penalised(y[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
           s.scores(y, r, live, x, v);
