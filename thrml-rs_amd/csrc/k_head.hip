@@ -1,5 +1,6 @@
 // k_head.hip -- rows of logits of a learned head: processing, sampling, and
 // distillation from a teacher's top candidates.
+#include "dev_util.hpp"
 #include "head.hpp"
 
 namespace thrml {
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
   const bool table = a.history || a.n_bias;
   const Table tab{lds, lds + CHUNK, reinterpret_cast<float *>(lds + CHUNK + hash), CHUNK, hash};
   if (table) table_clear(tab, P_BLOCK);
-  for (uint64_t task = blockIdx.x; task < n_tasks; task += gridDim.x) {
+  // neighbouring chunks on one XCD: its L2 then reads a row's lists once
+  for (uint64_t task = xcd_remap(blockIdx.x, gridDim.x); task < n_tasks; task += gridDim.x) {
     const uint64_t row = task / n_chunks;
     const uint32_t c0 = (uint32_t)(task % n_chunks) * CHUNK;
     const uint32_t n = min(CHUNK, a.q - c0);
@@ -270,6 +272,10 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
     TO *o = out + (int64_t)row * out_stride + c0;
     const uint8_t *mask =
         a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) + c0 / 8u : nullptr;
+    // the lists first: loads end in their order, and the table waits for these alone
+    RowLists<P_BLOCK> lists;
+    if (table) lists.load(a, row);
+    const RowParams p = row_params(a, row);
     Raw8<TI> r[V];
     uint32_t m[V];
 #pragma unroll
@@ -278,9 +284,6 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
       load_place(z, d, n, r[v]);
       m[v] = mask && d < n ? mask[d / 8u] : 255u;
     }
-    RowLists<P_BLOCK> lists;
-    if (table) lists.load(a, row);
-    const RowParams p = row_params(a, row);
     const Divisor t(p.t);
     if (table) table_fill(a, p, lists, row, c0, tab);
 #pragma unroll
@@ -658,7 +661,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
                     reinterpret_cast<float *>(lds + 2 * plan.slots + plan.part / 32u + plan.hash), plan.slots, plan.hash};
   const uint8_t *flags = reinterpret_cast<const uint8_t *>(named.flags);
   const uint64_t n_tasks = a.rows * n_seg;
-  for (uint64_t task = blockIdx.x; task < n_tasks; task += gridDim.x) {
+  for (uint64_t task = xcd_remap(blockIdx.x, gridDim.x); task < n_tasks; task += gridDim.x) {
     const uint64_t row = task / n_seg;
     const uint32_t s0 = (uint32_t)(task % n_seg) * seg, s1 = min(s0 + seg, a.q);
     RowLists<BLOCK> lists;
