@@ -108,17 +108,17 @@ struct RowLists {
   static constexpr int KEPT = BLOCK == 1024 ? 1 : 2;
   int32_t id[KEPT][4], bias_id;
   float bias;
-  __device__ __forceinline__ void load(const LogitRows &a, uint64_t row) {
+  __device__ __forceinline__ void load(const LogitRows &a, uint64_t row, uint32_t tid) {
     if (a.history) {
       const int32_t *h = a.history + (int64_t)row * a.history_stride;
 #pragma unroll
-      for (int k = 0; k < KEPT; ++k) get(h, a.history_len, (uint32_t)k * BLOCK * 4u + threadIdx.x * 4u, id[k]);
+      for (int k = 0; k < KEPT; ++k) get(h, a.history_len, (uint32_t)k * BLOCK * 4u + tid * 4u, id[k]);
     }
     bias_id = -1;
     bias = 0.0f;
-    if (threadIdx.x < a.n_bias) {
-      bias_id = a.bias_ids[(int64_t)row * a.bias_stride + threadIdx.x];
-      bias = a.bias_values[(int64_t)row * a.bias_stride + threadIdx.x];
+    if (tid < a.n_bias) {
+      bias_id = a.bias_ids[(int64_t)row * a.bias_stride + tid];
+      bias = a.bias_values[(int64_t)row * a.bias_stride + tid];
     }
   }
   static __device__ __forceinline__ void get(const int32_t *h, uint32_t len, uint32_t i, int32_t (&v)[4]) {
@@ -135,7 +135,7 @@ struct RowLists {
 };
 
 __device__ __forceinline__ void table_clear(const Table &t, uint32_t block) {
-  for (uint32_t i = threadIdx.x * 4u; i < t.chunk; i += block * 4u)
+  for (uint32_t i = here(threadIdx.x) * 4u; i < t.chunk; i += block * 4u)
     *reinterpret_cast<uint4 *>(t.tab + i) = make_uint4(0, 0, 0, 0);
 }
 
@@ -145,7 +145,7 @@ template <int BLOCK>
 __device__ __forceinline__ void table_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
                                            uint64_t row, uint32_t c0, const Table &t) {
   constexpr int KEPT = RowLists<BLOCK>::KEPT;
-  const uint32_t tid = threadIdx.x;
+  const uint32_t tid = here(threadIdx.x);
   __syncthreads();
   if (t.hash) {
     for (uint32_t i = tid; i < t.hash; i += BLOCK) t.keys[i] = NO_KEY;
@@ -256,7 +256,7 @@ __device__ __forceinline__ void hide(Raw8<T> &r) {
 constexpr int P_BLOCK = 512;
 
 template <class TI, class TO, int V>
-__global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
+__global__ __launch_bounds__(P_BLOCK, 6) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
                                                           uint32_t n_chunks, uint64_t n_tasks, uint32_t hash) {
   extern __shared__ uint32_t lds[];
   constexpr uint32_t CHUNK = P_BLOCK * 8 * V;
@@ -265,6 +265,7 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
   if (table) table_clear(tab, P_BLOCK);
   // neighbouring chunks on one XCD: its L2 then reads a row's lists once
   for (uint64_t task = xcd_remap(blockIdx.x, gridDim.x); task < n_tasks; task += gridDim.x) {
+    const uint32_t tid = here(threadIdx.x);  // (what follows from it is not kept over the loop)
     const uint64_t row = task / n_chunks;
     const uint32_t c0 = (uint32_t)(task % n_chunks) * CHUNK;
     const uint32_t n = min(CHUNK, a.q - c0);
@@ -274,13 +275,13 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
         a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) + c0 / 8u : nullptr;
     // the lists first: loads end in their order, and the table waits for these alone
     RowLists<P_BLOCK> lists;
-    if (table) lists.load(a, row);
+    if (table) lists.load(a, row, tid);
     const RowParams p = row_params(a, row);
     Raw8<TI> r[V];
     uint32_t m[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const uint32_t d = ((uint32_t)v * P_BLOCK + threadIdx.x) * 8u;
+      const uint32_t d = ((uint32_t)v * P_BLOCK + tid) * 8u;
       load_place(z, d, n, r[v]);
       m[v] = mask && d < n ? mask[d / 8u] : 255u;
     }
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(P_BLOCK, 4) void process_kernel(LogitRows a, TO *__
     if (table) table_fill(a, p, lists, row, c0, tab);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const uint32_t d = ((uint32_t)v * P_BLOCK + threadIdx.x) * 8u;
+      const uint32_t d = ((uint32_t)v * P_BLOCK + tid) * 8u;
       if (d >= n) break;
       float y[8];
       row_values(r[v], table, tab, d, p, y);
@@ -469,7 +470,7 @@ template <int BLOCK>
 __device__ __forceinline__ void named_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
                                            uint64_t row, uint32_t c0, uint32_t n, const Named &t) {
   constexpr int KEPT = RowLists<BLOCK>::KEPT;
-  const uint32_t tid = threadIdx.x;
+  const uint32_t tid = here(threadIdx.x);
   __syncthreads();
   for (uint32_t i = tid; i < t.slots; i += BLOCK) {
     t.keys[i] = NO_KEY;
@@ -662,10 +663,11 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
   const uint8_t *flags = reinterpret_cast<const uint8_t *>(named.flags);
   const uint64_t n_tasks = a.rows * n_seg;
   for (uint64_t task = xcd_remap(blockIdx.x, gridDim.x); task < n_tasks; task += gridDim.x) {
+    const uint32_t tid = here(threadIdx.x);
     const uint64_t row = task / n_seg;
     const uint32_t s0 = (uint32_t)(task % n_seg) * seg, s1 = min(s0 + seg, a.q);
     RowLists<BLOCK> lists;
-    if (table) lists.load(a, row);
+    if (table) lists.load(a, row, tid);
     const RowParams p = row_params(a, row);
     Sampler s;
     s.begin(p, u, a.temperature);
@@ -674,7 +676,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
     const uint8_t *mask = a.mask ? reinterpret_cast<const uint8_t *>(a.mask + (int64_t)row * a.mask_stride) : nullptr;
     for (bool bounded = true;; bounded = false) {
       SampleGroup<T> next{};
-      next.load(z, ur, mask, s0 + threadIdx.x * 8u, s1);
+      next.load(z, ur, mask, s0 + tid * 8u, s1);
       for (uint32_t c0 = s0; c0 < s1; c0 += plan.part) {
         const uint32_t end = min(c0 + plan.part, s1);
         if (table) named_fill(a, p, lists, row, c0, end - c0, named);
@@ -685,18 +687,18 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         };
         s.first = s.second = -INFINITY;
         s.at = c0;
-        for (uint32_t d0 = c0 + (threadIdx.x & ~63u) * 8u; d0 < end; d0 += BLOCK * 8u) {
-          const uint32_t d = d0 + (threadIdx.x & 63u) * 8u;
+        for (uint32_t d0 = c0 + (tid & ~63u) * 8u; d0 < end; d0 += BLOCK * 8u) {
+          const uint32_t d = d0 + (tid & 63u) * 8u;
           const SampleGroup<T> k = next;
           // the next one: in this part, or this wave's first in the next part
-          const uint32_t ahead = d0 + BLOCK * 8u < end ? d0 + BLOCK * 8u : end + (threadIdx.x & ~63u) * 8u;
-          if (ahead < s1) next.load(z, ur, mask, ahead + (threadIdx.x & 63u) * 8u, s1);
+          const uint32_t ahead = d0 + BLOCK * 8u < end ? d0 + BLOCK * 8u : end + (tid & ~63u) * 8u;
+          if (ahead < s1) next.load(z, ur, mask, ahead + (tid & 63u) * 8u, s1);
           float y[8];
           const uint32_t live = group(k, d, y);
           s.take(y, k.u.w, live, d);
         }
         const float w = wave_max(s.first);
-        if ((threadIdx.x & 63u) == 0) wave_best[threadIdx.x / 64u] = w;
+        if ((tid & 63u) == 0) wave_best[tid / 64u] = w;
         __syncthreads();
         float cut = -INFINITY;
         if (bounded) {
@@ -706,7 +708,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         }
         if (!(s.first < cut) && (s.first > -INFINITY || !bounded)) {
           const bool all = !(s.second < cut);
-          for (uint32_t d = all ? c0 + threadIdx.x * 8u : s.at; d < end; d += all ? BLOCK * 8u : end) {
+          for (uint32_t d = all ? c0 + tid * 8u : s.at; d < end; d += all ? BLOCK * 8u : end) {
             SampleGroup<T> k{};
             k.load(z, ur, mask, d, s1);
             float y[8], x[8], v[8];
@@ -722,7 +724,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
           uint32_t c[N], n[N], r[N], live = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const uint32_t i = b + (uint32_t)j * BLOCK + threadIdx.x, key = i < plan.slots ? named.keys[i] : NO_KEY;
+            const uint32_t i = b + (uint32_t)j * BLOCK + tid, key = i < plan.slots ? named.keys[i] : NO_KEY;
             c[j] = key == NO_KEY ? c0 : c0 + key;
             n[j] = key == NO_KEY ? 0u : named.words[i];
             if (key != NO_KEY) live |= 1u << j;
@@ -764,9 +766,9 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
     }
     SamplePart o = s.s;
     part_join_wave(o);
-    if ((threadIdx.x & 63u) == 0) wave_part[threadIdx.x / 64u] = o;
+    if ((tid & 63u) == 0) wave_part[tid / 64u] = o;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
 #pragma unroll 1
       for (int w = 1; w < BLOCK / 64; ++w) part_merge(o, wave_part[w]);
       if (n_seg > 1)
@@ -893,7 +895,7 @@ static size_t candidate_bytes(uint32_t k) { return (size_t)k * 16 + (size_t)cand
 // By the first wave alone: its LDS accesses are in order.
 template <class T>
 __device__ __forceinline__ void teacher_part(const DistillArgs &a, uint64_t row, const T *z, Candidates &c) {
-  const uint32_t l = threadIdx.x;
+  const uint32_t l = here(threadIdx.x);
   const int32_t *id_row = a.ids + (int64_t)row * a.ids_stride;
   const float *t_row = a.teacher + (int64_t)row * a.teacher_stride;
   for (uint32_t i = l; i < c.hash; i += 64u) c.keys[i] = -1;
@@ -943,7 +945,7 @@ __device__ __forceinline__ void teacher_part(const DistillArgs &a, uint64_t row,
 __device__ __forceinline__ void teacher_loss(const DistillArgs &a, uint64_t row, const Candidates &c, float m,
                                              float ls, float rtau) {
   float l = 0.0f;
-  for (uint32_t i = threadIdx.x; i < c.k; i += 64u) {
+  for (uint32_t i = here(threadIdx.x); i < c.k; i += 64u) {
     const float p = c.p[i];
     if (c.ids[i] >= 0 && p != 0.0f) l += p * (c.logp[i] - ((c.z[i] - m) * rtau - ls));
   }
@@ -956,7 +958,7 @@ __device__ __forceinline__ void teacher_loss(const DistillArgs &a, uint64_t row,
 template <class T>
 __device__ __forceinline__ void candidate_grads(const Candidates &c, bool again, T *g, float f, float m, float ls,
                                                 float rtau) {
-  for (uint32_t i = threadIdx.x; i < c.k; i += blockDim.x) {
+  for (uint32_t i = here(threadIdx.x); i < c.k; i += blockDim.x) {
     const int32_t id = c.ids[i];
     if (id < 0) continue;
     float p = c.p[i];
@@ -1009,16 +1011,17 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
   const float rtau = 1.0f / a.tau, l2 = rtau * LOG2E;
   constexpr int G = GROUPS ? GROUPS : 1;
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const uint32_t tid = here(threadIdx.x);
     const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
     Raw8<T> r[G];
     if constexpr (GROUPS > 0) {
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        if ((uint32_t)g * BLOCK * 8u < a.q) load_place(z, ((uint32_t)g * BLOCK + threadIdx.x) * 8u, a.q, r[g], LOWEST<T>);
+        if ((uint32_t)g * BLOCK * 8u < a.q) load_place(z, ((uint32_t)g * BLOCK + tid) * 8u, a.q, r[g], LOWEST<T>);
     }
-    if (threadIdx.x < 64u) {
+    if (tid < 64u) {
       teacher_part(a, row, z, c);
-      if (threadIdx.x == 0) flags = (c.some ? 1u : 0u) | (c.again ? 2u : 0u);
+      if (tid == 0) flags = (c.some ? 1u : 0u) | (c.again ? 2u : 0u);
     }
     MaxSum t{-__FLT_MAX__, 0.0f};
     if constexpr (GROUPS > 0) {
@@ -1039,7 +1042,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
           hide(r[g]);
         }
     } else {
-      for (uint32_t d = threadIdx.x * 8u; d < a.q; d += BLOCK * 8u) {
+      for (uint32_t d = tid * 8u; d < a.q; d += BLOCK * 8u) {
         load_place(z, d, a.q, r[0], LOWEST<T>);
         float x[8], m = t.m, s = 0.0f;
 #pragma unroll
@@ -1054,7 +1057,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
     }
     t = max_sum_block<BLOCK>(t, l2, buf);
     const float ls = logf(t.s);
-    if (threadIdx.x < 64u) teacher_loss(a, row, c, t.m, ls, rtau);
+    if (tid < 64u) teacher_loss(a, row, c, t.m, ls, rtau);
     if (a.weight) {
       const uint32_t fl = flags;
       const bool some = fl & 1u;
@@ -1074,11 +1077,11 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
       if constexpr (GROUPS > 0) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t d = ((uint32_t)g * BLOCK + threadIdx.x) * 8u;
+          const uint32_t d = ((uint32_t)g * BLOCK + tid) * 8u;
           if (d < a.q) write(d, r[g]);
         }
       } else {
-        for (uint32_t d = threadIdx.x * 8u; d < a.q; d += BLOCK * 8u) {
+        for (uint32_t d = tid * 8u; d < a.q; d += BLOCK * 8u) {
           load_place(z, d, a.q, r[0]);
           write(d, r[0]);
         }
