@@ -821,10 +821,18 @@ int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const fl
                          int32_t *index, float *logprob, void *work) {
   if (a.rows == 0) return THRML_OK;
   const SamplePlan p = sample_plan(ctx, a.rows, a.q);
-  // two workgroups of 512 in a compute unit's LDS, or one of 1024
-  NamedPlan named = named_plan(a, p.seg, 8192, 150 << 10);
-  const bool wide = p.wide && named.bytes <= 150 << 10;
-  if (!wide) named = named_plan(a, p.seg, 4096, 76 << 10);
+  // Two workgroups of 512 in a compute unit's LDS, or one of 1024, which also takes the
+  // segments whose lists would leave those several parts (512 x 65536 with histories of
+  // 8192: 257 us in 16 parts each).
+  NamedPlan named = named_plan(a, p.seg, 4096, 76 << 10);
+  bool wide = p.wide || named.part < std::min(p.seg, PART_MAX);
+  if (wide) {
+    const NamedPlan one = named_plan(a, p.seg, 8192, 150 << 10);
+    if (one.bytes <= 150 << 10)
+      named = one;
+    else
+      wide = false;
+  }
   const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows * p.n_seg, 1u << 20);
   SamplePart *parts = reinterpret_cast<SamplePart *>(work);
   const int rc = with_type(dtype, [&](auto t) -> int {
