@@ -179,6 +179,56 @@ def test_rows_without_a_distribution(device, dtype, q):
         assert abs(float(logprob[5]) + np.log(q)) < ref.EPS * (64 + 2 * q / 4096 + 4 * np.log(q)) and logprob[6] == 0.0
 
 
+@pytest.mark.parametrize("rows,q,history,bias", [(3, 40000, 8192, 0), (300, 9000, 8192, 300), (2, 9000, 30000, 5000),
+                                                (1, 300000, 20000, 3000), (40, 5000, 300, 4000)])
+def test_long_lists(device, rows, q, history, bias):
+    """Histories and bias lists that a workgroup's LDS holds for parts of a row alone; the
+    same bits from every call."""
+    log_case(f"long lists {rows} {q} {history} {bias}")
+    g = _gen(rows + q + history)
+    z = 2.5 * torch.randn(rows, q, generator=g)
+    u = torch.rand(rows, q, generator=g)
+    kw = _row_kw(g, rows, q, history, bias, "rows")
+    if rows > 5:  # (the reference takes a while for each row)
+        z, u = z[:5].repeat(rows // 5, 1), u[:5].repeat(rows // 5, 1)
+        kw = {k: v[:5].repeat(rows // 5, 1) if v.dim() == 2 else v[:5].repeat(rows // 5) for k, v in kw.items()}
+    few = {k: v[:5] for k, v in kw.items()}
+    times = max(1, rows // 5) if rows > 5 else 1
+    want, size = ref.processed(torch.float64, z[:5], **few)
+    got = th.process_logits(device, z.cuda(), **_cuda(kw))
+    ref.close(got, want.repeat(times, 1), (6 * ref.EPS * size).repeat(times, 1), "process")
+    want, lp, bound = ref.sampled(z[:5], u[:5], **few)
+    index, logprob = th.sample_logits(device, z.cuda(), u.cuda(), **_cuda(kw))
+    assert index.cpu().tolist() == want.tolist() * times
+    ref.close(logprob, lp.repeat(times), bound.repeat(times), "logprob")
+    for _ in range(3):
+        again, logprob_again = th.sample_logits(device, z.cuda(), u.cuda(), **_cuda(kw))
+        assert torch.equal(again, index) and torch.equal(logprob_again, logprob)
+
+
+def test_rows_past_32_bits(device):
+    """Rows that begin beyond 2^32 elements of their buffer."""
+    log_case("offsets past 2^32 elements")
+    rows, q = 70000, 65536
+    z = torch.zeros(rows, q, dtype=BF16, device="cuda")
+    g = _gen(21)
+    at = [0, 65535, 65536, rows - 1]
+    for r in at:
+        z[r] = (2.0 * torch.randn(q, generator=g)).to(BF16).cuda()
+    index, logprob = th.sample_logits(device, z)
+    ids = torch.full((rows, 1), 7, dtype=torch.int32, device="cuda")
+    loss = th.distill_loss(device, z, ids, torch.zeros(rows, 1, device="cuda"))
+    part = z[at].cpu()
+    want, lp, bound = ref.sampled(part)
+    assert index[at].cpu().tolist() == want.tolist() and int(index[at[1] - 1]) == 0
+    ref.close(logprob[at], lp, bound, "logprob")
+    want, lb, _, _ = ref.distilled(part, ids[at].cpu(), torch.zeros(len(at), 1))
+    ref.close(loss[at], want, lb, "loss")
+    assert th.process_logits(device, z, out=z, temperature=torch.full((rows,), 0.5, device="cuda")) is z
+    assert torch.equal(z[at].cpu(), (2.0 * part.float()).to(BF16)) and not z[65537].any()
+    del z
+
+
 def test_history_edges(device):
     """One category named thousands of times, lengths of zero, past the end and
     negative, a history of no entries."""

@@ -73,13 +73,14 @@ __device__ __forceinline__ bool bias_put(uint32_t *keys, float *vals, uint32_t h
     h = (h + 1u) & (hash - 1u);
   }
 }
-__device__ __forceinline__ uint32_t bias_slot(const uint32_t *keys, uint32_t hash, uint32_t d) {
+// a key's slot in a hash table that has it
+__device__ __forceinline__ uint32_t slot_of(const uint32_t *keys, uint32_t hash, uint32_t d) {
   uint32_t h = hash_at(d, hash);
-  while (keys[h] != d) h = (h + 1u) & (hash - 1u);  // it is there
+  while (keys[h] != d) h = (h + 1u) & (hash - 1u);
   return h;
 }
 __device__ __forceinline__ float bias_of(const uint32_t *keys, const float *vals, uint32_t hash, uint32_t d) {
-  return vals[bias_slot(keys, hash, d)];
+  return vals[slot_of(keys, hash, d)];
 }
 // Where a category is named more than once, its entries are added in list order by the
 // thread of the first one.
@@ -95,7 +96,7 @@ __device__ __forceinline__ void bias_sums(const LogitRows &a, const int32_t *ids
     float s = vals[i];
     for (uint32_t j = i + 1; j < a.n_bias; ++j)
       if (ids[j] == id) s += vals[j];
-    sums[bias_slot(keys, hash, (uint32_t)id - c0)] = s;
+    sums[slot_of(keys, hash, (uint32_t)id - c0)] = s;
   }
 }
 
@@ -429,52 +430,65 @@ __device__ __forceinline__ void part_write(const SamplePart &s, uint64_t row, in
 
 // What the lists name is few beside the row and goes apart: a hash table in LDS holds
 // the words (T_PROMPT, T_BIAS, count) of the categories named in a part of the row,
-// a bitmap says which these are.  The pass over the part leaves them out, and lanes
-// score them eight slots at a time.  So the lists are scanned once for a part, as
-// large as LDS allows, and the waves go over it without a barrier.
+// a bitmap says which these are, and a list has them in the bitmap's order.  The pass
+// over the part leaves them out, and lanes score them from the list.  So the lists of
+// the row are scanned once for a part, as large as LDS allows, and the waves go over it
+// without a barrier.  (Their places in the table depend on which lane came first; the
+// list does not, and with it the order in which exponentials are added.)
 struct Named {
-  uint32_t *keys, *words, *flags, *bias_keys;
+  uint32_t *keys, *words, *flags, *list, *bias_keys;
   float *bias_vals;
   uint32_t slots, hash;  // of the table, of the biases' table
 };
 constexpr uint32_t PART_MAX = 131072;  // categories that a bitmap of 16 KB holds
 
 struct NamedPlan {
-  uint32_t part, slots, hash;
+  uint32_t part, slots, list, hash;
   size_t bytes;
 };
 // The largest part (a multiple of unit, at least unit) whose tables take `limit` bytes.
 static NamedPlan named_plan(const LogitRows &a, uint32_t seg, uint32_t unit, size_t limit) {
-  NamedPlan p{std::min(seg, PART_MAX), 0, 0, 0};
+  NamedPlan p{std::min(seg, PART_MAX), 0, 0, 0, 0};
   if (!a.history && !a.n_bias) {
     p.part = seg;
     return p;
   }
   for (;;) {
     const uint64_t n = std::min<uint64_t>((uint64_t)a.history_len * (a.history ? 1 : 0) + a.n_bias, p.part);
-    p.slots = 512;  // at most three quarters are taken
-    while ((uint64_t)p.slots * 3 < n * 4) p.slots *= 2;
+    p.slots = (uint32_t)std::max<uint64_t>(512, (n * 4 / 3 + 4) & ~(uint64_t)3);  // at most three quarters are taken
+    p.list = (uint32_t)(n + 3) & ~3u;
     p.hash = hash_slots(a.n_bias, p.part);
-    p.bytes = (size_t)p.slots * 8 + p.part / 8 + (size_t)p.hash * 8;
+    p.bytes = (size_t)p.slots * 8 + p.part / 8 + (size_t)p.list * 4 + (size_t)p.hash * 8;
     if (p.bytes <= limit || p.part <= unit) return p;
     p.part = std::max(unit, p.part / 2 / unit * unit);
   }
 }
 
+// (any number of slots: a power of two would not fit 8192 entries beside the list)
+__device__ __forceinline__ uint32_t named_first(const Named &t, uint32_t d) { return __umulhi(d * 2654435761u, t.slots); }
+__device__ __forceinline__ uint32_t named_next(const Named &t, uint32_t h) { return h + 1u < t.slots ? h + 1u : 0u; }
+
 __device__ __forceinline__ uint32_t named_slot(const Named &t, uint32_t d, bool *fresh) {
-  uint32_t h = hash_at(d, t.slots);
+  uint32_t h = named_first(t, d);
   for (;;) {
     const uint32_t old = atomicCAS(&t.keys[h], NO_KEY, d);
     *fresh = old == NO_KEY;
     if (old == NO_KEY || old == d) return h;
-    h = (h + 1u) & (t.slots - 1u);
+    h = named_next(t, h);
   }
 }
+__device__ __forceinline__ uint32_t named_word(const Named &t, uint32_t d) {
+  uint32_t h = named_first(t, d);
+  while (t.keys[h] != d) h = named_next(t, h);  // it is there
+  return t.words[h];
+}
 
-// Fills the tables for the n categories from c0 on; begins and ends with a barrier.
+// Fills the tables for the n categories from c0 on, and gives the length of the list;
+// begins and ends with a barrier.
 template <int BLOCK>
-__device__ __forceinline__ void named_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
-                                           uint64_t row, uint32_t c0, uint32_t n, const Named &t) {
+__device__ __forceinline__ uint32_t named_fill(const LogitRows &a, const RowParams &p, const RowLists<BLOCK> &lists,
+                                               uint64_t row, uint32_t c0, uint32_t n, const Named &t,
+                                               uint32_t *wave_count) {
   constexpr int KEPT = RowLists<BLOCK>::KEPT;
   const uint32_t tid = here(threadIdx.x);
   __syncthreads();
@@ -529,6 +543,28 @@ __device__ __forceinline__ void named_fill(const LogitRows &a, const RowParams &
     if (__syncthreads_or(again)) bias_sums(a, ids, vals, c0, n, t.bias_keys, t.bias_vals, t.hash, BLOCK);
   }
   __syncthreads();
+  const uint32_t words = (n + 31u) / 32u, lane = tid & 63u;
+  uint32_t count = 0;
+  for (uint32_t i = tid; i < words; i += BLOCK) count += __popc(t.flags[i]);
+  uint32_t upto = count;
+#pragma unroll
+  for (uint32_t s = 1; s < 64; s *= 2) {
+    const uint32_t v = __shfl_up(upto, s);
+    if (lane >= s) upto += v;
+  }
+  if (lane == 63u) wave_count[tid / 64u] = upto;
+  __syncthreads();
+  uint32_t at = upto - count, total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < BLOCK / 64; ++w) {
+    const uint32_t c = wave_count[w];
+    at += w < tid / 64u ? c : 0u;
+    total += c;
+  }
+  for (uint32_t i = tid; i < words; i += BLOCK)
+    for (uint32_t bits = t.flags[i]; bits; bits &= bits - 1u) t.list[at++] = i * 32u + (uint32_t)__builtin_ctz(bits);
+  __syncthreads();
+  return total;
 }
 
 // One row's state in a lane.
@@ -668,9 +704,17 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
   extern __shared__ uint32_t lds[];
   __shared__ SamplePart wave_part[BLOCK / 64];
   __shared__ float wave_best[BLOCK / 64];
+  __shared__ uint32_t wave_count[BLOCK / 64];
   const bool table = a.history || a.n_bias;
-  const Named named{lds, lds + plan.slots, lds + 2 * plan.slots, lds + 2 * plan.slots + plan.part / 32u,
-                    reinterpret_cast<float *>(lds + 2 * plan.slots + plan.part / 32u + plan.hash), plan.slots, plan.hash};
+  Named named;
+  named.keys = lds;
+  named.words = named.keys + plan.slots;
+  named.flags = named.words + plan.slots;
+  named.list = named.flags + plan.part / 32u;
+  named.bias_keys = named.list + plan.list;
+  named.bias_vals = reinterpret_cast<float *>(named.bias_keys + plan.hash);
+  named.slots = plan.slots;
+  named.hash = plan.hash;
   const uint8_t *flags = reinterpret_cast<const uint8_t *>(named.flags);
   const uint64_t n_tasks = a.rows * n_seg;
   for (uint64_t task = xcd_remap(blockIdx.x, gridDim.x); task < n_tasks; task += gridDim.x) {
@@ -690,7 +734,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
       next.load(z, ur, mask, s0 + tid * 8u, s1);
       for (uint32_t c0 = s0; c0 < s1; c0 += plan.part) {
         const uint32_t end = min(c0 + plan.part, s1);
-        if (table) named_fill(a, p, lists, row, c0, end - c0, named);
+        const uint32_t n_named = table ? named_fill(a, p, lists, row, c0, end - c0, named, wave_count) : 0u;
         auto group = [&](const SampleGroup<T> &k, uint32_t d, float (&y)[8]) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = value(k.z, j);
@@ -730,15 +774,20 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         }
         // the named ones
         constexpr int N = 4;
-        for (uint32_t b = 0; b < plan.slots; b += BLOCK * N) {
+        for (uint32_t b = 0; b < n_named; b += BLOCK * N) {
           float y[N], x[N], v[N];
           uint32_t c[N], n[N], r[N], live = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const uint32_t i = b + (uint32_t)j * BLOCK + tid, key = i < plan.slots ? named.keys[i] : NO_KEY;
-            c[j] = key == NO_KEY ? c0 : c0 + key;
-            n[j] = key == NO_KEY ? 0u : named.words[i];
-            if (key != NO_KEY) live |= 1u << j;
+            const uint32_t i = b + (uint32_t)j * BLOCK + tid;
+            c[j] = c0;
+            n[j] = 0;
+            if (i < n_named) {
+              const uint32_t d = named.list[i];
+              c[j] = c0 + d;
+              n[j] = named_word(named, d);
+              live |= 1u << j;
+            }
           }
           if (!__any(live != 0u)) continue;
 #pragma unroll
