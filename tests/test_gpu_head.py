@@ -281,6 +281,7 @@ DISTILL = [
     (1, 1, 1, 1.0, 0), (3, 2, 4, 0.5, 1), (5, 37, 1, 2.0, 3), (7, 1000, 8, 1.0, 0), (4, 4097, 33, 2.0, 5),
     (3, 16385, 64, 1.0, 1), (2, 50001, 300, 0.7, 0), (2, 65536, 256, 1.0, 8), (1, 131072, 1000, 1.0, 0),
     (2, 131073, 5, 3.0, 0), (1, 262145, 4096, 1.0, 0), (1300, 64, 3, 1.0, 0), (9, 9000, 0, 1.0, 0),
+    (20, 65537, 40, 1.5, 3), (70, 33000, 12, 1.0, 0),
 ]
 
 
@@ -329,30 +330,31 @@ def test_distill_differences(device):
     assert ((up - down) / (2 * d) - grad[0].double()).abs().max() < d * d / 6 + 2 * float(lb[0]) / (2 * d)
 
 
-def test_distill_edges(device):
-    log_case("distill edges")
+@pytest.mark.parametrize("q", [50, 70000])
+def test_distill_edges(device, q):
+    """(70000 categories: the rows in segments)"""
+    log_case(f"distill edges {q}")
     inf, nan = float("inf"), float("nan")
-    z = torch.zeros(6, 50)
+    z = torch.zeros(6, q)
     z[0, 7] = -inf                     # a logit without probability that the teacher wants
     z[1, 7] = -inf                     # one that it does not
     z[2] = nan                         # no entry: nothing of the row counts
     z[3, 4] = nan
     z[4] = torch.finfo(F32).min        # a row of the lowest value is uniform
-    ids = torch.tensor([[7, 8], [3, 3], [-1, 99], [1, 2], [1, 1], [4, 5]], dtype=torch.int32)
+    ids = torch.tensor([[7, 8], [3, 3], [-1, q + 9], [1, 2], [1, 1], [4, 5]], dtype=torch.int32)
     teacher = torch.tensor([[1.0, 1.0], [0.0, 2.0], [0.0, 0.0], [0.0, 1.0], [0.0, 0.0], [-inf, -inf]])
     loss, grad = th.distill_grad(device, z.cuda(), ids.cuda(), teacher.cuda(), torch.ones(6, device="cuda"))
     loss, grad = loss.cpu(), grad.cpu()
     assert loss[0] == inf and grad[0].isfinite().all() and abs(float(grad[0, 7]) + 0.5) < 4 * ref.EPS
-    assert abs(float(loss[1]) - np.log(49) + 0.0 - float(_entropy([0.0, 2.0]))) < 64 * ref.EPS and grad[1, 7] == 0.0
+    p = np.exp([0.0, 2.0] - np.logaddexp(0.0, 2.0))  # both of one id
+    want = np.log(q - 1) + (p * np.log(p)).sum()
+    assert abs(float(loss[1]) - want) < (64 + 2 * q / 4096) * ref.EPS * 16 and grad[1, 7] == 0.0
     assert loss[2] == 0.0 and (grad[2] == 0.0).all()
     assert loss[3].isnan() and grad[3].isnan().all()
-    assert abs(float(grad[4, 0]) - 0.02) < 64 * ref.EPS * 0.02 and abs(float(grad[4, 1]) + 0.98) < 16 * ref.EPS
+    share = 1 / q
+    assert abs(float(grad[4, 0]) - share) < (64 + 2 * q / 4096) * ref.EPS * share
+    assert abs(float(grad[4, 1]) + 1 - share) < 16 * ref.EPS
     assert loss[5] == 0.0 and (grad[5] == 0.0).all()
-
-
-def _entropy(t):
-    p = np.exp(t - np.logaddexp.reduce(t))
-    return (p * np.log(p)).sum()
 
 
 # ---------------------------------------------------------------------------

@@ -66,6 +66,7 @@ REFUSED = [
     (_distill(z=None), "logits is NULL"), (_distill(ids=None), "ids is NULL"), (_distill(loss=None), "loss is NULL"),
     (_distill(grad=None), "grad is NULL"), (_distill(gs=69), "rows overlap"), (_distill(grad=P), "must not be the logits"),
     (_distill(weight=P + 1), "weight is not aligned"),
+    (_distill(q=1 << 17, zs=1 << 17, gs=1 << 17, work=None), "work holds 0 bytes"),
     (_linear(k=0), "k must be positive"), (_linear(k=131073), "at most 131072"), (_linear(q=0), "q must be positive"),
     (_linear(dtype=0), "x must be"), (_linear(od=7), "output must be"), (_linear(x=None), "x is NULL"),
     (_linear(w=None), "w is NULL"), (_linear(sc=None), "w_scale is NULL"), (_linear(y=None), "y is NULL"),

@@ -2173,8 +2173,8 @@ extern "C" int thrml_sample_logits(thrml_ctx *ctx, const thrml_logits *in, const
   return launch_sample_logits(ctx, a, in->dtype, u, u_stride, index, logprob, work);
 }
 
-extern "C" uint64_t thrml_distill_work(thrml_ctx *ctx, uint64_t rows, uint32_t q, uint32_t k) {
-  return ctx && rows && q && rows <= HEAD_MAX_ROWS && q <= HEAD_MAX_Q && k <= DISTILL_MAX_K ? distill_work(ctx, rows, q) : 0;
+extern "C" uint64_t thrml_distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q) {
+  return ctx && rows && q && rows <= HEAD_MAX_ROWS && q <= HEAD_MAX_Q ? distill_work(ctx, dtype, rows, q) : 0;
 }
 
 extern "C" int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint64_t rows, uint32_t q,
@@ -2197,7 +2197,7 @@ extern "C" int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint
     if (int rc = check_rows("grad", grad, size, rows, q, grad_stride, true)) return rc;
     if (grad && grad == logits) return fail(THRML_EINVAL, "grad must not be the logits");
   }
-  if (int rc = check_work(work, work_bytes, thrml_distill_work(ctx, rows, q, k))) return rc;
+  if (int rc = check_work(work, work_bytes, weight ? thrml_distill_work(ctx, dtype, rows, q) : 0)) return rc;
   THRML_HIP(hipSetDevice(ctx->device));
   const DistillArgs a{logits, logits_stride, rows, q, k, ids, teacher, ids_stride, teacher_stride, tau, weight, loss,
                       grad, grad_stride};

@@ -73,7 +73,7 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
 uint64_t sample_logits_work(thrml_ctx *ctx, uint64_t rows, uint32_t q);
 int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const float *u, int64_t u_stride,
                          int32_t *index, float *logprob, void *work);
-uint64_t distill_work(thrml_ctx *ctx, uint64_t rows, uint32_t q);
+uint64_t distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q);
 int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work);
 uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
 int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work);

@@ -1023,14 +1023,14 @@ __device__ __forceinline__ void teacher_loss(const DistillArgs &a, uint64_t row,
   if (threadIdx.x == 0) a.loss[row] = c.some ? a.tau * a.tau * l : 0.0f;
 }
 
-// The gradient at the candidates' places, by the whole workgroup: an id that comes
+// The gradient at the candidates' places from s0 to s1 - 1, by the whole workgroup: an id that comes
 // more than once has the sum of its probabilities, in the order of the list.
 template <class T>
-__device__ __forceinline__ void candidate_grads(const Candidates &c, bool again, T *g, float f, float m, float ls,
-                                                float rtau) {
+__device__ __forceinline__ void candidate_grads(const Candidates &c, bool again, uint32_t s0, uint32_t s1, T *g, float f,
+                                                float m, float ls, float rtau) {
   for (uint32_t i = here(threadIdx.x); i < c.k; i += blockDim.x) {
     const int32_t id = c.ids[i];
-    if (id < 0) continue;
+    if (id < 0 || (uint32_t)id - s0 >= s1 - s0) continue;
     float p = c.p[i];
     if (again) {
       bool first = true;
@@ -1063,6 +1063,53 @@ __device__ __forceinline__ MaxSum max_sum_block(MaxSum v, float c, MaxSum *buf) 
   return v;
 }
 
+// A lane's maximum and sum over the logits from d0 to end - 1.
+template <class T, int BLOCK>
+__device__ __forceinline__ MaxSum lane_max_sum(const T *z, uint32_t d0, uint32_t end, uint32_t tid, float l2) {
+  MaxSum t{-__FLT_MAX__, 0.0f};
+  for (uint32_t d = d0 + tid * 8u; d < end; d += BLOCK * 8u) {
+    Raw8<T> r;
+    load_place(z, d, end, r, LOWEST<T>);
+    float x[8], m = t.m, s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = value(r, j);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * l2);
+    t.s = t.s * __builtin_amdgcn_exp2f((t.m - m) * l2) + s;
+    t.m = m;
+  }
+  return t;
+}
+
+// Eight places of the gradient but for p; n: how many of them there are.
+template <class T>
+__device__ __forceinline__ void write_grad(T *o, uint32_t n, const Raw8<T> &v, bool some, float f, float m, float ls,
+                                           float rtau) {
+  float x[8];
+  if (some) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = f * softmax_of<T>(value(v, j), m, rtau, ls);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+  }
+  store8(o, n, x);
+}
+
+__device__ __forceinline__ Candidates candidates_in(uint32_t *lds, uint32_t k, uint32_t hash) {
+  Candidates c;
+  c.ids = reinterpret_cast<int32_t *>(lds);
+  c.p = reinterpret_cast<float *>(lds) + k;
+  c.logp = c.p + k;
+  c.z = c.logp + k;
+  c.keys = reinterpret_cast<int32_t *>(c.z + k);
+  c.k = k;
+  c.hash = hash;
+  return c;
+}
+
 // GROUPS > 0: the row, of at most BLOCK * 8 GROUPS logits, stays in registers;
 // 0: it is read twice.
 template <class T, int BLOCK, int GROUPS>
@@ -1070,14 +1117,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
   extern __shared__ uint32_t lds[];
   __shared__ MaxSum buf[BLOCK / 64];
   __shared__ uint32_t flags;  // 1: there is an entry, 2: an id comes twice
-  Candidates c;
-  c.ids = reinterpret_cast<int32_t *>(lds);
-  c.p = reinterpret_cast<float *>(lds) + a.k;
-  c.logp = c.p + a.k;
-  c.z = c.logp + a.k;
-  c.keys = reinterpret_cast<int32_t *>(c.z + a.k);
-  c.k = a.k;
-  c.hash = hash;
+  Candidates c = candidates_in(lds, a.k, hash);
   const float rtau = 1.0f / a.tau, l2 = rtau * LOG2E;
   constexpr int G = GROUPS ? GROUPS : 1;
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -1112,18 +1152,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
           hide(r[g]);
         }
     } else {
-      for (uint32_t d = tid * 8u; d < a.q; d += BLOCK * 8u) {
-        load_place(z, d, a.q, r[0], LOWEST<T>);
-        float x[8], m = t.m, s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = value(r[0], j);
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) m = max3(m, x[j], x[j + 1]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * l2);
-        t.s = t.s * __builtin_amdgcn_exp2f((t.m - m) * l2) + s;
-        t.m = m;
-      }
+      t = lane_max_sum<T, BLOCK>(z, 0, a.q, tid, l2);
     }
     t = max_sum_block<BLOCK>(t, l2, buf);
     const float ls = logf(t.s);
@@ -1133,41 +1162,108 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
       const bool some = fl & 1u;
       const float f = a.tau * a.weight[row];
       T *o = reinterpret_cast<T *>(a.grad) + (int64_t)row * a.grad_stride;
-      auto write = [&](uint32_t d, const Raw8<T> &v) {
-        float x[8];
-        if (some) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = f * softmax_of<T>(value(v, j), t.m, rtau, ls);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-        }
-        store8(o + d, a.q - d, x);
-      };
       if constexpr (GROUPS > 0) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t d = ((uint32_t)g * BLOCK + tid) * 8u;
-          if (d < a.q) write(d, r[g]);
+          if (d < a.q) write_grad(o + d, a.q - d, r[g], some, f, t.m, ls, rtau);
         }
       } else {
         for (uint32_t d = tid * 8u; d < a.q; d += BLOCK * 8u) {
           load_place(z, d, a.q, r[0]);
-          write(d, r[0]);
+          write_grad(o + d, a.q - d, r[0], some, f, t.m, ls, rtau);
         }
       }
       __syncthreads();
-      if (some) candidate_grads(c, fl & 2u, o, f, t.m, ls, rtau);
+      if (some) candidate_grads(c, fl & 2u, 0, a.q, o, f, t.m, ls, rtau);
     }
     __syncthreads();
   }
 }
 
-uint64_t distill_work(thrml_ctx *, uint64_t, uint32_t) { return 0; }
+// Few long rows: a row's segments in workgroups of their own, first their maxima and
+// sums, then, from all of a row's, their part of the gradient (and, in the first one,
+// the loss).
+constexpr int DS_BLOCK = 512;
 
-int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *) {
+template <class T>
+__global__ __launch_bounds__(DS_BLOCK) void distill_sum_kernel(DistillArgs a, uint32_t seg, uint32_t n_seg,
+                                                               MaxSum *__restrict__ parts) {
+  __shared__ MaxSum buf[DS_BLOCK / 64];
+  const uint32_t row = blockIdx.x / n_seg, s0 = blockIdx.x % n_seg * seg;
+  const float l2 = (1.0f / a.tau) * LOG2E;
+  const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
+  MaxSum t = lane_max_sum<T, DS_BLOCK>(z, s0, min(s0 + seg, a.q), threadIdx.x, l2);
+  t = max_sum_block<DS_BLOCK>(t, l2, buf);
+  if (threadIdx.x == 0) parts[blockIdx.x] = t;
+}
+
+template <class T>
+__global__ __launch_bounds__(DS_BLOCK) void distill_segment_kernel(DistillArgs a, uint32_t hash, uint32_t seg,
+                                                                   uint32_t n_seg, const MaxSum *__restrict__ parts) {
+  extern __shared__ uint32_t lds[];
+  __shared__ uint32_t flags;
+  Candidates c = candidates_in(lds, a.k, hash);
+  const uint32_t row = blockIdx.x / n_seg, s0 = blockIdx.x % n_seg * seg, s1 = min(s0 + seg, a.q), tid = threadIdx.x;
+  const float rtau = 1.0f / a.tau, l2 = rtau * LOG2E;
+  const T *z = reinterpret_cast<const T *>(a.z) + (int64_t)row * a.z_stride;
+  if (tid < 64u) {
+    teacher_part(a, row, z, c);
+    if (tid == 0) flags = (c.some ? 1u : 0u) | (c.again ? 2u : 0u);
+  }
+  // every wave joins the row's parts in the same order
+  MaxSum t{-__FLT_MAX__, 0.0f};
+  for (uint32_t i = tid & 63u; i < n_seg; i += 64u) t = max_sum_merge(t, parts[row * n_seg + i], l2);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) t = max_sum_merge(t, {__shfl_xor(t.m, k), __shfl_xor(t.s, k)}, l2);
+  const float ls = logf(t.s);
+  if (tid < 64u && s0 == 0) teacher_loss(a, row, c, t.m, ls, rtau);
+  __syncthreads();
+  const bool some = flags & 1u;
+  const float f = a.tau * a.weight[row];
+  T *o = reinterpret_cast<T *>(a.grad) + (int64_t)row * a.grad_stride;
+  for (uint32_t d = s0 + tid * 8u; d < s1; d += DS_BLOCK * 8u) {
+    Raw8<T> r;
+    load_place(z, d, s1, r);
+    write_grad(o + d, s1 - d, r, some, f, t.m, ls, rtau);
+  }
+  __syncthreads();
+  if (some) candidate_grads(c, flags & 2u, s0, s1, o, f, t.m, ls, rtau);
+}
+
+// Segments of a row where they pay: 0 for a workgroup per row.  One and two launches (us):
+//    8 x 65536 bf16 (128 KB a row) 13.5 / 17.1    32 rows: 21.4 / 16.8    64: 21.5 / 19.9
+//    8 x 131072 bf16 (256 KB)      19.8 / 16.7    32 rows: 28.0 / 19.1   128: 32.2 / 29.3
+//    8 x 131072 f32 (512 KB)       30.3 / 15.7    64 rows: 45.3 / 29.0   200: 55.9 / 55.8
+static uint32_t distill_segments(const thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q) {
+  const uint64_t bytes = (uint64_t)q * (dtype == THRML_DTYPE_F32 ? 4 : 2);
+  if (rows * 4 > (uint64_t)ctx->cu_count || bytes < (rows < 16 ? 256u << 10 : 128u << 10)) return 0;
+  return std::min<uint32_t>(64, std::min<uint32_t>(cdiv(q, 2 * DS_BLOCK * 8), 2 * ctx->cu_count / (uint32_t)rows));
+}
+uint64_t distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q) {
+  return rows * distill_segments(ctx, dtype, rows, q) * sizeof(MaxSum);
+}
+
+int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work) {
   if (a.rows == 0) return THRML_OK;
   const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows, 1u << 20);
+  if (const uint32_t n = a.weight ? distill_segments(ctx, dtype, a.rows, a.q) : 0) {
+    const uint32_t seg = cdiv(cdiv(a.q, n), 8) * 8, n_seg = cdiv(a.q, seg);
+    MaxSum *parts = reinterpret_cast<MaxSum *>(work);
+    return with_type(dtype, [&](auto t) -> int {
+      typedef decltype(t) T;
+      hipLaunchKernelGGL((distill_sum_kernel<T>), dim3((uint32_t)a.rows * n_seg), dim3(DS_BLOCK), 0, ctx->stream, a, seg,
+                         n_seg, parts);
+      THRML_HIP(hipGetLastError());
+      auto *f = &distill_segment_kernel<T>;
+      const size_t lds = candidate_bytes(a.k);
+      if (int rc = lds_limit(reinterpret_cast<const void *>(f), lds)) return rc;
+      hipLaunchKernelGGL(f, dim3((uint32_t)a.rows * n_seg), dim3(DS_BLOCK), lds, ctx->stream, a, candidate_slots(a.k), seg,
+                         n_seg, parts);
+      THRML_HIP(hipGetLastError());
+      return THRML_OK;
+    });
+  }
   return with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
     // 64 registers of logits a lane

@@ -234,14 +234,15 @@ def _distill(device, logits, ids, teacher, weight, tau, grad):
     _on_device(device, ("logits", "ids", "teacher", "weight", "out"), (z, ids, teacher, weight, grad))
     where = z.device
     loss = torch.empty(rows, dtype=torch.float32, device=where)
-    if weight is not None and grad is None:
-        grad = torch.empty((rows, q), dtype=z.dtype, device=where)
     lib = load()
-    n = lib.thrml_distill_work(device.handle, rows, q, k)
-    work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
-    wp, gp, gs = (weight.data_ptr(), grad.data_ptr(), grad.stride(0) if rows > 1 else q) if weight is not None else (
-        0, 0, q)
-    _run(device, lib.thrml_distill, z.data_ptr(), _TYPES[z.dtype], rows, q, z.stride(0) if rows > 1 else q,
+    dtype, n, wp, gp, gs = _TYPES[z.dtype], 0, 0, 0, q
+    if weight is not None:
+        if grad is None:
+            grad = torch.empty((rows, q), dtype=z.dtype, device=where)
+        wp, gp, gs = weight.data_ptr(), grad.data_ptr(), grad.stride(0) if rows > 1 else q
+        n = lib.thrml_distill_work(device.handle, dtype, rows, q)
+        work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    _run(device, lib.thrml_distill, z.data_ptr(), dtype, rows, q, z.stride(0) if rows > 1 else q,
          ids.data_ptr(), ids.stride(0) if rows > 1 else k, teacher.data_ptr(), teacher.stride(0) if rows > 1 else k, k,
          float(tau), wp, loss.data_ptr(), gp, gs, work.data_ptr() if n else 0, n)
     return loss, grad
