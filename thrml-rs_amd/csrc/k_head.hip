@@ -1268,8 +1268,11 @@ int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work) 
     typedef decltype(t) T;
     // 64 registers of logits a lane
     constexpr int G = sizeof(T) == 2 ? 16 : 8;
-    auto *f = &distill_kernel<T, 512, 0>;
-    uint32_t block = 512;
+    // rows that have a compute unit each: 16 waves for one (256 losses over 131072
+    // categories in bf16 14.8 us, with 8 waves 19.2); more rows: several workgroups in a
+    // compute unit
+    uint32_t block = a.rows <= (uint64_t)ctx->cu_count && a.q > 8192 ? 1024 : 512;
+    auto *f = block == 1024 ? &distill_kernel<T, 1024, 0> : &distill_kernel<T, 512, 0>;
     if (a.weight && a.q <= 1024 * 8 * G) {
       block = a.q <= 256 * 8 * G ? 256 : a.q <= 512 * 8 * G ? 512 : 1024;
       f = block == 256 ? &distill_kernel<T, 256, G> : block == 512 ? &distill_kernel<T, 512, G> : &distill_kernel<T, 1024, G>;
