@@ -330,6 +330,32 @@ def test_distill_differences(device):
     assert ((up - down) / (2 * d) - grad[0].double()).abs().max() < d * d / 6 + 2 * float(lb[0]) / (2 * d)
 
 
+@pytest.mark.parametrize("k,names", [(2, 1), (31, 7), (32, 31), (33, 1), (64, 63), (65, 20), (1000, 3), (4096, 2000), (4096, 1)])
+@pytest.mark.parametrize("q,rows", [(40, 300), (5001, 3), (70000, 2)])
+def test_distill_repeats(device, k, names, q, rows):
+    """Lists that name few categories many times; each sum of m probabilities adds m
+    roundings of itself to the bound (70000 categories: the rows in segments)."""
+    log_case(f"distill repeats {k} {names} {q} {rows}")
+    rows = rows if k < 1000 else 2
+    z, _, teacher, weight = _distill_inputs(rows, q, k, F32, q + k + names)
+    g = _gen(k)
+    pool = torch.stack([torch.randperm(q, generator=g)[:names] for _ in range(rows)])
+    pick = torch.randint(0, pool.shape[1], (rows, k), generator=g)
+    ids = torch.gather(pool, 1, pick).int()
+    ids[0, k // 2] = -1
+    loss, lb, grad, gb = ref.distilled(z, ids, teacher, weight)
+    p = torch.softmax(torch.where(ids < 0, -float("inf"), teacher.double()), 1)
+    total, times = torch.zeros_like(grad), torch.zeros_like(grad)
+    total.scatter_add_(1, ids.clamp(min=0).long(), p)
+    times.scatter_add_(1, ids.clamp(min=0).long(), torch.ones_like(p))
+    gb = gb + weight.abs().double()[:, None] * ref.EPS * times * total
+    args = (device, z.cuda(), ids.cuda(), teacher.cuda(), weight.cuda())
+    got_loss, got_grad = th.distill_grad(*args)
+    ref.close(got_loss, loss, lb, "loss")
+    ref.close(got_grad, grad, gb, "grad")
+    assert torch.equal(got_grad, th.distill_grad(*args)[1])
+
+
 @pytest.mark.parametrize("q", [50, 70000])
 def test_distill_edges(device, q):
     """(70000 categories: the rows in segments)"""

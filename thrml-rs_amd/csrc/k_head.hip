@@ -265,7 +265,7 @@ constexpr int P_BLOCK = 512;
 template <class TI, class TO, int V>
 __global__ __launch_bounds__(P_BLOCK, 6) void process_kernel(LogitRows a, TO *__restrict__ out, int64_t out_stride,
                                                           uint32_t n_chunks, uint64_t n_tasks, uint32_t hash) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   constexpr uint32_t CHUNK = P_BLOCK * 8 * V;
   const bool table = a.history || a.n_bias;
   const Table tab{lds, lds + CHUNK, reinterpret_cast<float *>(lds + CHUNK + hash), CHUNK, hash};
@@ -701,7 +701,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
                                                           uint32_t seg, uint32_t n_seg, NamedPlan plan,
                                                           SamplePart *__restrict__ parts, int32_t *__restrict__ index,
                                                           float *__restrict__ logprob) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   __shared__ SamplePart wave_part[BLOCK / 64];
   __shared__ float wave_best[BLOCK / 64];
   __shared__ uint32_t wave_count[BLOCK / 64];
@@ -1023,21 +1023,52 @@ __device__ __forceinline__ void teacher_loss(const DistillArgs &a, uint64_t row,
   if (threadIdx.x == 0) a.loss[row] = c.some ? a.tau * a.tau * l : 0.0f;
 }
 
+// The candidates that count as (id, place), sorted, where their hash table was; behind them
+// ones.  By the whole workgroup, a bitonic network.
+__device__ __forceinline__ uint64_t *sort_candidates(const Candidates &c) {
+  static_assert(DISTILL_MAX_K <= 4096, "12 bits for the place");
+  uint64_t *s = reinterpret_cast<uint64_t *>(c.keys);
+  const uint32_t n = c.hash / 2, tid = here(threadIdx.x);  // a power of two, k or more
+  for (uint32_t i = tid; i < n; i += blockDim.x) {
+    const int32_t id = i < c.k ? c.ids[i] : -1;
+    s[i] = id >= 0 ? (uint64_t)id << 12 | i : ~0ull;
+  }
+  for (uint32_t size = 2; size <= n; size *= 2)
+    for (uint32_t step = size / 2; step > 0; step /= 2) {
+      __syncthreads();
+      for (uint32_t i = tid; i < n / 2; i += blockDim.x) {
+        const uint32_t lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const uint64_t x = s[lo], y = s[hi];
+        if ((x > y) == !(lo & size)) {
+          s[lo] = y;
+          s[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+  return s;
+}
+
 // The gradient at the candidates' places from s0 to s1 - 1, by the whole workgroup: an id that comes
-// more than once has the sum of its probabilities, in the order of the list.
+// more than once has the sum of its probabilities, in the order of the list.  Such lists
+// are sorted first: 32 rows of 20000 categories with one repeat in 1024 candidates take
+// 50 us (without 31), where a search of the list for each entry took 317; with one in 64
+// 15, and 19.
 template <class T>
 __device__ __forceinline__ void candidate_grads(const Candidates &c, bool again, uint32_t s0, uint32_t s1, T *g, float f,
                                                 float m, float ls, float rtau) {
-  for (uint32_t i = here(threadIdx.x); i < c.k; i += blockDim.x) {
-    const int32_t id = c.ids[i];
+  const uint64_t *s = nullptr;
+  if (again) s = sort_candidates(c);
+  for (uint32_t e = here(threadIdx.x); e < c.k; e += blockDim.x) {
+    const uint32_t i = again ? (uint32_t)s[e] & 4095u : e;
+    const int32_t id = again ? (int32_t)(s[e] >> 12) : c.ids[e];  // (ones: -1)
     if (id < 0 || (uint32_t)id - s0 >= s1 - s0) continue;
-    float p = c.p[i];
+    float p = 0.0f;
     if (again) {
-      bool first = true;
-      for (uint32_t j = 0; j < i && first; ++j) first = c.ids[j] != id;
-      if (!first) continue;
-      for (uint32_t j = i + 1; j < c.k; ++j)
-        if (c.ids[j] == id) p += c.p[j];
+      if (e > 0 && (int32_t)(s[e - 1] >> 12) == id) continue;
+      for (uint32_t j = e; j < c.k && (int32_t)(s[j] >> 12) == id; ++j) p += c.p[(uint32_t)s[j] & 4095u];
+    } else {
+      p = c.p[e];
     }
     g[id] = (T)(f * (softmax_of<T>(c.z[i], m, rtau, ls) - p));
   }
@@ -1110,11 +1141,14 @@ __device__ __forceinline__ Candidates candidates_in(uint32_t *lds, uint32_t k, u
   return c;
 }
 
-// GROUPS > 0: the row, of at most BLOCK * 8 GROUPS logits, stays in registers;
-// 0: it is read twice.
+// GROUPS > 0: the row, of 8 to BLOCK * 8 GROUPS logits, stays in registers; 0: it is
+// read twice.  In registers a place behind the last eight logits stands for those eight:
+// the maximum does not mind, the sum leaves out what another lane has, and the gradient
+// there is written twice with the same bits.  With all loads under way at once 1021 rows of
+// 50001 f16 take 46 us and 200 of 20000 bf16 15; loads that wait for one another: 50, 19.
 template <class T, int BLOCK, int GROUPS>
 __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillArgs a, uint32_t hash) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   __shared__ MaxSum buf[BLOCK / 64];
   __shared__ uint32_t flags;  // 1: there is an entry, 2: an id comes twice
   Candidates c = candidates_in(lds, a.k, hash);
@@ -1127,7 +1161,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
     if constexpr (GROUPS > 0) {
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        if ((uint32_t)g * BLOCK * 8u < a.q) load_place(z, ((uint32_t)g * BLOCK + tid) * 8u, a.q, r[g], LOWEST<T>);
+        if ((uint32_t)g * BLOCK * 8u < a.q) load8(z + min(((uint32_t)g * BLOCK + tid) * 8u, a.q - 8u), r[g]);
     }
     if (tid < 64u) {
       teacher_part(a, row, z, c);
@@ -1142,12 +1176,25 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
           for (int j = 0; j < 8; j += 2) t.m = max3(t.m, value(r[g], j), value(r[g], j + 1));
           hide(r[g]);
         }
+      // vmcnt(0): nothing is under way here, but the compiler, with each load and its use
+      // under conditions, takes loads to be so at the next row and puts a wait before
+      // each of them
+      __builtin_amdgcn_s_waitcnt(0x0f70);
 #pragma unroll
       for (int g = 0; g < G; ++g)
         if ((uint32_t)g * BLOCK * 8u < a.q) {
           float s = 0.0f;
+          if ((uint32_t)(g + 1) * BLOCK * 8u <= a.q) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((value(r[g], j) - t.m) * l2);
+            for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((value(r[g], j) - t.m) * l2);
+          } else {
+            const uint32_t d = ((uint32_t)g * BLOCK + tid) * 8u, before = d - min(d, a.q - 8u);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+              const float e = __builtin_amdgcn_exp2f((value(r[g], j) - t.m) * l2);
+              s += j >= before ? e : 0.0f;
+            }
+          }
           t.s += s;
           hide(r[g]);
         }
@@ -1166,7 +1213,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t d = ((uint32_t)g * BLOCK + tid) * 8u;
-          if (d < a.q) write_grad(o + d, a.q - d, r[g], some, f, t.m, ls, rtau);
+          if (d < a.q) write_grad(o + min(d, a.q - 8u), 8, r[g], some, f, t.m, ls, rtau);
         }
       } else {
         for (uint32_t d = tid * 8u; d < a.q; d += BLOCK * 8u) {
@@ -1201,7 +1248,7 @@ __global__ __launch_bounds__(DS_BLOCK) void distill_sum_kernel(DistillArgs a, ui
 template <class T>
 __global__ __launch_bounds__(DS_BLOCK) void distill_segment_kernel(DistillArgs a, uint32_t hash, uint32_t seg,
                                                                    uint32_t n_seg, const MaxSum *__restrict__ parts) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   __shared__ uint32_t flags;
   Candidates c = candidates_in(lds, a.k, hash);
   const uint32_t row = blockIdx.x / n_seg, s0 = blockIdx.x % n_seg * seg, s1 = min(s0 + seg, a.q), tid = threadIdx.x;
@@ -1232,12 +1279,12 @@ __global__ __launch_bounds__(DS_BLOCK) void distill_segment_kernel(DistillArgs a
 }
 
 // Segments of a row where they pay: 0 for a workgroup per row.  One and two launches (us):
-//    8 x 65536 bf16 (128 KB a row) 13.5 / 17.1    32 rows: 21.4 / 16.8    64: 21.5 / 19.9
-//    8 x 131072 bf16 (256 KB)      19.8 / 16.7    32 rows: 28.0 / 19.1   128: 32.2 / 29.3
-//    8 x 131072 f32 (512 KB)       30.3 / 15.7    64 rows: 45.3 / 29.0   200: 55.9 / 55.8
+//   16 x 65536 bf16 (128 KB a row) 12.5 / 15.4    32 rows: 16.7 / 15.8    64: 17.5 / 15.8
+//    8 x 131072 bf16 (256 KB)      18.9 / 15.6    32 rows: 19.9 / 15.5    64: 21.3 / 18.2
+//    8 x 131072 f32 (512 KB)       24.2 / 15.8    32 rows: 25.7 / 15.1    64: 34.0 / 20.6
 static uint32_t distill_segments(const thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q) {
   const uint64_t bytes = (uint64_t)q * (dtype == THRML_DTYPE_F32 ? 4 : 2);
-  if (rows * 4 > (uint64_t)ctx->cu_count || bytes < (rows < 16 ? 256u << 10 : 128u << 10)) return 0;
+  if (rows * 4 > (uint64_t)ctx->cu_count || bytes < (rows < 32 ? 256u << 10 : 128u << 10)) return 0;
   return std::min<uint32_t>(64, std::min<uint32_t>(cdiv(q, 2 * DS_BLOCK * 8), 2 * ctx->cu_count / (uint32_t)rows));
 }
 uint64_t distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q) {
@@ -1273,7 +1320,7 @@ int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work) 
     // compute unit
     uint32_t block = a.rows <= (uint64_t)ctx->cu_count && a.q > 8192 ? 1024 : 512;
     auto *f = block == 1024 ? &distill_kernel<T, 1024, 0> : &distill_kernel<T, 512, 0>;
-    if (a.weight && a.q <= 1024 * 8 * G) {
+    if (a.weight && a.q >= 8 && a.q <= 1024 * 8 * G) {
       block = a.q <= 256 * 8 * G ? 256 : a.q <= 512 * 8 * G ? 512 : 1024;
       f = block == 256 ? &distill_kernel<T, 256, G> : block == 512 ? &distill_kernel<T, 512, G> : &distill_kernel<T, 1024, G>;
     }
