@@ -687,12 +687,12 @@ template <class T>
 struct SampleGroup {
   Raw8<T> z;
   Raw8<float> u;
-  uint32_t live;
+  uint32_t in, allowed;  // not joined before use: that would wait for all of the loads
   __device__ __forceinline__ void load(const T *z_, const float *u_, const uint8_t *mask, uint32_t c, uint32_t end) {
     load_place(z_, c, end, z);
     if (u_) load_place(u_, c, end, u);
-    const uint32_t in = c >= end ? 0u : c + 8u <= end ? 255u : (1u << (end - c)) - 1u;
-    live = mask && in ? mask[c / 8u] & in : in;
+    in = c >= end ? 0u : c + 8u <= end ? 255u : (1u << (end - c)) - 1u;
+    allowed = mask && in ? mask[c / 8u] : 255u;
   }
 };
 
@@ -738,7 +738,8 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         auto group = [&](const SampleGroup<T> &k, uint32_t d, float (&y)[8]) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = value(k.z, j);
-          return table && d < end ? k.live & ~(uint32_t)flags[(d - c0) / 8u] : k.live;
+          const uint32_t live = k.in & k.allowed;
+          return table && d < end ? live & ~(uint32_t)flags[(d - c0) / 8u] : live;
         };
         s.first = s.second = -INFINITY;
         s.at = c0;
@@ -790,19 +791,27 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
             }
           }
           if (!__any(live != 0u)) continue;
+          // (places without one read the part's first: all loads are under way at once)
+          T zc[N];
+          uint32_t m[N];
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            y[j] = 0.0f;
+            zc[j] = z[c[j]];
             r[j] = 0;
-            if (live >> j & 1u) {
-              y[j] = (float)z[c[j]];
-              if (ur) r[j] = __builtin_bit_cast(uint32_t, ur[c[j]]);
-              if (mask && !(mask[c[j] / 8u] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
-            }
+            m[j] = 255u;
+          }
+          if (ur) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) r[j] = __builtin_bit_cast(uint32_t, ur[c[j]]);
+          }
+          if (mask) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) m[j] = mask[c[j] / 8u];
           }
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            y[j] = penalised(y[j], n[j], p);
+            if (!(m[j] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
+            y[j] = penalised((float)zc[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
           s.scores(y, r, live, x, v);
