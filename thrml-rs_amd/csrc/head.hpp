@@ -111,6 +111,11 @@ __device__ __forceinline__ uint32_t here(uint32_t n) {
   return n;
 }
 
+// vmcnt(0), once in a loop over rows where nothing is under way any more.  The compiler,
+// with a load and its use under conditions of their own, takes the load to be under way
+// still at the next row, and there puts a wait before every load.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // p[0 .. n-1], and the bits `fill` for the rest, n < 8
 template <class T>
 __device__ __forceinline__ void load8_part(const T *p, uint32_t n_, Raw8<T> &r, uint32_t fill = 0) {

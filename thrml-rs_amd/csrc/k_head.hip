@@ -294,6 +294,7 @@ __global__ __launch_bounds__(P_BLOCK, 6) void process_kernel(LogitRows a, TO *__
     }
     const Divisor t(p.t);
     if (table) table_fill(a, p, lists, row, c0, tab);
+    loads_done();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t d = ((uint32_t)v * P_BLOCK + tid) * 8u;
@@ -846,6 +847,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
         part_write(o, row, index, logprob);
     }
     __syncthreads();
+    loads_done();
   }
 }
 
@@ -1185,10 +1187,7 @@ __global__ __launch_bounds__(BLOCK, GROUPS ? 4 : 1) void distill_kernel(DistillA
           for (int j = 0; j < 8; j += 2) t.m = max3(t.m, value(r[g], j), value(r[g], j + 1));
           hide(r[g]);
         }
-      // vmcnt(0): nothing is under way here, but the compiler, with each load and its use
-      // under conditions, takes loads to be so at the next row and puts a wait before
-      // each of them
-      __builtin_amdgcn_s_waitcnt(0x0f70);
+      loads_done();
 #pragma unroll
       for (int g = 0; g < G; ++g)
         if ((uint32_t)g * BLOCK * 8u < a.q) {
