@@ -143,9 +143,9 @@ def distilled(logits, ids, teacher, weight=None, tau=1.0):
 
 
 def integers(x):
-    """Rows as integers with a scale each, the quotients in f32."""
+    """Rows as integers with a scale each, 1 / 127 and the quotients in f32."""
     xf = x.float()
-    s = xf.abs().amax(1, keepdim=True) / 127.0
+    s = xf.abs().amax(1, keepdim=True) * torch.tensor(1 / 127)
     a = torch.round(xf / torch.where(s > 0, s, torch.ones(())))
     return a, s
 

@@ -1,10 +1,12 @@
 // k_linear.hip -- the product of a learned head in 8-bit integers: rows of
 // activations, quantised with a scale each, times weights with a scale for each
 // output channel.
-//   s_r = max |x_r| / 127,  a_r = round(x_r / s_r)   (ties to even)
+//   s_r = max |x_r| (1 / 127),  a_r = round(x_r / s_r)   (ties to even)
 //   y[r][c] = (sum_k a[r][k] w[c][k]) s_r w_scale[c] + bias[c]
 // The sum is exact in 32-bit integers (k <= 131072).  A row of zeros has zeros
-// for integers; a row with an infinity or a NaN has the scale NaN.
+// for integers; a row with an infinity or a NaN has the scale NaN.  1 / 127 is rounded
+// to 32 bits first, as torch on the device divides by a number: in one row of 22 a true
+// quotient is a step off that, and now and then an integer with it.
 #include "dev_util.hpp"
 #include "head.hpp"
 
@@ -36,6 +38,7 @@ __device__ __forceinline__ uint2 integers8(const Raw8<T> &r, const Divisor &d) {
   for (int j = 0; j < 8; ++j) v[j] = value(r, j);
   return make_uint2(integers4(v, d), integers4(v + 4, d));
 }
+__device__ __forceinline__ float scale_of(float peak) { return peak * (1.0f / 127.0f); }
 // a row's largest magnitude and whether it has an infinity or NaN
 struct Peak {
   float m = 0.0f;
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(256) void quantise_kernel(const T *__restrict__ x, 
     __syncthreads();
     const float m = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
     const int bad = bads[0] | bads[1] | bads[2] | bads[3];
-    const float s = m / 127.0f;
+    const float s = scale_of(m);
     const Divisor d(s > 0.0f ? s : 1.0f);
     if (threadIdx.x == 0) scale[row] = bad ? __builtin_nanf("") : s;
     int8_t *o = xq + row * kp;
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
               p.take(r);
             }
             p.join_wave();
-            const float sx = p.m / 127.0f;
+            const float sx = scale_of(p.m);
             const Divisor d(sx > 0.0f ? sx : 1.0f);
             if (l == 0) own_scales[i] = p.bad ? __builtin_nanf("") : sx;
             for (uint32_t c = l * 8u; c < kp; c += 512u) {
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(64 * LF_WAVES) void linear_few_kernel(LinearArgs a,
           __syncthreads();
           p.m = fmaxf(fmaxf(own_peak[0], own_peak[1]), fmaxf(own_peak[2], own_peak[3]));
           p.bad = own_bad[0] | own_bad[1] | own_bad[2] | own_bad[3];
-          own_scale = p.bad ? __builtin_nanf("") : p.m / 127.0f;
+          own_scale = p.bad ? __builtin_nanf("") : scale_of(p.m);
           const Divisor d(own_scale > 0.0f ? own_scale : 1.0f);
 #pragma unroll
           for (uint32_t g = 0; g < OWN_GROUPS; ++g) {
