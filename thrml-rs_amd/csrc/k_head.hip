@@ -681,7 +681,7 @@ struct Sampler {
 // A lane's next 8 logits and uniforms.
 //
 // 256 x 131072 bf16, a workgroup of 1024 for a row: 40 us without lists (201 MB, 5.0 TB/s),
-// 62 us with histories of 3000 entries on average.  The difference is a row's own: the
+// 60 us with histories of 3000 entries on average.  The difference is a row's own: the
 // table is filled before the pass over it begins, and the 2 % of categories that it names
 // are fetched again one by one, with half a kilobyte of cache lines for 8 of them.
 template <class T>
@@ -936,7 +936,7 @@ int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const fl
 // without p first, and at the candidates' places once more behind a barrier.
 //
 // Where the row fits the workgroup's registers, the gradient reads it there: one
-// read and one write of memory.  2048 x 131072 bf16: 249 us (1.07 GB, 4.3 TB/s; a copy
+// read and one write of memory.  2048 x 131072 bf16: 247 us (1.07 GB, 4.4 TB/s; a copy
 // reaches 4.8), 363 us reading the row twice.  Two exponentials and about 14 other
 // operations for a logit keep the vector unit busy for 160 us of that.
 // e^x: the hardware's 2^x of the rounded product, times what the rounding left
