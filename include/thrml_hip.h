@@ -538,7 +538,7 @@ int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint64_t rows, 
                   void *grad, int64_t grad_stride, void *work, uint64_t work_bytes);
 /* y[row][c] = (sum_j a[row][j] w[c][j]) s[row] w_scale[c] + bias[c] with s[row] =
  * max_j |x[row][j]| times 1 / 127 and a = x / s rounded to integers (ties to even; 1 / 127,
- * product and quotient in f32), the sum exact in integers, the rest in f32, rounded once to
+ * product and quotient in f32; a subnormal s is rounded up, |a| is at most 127), the sum exact in integers, the rest in f32, rounded once to
  * out_dtype.  bias may be NULL.  A row of x with an infinity or a NaN gives NaN. */
 uint64_t thrml_linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
 int thrml_linear_i8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,

@@ -3,6 +3,7 @@
 // output channel.
 //   s_r = max |x_r| (1 / 127),  a_r = round(x_r / s_r)   (ties to even)
 //   y[r][c] = (sum_k a[r][k] w[c][k]) s_r w_scale[c] + bias[c]
+// A subnormal scale is rounded up, so that |a| <= 127 (127 s >= max |x_r|).
 // The sum is exact in 32-bit integers (k <= 131072).  A row of zeros has zeros
 // for integers; a row with an infinity or a NaN has the scale NaN.  1 / 127 is rounded
 // to 32 bits first, as torch on the device divides by a number: in one row of 22 a true
@@ -23,8 +24,9 @@ typedef int32_t i32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 // up to 64, zeros behind k).
 static inline uint32_t padded_k(uint32_t k) { return (k + 63u) & ~63u; }
 static inline uint64_t scales_bytes(uint64_t rows) { return (rows * 4 + 255) & ~(uint64_t)255; }
-// x / d, rounded to integers; |x| is at most 127 d, so that only d decides whether
-// Divisor::fast is exact (a quotient below 2^-50 may be off and rounds to 0 either way).
+// x / d, rounded to integers; |x| is at most 127 d but for roundings of d, so that the
+// integers fit 8 bits and only d decides whether Divisor::fast is exact (a quotient below
+// 2^-50 may be off and rounds to 0 either way).
 __device__ __forceinline__ uint32_t integers4(const float *v, const Divisor &d) {
   uint32_t w = 0;
 #pragma unroll
@@ -38,7 +40,12 @@ __device__ __forceinline__ uint2 integers8(const Raw8<T> &r, const Divisor &d) {
   for (int j = 0; j < 8; ++j) v[j] = value(r, j);
   return make_uint2(integers4(v, d), integers4(v + 4, d));
 }
-__device__ __forceinline__ float scale_of(float peak) { return peak * (1.0f / 127.0f); }
+// A row's scale.  Where it is subnormal the product may lose up to all of its bits and
+// leave quotients far above 127 (190 for a peak of 190 x 2^-149): such scales are rounded up.
+__device__ __forceinline__ float scale_of(float peak) {
+  const float s = peak * (1.0f / 127.0f);
+  return s < 0x1p-126f && s * 127.0f < peak ? s + 0x1p-149f : s;
+}
 // a row's largest magnitude and whether it has an infinity or NaN
 struct Peak {
   float m = 0.0f;

@@ -272,8 +272,8 @@ def linear_i8(device, x, w, w_scale, bias=None, out_dtype=None):
     """y [rows, q] = (a @ w.T) * s * w_scale + bias in out_dtype (default: x's): w
     [q, k] int8 weights with a scale w_scale [q] float32 for each output channel, x
     [rows, k] activations that the call quantises row by row, s = max |x| * (1 /
-    127) in f32, a = x / s rounded to integers (ties to even).  The sum is exact in integers, the
-    rest is in f32.  A row of x with an infinity or a NaN gives NaN.  k is at most
+    127) in f32 (a subnormal s is rounded up: |a| is at most 127), a = x / s rounded to
+    integers (ties to even).  The sum is exact in integers, the rest is in f32.  A row of x with an infinity or a NaN gives NaN.  k is at most
     131072."""
     if torch is None:
         _setup()
