@@ -574,14 +574,16 @@ struct Sampler {
   // of a part's groups: the best v, the place of its group, the best v of the others
   float first, second;
   uint32_t at;
-  float t, rt;
+  float t, by, rt;  // x = y by rt, y / t but for roundings
   bool scaled, noisy, odd = false;
 
   __device__ __forceinline__ void begin(const RowParams &p, const float *u, const float *temperature) {
     t = p.t;
     scaled = p.t > 0.0f;
     noisy = u && (scaled || !temperature);
-    rt = scaled ? 1.0f / p.t : 1.0f;
+    const Scaled d(scaled ? p.t : 1.0f);
+    by = d.by;
+    rt = 1.0f / d.d;
   }
 
   // What v has to reach where the best is b.  Greedy rows without a temperature have
@@ -595,7 +597,7 @@ struct Sampler {
   __device__ __forceinline__ void scores(const float (&y)[N], const uint32_t (&u)[N], uint32_t live, float (&x)[N],
                                          float (&v)[N]) const {
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = y[j] * rt;
+    for (int j = 0; j < N; ++j) x[j] = y[j] * by * rt;
     if (__any(live != (1u << N) - 1u)) {
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
@@ -830,6 +832,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
       const Sampler again = s;
       s = Sampler{};
       s.t = again.t;
+      s.by = again.by;
       s.rt = again.rt;
       s.scaled = again.scaled;
       s.noisy = again.noisy;
