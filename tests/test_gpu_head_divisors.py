@@ -55,6 +55,42 @@ def test_repetition(device, times):
     _held(got, want, "repetition")
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("rows_times", [1, 16])
+def test_both_in_place(device, rows_times, out):
+    """Penalties and temperatures of every kind together, biases and a mask, into the logits
+    themselves: one rounding for each of the steps, relative to the larger of its two
+    sides, which the temperature divides too."""
+    n = len(DIVISORS)
+    t = torch.tensor(DIVISORS, dtype=F32).repeat_interleave(n).repeat(rows_times)
+    theta = torch.tensor(DIVISORS, dtype=F32).repeat(n).repeat(rows_times)
+    rows, q = len(t), 5000 // rows_times
+    log_case(f"both {rows} {q} {out}")
+    g = torch.Generator().manual_seed(rows)
+    z = torch.tensor(VALUES, dtype=F32).repeat(q // len(VALUES) + 1)[:q].to(out).expand(rows, -1).contiguous()
+    kw = {"history": torch.randint(0, q, (rows, 40), generator=g, dtype=torch.int32), "repetition": theta,
+          "prompt_lengths": torch.full((rows,), 40, dtype=torch.int32), "temperature": t,
+          "bias_ids": torch.randint(0, q, (rows, 5), generator=g, dtype=torch.int32),
+          "bias_values": torch.randn(rows, 5, generator=g),
+          "mask": torch.randint(-2**31, 2**31, (rows, (q + 31) // 32), generator=g).to(torch.int32)}
+    want, _ = ref.processed(F32, z, **kw)
+    zd = z.cuda()
+    assert th.process_logits(device, zd, out=zd, **{k: v.cuda() for k, v in kw.items()}) is zd
+    got, want = zd.cpu().double(), want.double()
+    first, _ = ref.processed(F32, z, **{k: v for k, v in kw.items() if k not in ("temperature", "mask")})
+    # each quotient as in _held: 3 roundings or a unit; the sum with a bias, below 8, is
+    # relative to a penalised logit of at most 1.5 times itself or 8
+    size = torch.where(first.isfinite(), torch.clamp(first.double().abs(), min=8.0), 0.0)
+    off = (10 * ref.EPS * size + 2 * 2.0**-149) / t.double()[:, None]
+    same = (got == want) | (got.isnan() & want.isnan())
+    half = ref.HALF_STEP[out]
+    near = ((got - want).abs() <= off + half * want.abs() + 2.0**-133) & want.isfinite()
+    # beyond the type's range by its last rounding
+    over = got.isinf() & (got.sign() == want.sign()) & (want.abs() > torch.finfo(out).max * (1 - 2 * half))
+    bad = (~(same | near | over)).nonzero()
+    assert not bad.numel(), [(i.tolist(), float(got[tuple(i)]), float(want[tuple(i)])) for i in bad[:6]]
+
+
 def _logprob(z, index, kw):
     """In 64 bits from the steps before the temperature in f32, as they are defined: a
     penalty's rounding of a subnormal logit is no small part of it."""

@@ -208,37 +208,27 @@ __device__ __forceinline__ void store4(T *p, uint32_t n, const float (&v)[4]) {
   }
 }
 
-// A row's divisor as what multiplies the dividends first (exact, but for overflows that the
-// quotient shares) and a divisor whose reciprocal is finite and above 0.  A subnormal one
-// is brought up by 2^64; an infinite one divides as 0 times the dividend over 1 (0, or NaN
-// of an infinity).
-struct Scaled {
-  float by, d;
-  __device__ __forceinline__ explicit Scaled(float b) : by(1.0f), d(b) {
-    if (__builtin_fabsf(b) < 0x1p-126f) {
-      by = 0x1p64f;
-      d = b * 0x1p64f;
-    } else if (__builtin_isinf(b)) {
-      by = 0.0f;
-      d = 1.0f;
-    }
-  }
-};
-
 // a / b for many a: q = a r with r = 1 / b rounded, and one step of the remainder,
 // which an fma gives exactly, leave the correctly rounded quotient (Markstein 1990)
 // for |b| within 2^-100 .. 2^100 and |a| from 2^-100 on, but for one within a step of
 // overflow, and elsewhere one a step off it at most; infinities, zeros and NaN divide as
-// they should.  6 operations instead of the 10 of a full division, in line.
+// they should.  5 operations instead of the 10 of a full division, in line.  Not for a b
+// below 2^-128, whose reciprocal is infinite (0 would give NaN, small dividends infinities).
 struct Divisor {
-  Scaled s;
-  float b, r;
-  bool plain;  // b is within 2^-100 .. 2^100
+  float b, r, m;  // m: b, or 1 for an infinite one
+  bool plain;     // b is within 2^-100 .. 2^100
   __device__ __forceinline__ explicit Divisor(float b_)
-      : s(b_), b(b_), r(1.0f / s.d), plain(b_ >= 0x1p-100f && b_ <= 0x1p100f) {}
-  __device__ __forceinline__ float fast(float a_) const {
-    const float a = a_ * s.by, q = a * r;
-    return __builtin_isinf(q) ? q : __builtin_fmaf(__builtin_fmaf(-q, s.d, a), r, q);
+      : b(b_), r(1.0f / b_), m(__builtin_isinf(b_) ? 1.0f : b_), plain(b_ >= 0x1p-100f && b_ <= 0x1p100f) {}
+  __device__ __forceinline__ bool fine() const { return !__builtin_isinf(r); }
+  __device__ __forceinline__ float fast(float a) const {  // where fine()
+    const float q = a * r;
+    return __builtin_isinf(q) ? q : __builtin_fmaf(__builtin_fmaf(-q, m, a), r, q);
+  }
+  // r and m, the same in all lanes of the wave, in scalar registers (where it is called: b
+  // has to be there)
+  __device__ __forceinline__ void scalar() {
+    r = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, r)));
+    m = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, m)));
   }
 };
 

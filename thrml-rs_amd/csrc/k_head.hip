@@ -199,11 +199,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-// z with its row's penalties, each step rounded to f32 (w = 0: none)
+// z with its row's penalties, each step rounded to f32 (w = 0: none); ANY: for a repetition
+// penalty that is not fine(), too
+template <bool ANY>
 __device__ __forceinline__ float penalised(float z, uint32_t w, const RowParams &p) {
   const uint32_t n = w & T_COUNT;
   const float fn = (float)n;
-  float y = z > 0.0f ? p.theta.fast(z) : z * p.theta.b;
+  float y = z > 0.0f ? ANY ? z / p.theta.b : p.theta.fast(z) : z * p.theta.b;
   y = (w & ~T_BIAS) ? y : z;
   const float less = (y - p.frequency * fn) - p.presence;
   return n ? less : y;
@@ -222,7 +224,7 @@ __device__ __forceinline__ void row_values(const Raw8<T> &r, bool table, const T
     if ((t0.x | t0.y | t0.z | t0.w | t1.x | t1.y | t1.z | t1.w) != 0u) {
       const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = penalised(y[j], w[j], p);
+      for (int j = 0; j < 8; ++j) y[j] = penalised<false>(y[j], w[j], p);
       if (((w[0] | w[1] | w[2] | w[3] | w[4] | w[5] | w[6] | w[7]) & T_BIAS) != 0u) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -283,7 +285,8 @@ __global__ __launch_bounds__(P_BLOCK, 6) void process_kernel(LogitRows a, TO *__
     // the lists first: loads end in their order, and the table waits for these alone
     RowLists<P_BLOCK> lists;
     if (table) lists.load(a, row, tid);
-    const RowParams p = row_params(a, row);
+    RowParams p = row_params(a, row);
+    p.theta.scalar();
     Raw8<TI> r[V];
     uint32_t m[V];
 #pragma unroll
@@ -292,24 +295,44 @@ __global__ __launch_bounds__(P_BLOCK, 6) void process_kernel(LogitRows a, TO *__
       load_place(z, d, n, r[v]);
       m[v] = mask && d < n ? mask[d / 8u] : 255u;
     }
-    const Divisor t(p.t);
+    Divisor t(p.t > 0.0f ? p.t : 1.0f);
+    t.scalar();
     if (table) table_fill(a, p, lists, row, c0, tab);
     loads_done();
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const uint32_t d = ((uint32_t)v * P_BLOCK + tid) * 8u;
-      if (d >= n) break;
-      float y[8];
-      row_values(r[v], table, tab, d, p, y);
-      if (p.t > 0.0f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = t.fast(y[j]);
+    if (__builtin_expect(!p.theta.fine() || !t.fine(), 0)) {
+      // a subnormal divisor: full divisions, one category at a time, from pointers of its own
+      // (a second form of the divisions in the loop below, or its pointers kept for this one,
+      // cost the rows of other divisors: 512 x 65536 takes 69 us, and took 76 to 102)
+      const int64_t row_ = opaque((uint32_t)row);
+      const TI *z_ = reinterpret_cast<const TI *>(a.z) + row_ * a.z_stride;
+      const uint8_t *mask_ = reinterpret_cast<const uint8_t *>(a.mask + row_ * a.mask_stride);
+#pragma unroll 1
+      for (uint32_t d = tid; d < n; d += P_BLOCK) {
+        const uint32_t w = table ? tab.tab[d] : 0u, c = c0 + d;
+        float y = penalised<true>((float)z_[c], w, p);
+        if (w & T_BIAS) y = y + bias_of(tab.keys, tab.vals, hash, d);
+        if (p.t > 0.0f) y = y / p.t;
+        if (a.mask && !(mask_[c / 8u] >> (c % 8u) & 1u)) y = -INFINITY;
+        o[d] = (TO)y;
+        if (table) tab.tab[d] = 0;
       }
-      if (mask) {
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (m[v] >> j & 1u) ? y[j] : -INFINITY;
+      for (int v = 0; v < V; ++v) {
+        const uint32_t d = ((uint32_t)v * P_BLOCK + tid) * 8u;
+        if (d >= n) break;
+        float y[8];
+        row_values(r[v], table, tab, d, p, y);
+        if (p.t > 0.0f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = t.fast(y[j]);
+        }
+        if (mask) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = (m[v] >> j & 1u) ? y[j] : -INFINITY;
+        }
+        store8(o + d, n - d, y);
       }
-      store8(o + d, n - d, y);
     }
     // (the last chunk's words behind the row's end belong to no one)
     if (table && gridDim.x < n_tasks) {
@@ -568,6 +591,22 @@ __device__ __forceinline__ uint32_t named_fill(const LogitRows &a, const RowPara
   return total;
 }
 
+// What multiplies a row's logits (exact, but for overflows that their quotients share) and
+// the divisor that is left of its temperature, with a reciprocal that is finite and above 0.
+// A subnormal temperature is brought up by 2^64; over an infinite one a logit is 0, or NaN.
+struct Scaled {
+  float by, d;
+  __device__ __forceinline__ explicit Scaled(float t) : by(1.0f), d(t) {
+    if (t < 0x1p-126f) {
+      by = 0x1p64f;
+      d = t * 0x1p64f;
+    } else if (__builtin_isinf(t)) {
+      by = 0.0f;
+      d = 1.0f;
+    }
+  }
+};
+
 // One row's state in a lane.
 struct Sampler {
   SamplePart s{-__FLT_MAX__, 0.0f, -INFINITY, 0.0f, -1.0f, -1};
@@ -814,7 +853,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             if (!(m[j] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
-            y[j] = penalised((float)zc[j], n[j], p);
+            y[j] = penalised<true>((float)zc[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
           s.scores(y, r, live, x, v);
