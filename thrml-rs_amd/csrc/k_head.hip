@@ -369,11 +369,13 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
 // ---------------------------------------------------------------------------
 // Sampling.  With x the processed logits, a row's category is the first argmax
 // over the allowed ones of x - log(-log u) (Gumbel-max), or of x for a greedy
-// row, and its log-probability is x - m - log(sum exp(x - m)), all in one pass
-// over the row: the running maximum and sum of a softmax per lane, and the pick.
+// row, all in one pass over the row: the running maximum and sum of a softmax per lane,
+// and the pick.  With y the logits before the temperature t and m the largest of them,
+// the log-probability is (y - m) / t - log(sum exp((y - m) / t)): its error follows the
+// distance from the largest logit, and it is never above 0.
 //
 // The pick is exact in 64 bits at f32 cost.  v, the score from hardware logarithms and
-// x from a reciprocal of the temperature, is within S_MARGIN / 2 + |v| S_REL / 2 of the
+// y times a reciprocal of the temperature, is within S_MARGIN / 2 + |v| S_REL / 2 of the
 // score in 64 bits; picks are compared by v where that decides and in 64 bits, from x as
 // the steps in f32 give it, where it does not.  A lane keeps its best group of 8 by v
 // and the best v of its other groups; at the end of a part of the row the workgroup's
@@ -382,6 +384,8 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
 // of 2^-126, no less than its own: where one comes into play, the row is done again
 // without a bound.  An allowed category whose own score is -inf (u = 0) is taken only
 // where there is no other, a masked one never.
+// (The noise from hardware logarithms is within 1.98e-6 of -log(-log u) for every f32 u from
+// 2^-126 to 1, all of them tried.)
 constexpr float S_MARGIN = 1e-4f, S_REL = 0x1p-18f;
 constexpr float LOG2E = 1.44269504f;
 
@@ -396,9 +400,23 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// What multiplies a row's logits (exact, but for overflows that their quotients share) and
+// the divisor that is left of its temperature, with a reciprocal that is finite and above 0.
+// A subnormal temperature is brought up by 2^64; over an infinite one a logit is 0, or NaN.
+// A temperature that is not above 0 leaves the logits as they are.
+struct Scaled {
+  float by, d;
+  __device__ __forceinline__ explicit Scaled(float t) {  // (no branches: loads behind it would wait for t)
+    const bool tiny = t > 0.0f && t < 0x1p-126f, endless = t == INFINITY;
+    by = tiny ? 0x1p64f : endless ? 0.0f : 1.0f;
+    d = tiny ? t * 0x1p64f : t > 0.0f && !endless ? t : 1.0f;
+  }
+};
+
+// Here and below y is a logit as Scaled::by makes it: x = y / d.
 struct SamplePart {
-  float m, sum;   // running maximum and sum of exponentials
-  float v, x, u;  // of the pick: its score in 32 bits, logit and uniform (-1: the logit is the score)
+  float m, sum;   // running maximum of y, and sum of exp((y - m) / d)
+  float v, y, u;  // of the pick: its score in 32 bits, logit and uniform (-1: the logit is the score)
   int32_t arg;    // -1: none yet
 };
 constexpr float U_MIN = 0x1p-126f;
@@ -409,47 +427,49 @@ __device__ __forceinline__ double exact_score(float x, float u) {
   return e == -INFINITY && x > -INFINITY ? -__DBL_MAX__ : e;
 }
 // b's pick comes before a's: by v where that decides, else in 64 bits.
-__device__ __forceinline__ bool beats(const SamplePart &b, const SamplePart &a) {
+__device__ __forceinline__ bool beats(const SamplePart &b, const SamplePart &a, float d) {
   if (b.arg < 0 || a.arg < 0) return b.arg >= 0;
-  const float margin = 2.0f * S_MARGIN + (fabsf(a.v) + fabsf(b.v)) * S_REL, d = b.v - a.v;
-  if (d > margin && b.u >= U_MIN) return true;
-  if (d < -margin && a.u >= U_MIN) return false;
-  const double ea = exact_score(a.x, a.u), eb = exact_score(b.x, b.u);
+  const float margin = 2.0f * S_MARGIN + (fabsf(a.v) + fabsf(b.v)) * S_REL, lead = b.v - a.v;
+  if (lead > margin && b.u >= U_MIN) return true;
+  if (lead < -margin && a.u >= U_MIN) return false;
+  const double ea = exact_score(a.y / d, a.u), eb = exact_score(b.y / d, b.u);
   return eb > ea || (eb == ea && b.arg < a.arg);
 }
 
-__device__ __forceinline__ void part_merge(SamplePart &a, const SamplePart &b) {
+// c: log2 e / d
+__device__ __forceinline__ void part_merge(SamplePart &a, const SamplePart &b, float d, float c) {
   const float m = fmaxf(a.m, b.m);
-  a.sum = a.sum * __builtin_amdgcn_exp2f((a.m - m) * LOG2E) + b.sum * __builtin_amdgcn_exp2f((b.m - m) * LOG2E);
+  a.sum = a.sum * __builtin_amdgcn_exp2f((a.m - m) * c) + b.sum * __builtin_amdgcn_exp2f((b.m - m) * c);
   a.m = m;
-  if (beats(b, a)) {
+  if (beats(b, a, d)) {
     a.v = b.v;
-    a.x = b.x;
+    a.y = b.y;
     a.u = b.u;
     a.arg = b.arg;
   }
 }
 
 // of all lanes of a wave, in lane 0 (a loop, so that there is one merge to compile)
-__device__ __forceinline__ void part_join_wave(SamplePart &a) {
+__device__ __forceinline__ void part_join_wave(SamplePart &a, float d, float c) {
 #pragma unroll 1
   for (int s = 32; s > 0; s >>= 1) {
     SamplePart b;
     b.m = __shfl_xor(a.m, s);
     b.sum = __shfl_xor(a.sum, s);
     b.v = __shfl_xor(a.v, s);
-    b.x = __shfl_xor(a.x, s);
+    b.y = __shfl_xor(a.y, s);
     b.u = __shfl_xor(a.u, s);
     b.arg = __shfl_xor(a.arg, s);
-    part_merge(a, b);
+    part_merge(a, b, d, c);
   }
 }
 
-__device__ __forceinline__ void part_write(const SamplePart &s, uint64_t row, int32_t *index, float *logprob) {
-  // no sum: nothing is allowed; NaN: a NaN or +inf among the logits
-  const bool ok = s.sum > 0.0f && s.arg >= 0;
+__device__ __forceinline__ void part_write(const SamplePart &s, float d, uint64_t row, int32_t *index, float *logprob) {
+  // no sum: nothing is allowed; NaN: a NaN or +inf among the logits; and the largest
+  // quotient may be infinite where the logit is not
+  const bool ok = s.sum > 0.0f && s.arg >= 0 && fabsf(s.m / d) < INFINITY;
   index[row] = ok ? s.arg : -1;
-  logprob[row] = ok ? (s.x - s.m) - logf(s.sum) : __builtin_nanf("");
+  logprob[row] = ok ? (s.y - s.m) / d - logf(s.sum) : __builtin_nanf("");
 }
 
 // What the lists name is few beside the row and goes apart: a hash table in LDS holds
@@ -591,38 +611,22 @@ __device__ __forceinline__ uint32_t named_fill(const LogitRows &a, const RowPara
   return total;
 }
 
-// What multiplies a row's logits (exact, but for overflows that their quotients share) and
-// the divisor that is left of its temperature, with a reciprocal that is finite and above 0.
-// A subnormal temperature is brought up by 2^64; over an infinite one a logit is 0, or NaN.
-struct Scaled {
-  float by, d;
-  __device__ __forceinline__ explicit Scaled(float t) : by(1.0f), d(t) {
-    if (t < 0x1p-126f) {
-      by = 0x1p64f;
-      d = t * 0x1p64f;
-    } else if (__builtin_isinf(t)) {
-      by = 0.0f;
-      d = 1.0f;
-    }
-  }
-};
-
 // One row's state in a lane.
 struct Sampler {
   SamplePart s{-__FLT_MAX__, 0.0f, -INFINITY, 0.0f, -1.0f, -1};
   // of a part's groups: the best v, the place of its group, the best v of the others
   float first, second;
   uint32_t at;
-  float t, by, rt;  // x = y by rt, y / t but for roundings
+  float t, rd;  // the temperature, 1 / Scaled::d (what follows from them is not kept in registers)
   bool scaled, noisy, odd = false;
 
+  __device__ __forceinline__ float d() const { return Scaled(t).d; }
+  __device__ __forceinline__ float c() const { return rd * LOG2E; }
   __device__ __forceinline__ void begin(const RowParams &p, const float *u, const float *temperature) {
     t = p.t;
-    scaled = p.t > 0.0f;
+    scaled = t > 0.0f;
     noisy = u && (scaled || !temperature);
-    const Scaled d(scaled ? p.t : 1.0f);
-    by = d.by;
-    rt = 1.0f / d.d;
+    rd = 1.0f / Scaled(t).d;
   }
 
   // What v has to reach where the best is b.  Greedy rows without a temperature have
@@ -631,51 +635,55 @@ struct Sampler {
     return noisy || scaled ? b - (S_MARGIN + fabsf(b) * S_REL) : b;
   }
 
-  // v of N logits with penalties and biases; -inf where the bit in live is clear
+  // v of N logits with penalties and biases, which become y, -inf where the bit in live is
+  // clear
   template <int N>
-  __device__ __forceinline__ void scores(const float (&y)[N], const uint32_t (&u)[N], uint32_t live, float (&x)[N],
-                                         float (&v)[N]) const {
+  __device__ __forceinline__ void scores(float (&y)[N], const uint32_t (&u)[N], uint32_t live, float (&v)[N]) const {
+    if (__builtin_expect(__builtin_amdgcn_classf(t, 0x280), 0)) {  // a subnormal or infinite temperature
+      const float by = Scaled(t).by;
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = y[j] * by * rt;
+      for (int j = 0; j < N; ++j) y[j] *= by;
+    }
     if (__any(live != (1u << N) - 1u)) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = (live >> j & 1u) ? x[j] : -INFINITY;
+      for (int j = 0; j < N; ++j) y[j] = (live >> j & 1u) ? y[j] : -INFINITY;
     }
     if (noisy) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float l =
             __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(__builtin_bit_cast(float, u[j]), U_MIN, INFINITY));
-        v[j] = x[j] + __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f);
+        v[j] = __builtin_fmaf(y[j], rd, __builtin_fmaf(__builtin_amdgcn_logf(-l), -0.693147182f, 0.366512921f));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = x[j];
+      for (int j = 0; j < N; ++j) v[j] = y[j] * rd;
     }
   }
 
   template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N]) {
+  __device__ __forceinline__ void add(const float (&y)[N]) {
     float m = s.m;
+    const float c = this->c();
 #pragma unroll
-    for (int j = 0; j < N; j += 2) m = max3(m, x[j], x[j + 1]);
+    for (int j = 0; j < N; j += 2) m = max3(m, y[j], y[j + 1]);
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * LOG2E);
-    s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * LOG2E) + sum;
+    for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f((y[j] - m) * c);
+    s.sum = s.sum * __builtin_amdgcn_exp2f((s.m - m) * c) + sum;
     s.m = m;
   }
 
   // Eight logits from place d on.
-  __device__ __forceinline__ void take(const float (&y)[8], const uint32_t (&u)[8], uint32_t live, uint32_t d) {
-    float x[8], v[8];
-    scores(y, u, live, x, v);
-    add(x);
+  __device__ __forceinline__ void take(float (&y)[8], const uint32_t (&u)[8], uint32_t live, uint32_t place) {
+    float v[8];
+    scores(y, u, live, v);
+    add(y);
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) top = max3(top, v[j], v[j + 1]);
     second = __builtin_amdgcn_fmed3f(second, first, top);
-    at = top > first ? d : at;
+    at = top > first ? place : at;
     first = fmaxf(first, top);
   }
 
@@ -696,14 +704,14 @@ struct Sampler {
       }
       SamplePart b;
       b.v = vj;
-      b.x = scaled ? yj / t : yj;
+      b.y = yj;
       b.u = noisy ? __builtin_bit_cast(float, uj) : -1.0f;
       b.arg = id(j);
       // (v of a u below 2^-126 is too high, and so are bounds that come from it)
       odd = odd || (noisy && b.u < U_MIN);
-      if (beats(b, s)) {
+      if (beats(b, s, d())) {
         s.v = b.v;
-        s.x = b.x;
+        s.y = b.y;
         s.u = b.u;
         s.arg = b.arg;
       }
@@ -711,10 +719,10 @@ struct Sampler {
   }
 
   template <int N>
-  static __device__ __forceinline__ uint32_t reach(const float (&v)[N], const float (&x)[N], float cut) {
+  static __device__ __forceinline__ uint32_t reach(const float (&v)[N], const float (&y)[N], float cut) {
     uint32_t todo = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) todo |= (x[j] > -INFINITY && !(v[j] < cut) ? 1u : 0u) << j;
+    for (int j = 0; j < N; ++j) todo |= (y[j] > -INFINITY && !(v[j] < cut) ? 1u : 0u) << j;
     return todo;
   }
 };
@@ -809,16 +817,16 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
           for (uint32_t d = all ? c0 + tid * 8u : s.at; d < end; d += all ? BLOCK * 8u : end) {
             SampleGroup<T> k{};
             k.load(z, ur, mask, d, s1);
-            float y[8], x[8], v[8];
+            float y[8], v[8];
             const uint32_t live = group(k, d, y);
-            s.scores(y, k.u.w, live, x, v);
-            s.settle(y, k.u.w, v, Sampler::reach(v, x, cut), [&](int j) { return (int32_t)(d + j); });
+            s.scores(y, k.u.w, live, v);
+            s.settle(y, k.u.w, v, Sampler::reach(v, y, cut), [&](int j) { return (int32_t)(d + j); });
           }
         }
         // the named ones
         constexpr int N = 4;
         for (uint32_t b = 0; b < n_named; b += BLOCK * N) {
-          float y[N], x[N], v[N];
+          float y[N], v[N];
           uint32_t c[N], n[N], r[N], live = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
@@ -853,13 +861,13 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             if (!(m[j] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
-            y[j] = penalised<true>((float)zc[j], n[j], p);
+            y[j] = p.theta.fine() ? penalised<false>((float)zc[j], n[j], p) : penalised<true>((float)zc[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
-          s.scores(y, r, live, x, v);
-          s.add(x);
+          s.scores(y, r, live, v);
+          s.add(y);
           // (no bound but the other categories': few of these reach it)
-          s.settle(y, r, v, Sampler::reach(v, x, cut), [&](int j) {
+          s.settle(y, r, v, Sampler::reach(v, y, cut), [&](int j) {
             uint32_t cj = c[0];
 #pragma unroll
             for (int i = 1; i < N; ++i) cj = i == j ? c[i] : cj;
@@ -871,22 +879,21 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
       const Sampler again = s;
       s = Sampler{};
       s.t = again.t;
-      s.by = again.by;
-      s.rt = again.rt;
+      s.rd = again.rd;
       s.scaled = again.scaled;
       s.noisy = again.noisy;
     }
     SamplePart o = s.s;
-    part_join_wave(o);
+    part_join_wave(o, s.d(), s.c());
     if ((tid & 63u) == 0) wave_part[tid / 64u] = o;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll 1
-      for (int w = 1; w < BLOCK / 64; ++w) part_merge(o, wave_part[w]);
+      for (int w = 1; w < BLOCK / 64; ++w) part_merge(o, wave_part[w], s.d(), s.c());
       if (n_seg > 1)
         parts[task] = o;
       else
-        part_write(o, row, index, logprob);
+        part_write(o, s.d(), row, index, logprob);
     }
     __syncthreads();
     loads_done();
@@ -895,13 +902,14 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
 
 // one wave per row
 __global__ __launch_bounds__(64) void sample_join_kernel(const SamplePart *__restrict__ parts, uint64_t rows,
-                                                         uint32_t n_seg, int32_t *__restrict__ index,
-                                                         float *__restrict__ logprob) {
+                                                         uint32_t n_seg, const float *__restrict__ temperature,
+                                                         int32_t *__restrict__ index, float *__restrict__ logprob) {
   for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float d = Scaled(temperature ? temperature[row] : 0.0f).d, c = 1.0f / d * LOG2E;
     SamplePart s{-__FLT_MAX__, 0.0f, -INFINITY, 0.0f, -1.0f, -1};
-    for (uint32_t i = threadIdx.x; i < n_seg; i += 64u) part_merge(s, parts[row * n_seg + i]);
-    part_join_wave(s);
-    if (threadIdx.x == 0) part_write(s, row, index, logprob);
+    for (uint32_t i = threadIdx.x; i < n_seg; i += 64u) part_merge(s, parts[row * n_seg + i], d, c);
+    part_join_wave(s, d, c);
+    if (threadIdx.x == 0) part_write(s, d, row, index, logprob);
   }
 }
 
@@ -959,7 +967,7 @@ int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const fl
   });
   if (rc || p.n_seg == 1) return rc;
   hipLaunchKernelGGL(sample_join_kernel, dim3((uint32_t)std::min<uint64_t>(a.rows, 1u << 20)), dim3(64), 0, ctx->stream,
-                     parts, a.rows, p.n_seg, index, logprob);
+                     parts, a.rows, p.n_seg, a.temperature, index, logprob);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
 }
