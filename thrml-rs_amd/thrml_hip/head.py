@@ -11,6 +11,9 @@ Every call queues its kernels on the device's stream and returns tensors.  Where
 that is another stream than torch's current one, the kernels wait for what torch
 has queued there, and what torch queues there afterwards waits for them.  Calls
 may be captured into a graph.
+
+torch's gradients do not go through these calls: but for distill_grad, which returns the
+gradient, they refuse tensors that require one unless gradients are off.
 """
 import struct
 
@@ -72,11 +75,24 @@ def _out(name, t, rows, q, dtype):
     return t
 
 
-def _on_device(device, names, tensors):
+def _on_device(device, names, tensors, differentiable=True):
+    ordinal = device.ordinal
     for t in tensors:
-        if t is not None and t.get_device() != device.ordinal:
-            name = next(n for n, x in zip(names, tensors) if x is t)
-            _refuse(f"{name} is on {t.device}, the device is cuda:{device.ordinal}")
+        if t is not None and (t.requires_grad or t.get_device() != ordinal):
+            _check_tensors(ordinal, names, tensors, differentiable)
+            return
+
+
+def _check_tensors(ordinal, names, tensors, differentiable):
+    """differentiable: torch's gradients would have to go through the call, and do not"""
+    given = [(n, t) for n, t in zip(names, tensors) if t is not None]
+    for name, t in given:
+        if differentiable and t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name} requires a gradient, which this call does not carry on: detach it, or call under "
+                    "torch.no_grad() (distill_grad gives the gradient of the logits itself)")
+    for name, t in given:
+        if t.get_device() != ordinal:
+            _refuse(f"{name} is on {t.device}, the device is cuda:{ordinal}")
 
 
 def _run(device, fn, *args):
@@ -94,6 +110,7 @@ def _run(device, fn, *args):
 
 _ROW_NAMES = ("logits", "history", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "bias_ids",
               "bias_values", "temperature", "mask")
+_SAMPLE_NAMES = _ROW_NAMES + ("u",)
 
 
 def _rows(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
@@ -178,14 +195,14 @@ def process_logits(device, logits, *, history=None, lengths=None, prompt_lengths
                              bias_values, temperature, mask)
     z = keep[0]
     dtype = out_dtype or z.dtype
-    code = _type("out_dtype", dtype)
-    if out is not None:
+    code = _TYPES.get(dtype) or _type("out_dtype", dtype)
+    if out is None:
+        _on_device(device, _ROW_NAMES, keep)
+        out = torch.empty((rows, q), dtype=dtype, device=z.device)
+    else:
         if out is logits and z is not logits:
             _refuse("out may be the logits only where their rows are contiguous")
-        _out("out", out, rows, q, dtype)
-    _on_device(device, _ROW_NAMES + ("out",), keep + (out,))
-    if out is None:
-        out = torch.empty((rows, q), dtype=dtype, device=z.device)
+        _on_device(device, _ROW_NAMES + ("out",), keep + (_out("out", out, rows, q, dtype),))
     _run(device, load().thrml_process_logits, d, out.data_ptr(), code, out.stride(0) if rows > 1 else q)
     return out
 
@@ -203,7 +220,7 @@ def sample_logits(device, logits, u=None, *, history=None, lengths=None, prompt_
                              bias_values, temperature, mask)
     if u is not None:
         u = _matrix("u", u, _FLOAT32, rows, q)
-    _on_device(device, _ROW_NAMES + ("u",), keep + (u,))
+    _on_device(device, _SAMPLE_NAMES, keep + (u,))
     where = keep[0].device
     index = torch.empty(rows, dtype=torch.int32, device=where)
     logprob = torch.empty(rows, dtype=torch.float32, device=where)
@@ -231,7 +248,7 @@ def _distill(device, logits, ids, teacher, weight, tau, grad):
         weight = _vector("weight", weight, rows, _FLOAT32)
         if grad is not None:
             _out("out", grad, rows, q, z.dtype)
-    _on_device(device, ("logits", "ids", "teacher", "weight", "out"), (z, ids, teacher, weight, grad))
+    _on_device(device, ("logits", "ids", "teacher", "weight", "out"), (z, ids, teacher, weight, grad), weight is None)
     where = z.device
     loss = torch.empty(rows, dtype=torch.float32, device=where)
     lib = load()
