@@ -1,5 +1,7 @@
 """Arguments that the functions around a learned head have to refuse or take, on CPU
 tensors: no GPU is used."""
+import threading
+
 import pytest
 import torch
 
@@ -47,3 +49,34 @@ def test_distill_grad_takes_leaves():
     for z, t, w in ((_grad(Z), F, V), (Z, _grad(F), V), (Z, F, _grad(V))):
         with pytest.raises(th.ThrmlError, match="is on cpu"):
             th.distill_grad(_Device(), z, I, t, w)
+
+
+def test_second_thread_during_the_first_call(monkeypatch):
+    """Nothing of the module is seen half set up: a call from another thread, made between
+    any two steps of the first call's setup, is checked as any other."""
+    from thrml_hip import head
+
+    seen = []
+
+    class Types(dict):
+        def update(self, *args):
+            if not seen:
+                seen.append(None)
+                t = threading.Thread(target=other)
+                t.start()
+                t.join()
+            super().update(*args)
+
+    def other():
+        try:
+            th.process_logits(_Device(), Z)
+        except th.ThrmlError as e:
+            seen.append(str(e))
+
+    for name in ("_FLOATS", "_INT32", "_FLOAT32", "_INT8", "_WORDS"):
+        monkeypatch.setattr(head, name, ())
+    monkeypatch.setattr(head, "torch", None)
+    monkeypatch.setattr(head, "_TYPES", Types())
+    with pytest.raises(th.ThrmlError, match="is on cpu"):
+        th.process_logits(_Device(), Z)
+    assert len(seen) == 2 and "is on cpu" in seen[1]

@@ -29,15 +29,16 @@ _PACK = struct.Struct("@PiIQqPqIPPPPPPPqIPPq").pack  # thrml_logits
 
 def _setup():
     global torch, _raw_stream, _FLOATS, _INT32, _FLOAT32, _INT8, _WORDS
-    import torch
+    import torch as t
 
     # (without the stream object that torch.cuda.current_stream makes: 1 us of a call's 11)
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: t.cuda.current_stream(index).cuda_stream)
 
-    _TYPES.update({torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16})
-    _FLOATS, _INT32, _FLOAT32, _INT8 = tuple(_TYPES), (torch.int32,), (torch.float32,), (torch.int8,)
-    _WORDS = (torch.int32, torch.uint32)
+    _TYPES.update({t.float32: _lib.DTYPE_F32, t.bfloat16: _lib.DTYPE_BF16, t.float16: _lib.DTYPE_F16})
+    _FLOATS, _INT32, _FLOAT32, _INT8 = tuple(_TYPES), (t.int32,), (t.float32,), (t.int8,)
+    _WORDS = (t.int32, t.uint32)
+    torch = t  # last: with it a call, from any thread, takes the rest to be there
 
 
 def _refuse(msg):
