@@ -38,8 +38,7 @@ class PottsTorus:
     def states(self, key, chains, sweeps):
         """[chains, n] categories by node after a run from uniform states."""
         st = self.program.new_state(chains)
-        init = np.random.default_rng(key.seed).integers(0, self.q, (chains, self.n)).astype(np.uint8)
-        st.set_global(init)
+        st.set_global(np.random.default_rng(key.seed).integers(0, self.q, (chains, self.n)))
         run_blocks(key, self.program, st, (), sweeps)
         by_node = np.empty((chains, self.n), np.int64)
         by_node[:, self.order] = st.get_global()
