@@ -530,7 +530,8 @@ int thrml_sample_logits(thrml_ctx *ctx, const thrml_logits *in, const float *u, 
  * an id named twice has both probabilities),
  *   loss[row] = tau^2 sum_i p_i (log p_i - log softmax(logits / tau)[ids_i])
  *   grad[row][c] = d(weight[row] loss[row]) / d logits[row][c], in the logits' type
- * (weight NULL: the loss alone, without work memory).  A row without an entry has loss and gradient 0. */
+ * (weight NULL: the loss alone, without work memory).  A row without an entry has loss and gradient 0.
+ * tau is positive, finite and not subnormal. */
 uint64_t thrml_distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q);
 int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint64_t rows, uint32_t q,
                   int64_t logits_stride, const int32_t *ids, int64_t ids_stride, const float *teacher,

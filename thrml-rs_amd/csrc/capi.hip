@@ -2187,7 +2187,8 @@ extern "C" int thrml_distill(thrml_ctx *ctx, const void *logits, int dtype, uint
   if (!size) return fail(THRML_EINVAL, "logits must be f32, bf16 or f16");
   if (k > DISTILL_MAX_K)
     return fail(THRML_EUNSUPPORTED, "at most " + std::to_string(DISTILL_MAX_K) + " candidates per row");
-  if (!(tau > 0.0f) || !std::isfinite(tau)) return fail(THRML_EINVAL, "tau must be positive and finite");
+  // (of a subnormal tau 1 / tau may be infinite, and 0 / tau then NaN)
+  if (!(tau > 0.0f) || !std::isnormal(tau)) return fail(THRML_EINVAL, "tau must be positive, finite and not subnormal");
   if (int rc = check_rows("logits", logits, size, rows, q, logits_stride, false)) return rc;
   if (int rc = check_rows("ids", ids, 4, rows, k, ids_stride, false)) return rc;
   if (int rc = check_rows("teacher", teacher, 4, rows, k, teacher_stride, false)) return rc;

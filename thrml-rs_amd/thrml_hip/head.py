@@ -271,7 +271,8 @@ def distill_loss(device, logits, ids, teacher, tau=1.0):
     ids [rows, k] int32 (those outside 0 .. q-1 fill up shorter rows) with their
     logits teacher [rows, k] float32.  With p = softmax(teacher / tau) over the
     row's candidates, tau^2 sum_i p_i (log p_i - log softmax(logits / tau)[ids_i]);
-    0 for a row without candidates.  k is at most 4096."""
+    0 for a row without candidates.  k is at most 4096, tau positive, finite and not
+    subnormal."""
     return _distill(device, logits, ids, teacher, None, tau, None)[0]
 
 
