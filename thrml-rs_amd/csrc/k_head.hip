@@ -257,11 +257,13 @@ __device__ __forceinline__ void hide(Raw8<T> &r) {
 // Processing: a workgroup writes P_BLOCK * 8 V categories of one row.  Their logits
 // are on their way while it fills its table.
 //
-// Memory bounds it: 512 x 65536 f32 without lists take 42 us (6.4 TB/s, part of it from
-// the last-level cache).  Histories of 6144 entries on average bring that to 70 us (285
+// Memory bounds it: 512 x 65536 f32 without lists take 47 us (5.7 TB/s, part of it from
+// the last-level cache).  Histories of 6144 entries on average bring that to 69 us (285
 // MB, 4.1 TB/s): each of a row's 8 workgroups scans them, 0.75 entries per logit, and
-// waits for the scan at two barriers.  At 79 registers three workgroups of a compute
-// unit cover each other's waits (two, at 128 registers: 85 us).
+// waits for the scan at two barriers.  At 80 registers three workgroups of a compute
+// unit cover each other's waits (two, at 128 registers: 76 us).  A call whose workgroups are
+// all there at once has no such cover: 48 x 131071 f16 in 768 of them take 14.2 us, and 10.3
+// without lists.
 constexpr int P_BLOCK = 512;
 
 template <class TI, class TO, int V>
@@ -346,8 +348,8 @@ int launch_process_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, void *o
                           int64_t out_stride) {
   if (a.rows == 0) return THRML_OK;
   // two groups of 8 per lane where that leaves two workgroups for each compute unit, and
-  // LDS for many biases (48 x 131071: 18 us, 23 with one group; four groups, which spill
-  // registers, take 101 us at 512 x 65536 where two take 87)
+  // LDS for many biases (one, two and four groups, of which the last spill registers: 48 x
+  // 131071 17.7, 14.2 and 16.8 us, 512 x 65536 83.5, 68.5 and 115)
   const bool two = a.rows * cdiv(a.q, P_BLOCK * 16) >= 2ull * ctx->cu_count && a.n_bias <= 1024;
   const uint32_t chunk = P_BLOCK * (two ? 16 : 8), nc = cdiv(a.q, chunk);
   const uint64_t tasks = a.rows * nc;
@@ -732,7 +734,9 @@ struct Sampler {
 // 256 x 131072 bf16, a workgroup of 1024 for a row: 40 us without lists (201 MB, 5.0 TB/s),
 // 60 us with histories of 3000 entries on average.  The difference is a row's own: the
 // table is filled before the pass over it begins, and the 2 % of categories that it names
-// are fetched again one by one, with half a kilobyte of cache lines for 8 of them.
+// are fetched again one by one, with half a kilobyte of cache lines for 8 of them.  One
+// instance does it all, at 128 registers, with 3 to 8 of them and about 110 scalars spilled
+// (32 to 64 bytes of scratch a lane).
 template <class T>
 struct SampleGroup {
   Raw8<T> z;
@@ -990,7 +994,7 @@ int launch_sample_logits(thrml_ctx *ctx, const LogitRows &a, int dtype, const fl
 // reaches 4.8), 363 us reading the row twice.  Two exponentials and about 14 other
 // operations for a logit keep the vector unit busy for 160 us of that.
 // e^x: the hardware's 2^x of the rounded product, times what the rounding left
-// out (the relative error stays at 2 in 10^7 for x down to -100, 2 in 10^6 without)
+// out (the relative error stays at 1.4 in 10^7 down to e^x = 2^-125, 3.9 in 10^6 without)
 __device__ __forceinline__ float exp_wide(float x) {
   const float p = x * LOG2E;
   const float e = __builtin_fmaf(x, LOG2E, -p) + x * 1.92596299e-8f;
@@ -999,8 +1003,8 @@ __device__ __forceinline__ float exp_wide(float x) {
 }
 
 // The scaled logit's exponential against the row's sum, for the gradient.  16-bit
-// gradients take the hardware's 2^x as it is (2 in 10^6 off where their own step is
-// 5 in 10^4 or more).
+// gradients take the hardware's 2^x as it is: with the roundings of its exponent, up to 125,
+// it is within 2 in 10^5, where half of a step of theirs is 5 in 10^4 or more.
 template <class T>
 __device__ __forceinline__ float softmax_of(float z, float m, float rtau, float ls) {
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(__builtin_fmaf(z - m, rtau * LOG2E, -(ls * LOG2E)));
