@@ -48,14 +48,18 @@ def _refuse(msg):
 # The checks read few attributes of a tensor: a call's time on the host is what small
 # calls cost (each attribute is about 0.1 us).
 def _matrix(name, t, dtypes, rows=None, cols=None):
-    """t, a [rows, cols] tensor, with contiguous rows."""
+    """(t, a [rows, cols] tensor, with contiguous rows; its rows' stride)"""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         _refuse(f"{name} must be a {' or '.join(str(d)[6:] for d in dtypes)} tensor")
     s = t.shape
     if len(s) != 2 or (rows is not None and s[0] != rows) or (cols is not None and s[1] != cols):
         _refuse(f"{name} must have shape [{'rows' if rows is None else rows}, "
                 f"{'n' if cols is None else cols}], got {list(s)}")
-    return t if t.stride(1) == 1 or s[1] <= 1 else t.contiguous()
+    stride = t.stride()
+    if stride[1] == 1 or s[1] <= 1:
+        return t, stride[0]
+    t = t.contiguous()
+    return t, t.stride(0)
 
 
 def _vector(name, t, n, dtypes):
@@ -119,14 +123,14 @@ def _rows(logits, history, lengths, prompt_lengths, repetition, presence, freque
     """(the C descriptor, the tensors that it points into, rows, q)"""
     if torch is None:
         _setup()
-    z = _matrix("logits", logits, _FLOATS)
+    z, zs = _matrix("logits", logits, _FLOATS)
     rows, q = z.shape
     if q == 0:
         _refuse("logits must have at least one category")
     hp = hs = hn = lp = pp = rp = np_ = fp = bp = vp = bs = bn = tp = mp = ms = 0
     if history is not None:
-        history = _matrix("history", history, _INT32, rows)
-        hp, hs, hn = history.data_ptr(), history.stride(0), history.shape[1]
+        history, hs = _matrix("history", history, _INT32, rows)
+        hp, hn = history.data_ptr(), history.shape[1]
         if lengths is not None:
             lengths = _vector("lengths", lengths, rows, _INT32)
             lp = lengths.data_ptr()
@@ -147,11 +151,10 @@ def _rows(logits, history, lengths, prompt_lengths, repetition, presence, freque
             if t is not None:
                 _refuse(f"{name} needs a history")
     if bias_ids is not None and bias_values is not None:
-        bias_ids = _matrix("bias_ids", bias_ids, _INT32, rows)
+        bias_ids, bs = _matrix("bias_ids", bias_ids, _INT32, rows)
         bn = bias_ids.shape[1]
-        bias_values = _matrix("bias_values", bias_values, _FLOAT32, rows, bn)
-        bs = bias_ids.stride(0)
-        if rows > 1 and bs != bias_values.stride(0):
+        bias_values, vs = _matrix("bias_values", bias_values, _FLOAT32, rows, bn)
+        if rows > 1 and bs != vs:
             bias_ids, bias_values, bs = bias_ids.contiguous(), bias_values.contiguous(), bn
         bp, vp = bias_ids.data_ptr(), bias_values.data_ptr()
     elif bias_ids is not None or bias_values is not None:
@@ -160,12 +163,12 @@ def _rows(logits, history, lengths, prompt_lengths, repetition, presence, freque
         temperature = _vector("temperature", temperature, rows, _FLOAT32)
         tp = temperature.data_ptr()
     if mask is not None:
-        mask = _matrix("mask", mask, _WORDS, None, (q + 31) // 32)
+        mask, ms = _matrix("mask", mask, _WORDS, None, (q + 31) // 32)
         n = mask.shape[0]
         if n != 1 and n != rows:
             _refuse(f"mask must have 1 or {rows} rows, got {n}")
-        mp, ms = mask.data_ptr(), mask.stride(0) if n > 1 else 0
-    d = _PACK(z.data_ptr(), _TYPES[z.dtype], q, rows, z.stride(0) if rows > 1 else q, hp, hs, hn, lp, pp, rp, np_, fp,
+        mp, ms = mask.data_ptr(), ms if n > 1 else 0
+    d = _PACK(z.data_ptr(), _TYPES[z.dtype], q, rows, zs if rows > 1 else q, hp, hs, hn, lp, pp, rp, np_, fp,
               bp, vp, bs, bn, tp, mp, ms)
     return d, (z, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
                temperature, mask), rows, q
@@ -197,6 +200,7 @@ def process_logits(device, logits, *, history=None, lengths=None, prompt_lengths
     z = keep[0]
     dtype = out_dtype or z.dtype
     code = _TYPES.get(dtype) or _type("out_dtype", dtype)
+    stride = q
     if out is None:
         _on_device(device, _ROW_NAMES, keep)
         out = torch.empty((rows, q), dtype=dtype, device=z.device)
@@ -204,7 +208,9 @@ def process_logits(device, logits, *, history=None, lengths=None, prompt_lengths
         if out is logits and z is not logits:
             _refuse("out may be the logits only where their rows are contiguous")
         _on_device(device, _ROW_NAMES + ("out",), keep + (_out("out", out, rows, q, dtype),))
-    _run(device, load().thrml_process_logits, d, out.data_ptr(), code, out.stride(0) if rows > 1 else q)
+        if rows > 1:
+            stride = out.stride(0)
+    _run(device, load().thrml_process_logits, d, out.data_ptr(), code, stride)
     return out
 
 
@@ -219,8 +225,9 @@ def sample_logits(device, logits, u=None, *, history=None, lengths=None, prompt_
     logits) gets index -1 and logprob NaN."""
     d, keep, rows, q = _rows(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids,
                              bias_values, temperature, mask)
+    us = q
     if u is not None:
-        u = _matrix("u", u, _FLOAT32, rows, q)
+        u, us = _matrix("u", u, _FLOAT32, rows, q)
     _on_device(device, _SAMPLE_NAMES, keep + (u,))
     where = keep[0].device
     index = torch.empty(rows, dtype=torch.int32, device=where)
@@ -229,7 +236,7 @@ def sample_logits(device, logits, u=None, *, history=None, lengths=None, prompt_
     n = lib.thrml_sample_logits_work(device.handle, rows, q)
     work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
     _run(device, lib.thrml_sample_logits, d, u.data_ptr() if u is not None else 0,
-         u.stride(0) if u is not None and rows > 1 else q, index.data_ptr(), logprob.data_ptr(),
+         us if rows > 1 else q, index.data_ptr(), logprob.data_ptr(),
          work.data_ptr() if n else 0, n)
     return index, logprob
 
@@ -238,13 +245,13 @@ def _distill(device, logits, ids, teacher, weight, tau, grad):
     """weight None: the loss alone; grad: a tensor for the gradient, or None"""
     if torch is None:
         _setup()
-    z = _matrix("logits", logits, _FLOATS)
+    z, zs = _matrix("logits", logits, _FLOATS)
     rows, q = z.shape
     if q == 0:
         _refuse("logits must have at least one category")
-    ids = _matrix("ids", ids, _INT32, rows)
+    ids, ids_stride = _matrix("ids", ids, _INT32, rows)
     k = ids.shape[1]
-    teacher = _matrix("teacher", teacher, _FLOAT32, rows, k)
+    teacher, teacher_stride = _matrix("teacher", teacher, _FLOAT32, rows, k)
     if weight is not None:
         weight = _vector("weight", weight, rows, _FLOAT32)
         if grad is not None:
@@ -257,11 +264,13 @@ def _distill(device, logits, ids, teacher, weight, tau, grad):
     if weight is not None:
         if grad is None:
             grad = torch.empty((rows, q), dtype=z.dtype, device=where)
-        wp, gp, gs = weight.data_ptr(), grad.data_ptr(), grad.stride(0) if rows > 1 else q
+        elif rows > 1:
+            gs = grad.stride(0)
+        wp, gp = weight.data_ptr(), grad.data_ptr()
         n = lib.thrml_distill_work(device.handle, dtype, rows, q)
         work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
-    _run(device, lib.thrml_distill, z.data_ptr(), dtype, rows, q, z.stride(0) if rows > 1 else q,
-         ids.data_ptr(), ids.stride(0) if rows > 1 else k, teacher.data_ptr(), teacher.stride(0) if rows > 1 else k, k,
+    _run(device, lib.thrml_distill, z.data_ptr(), dtype, rows, q, zs if rows > 1 else q, ids.data_ptr(),
+         ids_stride if rows > 1 else k, teacher.data_ptr(), teacher_stride if rows > 1 else k, k,
          float(tau), wp, loss.data_ptr(), gp, gs, work.data_ptr() if n else 0, n)
     return loss, grad
 
@@ -296,9 +305,9 @@ def linear_i8(device, x, w, w_scale, bias=None, out_dtype=None):
     131072."""
     if torch is None:
         _setup()
-    x = _matrix("x", x, _FLOATS)
+    x, xs = _matrix("x", x, _FLOATS)
     rows, k = x.shape
-    w = _matrix("w", w, _INT8, None, k)
+    w, ws = _matrix("w", w, _INT8, None, k)
     q = w.shape[0]
     if k == 0 or q == 0:
         _refuse("w must have at least one row and column")
@@ -315,7 +324,7 @@ def linear_i8(device, x, w, w_scale, bias=None, out_dtype=None):
     lib = load()
     n = lib.thrml_linear_i8_work(device.handle, rows, k, q)
     work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
-    _run(device, lib.thrml_linear_i8, x.data_ptr(), _TYPES[x.dtype], rows, k, x.stride(0) if rows > 1 else k,
-         w.data_ptr(), q, w.stride(0) if q > 1 else k, w_scale.data_ptr(), bias.data_ptr() if bias is not None else 0,
+    _run(device, lib.thrml_linear_i8, x.data_ptr(), _TYPES[x.dtype], rows, k, xs if rows > 1 else k,
+         w.data_ptr(), q, ws if q > 1 else k, w_scale.data_ptr(), bias.data_ptr() if bias is not None else 0,
          y.data_ptr(), code, q, work.data_ptr() if n else 0, n)
     return y
