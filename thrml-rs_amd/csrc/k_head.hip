@@ -735,8 +735,8 @@ struct Sampler {
 // 60 us with histories of 3000 entries on average.  The difference is a row's own: the
 // table is filled before the pass over it begins, and the 2 % of categories that it names
 // are fetched again one by one, with half a kilobyte of cache lines for 8 of them.  One
-// instance does it all, at 128 registers, with 3 to 8 of them and about 110 scalars spilled
-// (32 to 64 bytes of scratch a lane).
+// instance does it all, at 128 registers, with up to 6 of them and about 110 scalars spilled
+// (32 or 48 bytes of scratch a lane).
 template <class T>
 struct SampleGroup {
   Raw8<T> z;
@@ -865,7 +865,7 @@ __global__ __launch_bounds__(BLOCK, 4) void sample_kernel(LogitRows a, const flo
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             if (!(m[j] >> (c[j] % 8u) & 1u)) live &= ~(1u << j);
-            y[j] = p.theta.fine() ? penalised<false>((float)zc[j], n[j], p) : penalised<true>((float)zc[j], n[j], p);
+            y[j] = penalised<true>((float)zc[j], n[j], p);
             if (n[j] & T_BIAS) y[j] = y[j] + bias_of(named.bias_keys, named.bias_vals, plan.hash, c[j] - c0);
           }
           s.scores(y, r, live, v);
