@@ -546,6 +546,47 @@ int thrml_linear_i8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uin
                     const int8_t *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,
                     void *y, int out_dtype, int64_t y_stride, void *work, uint64_t work_bytes);
 
+/* ---- operators of a learned head's hidden block; no counterpart in the reference
+ * The conventions are those of the operators around a learned head.
+ *
+ * thrml_gated: rows of k features and the two weights [n][k] of a gated block, all
+ * bf16 or f16 (one type), with
+ *   z = x w_gate^T,  u = x w_up^T,  h = act(z) u
+ * act: THRML_ACT_SILU z / (1 + e^-z), THRML_ACT_GELU z (1 + erf(z / sqrt 2)) / 2 or
+ * THRML_ACT_RELU max(z, 0).  Sums are f32.  k and n are at most 2^20. */
+#define THRML_ACT_SILU 0
+#define THRML_ACT_GELU 1
+#define THRML_ACT_RELU 2
+typedef struct {
+  const void *x;
+  int32_t dtype; /* THRML_DTYPE_BF16 or _F16 */
+  int32_t act;
+  uint64_t rows;
+  uint32_t k;
+  uint32_t n;
+  int64_t x_stride;
+  const void *w_gate;
+  int64_t gate_stride;
+  const void *w_up;
+  int64_t up_stride;
+} thrml_gated;
+/* h[row][c] rounded once to the type; gate and up, both or neither NULL, receive z and
+ * u, [rows][n] contiguous, for thrml_gated_backward.  work: thrml_gated_work(in, 0)
+ * bytes.  The operands are read as they lie where their rows are whole 16-byte pieces
+ * (k a multiple of 8, pointers of 16 bytes, strides of 8 elements, those of the two
+ * weights alike), else from a copy in work. */
+uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward);
+int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, void *gate,
+                        void *up, void *work, uint64_t work_bytes);
+/* From grad = d loss / d h [rows][n] and the z and u that the forward call kept:
+ *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
+ *   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x
+ * dx [rows][k] in rows of dx_stride (NULL: not computed), dw_gate and dw_up [n][k]
+ * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes. */
+int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
+                         const void *gate, const void *up, void *dx, int64_t dx_stride, void *dw_gate,
+                         void *dw_up, void *work, uint64_t work_bytes);
+
 /* ---- self-check; no counterpart in the reference ---------------------------
  * Worst-case errors of the hardware-math fast paths of the sweep kernels,
  * which their exact decisions rely on (host output, 3 floats):

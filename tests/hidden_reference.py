@@ -1,0 +1,78 @@
+"""The operators of a learned head's hidden block from their definitions in 64 bits, on
+the CPU or the device, with bounds of the error that 32-bit sums and the documented
+roundings allow.  Nothing here is the library's."""
+import math
+
+import torch
+
+U32 = 2.0**-24  # half a step of f32, relative
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """half the distance of the smallest values"""
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def act(z, name):
+    """(act(z), act'(z))"""
+    if name == "relu":
+        return z.clamp(min=0.0), (z > 0).double()
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * torch.sigmoid(-z)
+    phi = 0.5 * torch.erfc(-z * math.sqrt(0.5))
+    return z * phi, phi + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+
+
+STEEPEST = 1.13  # of the activations (gelu at sqrt 2: 1.129)
+
+
+def gated(x, wg, wu, name):
+    """{h, gate, up} and the error allowed for each: a sum of k products in f32 is off by at
+    most k u sum |terms|, the activation by 8 u of its value or, where that is small, of
+    its argument's (its exponential or error function by a few steps)."""
+    dtype, k = x.dtype, x.shape[1]
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    z, u = torch.mm(x, wg.t().contiguous()), torch.mm(x, wu.t().contiguous())
+    ez, eu = (k * U32 * torch.mm(x.abs(), w.abs().t().contiguous()) for w in (wg, wu))
+    a, _ = act(z, name)
+    h = a * u
+    eh = STEEPEST * ez * (u.abs() + eu) + (a.abs() + STEEPEST * ez) * eu + 16 * U32 * z.abs() * u.abs()
+    out = {}
+    for n, v, e in (("h", h, eh), ("gate", z, ez), ("up", u, eu)):
+        out[n] = v, e + half_step(dtype) * (v.abs() + e) + tiny(dtype)
+    return out
+
+
+def gated_grad(dh, x, wg, wu, z, u, name):
+    """{dx, dw_gate, dw_up} and the error allowed for each, from the kept z and u: dz and du
+    are rounded to the type (and computed in f32: 16 u of the factors), the sums are in f32."""
+    dtype = x.dtype
+    dh, x, wg, wu, z, u = (t.double() for t in (dh, x, wg, wu, z, u))
+    a, slope = act(z, name)
+    dz, du = dh * u * slope, dh * a
+    ez = 16 * U32 * (dh * u).abs() * (1 + z.abs())
+    eu = 16 * U32 * (dh * z).abs()
+    ez, eu = (e + half_step(dtype) * (v.abs() + e) + tiny(dtype) for e, v in ((ez, dz), (eu, du)))
+    terms = 2 * wg.shape[0]
+    dx = torch.mm(dz, wg) + torch.mm(du, wu)
+    ex = torch.mm(ez, wg.abs()) + torch.mm(eu, wu.abs())
+    ex = ex + terms * U32 * (torch.mm(dz.abs() + ez, wg.abs()) + torch.mm(du.abs() + eu, wu.abs()))
+    out = {"dx": (dx, ex)}
+    rows = x.shape[0]
+    for n, d, e in (("dw_gate", dz, ez), ("dw_up", du, eu)):
+        dt, et = d.t().contiguous(), e.t().contiguous()
+        out[n] = torch.mm(dt, x), torch.mm(et, x.abs()) + rows * U32 * torch.mm(dt.abs() + et, x.abs())
+    return {n: (v, e + half_step(dtype) * (v.abs() + e) + tiny(dtype)) for n, (v, e) in out.items()}
+
+
+def close(got, want, bound, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} off, the worst by "
+                           f"{float((err / bound).nan_to_num(1e30).max()):.3g} times what is allowed, first at "
+                           f"{bad.nonzero()[0].tolist()}")

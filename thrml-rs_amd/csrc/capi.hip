@@ -2233,6 +2233,65 @@ extern "C" int thrml_linear_i8(thrml_ctx *ctx, const void *x, int dtype, uint64_
   return launch_linear_i8(ctx, a, dtype, out_dtype, work);
 }
 
+// ---------------------------------------------------------------------------
+// Operators of a learned head's hidden block
+namespace {
+
+constexpr uint32_t GATED_MAX = 1u << 20;  // features and units: a tile's rows lie within 32 bits
+
+int check_gated(const thrml_gated *in) {
+  if (in->dtype != THRML_DTYPE_BF16 && in->dtype != THRML_DTYPE_F16)
+    return fail(THRML_EINVAL, "x and the weights must be bf16 or f16");
+  if (in->act != THRML_ACT_SILU && in->act != THRML_ACT_GELU && in->act != THRML_ACT_RELU)
+    return fail(THRML_EINVAL, "unknown activation");
+  if (in->k == 0 || in->n == 0) return fail(THRML_EINVAL, "k and n must be positive");
+  if (in->k > GATED_MAX || in->n > GATED_MAX) return fail(THRML_EUNSUPPORTED, "k and n are at most 2^20");
+  if (in->rows > HEAD_MAX_ROWS) return fail(THRML_EUNSUPPORTED, "at most 2^30 rows");
+  if (int rc = check_rows("x", in->x, 2, in->rows, in->k, in->x_stride, false)) return rc;
+  if (int rc = check_rows("w_gate", in->w_gate, 2, in->n, in->k, in->gate_stride, false)) return rc;
+  return check_rows("w_up", in->w_up, 2, in->n, in->k, in->up_stride, false);
+}
+
+}  // namespace
+
+extern "C" uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward) {
+  return ctx && in && in->rows && in->k && in->n && in->rows <= HEAD_MAX_ROWS && in->k <= GATED_MAX && in->n <= GATED_MAX
+             ? gated_work(ctx, *in, backward != 0)
+             : 0;
+}
+
+extern "C" int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, void *gate,
+                                   void *up, void *work, uint64_t work_bytes) {
+  if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
+  if (int rc = check_gated(in)) return rc;
+  if (int rc = check_rows("h", h, 2, in->rows, in->n, h_stride, true)) return rc;
+  if (in->rows && !gate != !up) return fail(THRML_EINVAL, "gate and up go together");
+  if (gate) {
+    if (int rc = check_rows("gate", gate, 2, in->rows, in->n, in->n, true)) return rc;
+    if (int rc = check_rows("up", up, 2, in->rows, in->n, in->n, true)) return rc;
+  }
+  if (int rc = check_work(work, work_bytes, thrml_gated_work(ctx, in, 0))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  return launch_gated(ctx, *in, h, h_stride, gate, up, work);
+}
+
+extern "C" int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
+                                    const void *gate, const void *up, void *dx, int64_t dx_stride, void *dw_gate,
+                                    void *dw_up, void *work, uint64_t work_bytes) {
+  if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
+  if (int rc = check_gated(in)) return rc;
+  if (int rc = check_rows("grad", grad, 2, in->rows, in->n, grad_stride, false)) return rc;
+  if (int rc = check_rows("gate", gate, 2, in->rows, in->n, in->n, false)) return rc;
+  if (int rc = check_rows("up", up, 2, in->rows, in->n, in->n, false)) return rc;
+  if (dx)
+    if (int rc = check_rows("dx", dx, 2, in->rows, in->k, dx_stride, true)) return rc;
+  if (int rc = check_rows("dw_gate", dw_gate, 2, in->n, in->k, in->k, true)) return rc;
+  if (int rc = check_rows("dw_up", dw_up, 2, in->n, in->k, in->k, true)) return rc;
+  if (int rc = check_work(work, work_bytes, thrml_gated_work(ctx, in, 1))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  return launch_gated_grad(ctx, *in, grad, grad_stride, gate, up, dx, dx_stride, dw_gate, dw_up, work);
+}
+
 extern "C" int thrml_fast_math_check(thrml_ctx *ctx, float *out) {
   if (!ctx || !out) return fail(THRML_EINVAL, "NULL argument");
   THRML_HIP(hipSetDevice(ctx->device));

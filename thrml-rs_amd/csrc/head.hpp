@@ -77,6 +77,10 @@ uint64_t distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q);
 int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work);
 uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
 int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work);
+uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward);
+int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, void *gate, void *up, void *work);
+int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const void *gate,
+                      const void *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work);
 
 // ---------------------------------------------------------------------------
 // Device helpers

@@ -1,0 +1,585 @@
+// k_gated.hip -- the hidden block of a learned head: h = act(z) u with z = x w_gate^T,
+// u = x w_up^T, and its gradient,
+//   dz = dh u act'(z), du = dh act(z)
+//   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x.
+//
+// Operands are 16-bit, sums f32, on v_mfma_f32_32x32x16.  Forward is one product with a
+// fused end: a tile has the same channels of both weights.  Backward is one pass that
+// writes dz and du, rounded to 16 bits as operands of the two products behind it have to
+// be (half a step of 2^-8 or 2^-11, as is every operand), and those products, whose
+// operands lie across the reduction and are transposed on their way from LDS.
+// z and u are kept between the two in 16 bits: recomputing them in f32 would cost half
+// of the backward pass again.
+#include "tile.hpp"
+
+namespace thrml {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <class T>
+struct Frag;
+template <>
+struct Frag<bf16_t> {
+  typedef bf16x8 type;
+  __device__ static __forceinline__ f32x16 mul(type a, type b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Frag<f16_t> {
+  typedef f16x8 type;
+  __device__ static __forceinline__ f32x16 mul(type a, type b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+// ---------------------------------------------------------------------------
+// The activation and its derivative
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == THRML_ACT_RELU) return z < 0.0f ? 0.0f : z;  // (NaN stays)
+  if constexpr (ACT == THRML_ACT_SILU) return z / (1.0f + expf(-z));
+  return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+}
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float &value, float &slope) {
+  if constexpr (ACT == THRML_ACT_RELU) {
+    value = z < 0.0f ? 0.0f : z;
+    slope = z > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == THRML_ACT_SILU) {
+    const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
+    const float sig = z < 0.0f ? e * r : r, other = z < 0.0f ? r : e * r;  // sig and 1 - sig
+    value = z * sig;
+    slope = sig * (1.0f + z * other);
+  } else {
+    const float cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
+    value = z * cdf;
+    slope = cdf + z * expf(-0.5f * z * z) * 0.39894228f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The products
+enum { G_FORWARD = 0, G_INPUT = 1, G_WEIGHT = 2 };  // h; dx; dw_gate and dw_up
+
+struct GatedTiles {
+  const void *a0, *a1;  // G_FORWARD, G_INPUT: w_gate, w_up; G_WEIGHT: x
+  const void *b;        // G_FORWARD: x; else dz and du, a row's du behind its dz
+  uint64_t a_stride, b_stride;  // bytes
+  uint64_t rows;        // of x
+  uint32_t k, n;
+  uint32_t np;          // columns from a row's dz to its du
+  uint32_t ta, tb;      // tiles
+  uint32_t splits, steps;  // of the reduction; stages in all
+  // G_FORWARD: h and, unless null, z and u; G_INPUT: dx; G_WEIGHT: dw_gate and dw_up
+  void *out, *out1, *out2;
+  int64_t out_stride;   // elements
+  float *part;          // sums of the splits, [split][row][column], in place of the above
+};
+
+template <class S, int OP, class T, int ACT, bool PART>
+__global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
+  constexpr bool A_CROSS = OP != G_FORWARD, B_CROSS = OP == G_WEIGHT;
+  constexpr uint32_t HALF = OP == G_FORWARD ? S::NA / 2 : S::NA;  // channels of a tile
+  constexpr int TA = S::MA / 32, TB = S::MB / 32, SLICES = 4 / S::WK;
+  constexpr uint32_t STAGE = (S::NA + S::NB) * 128u;
+  typedef typename Frag<T>::type V;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const uint32_t tid = threadIdx.x, l = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid / 64u);
+  const uint32_t lo = l & 31u, hi = l >> 5;
+  const uint32_t wk = wave / (S::WA * S::WB), wa = wave % (S::WA * S::WB) / S::WB, wb = wave % S::WB;
+  uint32_t ia, ib;
+  tile_place(blockIdx.x, gridDim.x, g.ta, g.tb, ia, ib);
+  const uint32_t c0 = ia * HALF;
+  // G_WEIGHT: the tiles of dw_up's rows come behind those of dw_gate's
+  const uint32_t up = OP == G_WEIGHT && ib >= g.tb / 2u ? 1u : 0u;
+  const uint64_t r0 = (uint64_t)(ib - up * (g.tb / 2u)) * S::NB;
+  const uint32_t s0 = (uint32_t)((uint64_t)g.steps * blockIdx.y / g.splits);
+  const uint32_t s1 = (uint32_t)((uint64_t)g.steps * (blockIdx.y + 1u) / g.splits);
+
+  Side<S, S::NA, A_CROSS> sa;
+  Side<S, S::NB, B_CROSS> sb;
+  // the block of 32 rows of side A is one wave's and one weight's
+  auto is_up = [&](uint32_t r) { return OP == G_FORWARD && r % S::MA >= S::MA / 2u; };
+  sa.init((uint32_t)g.a_stride, [&](uint32_t r) -> uint32_t {
+    if (OP == G_FORWARD) {
+      const uint32_t c = r / S::MA * (S::MA / 2u) + r % (S::MA / 2u);
+      return min(c, g.n - 1u - c0);
+    }
+    return c0 + r < ((g.k + 7u) & ~7u) ? r : 0u;  // 8 columns of w or x
+  });
+  sb.init((uint32_t)g.b_stride, [&](uint32_t r) -> uint32_t {
+    if (OP == G_WEIGHT) return r0 + r < g.np ? r : 0u;  // 8 columns of dz or du
+    return (uint32_t)min((uint64_t)r, g.rows - 1u - r0);
+  });
+  const uint32_t half_steps = g.steps / 2u;  // G_INPUT: the stages of w_gate
+  const uint8_t *a0 = reinterpret_cast<const uint8_t *>(g.a0), *a1 = reinterpret_cast<const uint8_t *>(g.a1);
+  const uint8_t *b0 = reinterpret_cast<const uint8_t *>(g.b);
+  if (OP == G_FORWARD) {
+    a0 += (uint64_t)c0 * g.a_stride;
+    a1 += (uint64_t)c0 * g.a_stride;
+  } else {
+    a0 += (uint64_t)c0 * 2u;
+    a1 += (uint64_t)c0 * 2u;
+  }
+  b0 += OP == G_WEIGHT ? (r0 + (uint64_t)up * g.np) * 2u : r0 * g.b_stride;
+  const uint32_t lds0 = lds_address(lds);
+  auto fetch = [&](uint32_t s, uint32_t buffer) {
+    const uint32_t to = lds0 + buffer * STAGE + wave * 1024u, to_b = to + S::NA * 128u;
+    // what is left of the reduction: bytes of a row, or rows
+    const uint32_t sa_step = OP == G_INPUT && s >= half_steps ? s - half_steps : s;
+    const uint64_t left = OP == G_FORWARD ? (uint64_t)g.k * 2u - (uint64_t)s * 128u
+                          : OP == G_INPUT ? (uint64_t)g.n - (uint64_t)sa_step * 64u
+                                          : g.rows - (uint64_t)s * 64u;
+    const uint8_t *seg = OP == G_INPUT && s >= half_steps ? a1 : a0;
+    const uint64_t ao = A_CROSS ? (uint64_t)sa_step * 64u * g.a_stride : (uint64_t)s * 128u;
+    const uint64_t bo = B_CROSS ? (uint64_t)s * 64u * g.b_stride : (uint64_t)s * 128u;
+    auto a_base = [&](int p) -> const void * {
+      // (a wave's 8 rows of a piece are one weight's)
+      if (OP == G_FORWARD) return (is_up(((uint32_t)p * S::THREADS + wave * 64u) / 8u) ? a1 : a0) + ao;
+      return seg + ao;
+    };
+    auto b_base = [&](int) -> const void * { return b0 + bo; };
+    const bool whole = left >= (OP == G_FORWARD ? 128u : 64u);
+    if (whole) {
+      sa.fetch(a_base, to);
+      sb.fetch(b_base, to_b);
+    } else {
+      sa.fetch_end(a_base, to, (uint32_t)left);
+      if (OP == G_INPUT)
+        sb.fetch(b_base, to_b);  // (dz and du have zeros behind their ends)
+      else
+        sb.fetch_end(b_base, to_b, (uint32_t)left);
+    }
+  };
+
+  V va[SLICES][TA], vb[SLICES][TB];
+  f32x16 acc[TA][TB] = {};
+  // 8 reduction indices of a slice of 16 (the lane's half of it) for 32 rows of a side
+  auto take = [&](uint32_t base, uint32_t row, uint32_t ks) -> V {
+    return *reinterpret_cast<const V *>(lds + base + row * 128u + lo * 128u + (((2u * ks + hi) ^ (lo >> 1 & 7u)) * 16u));
+  };
+  auto take_cross = [&](uint32_t base, uint32_t pitch, uint32_t chunks, uint32_t chunk, uint32_t ks) -> V {
+    const uint32_t q = (l & 15u) / 4u, turn = chunks >= 4 ? q : chunks == 2 ? q >> 1 : 0u;
+    const uint32_t at = base + (16u * ks + 8u * hi + q) * pitch + ((chunk ^ turn) * 64u) + (l >> 4 & 1u) * 32u + (l & 3u) * 8u;
+    typedef __attribute__((address_space(3))) s16x4 *P;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at + 4u * pitch));
+    return __builtin_bit_cast(V, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto read = [&](uint32_t buffer) {
+    const uint32_t base = buffer * STAGE, base_b = base + S::NA * 128u;
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k) {
+      const uint32_t ks = wk * SLICES + k;
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+        va[k][i] = A_CROSS ? take_cross(base, S::NA * 2u, S::NA / 32, wa * TA + i, ks) : take(base, wa * S::MA + 32u * i, ks);
+#pragma unroll
+      for (int j = 0; j < TB; ++j)
+        vb[k][j] = B_CROSS ? take_cross(base_b, S::NB * 2u, S::NB / 32, wb * TB + j, ks) : take(base_b, wb * S::MB + 32u * j, ks);
+    }
+  };
+  auto multiply = [&]() {
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k)
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int j = 0; j < TB; ++j) acc[i][j] = Frag<T>::mul(va[k][i], vb[k][j], acc[i][j]);
+  };
+  tile_loop<S, S::PA + S::PB>(s0, s1, fetch, read, multiply);
+
+  // The end: a wave turns 32 rows x MA columns at a time through its part of LDS, so that
+  // 8 neighbouring columns come to a lane (rows are padded by 16 bytes: 16 lanes that write
+  // together fall on all banks).
+  constexpr uint32_t PITCH = S::MA + 4, LPR = HALF / S::WA / 8u, RPI = 64u / LPR;  // floats; lanes per row, rows at a time
+  constexpr uint32_t PARTS = S::WA * S::WB;
+  float *mine = reinterpret_cast<float *>(lds) + (wave % PARTS) * 32u * PITCH;
+  T *out = reinterpret_cast<T *>(up ? g.out1 : g.out);
+  const uint64_t limit = OP == G_WEIGHT ? g.n : g.rows;  // rows of the output
+  const uint32_t cols = OP == G_FORWARD ? g.n : g.k;
+  const uint32_t cl = (l % LPR) * 8u, c = c0 + wa * (HALF / S::WA) + cl;
+#pragma unroll
+  for (int j = 0; j < TB; ++j) {
+    // (the waves that share a tile add their sums one after another)
+    for (int turn = 0; turn < S::WK; ++turn) {
+      if (S::WK == 1 || wk == (uint32_t)turn) {
+#pragma unroll
+        for (int i = 0; i < TA; ++i)
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            f32x4 *p = reinterpret_cast<f32x4 *>(mine + lo * PITCH + 32u * i + 8u * q + 4u * hi);
+            f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            if (turn) v += *p;
+            *p = v;
+          }
+      }
+      if (S::WK > 1) __syncthreads();
+    }
+    __builtin_amdgcn_wave_barrier();
+    wait_reads();
+    if (S::WK == 1 || wk == 0) {
+#pragma unroll
+      for (uint32_t t = 0; t < 32u / RPI; ++t) {
+        const uint32_t rl = t * RPI + l / LPR;
+        const uint64_t row = r0 + wb * S::MB + 32u * j + rl;
+        if (row >= limit || c >= cols) continue;
+        const uint32_t m = cols - c;
+        float v[8], w[8];
+        const float *at = mine + rl * PITCH + cl;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = at[e];
+          if (OP == G_FORWARD) w[e] = at[S::MA / 2 + e];
+        }
+        if constexpr (PART) {
+          const uint64_t all = OP == G_WEIGHT ? 2ull * g.n : g.rows, vr = row + (uint64_t)up * g.n;
+          float *to = g.part + ((uint64_t)blockIdx.y * all + vr) * (OP == G_FORWARD ? 2ull * g.n : g.k) + c;
+          store8(to, m, v);
+          if (OP == G_FORWARD) store8(to + g.n, m, w);
+        } else if constexpr (OP == G_FORWARD) {
+          const int64_t saved = (int64_t)row * g.n + c;
+          if (g.out1) {
+            store8(reinterpret_cast<T *>(g.out1) + saved, m, v);
+            store8(reinterpret_cast<T *>(g.out2) + saved, m, w);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
+          store8(out + (int64_t)row * g.out_stride + c, m, v);
+        } else {
+          store8(out + (int64_t)row * g.out_stride + c, m, v);
+        }
+      }
+    }
+    if (S::WK > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_wave_barrier();
+    wait_reads();
+  }
+}
+
+// The sums of the splits, added in their order.
+template <int OP, class T, int ACT>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
+  const uint32_t cols = OP == G_FORWARD ? g.n : g.k, groups = (cols + 7u) / 8u;
+  const uint64_t rows = OP == G_WEIGHT ? 2ull * g.n : g.rows, pitch = OP == G_FORWARD ? 2ull * g.n : g.k;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t row = i / groups;
+    const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = cols - c;
+    float v[8] = {}, w[8] = {};
+    for (uint32_t s = 0; s < g.splits; ++s) {
+      const float *p = g.part + (s * rows + row) * pitch + c;
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e)
+        if (e < m) {
+          v[e] += p[e];
+          if (OP == G_FORWARD) w[e] += p[g.n + e];
+        }
+    }
+    if constexpr (OP == G_FORWARD) {
+      const int64_t saved = (int64_t)row * g.n + c;
+      if (g.out1) {
+        store8(reinterpret_cast<T *>(g.out1) + saved, m, v);
+        store8(reinterpret_cast<T *>(g.out2) + saved, m, w);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
+      store8(reinterpret_cast<T *>(g.out) + (int64_t)row * g.out_stride + c, m, v);
+    } else if constexpr (OP == G_INPUT) {
+      store8(reinterpret_cast<T *>(g.out) + (int64_t)row * g.out_stride + c, m, v);
+    } else {
+      T *out = reinterpret_cast<T *>(row < g.n ? g.out : g.out1);
+      store8(out + (int64_t)(row < g.n ? row : row - g.n) * g.out_stride + c, m, v);
+    }
+  }
+}
+
+// dz and du from dh and the z and u that the forward pass kept: rows of 2 np elements,
+// zeros behind the n of each half.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ grad, int64_t grad_stride,
+                                                          const T *__restrict__ z, const T *__restrict__ u, uint64_t rows,
+                                                          uint32_t n, uint32_t np, T *__restrict__ d) {
+  const uint32_t groups = np / 8u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t row = i / groups;
+    const uint32_t c = (uint32_t)(i - row * groups) * 8u;
+    float a[8], b[8];
+    if (c < n) {
+      Raw8<T> rg, rz, ru;
+      const T *pg = grad + (int64_t)row * grad_stride + c, *pz = z + row * n + c, *pu = u + row * n + c;
+      if (c + 8u <= n) {
+        load8(pg, rg);
+        load8(pz, rz);
+        load8(pu, ru);
+      } else {
+        load8_part(pg, n - c, rg);
+        load8_part(pz, n - c, rz);
+        load8_part(pu, n - c, ru);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float value_, slope;
+        act_both<ACT>(value(rz, e), value_, slope);
+        const float dh = value(rg, e);
+        // (behind the end: zeros)
+        a[e] = c + e < n ? dh * value(ru, e) * slope : 0.0f;
+        b[e] = c + e < n ? dh * value_ : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.0f;
+    }
+    T *o = d + row * 2u * np + c;
+    store8(o, 8, a);
+    store8(o + np, 8, b);
+  }
+}
+
+// Rows of k elements to rows of kp, zeros behind k.
+__global__ __launch_bounds__(256) void gated_pack_kernel(const uint16_t *__restrict__ x, int64_t stride, uint64_t rows, uint32_t k,
+                                                         uint32_t kp, uint16_t *__restrict__ out) {
+  const uint32_t groups = kp / 8u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t row = i / groups;
+    const uint32_t c = (uint32_t)(i - row * groups) * 8u;
+    const f16_t *p = reinterpret_cast<const f16_t *>(x) + (int64_t)row * stride + c;
+    Raw8<f16_t> r;
+    if (c + 8u <= k)
+      load8(p, r);
+    else
+      load8_part(p, k - c, r);
+    *reinterpret_cast<u32x4 *>(out + row * kp + c) = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+  }
+}
+
+// n 16-bit zeros to each of a and b
+__global__ __launch_bounds__(256) void gated_zero_kernel(uint16_t *a, uint16_t *b, uint64_t n) {
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) a[i] = b[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Calls
+static uint64_t round256(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
+static uint32_t padded(uint32_t n, uint32_t to) { return (n + to - 1u) / to * to; }
+
+// rows that tiles load as they lie: whole 16-byte pieces, and 256 rows within 32 bits
+static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) {
+  return k % 8u == 0 && reinterpret_cast<uintptr_t>(p) % 16u == 0 &&
+         (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
+}
+
+struct Kind {
+  uint32_t na, nb;
+  float alone, many;  // us a stage: a tile alone on a compute unit, and one of several
+};
+static constexpr Kind kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
+typedef TileShape<64, 32, 1, 1, 4, 6, false> Tile32;
+typedef TileShape<64, 32, 1, 2, 2, 4, false> Tile64;
+typedef TileShape<64, 64, 2, 2, 1, 3, false> Tile128;
+typedef TileShape<128, 64, 2, 4, 1, 2, true> Tile256;
+
+struct Plan {
+  int kind = 0;
+  uint32_t ta = 0, tb = 0, splits = 1, steps = 0;
+  uint64_t part = 0;  // bytes
+};
+
+// cols: of the output, counted as side A's rows; halves: side B's rows are two matrices'
+static Plan plan_tiles(const thrml_ctx *ctx, uint64_t cols, uint64_t rows, bool halves, uint32_t steps, uint64_t out_values) {
+  Plan best;
+  double best_t = 0.0;
+  for (int i = 0; i < 4; ++i) {
+    const Kind &kd = kinds[i];
+    const uint32_t ta = tile_cdiv(cols, kd.na), tb = tile_cdiv(rows, kd.nb) * (halves ? 2u : 1u);
+    const uint64_t tiles = (uint64_t)ta * tb;
+    for (uint32_t splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (steps < 8 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
+      const double one = std::max<double>(kd.alone, (double)kd.many * (double)tile_cdiv(tiles * splits, ctx->cu_count));
+      // a join reads what the splits wrote, at about 3 bytes a ps, and is a launch
+      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 5.0 + (double)out_values * 4 * 2 * splits / 3e6 : 0.0);
+      if (best_t == 0.0 || t < best_t) {
+        best_t = t;
+        best.kind = i;
+        best.ta = ta;
+        best.tb = tb;
+        best.splits = splits;
+        best.steps = steps;
+        best.part = splits > 1 ? round256(out_values * 4 * splits) : 0;
+      }
+    }
+  }
+  return best;
+}
+
+struct GatedPlan {
+  bool pack_x, pack_w;
+  uint32_t kp, np;
+  uint64_t x_bytes, w_bytes, d_bytes;  // packed x, each packed weight, dz and du
+  Plan forward, input, weight;
+  GatedPlan(const thrml_ctx *ctx, const thrml_gated &g) {
+    kp = padded(g.k, 8);
+    np = padded(g.n, 64);
+    pack_x = !tile_rows(g.x, g.x_stride, g.rows, g.k);
+    pack_w = !tile_rows(g.w_gate, g.gate_stride, g.n, g.k) || !tile_rows(g.w_up, g.up_stride, g.n, g.k) || (g.n > 1 && g.gate_stride != g.up_stride);
+    x_bytes = pack_x ? round256(g.rows * kp * 2u) : 0;
+    w_bytes = pack_w ? round256((uint64_t)g.n * kp * 2u) : 0;
+    d_bytes = round256(g.rows * 2u * np * 2u);
+    forward = plan_tiles(ctx, 2ull * g.n, g.rows, false, tile_cdiv(g.k, 64), g.rows * 2u * g.n);
+    input = plan_tiles(ctx, g.k, g.rows, false, 2u * (np / 64u), g.rows * g.k);
+    weight = plan_tiles(ctx, g.k, g.n, true, tile_cdiv(g.rows, 64), 2ull * g.n * g.k);
+  }
+};
+
+uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward) {
+  const GatedPlan p(ctx, g);
+  return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
+}
+
+static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t rows, uint32_t k, uint32_t kp, void *out) {
+  const uint64_t n = rows * (kp / 8u);
+  hipLaunchKernelGGL(gated_pack_kernel, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
+                     reinterpret_cast<const uint16_t *>(x), stride, rows, k, kp, reinterpret_cast<uint16_t *>(out));
+  THRML_HIP(hipGetLastError());
+  return THRML_OK;
+}
+
+template <class S, int OP, class T, int ACT>
+static int launch_kind(thrml_ctx *ctx, const GatedTiles &g) {
+  if ((uint64_t)g.ta * g.tb * S::THREADS >> 32) {
+    set_error("more tiles than a launch takes");
+    return THRML_EUNSUPPORTED;
+  }
+  constexpr size_t stage = (S::NA + S::NB) * 128u;
+  const size_t lds = std::max<size_t>(stage * S::STAGES, (size_t)S::WA * S::WB * 32 * (S::MA + 4) * 4);
+  auto *f = g.splits > 1 ? &gated_tile_kernel<S, OP, T, ACT, true> : &gated_tile_kernel<S, OP, T, ACT, false>;
+  if (lds > 65536)
+    THRML_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL(f, dim3(g.ta * g.tb, g.splits), dim3(S::THREADS), lds, ctx->stream, g);
+  THRML_HIP(hipGetLastError());
+  return THRML_OK;
+}
+
+template <int OP, class T, int ACT>
+static int launch_product(thrml_ctx *ctx, const Plan &p, GatedTiles g) {
+  g.ta = p.ta;
+  g.tb = p.tb;
+  g.splits = p.splits;
+  g.steps = p.steps;
+  int rc;
+  switch (p.kind) {
+    case 0: rc = launch_kind<Tile32, OP, T, ACT>(ctx, g); break;
+    case 1: rc = launch_kind<Tile64, OP, T, ACT>(ctx, g); break;
+    case 2: rc = launch_kind<Tile128, OP, T, ACT>(ctx, g); break;
+    default: rc = launch_kind<Tile256, OP, T, ACT>(ctx, g); break;
+  }
+  if (rc || p.splits == 1) return rc;
+  const uint64_t n = (OP == G_WEIGHT ? 2ull * g.n : g.rows) * tile_cdiv(OP == G_FORWARD ? g.n : g.k, 8);
+  auto *f = &gated_join_kernel<OP, T, ACT>;
+  hipLaunchKernelGGL(f, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream, g);
+  THRML_HIP(hipGetLastError());
+  return THRML_OK;
+}
+
+// f(an element, std::integral_constant of the activation)
+template <class F>
+static int with_gated(const thrml_gated &g, F &&f) {
+  auto typed = [&](auto t) {
+    if (g.act == THRML_ACT_RELU) return f(t, std::integral_constant<int, THRML_ACT_RELU>{});
+    if (g.act == THRML_ACT_GELU) return f(t, std::integral_constant<int, THRML_ACT_GELU>{});
+    return f(t, std::integral_constant<int, THRML_ACT_SILU>{});
+  };
+  return g.dtype == THRML_DTYPE_F16 ? typed(f16_t{}) : typed(bf16_t{});
+}
+
+// The operands as the tiles read them, packed into work where they have to be.
+static int operands(thrml_ctx *ctx, const thrml_gated &g, const GatedPlan &p, uint8_t *&work, GatedTiles &t, const void *&x, uint64_t &x_stride) {
+  t = GatedTiles{};
+  t.rows = g.rows;
+  t.k = g.k;
+  t.n = g.n;
+  t.np = p.np;
+  x = g.x;
+  x_stride = (uint64_t)(g.rows > 1 ? g.x_stride : p.kp) * 2u;
+  if (p.pack_x) {
+    if (int rc = launch_pack(ctx, g.x, g.x_stride, g.rows, g.k, p.kp, work)) return rc;
+    x = work;
+    x_stride = (uint64_t)p.kp * 2u;
+    work += p.x_bytes;
+  }
+  t.a0 = g.w_gate;
+  t.a1 = g.w_up;
+  t.a_stride = (uint64_t)(g.n > 1 ? g.gate_stride : p.kp) * 2u;
+  if (p.pack_w) {
+    if (int rc = launch_pack(ctx, g.w_gate, g.gate_stride, g.n, g.k, p.kp, work)) return rc;
+    if (int rc = launch_pack(ctx, g.w_up, g.up_stride, g.n, g.k, p.kp, work + p.w_bytes)) return rc;
+    t.a0 = work;
+    t.a1 = work + p.w_bytes;
+    t.a_stride = (uint64_t)p.kp * 2u;
+    work += 2 * p.w_bytes;
+  }
+  return THRML_OK;
+}
+
+int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, void *gate, void *up, void *work) {
+  if (g.rows == 0) return THRML_OK;
+  const GatedPlan p(ctx, g);
+  uint8_t *w = reinterpret_cast<uint8_t *>(work);
+  GatedTiles t;
+  const void *x;
+  uint64_t x_stride;
+  if (int rc = operands(ctx, g, p, w, t, x, x_stride)) return rc;
+  t.b = x;
+  t.b_stride = x_stride;
+  t.out = h;
+  t.out_stride = h_stride;
+  t.out1 = gate;
+  t.out2 = up;
+  t.part = reinterpret_cast<float *>(w);
+  return with_gated(g, [&](auto e, auto act) { return launch_product<G_FORWARD, decltype(e), decltype(act)::value>(ctx, p.forward, t); });
+}
+
+int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const void *gate,
+                      const void *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work) {
+  if (g.rows == 0) {
+    const uint64_t n = (uint64_t)g.n * g.k;
+    hipLaunchKernelGGL(gated_zero_kernel, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
+                       reinterpret_cast<uint16_t *>(dw_gate), reinterpret_cast<uint16_t *>(dw_up), n);
+    THRML_HIP(hipGetLastError());
+    return THRML_OK;
+  }
+  const GatedPlan p(ctx, g);
+  uint8_t *w = reinterpret_cast<uint8_t *>(work);
+  GatedTiles t;
+  const void *x;
+  uint64_t x_stride;
+  if (int rc = operands(ctx, g, p, w, t, x, x_stride)) return rc;
+  t.b = w;
+  t.b_stride = (uint64_t)p.np * 4u;
+  w += p.d_bytes;
+  t.part = reinterpret_cast<float *>(w);
+  return with_gated(g, [&](auto e, auto act) -> int {
+    typedef decltype(e) T;
+    const uint64_t n = g.rows * (p.np / 8u);
+    auto *slope = &gated_slope_kernel<T, decltype(act)::value>;
+    hipLaunchKernelGGL(slope, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
+                       reinterpret_cast<const T *>(grad), grad_stride, reinterpret_cast<const T *>(gate),
+                       reinterpret_cast<const T *>(up), g.rows, g.n, p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)));
+    THRML_HIP(hipGetLastError());
+    // (the products do not use the activation)
+    if (dx) {
+      GatedTiles i = t;
+      i.out = dx;
+      i.out_stride = dx_stride;
+      if (int rc = launch_product<G_INPUT, T, THRML_ACT_RELU>(ctx, p.input, i)) return rc;
+    }
+    GatedTiles i = t;
+    i.a0 = i.a1 = x;
+    i.a_stride = x_stride;
+    i.out = dw_gate;
+    i.out1 = dw_up;
+    i.out_stride = g.k;
+    return launch_product<G_WEIGHT, T, THRML_ACT_RELU>(ctx, p.weight, i);
+  });
+}
+
+}  // namespace thrml

@@ -18,6 +18,9 @@ DTYPE_U8 = 0
 DTYPE_F32 = 1
 DTYPE_BF16 = 2
 DTYPE_F16 = 3
+ACT_SILU = 0
+ACT_GELU = 1
+ACT_RELU = 2
 
 KIND_NAMES = {0: "lattice", 1: "csr", 2: "potts", 3: "dense", 4: "discrete"}
 
@@ -285,6 +288,13 @@ SIGNATURES = [
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int64,
       ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
       ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_uint64]),
+    ("thrml_gated_work", ctypes.c_uint64, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]),
+    ("thrml_gated_forward", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+      ctypes.c_void_p, ctypes.c_uint64]),
+    ("thrml_gated_backward", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+      ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64]),
     ("thrml_fast_math_check", ctypes.c_int, [ctypes.c_void_p, c_f32p]),
     ("thrml_fast_math_status", ctypes.c_int,
      [ctypes.c_void_p, c_f32p, ctypes.POINTER(ctypes.c_int)]),
