@@ -586,6 +586,34 @@ int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t 
 int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
                          const void *gate, const void *up, void *dx, int64_t dx_stride, void *dw_gate,
                          void *dw_up, void *work, uint64_t work_bytes);
+/* Dropout from a key: with the half words b of the ChaCha8 stream of seed_from_u64(seed)
+ * (the generator of thrml_rng_split; 32 half words in a block, the lower one of a word
+ * first), i = (first_row + row) cols + col and border = 65536 p rounded (ties to even),
+ *   y[row][col] = (residual[row][col] +) (b[i] >= border ? x[row][col] scale : 0)
+ * scale = 65536 / (65536 - border) in f32 (p rounded to border / 65536, so that the mean
+ * is kept), product and sum in f32, rounded once to the type.  A dropped unit counts as 0
+ * whatever it holds.  seed_at, unless NULL, is device memory with the seed, read when
+ * the kernel runs, in place of seed.  residual may be NULL.  y may be x or residual (with
+ * its stride).  With x the gradient in y and no residual it gives the gradient in x.
+ * (first_row + rows) cols is at most 2^37. */
+int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint64_t cols, int64_t x_stride,
+                  const void *residual, int64_t residual_stride, uint64_t seed, const int64_t *seed_at,
+                  uint64_t first_row, double p, void *y, int64_t y_stride);
+/* The product of a learned head in 8-bit floating point (e4m3, without infinities): for
+ * weights w [q][k], a byte each, with a scale for each block of 128 x 128, and rows x
+ * that are quantised for each 128 of a row,
+ *   s[row][b] = max(2^-126, max |x[row][128 b ..]| times 1 / 448)
+ *   a = x / s rounded to e4m3 (ties to even; 1 / 448, product and quotient in f32)
+ *   y[row][c] = sum over b of (sum over j of a[row][j] w[c][j]) s[row][b] w_scale[c / 128][b] + bias[c]
+ * w_scale [ceil(q / 128)][ceil(k / 128)], bias may be NULL.  Sums are f32.  For y in bf16
+ * or f16 the products of a block are added by the 8-bit matrix unit, which keeps 2^-16 of
+ * the largest; for y in f32 exactly.  A row of x with an infinity or a NaN gives NaN.
+ * work: thrml_linear_f8_work bytes, for the same arguments. */
+uint64_t thrml_linear_f8_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t k, const void *w, uint32_t q,
+                              int64_t w_stride, int out_dtype);
+int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
+                    const void *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,
+                    void *y, int out_dtype, int64_t y_stride, void *work, uint64_t work_bytes);
 
 /* ---- self-check; no counterpart in the reference ---------------------------
  * Worst-case errors of the hardware-math fast paths of the sweep kernels,

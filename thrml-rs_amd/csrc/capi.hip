@@ -2292,6 +2292,68 @@ extern "C" int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const
   return launch_gated_grad(ctx, *in, grad, grad_stride, gate, up, dx, dx_stride, dw_gate, dw_up, work);
 }
 
+extern "C" int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint64_t cols, int64_t x_stride,
+                             const void *residual, int64_t residual_stride, uint64_t seed, const int64_t *seed_at,
+                             uint64_t first_row, double p, void *y, int64_t y_stride) {
+  if (!ctx) return fail(THRML_EINVAL, "NULL argument");
+  const uint32_t size = head_type_size(dtype);
+  if (!size) return fail(THRML_EINVAL, "x must be f32, bf16 or f16");
+  if (!(p >= 0.0 && p <= 1.0)) return fail(THRML_EINVAL, "p must lie in [0, 1]");
+  constexpr uint64_t most = 1ull << 37;  // 32 half words in each of 2^32 blocks
+  if (cols && (first_row > most || rows > most || (first_row + rows) > most / cols))
+    return fail(THRML_EUNSUPPORTED, "(first_row + rows) * cols is at most 2^37");
+  if (int rc = check_rows("x", x, size, rows, cols, x_stride, false)) return rc;
+  if (residual)
+    if (int rc = check_rows("residual", residual, size, rows, cols, residual_stride, false)) return rc;
+  if (int rc = check_rows("y", y, size, rows, cols, y_stride, true)) return rc;
+  if (rows && (reinterpret_cast<uintptr_t>(seed_at) & 7u)) return fail(THRML_EINVAL, "seed_at is not aligned to 8 bytes");
+  const uint32_t border = (uint32_t)std::nearbyint(p * 65536.0);
+  const float scale = border == 65536u ? 0.0f : (float)(65536.0 / (65536.0 - border));
+  THRML_HIP(hipSetDevice(ctx->device));
+  return launch_dropout(ctx, DropoutArgs{x, residual, y, x_stride, residual_stride, y_stride, rows, cols, first_row * cols, seed,
+                                         seed_at, border, scale}, dtype);
+}
+
+namespace {
+
+constexpr uint32_t F8_MAX_K = 1u << 20;  // a tile's rows lie within 32 bits
+
+}  // namespace
+
+extern "C" uint64_t thrml_linear_f8_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t k, const void *w, uint32_t q,
+                                         int64_t w_stride, int out_dtype) {
+  if (!ctx || !rows || !k || !q || rows > HEAD_MAX_ROWS || q > HEAD_MAX_Q || k > F8_MAX_K) return 0;
+  F8Args a{};
+  a.rows = rows;
+  a.k = k;
+  a.q = q;
+  a.w = reinterpret_cast<const uint8_t *>(w);
+  a.w_stride = w_stride;
+  return linear_f8_work(ctx, a, dtype, out_dtype);
+}
+
+extern "C" int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
+                               const void *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,
+                               void *y, int out_dtype, int64_t y_stride, void *work, uint64_t work_bytes) {
+  if (!ctx) return fail(THRML_EINVAL, "NULL argument");
+  if (int rc = check_sizes(rows, q)) return rc;
+  if (k == 0) return fail(THRML_EINVAL, "k must be positive");
+  if (k > F8_MAX_K) return fail(THRML_EUNSUPPORTED, "k is at most 2^20");
+  const uint32_t size = head_type_size(dtype), out_size = head_type_size(out_dtype);
+  if (!size) return fail(THRML_EINVAL, "x must be f32, bf16 or f16");
+  if (!out_size) return fail(THRML_EINVAL, "the output must be f32, bf16 or f16");
+  if (int rc = check_rows("x", x, size, rows, k, x_stride, false)) return rc;
+  if (int rc = check_rows("w", w, 1, q, k, w_stride, false)) return rc;
+  if (rows && !w_scale) return fail(THRML_EINVAL, "w_scale is NULL");
+  if (int rc = check_vector("w_scale", w_scale)) return rc;
+  if (int rc = check_vector("bias", bias)) return rc;
+  if (int rc = check_rows("y", y, out_size, rows, q, y_stride, true)) return rc;
+  if (int rc = check_work(work, work_bytes, thrml_linear_f8_work(ctx, dtype, rows, k, w, q, w_stride, out_dtype))) return rc;
+  THRML_HIP(hipSetDevice(ctx->device));
+  const F8Args a{x, x_stride, rows, k, q, reinterpret_cast<const uint8_t *>(w), w_stride, w_scale, bias, y, y_stride};
+  return launch_linear_f8(ctx, a, dtype, out_dtype, work);
+}
+
 extern "C" int thrml_fast_math_check(thrml_ctx *ctx, float *out) {
   if (!ctx || !out) return fail(THRML_EINVAL, "NULL argument");
   THRML_HIP(hipSetDevice(ctx->device));

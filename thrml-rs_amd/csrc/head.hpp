@@ -64,6 +64,30 @@ struct LinearArgs {
   int64_t y_stride;
 };
 
+struct DropoutArgs {
+  const void *x, *residual;  // residual: null for none
+  void *y;
+  int64_t x_stride, residual_stride, y_stride;
+  uint64_t rows, cols, begin;  // begin: the half word of row 0's first unit
+  uint64_t seed;
+  const int64_t *seed_at;      // null, or where the seed is
+  uint32_t border;             // units whose half word is below it are dropped
+  float scale;
+};
+
+struct F8Args {
+  const void *x;
+  int64_t x_stride;
+  uint64_t rows;
+  uint32_t k, q;
+  const uint8_t *w;
+  int64_t w_stride;
+  const float *w_scale;  // [ceil(q / 128)][ceil(k / 128)]
+  const float *bias;
+  void *y;
+  int64_t y_stride;
+};
+
 constexpr uint32_t HEAD_MAX_HISTORY = (1u << 29) - 1;  // the counter bits of a table word
 constexpr uint32_t DISTILL_MAX_K = 4096;               // candidates kept in LDS
 constexpr uint32_t LINEAR_MAX_K = 131072;              // 127 * 128 * k stays below 2^31
@@ -77,6 +101,9 @@ uint64_t distill_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t q);
 int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work);
 uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
 int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work);
+int launch_dropout(thrml_ctx *ctx, DropoutArgs a, int dtype);
+uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype);
+int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, void *work);
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward);
 int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, void *gate, void *up, void *work);
 int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const void *gate,

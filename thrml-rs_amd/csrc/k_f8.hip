@@ -1,0 +1,383 @@
+// k_f8.hip -- the product of a learned head in 8-bit floating point (e4m3), with a scale
+// for each 128 of a row of activations and each 128 x 128 of the weights.
+//   s[r][b] = max(2^-126, max |x[r][128 b ..]| (1 / 448)),  a = x / s rounded to e4m3
+//   y[r][c] = sum_b (sum_j a[r][j] w[c][j]) s[r][b] w_scale[c / 128][b] + bias[c]
+//
+// A stage of the tiles (tile.hpp) is one block of 128, and so is one
+// v_mfma_f32_16x16x128_f8f6f4: its result times the two scales is added in f32.  The
+// weights are side A, so that a wave's 128 channels have one scale and a lane's column is
+// one row of activations with another.
+//
+// The 8-bit matrix unit keeps of the sum of a block what lies within about 2^-16 of its
+// largest product (against 64 bits, 1.5e-5 of the norm).  That is far below the rounding of
+// a result in 16 bits.  For results in f32, EXACT widens the operands to bf16, which holds
+// every e4m3 value, and uses v_mfma_f32_16x16x32_bf16 (8e-9), at half the rate.
+#include "tile.hpp"
+
+namespace thrml {
+
+typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// rows of the scales of one block, so that any tile's 256 are there
+static uint64_t scale_rows(uint64_t rows) { return ((rows + 255u) & ~(uint64_t)255u) + 64u; }
+
+// A wave quantises 512 values of a row: 16 lanes have a block.
+template <class T>
+__global__ __launch_bounds__(256) void f8_quantise_kernel(const T *__restrict__ x, int64_t x_stride, uint64_t rows, uint32_t k,
+                                                          uint32_t kp, float *__restrict__ scale, uint64_t scale_pitch,
+                                                          uint8_t *__restrict__ xq) {
+  const uint32_t l = threadIdx.x & 63u, parts = (kp + 511u) / 512u;
+  const uint64_t waves = (uint64_t)gridDim.x * 4u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 4u + threadIdx.x / 64u; i < rows * parts; i += waves) {
+    const uint64_t row = i / parts;
+    const uint32_t c = (uint32_t)(i - row * parts) * 512u + l * 8u;
+    const T *p = x + (int64_t)row * x_stride + c;
+    Raw8<T> r;
+    if (c + 8u <= k)
+      load8(p, r);
+    else
+      load8_part(p, c < k ? k - c : 0u, r);
+    float v[8], m = 0.0f;
+    int bad = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = value(r, j);
+      bad |= !(fabsf(v[j]) < INFINITY);
+      m = fmaxf(m, fabsf(v[j]));
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) {
+      m = fmaxf(m, __shfl_xor(m, s));
+      bad |= __shfl_xor(bad, s);
+    }
+    // 1 / 448 is rounded first, as a division by a number is on the device; a scale below
+    // 2^-126 would be rounded to so few bits that quotients leave e4m3's range
+    const float s = fmaxf(m * (1.0f / 448.0f), 0x1p-126f);
+    if (c < kp) {
+      uint32_t w[2] = {0, 0};
+      if (!bad) {
+        const Divisor d(s);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = d.plain ? d.fast(v[j]) : v[j] / s;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int t = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h], f[4 * h + 1], 0, false);
+          w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h + 2], f[4 * h + 3], t, true);
+        }
+      }
+      *reinterpret_cast<uint2 *>(xq + row * kp + c) = make_uint2(w[0], w[1]);
+      if ((l & 15u) == 0) scale[(uint64_t)(c / 128u) * scale_pitch + row] = bad ? __builtin_nanf("") : s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+struct F8Tiles {
+  const uint8_t *w, *x;   // x: quantised, rows of kp
+  const float *scale;     // [block][scale_pitch]
+  const float *w_scale, *bias;
+  uint64_t w_stride, scale_pitch, rows;
+  uint32_t k, kp, q;
+  uint32_t ta, tb, splits, steps;
+  void *y;
+  int64_t y_stride;
+  float *part;            // [split][row][column]
+};
+
+__device__ __forceinline__ bf16x8 widen8(uint32_t a, uint32_t b) {
+  const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+  const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false), s = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+  return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+
+// what a wave holds of 16 rows of a side: 32 reduction indices a lane
+template <bool EXACT>
+struct F8Frag {
+  i32x8 v;
+  __device__ __forceinline__ void set(u32x4 a, u32x4 b) { v = i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]}; }
+  __device__ static __forceinline__ f32x4 mul(const F8Frag &a, const F8Frag &b) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+  }
+};
+template <>
+struct F8Frag<true> {
+  bf16x8 v[4];
+  __device__ __forceinline__ void set(u32x4 a, u32x4 b) {
+    v[0] = widen8(a[0], a[1]);
+    v[1] = widen8(a[2], a[3]);
+    v[2] = widen8(b[0], b[1]);
+    v[3] = widen8(b[2], b[3]);
+  }
+  __device__ static __forceinline__ f32x4 mul(const F8Frag &a, const F8Frag &b) {
+    f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <class S, class TO, bool EXACT, bool PART>
+__global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
+  constexpr int TA = S::MA / 16, TB = S::MB / 16;
+  constexpr uint32_t SCALES = (S::NB < 64 ? 64 : S::NB), STAGE = (S::NA + S::NB) * 128u + SCALES * 4u;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const uint32_t tid = threadIdx.x, l = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid / 64u);
+  const uint32_t lo = l & 15u, hi = l >> 4, wa = wave / S::WB, wb = wave % S::WB;
+  uint32_t ia, ib;
+  tile_place(blockIdx.x, gridDim.x, g.ta, g.tb, ia, ib);
+  const uint32_t c0 = ia * S::NA;
+  const uint64_t r0 = (uint64_t)ib * S::NB;
+  const uint32_t s0 = (uint32_t)((uint64_t)g.steps * blockIdx.y / g.splits);
+  const uint32_t s1 = (uint32_t)((uint64_t)g.steps * (blockIdx.y + 1u) / g.splits);
+
+  Side<S, S::NA, false> sa;
+  Side<S, S::NB, false> sb;
+  sa.init((uint32_t)g.w_stride, [&](uint32_t r) { return min(r, g.q - 1u - c0); });
+  sb.init(g.kp, [&](uint32_t r) { return (uint32_t)min((uint64_t)r, g.rows - 1u - r0); });
+  const uint8_t *a0 = g.w + (uint64_t)c0 * g.w_stride, *b0 = g.x + r0 * g.kp;
+  const uint32_t part = wave % (SCALES / 64u) * 64u;
+  const float *sx0 = g.scale + r0 + part;
+  // the wave's block of channels (of 128: MA divides it)
+  const float *sw0 = g.w_scale + (uint64_t)(min(c0 + wa * S::MA, g.q - 1u) / 128u) * g.steps;
+  const uint32_t lds0 = lds_address(lds);
+  auto fetch = [&](uint32_t s, uint32_t buffer) {
+    const uint32_t to = lds0 + buffer * STAGE, to_a = to + wave * 1024u, to_b = to_a + S::NA * 128u;
+    const uint32_t left = g.k - s * 128u;
+    auto a_base = [&](int) -> const void * { return a0 + s * 128u; };
+    auto b_base = [&](int) -> const void * { return b0 + s * 128u; };
+    if (left >= 128u)
+      sa.fetch(a_base, to_a);
+    else
+      sa.fetch_end(a_base, to_a, left);
+    sb.fetch(b_base, to_b);  // (rows of kp, zeros behind k)
+    word_to_lds(sx0 + s * g.scale_pitch, l * 4u, to + (S::NA + S::NB) * 128u + part * 4u);
+  };
+  F8Frag<EXACT> va[TA], vb[TB];
+  float sx[TB];
+  f32x4 acc[TA][TB] = {};
+  uint32_t stage = s0;
+  auto take = [&](uint32_t base, uint32_t row, F8Frag<EXACT> &f) {
+    // (pieces hi and hi + 4 of the row: any order of the block's indices, the same on both sides)
+    const uint32_t at = base + (row + lo) * 128u + ((hi ^ (lo >> 1 & 7u)) * 16u);
+    f.set(*reinterpret_cast<const u32x4 *>(lds + at), *reinterpret_cast<const u32x4 *>(lds + (at ^ 64u)));
+  };
+  auto read = [&](uint32_t buffer) {
+    const uint32_t base = buffer * STAGE, base_b = base + S::NA * 128u, base_s = base_b + S::NB * 128u;
+    const float sw = sw0[stage++];
+#pragma unroll
+    for (int j = 0; j < TB; ++j) take(base_b, wb * S::MB + 16u * j, vb[j]);
+#pragma unroll
+    for (int j = 0; j < TB; ++j) sx[j] = *reinterpret_cast<const float *>(lds + base_s + (wb * S::MB + 16u * j + lo) * 4u) * sw;
+#pragma unroll
+    for (int i = 0; i < TA; ++i) take(base, wa * S::MA + 16u * i, va[i]);
+  };
+  // two products at a time, the results of the two before added meanwhile (the fences keep
+  // the compiler from holding more of them: operands and sums take 224 registers of a
+  // 256 x 256 tile's 256)
+  auto multiply = [&]() {
+    constexpr int G = TA % 2 ? 1 : 2, GROUPS = TA / G * TB;
+    f32x4 t[2][G];
+#pragma unroll
+    for (int n = 0; n <= GROUPS; ++n) {
+      if (n < GROUPS) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) t[n & 1][e] = F8Frag<EXACT>::mul(va[n * G % TA + e], vb[n * G / TA]);
+      }
+      if (n > 0) {
+        const int m = n - 1;
+        const float s = sx[m * G / TA];
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) acc[m * G % TA + e][m * G / TA][h] = __builtin_fmaf(t[m & 1][e][h], s, acc[m * G % TA + e][m * G / TA][h]);
+      }
+      if (S::PING) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  tile_loop<S, S::PA + S::PB + 1>(s0, s1, fetch, read, multiply);
+
+  // The end: 16 rows x MA channels at a time through LDS, 8 neighbouring channels to a lane.
+  constexpr uint32_t PITCH = S::MA + 4, LPR = S::MA / 8u;
+  float *mine = reinterpret_cast<float *>(lds) + wave * 16u * PITCH;
+#pragma unroll
+  for (int j = 0; j < TB; ++j) {
+#pragma unroll
+    for (int i = 0; i < TA; ++i) *reinterpret_cast<f32x4 *>(mine + lo * PITCH + 16u * i + 4u * hi) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();
+    wait_reads();
+#pragma unroll
+    for (uint32_t t = 0; t < (16u * LPR + 63u) / 64u; ++t) {
+      const uint32_t rl = (t * 64u + l) / LPR, cl = (t * 64u + l) % LPR * 8u, c = c0 + wa * S::MA + cl;
+      const uint64_t row = r0 + wb * S::MB + 16u * j + rl;
+      if (rl >= 16u || row >= g.rows || c >= g.q) continue;
+      const uint32_t m = g.q - c;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = mine[rl * PITCH + cl + e];
+      if constexpr (PART) {
+        store8(g.part + ((uint64_t)blockIdx.y * g.rows + row) * g.q + c, m, v);
+      } else {
+        if (g.bias) {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e)
+            if (e < m) v[e] += g.bias[c + e];
+        }
+        store8(reinterpret_cast<TO *>(g.y) + (int64_t)row * g.y_stride + c, m, v);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    wait_reads();
+  }
+}
+
+// The sums of the splits, added in their order.
+template <class TO>
+__global__ __launch_bounds__(256) void f8_join_kernel(F8Tiles g) {
+  const uint32_t groups = (g.q + 7u) / 8u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < g.rows * groups; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t row = i / groups;
+    const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = g.q - c;
+    float v[8] = {};
+    for (uint32_t s = 0; s < g.splits; ++s) {
+      const float *p = g.part + (s * g.rows + row) * g.q + c;
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e)
+        if (e < m) v[e] += p[e];
+    }
+    if (g.bias) {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e)
+        if (e < m) v[e] += g.bias[c + e];
+    }
+    store8(reinterpret_cast<TO *>(g.y) + (int64_t)row * g.y_stride + c, m, v);
+  }
+}
+
+// Weight rows of k bytes to rows of kp, zeros behind k.
+__global__ __launch_bounds__(256) void f8_pack_kernel(const uint8_t *__restrict__ w, int64_t stride, uint32_t q, uint32_t k, uint32_t kp,
+                                                      uint8_t *__restrict__ out) {
+  typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
+  const uint32_t groups = kp / 16u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < (uint64_t)q * groups; i += (uint64_t)gridDim.x * 256u) {
+    const uint64_t row = i / groups;
+    const uint32_t c = (uint32_t)(i - row * groups) * 16u;
+    const uint8_t *p = w + (int64_t)row * stride + c;
+    u32x4 v = {0, 0, 0, 0};
+    if (c + 16u <= k) {
+      v = *reinterpret_cast<const u32x4_a1 *>(p);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j)
+        if (c + j < k) v[j / 4u] |= (uint32_t)p[j] << (8u * (j & 3u));
+    }
+    *reinterpret_cast<u32x4 *>(out + row * kp + c) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Calls
+static constexpr TileKind f8_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
+static constexpr TileKind f8_exact_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.3f, 0.25f}, {128, 128, 0.8f, 0.7f}};
+typedef TileShape<16, 32, 4, 1, 1, 6, false> F8Tile32;
+typedef TileShape<32, 32, 2, 2, 1, 4, false> F8Tile64;
+typedef TileShape<64, 64, 2, 2, 1, 3, false> F8Tile128;
+typedef TileShape<128, 64, 2, 4, 1, 2, true> F8Tile256;
+
+struct F8Plan {
+  bool pack;
+  uint32_t kp;
+  uint64_t scale_bytes, x_bytes, w_bytes;
+  TilePlan tiles;
+  F8Plan(const thrml_ctx *ctx, const F8Args &a, int out_dtype) {
+    kp = (a.k + 127u) & ~127u;
+    pack = a.k % 16u != 0 || reinterpret_cast<uintptr_t>(a.w) % 16u != 0 ||
+           (a.q > 1 && (a.w_stride % 16 != 0 || a.w_stride >= (1 << 23)));
+    scale_bytes = tile_bytes(scale_rows(a.rows) * (kp / 128u) * 4u);
+    x_bytes = tile_bytes(a.rows * kp);
+    w_bytes = pack ? tile_bytes((uint64_t)a.q * kp) : 0;
+    const bool exact = out_dtype == THRML_DTYPE_F32;
+    tiles = plan_tiles(ctx, exact ? f8_exact_kinds : f8_kinds, exact ? 3 : 4, a.q, a.rows, false, kp / 128u, a.rows * a.q);
+  }
+};
+
+uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int, int out_dtype) {
+  const F8Plan p(ctx, a, out_dtype);
+  return p.scale_bytes + p.x_bytes + p.w_bytes + p.tiles.part;
+}
+
+template <class S, class TO, bool EXACT>
+static int launch_f8_kind(thrml_ctx *ctx, const F8Tiles &g) {
+  constexpr size_t stage = (S::NA + S::NB) * 128u + (S::NB < 64 ? 64 : S::NB) * 4u;
+  const size_t lds = std::max<size_t>(stage * S::STAGES, (size_t)S::WAVES * 16 * (S::MA + 4) * 4);
+  auto *f = g.splits > 1 ? &f8_tile_kernel<S, TO, EXACT, true> : &f8_tile_kernel<S, TO, EXACT, false>;
+  return launch_tiles(ctx, f, g, S::THREADS, lds);
+}
+
+int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, void *work) {
+  if (a.rows == 0) return THRML_OK;
+  const F8Plan p(ctx, a, out_dtype);
+  uint8_t *at = reinterpret_cast<uint8_t *>(work);
+  F8Tiles g{};
+  g.rows = a.rows;
+  g.k = a.k;
+  g.kp = p.kp;
+  g.q = a.q;
+  g.scale = reinterpret_cast<const float *>(at);
+  g.scale_pitch = scale_rows(a.rows);
+  at += p.scale_bytes;
+  g.x = at;
+  at += p.x_bytes;
+  const int rc = with_type(dtype, [&](auto t) -> int {
+    typedef decltype(t) T;
+    const uint64_t n = a.rows * ((p.kp + 511u) / 512u);
+    hipLaunchKernelGGL((f8_quantise_kernel<T>), dim3((uint32_t)std::min<uint64_t>((n + 3u) / 4u, 1u << 16)), dim3(256), 0, ctx->stream,
+                       reinterpret_cast<const T *>(a.x), a.x_stride, a.rows, a.k, p.kp, const_cast<float *>(g.scale), g.scale_pitch,
+                       const_cast<uint8_t *>(g.x));
+    THRML_HIP(hipGetLastError());
+    return THRML_OK;
+  });
+  if (rc) return rc;
+  g.w = a.w;
+  g.w_stride = a.q > 1 ? (uint64_t)a.w_stride : p.kp;
+  if (p.pack) {
+    const uint64_t n = (uint64_t)a.q * (p.kp / 16u);
+    hipLaunchKernelGGL(f8_pack_kernel, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
+                       a.w, a.w_stride, a.q, a.k, p.kp, at);
+    THRML_HIP(hipGetLastError());
+    g.w = at;
+    g.w_stride = p.kp;
+    at += p.w_bytes;
+  }
+  g.part = reinterpret_cast<float *>(at);
+  g.w_scale = a.w_scale;
+  g.bias = a.bias;
+  g.y = a.y;
+  g.y_stride = a.y_stride;
+  g.ta = p.tiles.ta;
+  g.tb = p.tiles.tb;
+  g.splits = p.tiles.splits;
+  g.steps = p.tiles.steps;
+  return with_type(out_dtype, [&](auto t) -> int {
+    typedef decltype(t) TO;
+    constexpr bool EXACT = sizeof(TO) == 4;
+    int rc = THRML_OK;
+    switch (p.tiles.kind) {
+      case 0: rc = launch_f8_kind<F8Tile32, TO, EXACT>(ctx, g); break;
+      case 1: rc = launch_f8_kind<F8Tile64, TO, EXACT>(ctx, g); break;
+      case 2: rc = launch_f8_kind<F8Tile128, TO, EXACT>(ctx, g); break;
+      default:
+        if constexpr (!EXACT) rc = launch_f8_kind<F8Tile256, TO, false>(ctx, g);
+        break;
+    }
+    if (rc || g.splits == 1) return rc;
+    const uint64_t n = a.rows * tile_cdiv(a.q, 8);
+    hipLaunchKernelGGL((f8_join_kernel<TO>), dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream, g);
+    THRML_HIP(hipGetLastError());
+    return THRML_OK;
+  });
+}
+
+}  // namespace thrml

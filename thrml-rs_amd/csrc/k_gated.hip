@@ -359,7 +359,6 @@ __global__ __launch_bounds__(256) void gated_zero_kernel(uint16_t *a, uint16_t *
 
 // ---------------------------------------------------------------------------
 // Calls
-static uint64_t round256(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
 static uint32_t padded(uint32_t n, uint32_t to) { return (n + to - 1u) / to * to; }
 
 // rows that tiles load as they lie: whole 16-byte pieces, and 256 rows within 32 bits
@@ -368,65 +367,28 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
          (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
 }
 
-struct Kind {
-  uint32_t na, nb;
-  float alone, many;  // us a stage: a tile alone on a compute unit, and one of several
-};
-static constexpr Kind kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
+static constexpr TileKind gated_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
 typedef TileShape<64, 32, 1, 1, 4, 6, false> Tile32;
 typedef TileShape<64, 32, 1, 2, 2, 4, false> Tile64;
 typedef TileShape<64, 64, 2, 2, 1, 3, false> Tile128;
 typedef TileShape<128, 64, 2, 4, 1, 2, true> Tile256;
 
-struct Plan {
-  int kind = 0;
-  uint32_t ta = 0, tb = 0, splits = 1, steps = 0;
-  uint64_t part = 0;  // bytes
-};
-
-// cols: of the output, counted as side A's rows; halves: side B's rows are two matrices'
-static Plan plan_tiles(const thrml_ctx *ctx, uint64_t cols, uint64_t rows, bool halves, uint32_t steps, uint64_t out_values) {
-  Plan best;
-  double best_t = 0.0;
-  for (int i = 0; i < 4; ++i) {
-    const Kind &kd = kinds[i];
-    const uint32_t ta = tile_cdiv(cols, kd.na), tb = tile_cdiv(rows, kd.nb) * (halves ? 2u : 1u);
-    const uint64_t tiles = (uint64_t)ta * tb;
-    for (uint32_t splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (steps < 8 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
-      const double one = std::max<double>(kd.alone, (double)kd.many * (double)tile_cdiv(tiles * splits, ctx->cu_count));
-      // a join reads what the splits wrote, at about 3 bytes a ps, and is a launch
-      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 5.0 + (double)out_values * 4 * 2 * splits / 3e6 : 0.0);
-      if (best_t == 0.0 || t < best_t) {
-        best_t = t;
-        best.kind = i;
-        best.ta = ta;
-        best.tb = tb;
-        best.splits = splits;
-        best.steps = steps;
-        best.part = splits > 1 ? round256(out_values * 4 * splits) : 0;
-      }
-    }
-  }
-  return best;
-}
-
 struct GatedPlan {
   bool pack_x, pack_w;
   uint32_t kp, np;
   uint64_t x_bytes, w_bytes, d_bytes;  // packed x, each packed weight, dz and du
-  Plan forward, input, weight;
+  TilePlan forward, input, weight;
   GatedPlan(const thrml_ctx *ctx, const thrml_gated &g) {
     kp = padded(g.k, 8);
     np = padded(g.n, 64);
     pack_x = !tile_rows(g.x, g.x_stride, g.rows, g.k);
     pack_w = !tile_rows(g.w_gate, g.gate_stride, g.n, g.k) || !tile_rows(g.w_up, g.up_stride, g.n, g.k) || (g.n > 1 && g.gate_stride != g.up_stride);
-    x_bytes = pack_x ? round256(g.rows * kp * 2u) : 0;
-    w_bytes = pack_w ? round256((uint64_t)g.n * kp * 2u) : 0;
-    d_bytes = round256(g.rows * 2u * np * 2u);
-    forward = plan_tiles(ctx, 2ull * g.n, g.rows, false, tile_cdiv(g.k, 64), g.rows * 2u * g.n);
-    input = plan_tiles(ctx, g.k, g.rows, false, 2u * (np / 64u), g.rows * g.k);
-    weight = plan_tiles(ctx, g.k, g.n, true, tile_cdiv(g.rows, 64), 2ull * g.n * g.k);
+    x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;
+    w_bytes = pack_w ? tile_bytes((uint64_t)g.n * kp * 2u) : 0;
+    d_bytes = tile_bytes(g.rows * 2u * np * 2u);
+    forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, tile_cdiv(g.k, 64), g.rows * 2u * g.n);
+    input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, 2u * (np / 64u), g.rows * g.k);
+    weight = plan_tiles(ctx, gated_kinds, 4, g.k, g.n, true, tile_cdiv(g.rows, 64), 2ull * g.n * g.k);
   }
 };
 
@@ -445,22 +407,14 @@ static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t r
 
 template <class S, int OP, class T, int ACT>
 static int launch_kind(thrml_ctx *ctx, const GatedTiles &g) {
-  if ((uint64_t)g.ta * g.tb * S::THREADS >> 32) {
-    set_error("more tiles than a launch takes");
-    return THRML_EUNSUPPORTED;
-  }
   constexpr size_t stage = (S::NA + S::NB) * 128u;
   const size_t lds = std::max<size_t>(stage * S::STAGES, (size_t)S::WA * S::WB * 32 * (S::MA + 4) * 4);
   auto *f = g.splits > 1 ? &gated_tile_kernel<S, OP, T, ACT, true> : &gated_tile_kernel<S, OP, T, ACT, false>;
-  if (lds > 65536)
-    THRML_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  hipLaunchKernelGGL(f, dim3(g.ta * g.tb, g.splits), dim3(S::THREADS), lds, ctx->stream, g);
-  THRML_HIP(hipGetLastError());
-  return THRML_OK;
+  return launch_tiles(ctx, f, g, S::THREADS, lds);
 }
 
 template <int OP, class T, int ACT>
-static int launch_product(thrml_ctx *ctx, const Plan &p, GatedTiles g) {
+static int launch_product(thrml_ctx *ctx, const TilePlan &p, GatedTiles g) {
   g.ta = p.ta;
   g.tb = p.tb;
   g.splits = p.splits;

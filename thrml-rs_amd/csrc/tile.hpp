@@ -182,4 +182,63 @@ __device__ __forceinline__ void tile_place(uint32_t index, uint32_t tiles, uint3
   a = j / n;
 }
 
+// ---------------------------------------------------------------------------
+// On the host: which tiles a call takes
+static inline uint64_t tile_bytes(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
+
+struct TileKind {
+  uint32_t na, nb;
+  float alone, many;  // us a stage: of a tile alone on a compute unit, and of one of several
+};
+
+struct TilePlan {
+  int kind = 0;
+  uint32_t ta = 0, tb = 0, splits = 1, steps = 0;
+  uint64_t part = 0;  // bytes of the splits' sums
+};
+
+// The kind of tile, and into how many parts the reduction goes, by an estimate of each
+// one's time: its stages, and about 6 more for beginning and end, at its time for one.
+// cols: the rows of side A; rows: those of side B, of two matrices where `halves`.
+static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, int n, uint64_t cols, uint64_t rows, bool halves,
+                                  uint32_t steps, uint64_t out_values) {
+  TilePlan best;
+  double best_t = 0.0;
+  for (int i = 0; i < n; ++i) {
+    const TileKind &kd = kinds[i];
+    const uint32_t ta = tile_cdiv(cols, kd.na), tb = tile_cdiv(rows, kd.nb) * (halves ? 2u : 1u);
+    const uint64_t tiles = (uint64_t)ta * tb;
+    for (uint32_t splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (steps < 8 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
+      const double one = std::max<double>(kd.alone, (double)kd.many * (double)tile_cdiv(tiles * splits, ctx->cu_count));
+      // a join reads what the splits wrote, 3 bytes a ps, and is a launch
+      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 5.0 + (double)out_values * 4 * 2 * splits / 3e6 : 0.0);
+      if (best_t == 0.0 || t < best_t) {
+        best_t = t;
+        best.kind = i;
+        best.ta = ta;
+        best.tb = tb;
+        best.splits = splits;
+        best.steps = steps;
+        best.part = splits > 1 ? tile_bytes(out_values * 4 * splits) : 0;
+      }
+    }
+  }
+  return best;
+}
+
+// One workgroup for each tile and split.
+template <class G>
+static int launch_tiles(thrml_ctx *ctx, void (*f)(G), const G &g, uint32_t threads, size_t lds) {
+  if ((uint64_t)g.ta * g.tb * threads >> 32) {
+    set_error("more tiles than a launch takes");
+    return THRML_EUNSUPPORTED;
+  }
+  if (lds > 65536)
+    THRML_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL(f, dim3(g.ta * g.tb, g.splits), dim3(threads), lds, ctx->stream, g);
+  THRML_HIP(hipGetLastError());
+  return THRML_OK;
+}
+
 }  // namespace thrml

@@ -45,7 +45,7 @@ __all__ = [
     "MomentAccumulatorObserver", "make_nearest_neighbor_lattice",
     "greedy_coloring", "coloring_to_blocks", "erdos_renyi", "double_grid", "param_normal", "bf16_round",
     "process_logits", "sample_logits", "distill_loss", "distill_grad", "linear_i8",
-    "gated_linear", "gated_linear_grad",
+    "gated_linear", "gated_linear_grad", "dropout", "linear_f8",
 ]
 
 
@@ -1083,4 +1083,4 @@ def param_normal(seed, n, mean, std):
 # the operators around a learned head
 from .head import distill_grad, distill_loss, linear_i8, process_logits, sample_logits  # noqa: E402
 # the operators of its hidden block
-from .hidden import gated_linear, gated_linear_grad  # noqa: E402
+from .hidden import dropout, gated_linear, gated_linear_grad, linear_f8  # noqa: E402

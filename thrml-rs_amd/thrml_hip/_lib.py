@@ -295,6 +295,17 @@ SIGNATURES = [
     ("thrml_gated_backward", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64]),
+    ("thrml_dropout", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int64,
+      ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_double,
+      ctypes.c_void_p, ctypes.c_int64]),
+    ("thrml_linear_f8_work", ctypes.c_uint64,
+     [ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint32,
+      ctypes.c_int64, ctypes.c_int]),
+    ("thrml_linear_f8", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int64,
+      ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+      ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_uint64]),
     ("thrml_fast_math_check", ctypes.c_int, [ctypes.c_void_p, c_f32p]),
     ("thrml_fast_math_status", ctypes.c_int,
      [ctypes.c_void_p, c_f32p, ctypes.POINTER(ctypes.c_int)]),

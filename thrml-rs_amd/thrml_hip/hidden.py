@@ -3,6 +3,8 @@ counterpart in the reference):
 
   gated_linear       hidden units act(x @ w_gate.T) * (x @ w_up.T)
   gated_linear_grad  the gradients of a loss in x and both weights
+  dropout            units kept or zeroed by the bits of a key
+  linear_f8          a product in 8-bit floating point with a scale for each block
 
 Streams, graphs and tensors that require a gradient are as in `head`: calls queue their
 kernels on the device's stream, in order with torch's current one, and torch's gradients
@@ -101,3 +103,89 @@ def gated_linear_grad(device, grad, x, w_gate, w_up, gate, up, activation="silu"
          up.data_ptr(), dx.data_ptr() if input_grad else 0, k, dw_gate.data_ptr(), dw_up.data_ptr(),
          work.data_ptr() if size else 0, size)
     return dx, dw_gate, dw_up
+
+
+def dropout(device, x, key, p, residual=None, first_row=0, out=None):
+    """y [rows, cols] = (residual +) x with each unit kept and scaled, or replaced by 0, by
+    the bits of a key: with the half words b of the key's ChaCha8 stream, i = (first_row +
+    row) * cols + col and border = round(65536 p), kept where b[i] >= border and times
+    65536 / (65536 - border), in float32, rounded once (p counts as border / 65536).  No
+    mask is kept: the gradient in x is dropout(device, grad, key, p, first_row=first_row).
+
+    key: an RngKey, used for nothing else, or its seed in an int64 tensor of one element
+    on the device, which is read when the kernel runs: a captured call draws other bits
+    when it changes.  first_row: where x is a part of a larger batch, its first row
+    there.  out: a tensor for the result; it may be x or residual."""
+    if head.torch is None:
+        head._setup()
+    torch = head.torch
+    x0, residual0 = x, residual
+    x, xs = _matrix("x", x, head._FLOATS)
+    rows, cols = x.shape
+    rs = rp = 0
+    if residual is not None:
+        residual, rs = _matrix("residual", residual, (x.dtype,), rows, cols)
+        rp = residual.data_ptr()
+    seed = at = 0
+    seed_at = None
+    if isinstance(key, torch.Tensor):
+        if key.dtype != torch.int64 or key.numel() != 1:
+            _refuse("key must be an RngKey or an int64 tensor of one element")
+        seed_at, at = key, key.data_ptr()
+    else:
+        seed = getattr(key, "seed", None)
+        if seed is None:
+            _refuse("key must be an RngKey or an int64 tensor of one element")
+    first_row = int(first_row)
+    if first_row < 0:
+        _refuse("first_row must not be negative")
+    if out is not None:
+        _out("out", out, rows, cols, x.dtype)
+        if (out is x0 and x is not x0) or (out is residual0 and residual is not residual0):
+            _refuse("out may be x or residual only where their rows are contiguous")
+    _on_device(device, ("x", "residual", "key", "out"), (x, residual, seed_at, out))
+    if out is None:
+        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    _run(device, load().thrml_dropout, x.data_ptr(), head._TYPES[x.dtype], rows, cols, xs if rows > 1 else cols, rp,
+         rs if rows > 1 else cols, seed, at, first_row, float(p), out.data_ptr(), out.stride(0) if rows > 1 else cols)
+    return out
+
+
+def linear_f8(device, x, w, w_scale, bias=None, out_dtype=None):
+    """y [rows, q] = x @ w.T + bias in out_dtype (default: x's) with both sides in 8-bit
+    floating point: w [q, k] float8_e4m3fn weights with a scale w_scale [ceil(q / 128),
+    ceil(k / 128)] float32 for each block of 128 x 128, x [rows, k] activations that the
+    call quantises in blocks of 128 of a row, s = max(2^-126, max |x| * (1 / 448)), a = x / s
+    rounded to e4m3 (ties to even; in float32).  A block's sum times s w_scale is added in
+    float32.  For results in 16 bits the sum within a block keeps 2^-16 of its largest
+    product, for float32 all.  A row of x with an infinity or a NaN gives NaN.
+
+    k is at most 2^20.  Weights whose rows are not whole 16-byte pieces are copied
+    first."""
+    if head.torch is None:
+        head._setup()
+    torch = head.torch
+    x, xs = _matrix("x", x, head._FLOATS)
+    rows, k = x.shape
+    w, ws = _matrix("w", w, (torch.float8_e4m3fn,), None, k)
+    q = w.shape[0]
+    if k == 0 or q == 0:
+        _refuse("w must have at least one row and column")
+    w_scale, scale_stride = _matrix("w_scale", w_scale, head._FLOAT32, (q + 127) // 128, (k + 127) // 128)
+    if scale_stride != w_scale.shape[1]:
+        w_scale = w_scale.contiguous()
+    if bias is not None:
+        bias = head._vector("bias", bias, q, head._FLOAT32)
+    dtype = out_dtype or x.dtype
+    code, in_code = head._type("out_dtype", dtype), head._TYPES[x.dtype]
+    _on_device(device, ("x", "w", "w_scale", "bias"), (x, w, w_scale, bias))
+    where = x.device
+    y = torch.empty((rows, q), dtype=dtype, device=where)
+    lib = load()
+    wp, ws = w.data_ptr(), ws if q > 1 else k
+    n = lib.thrml_linear_f8_work(device.handle, in_code, rows, k, wp, q, ws, code)
+    work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    _run(device, lib.thrml_linear_f8, x.data_ptr(), in_code, rows, k, xs if rows > 1 else k, wp, q, ws,
+         w_scale.data_ptr(), bias.data_ptr() if bias is not None else 0, y.data_ptr(), code, q,
+         work.data_ptr() if n else 0, n)
+    return y
