@@ -119,13 +119,19 @@ struct F8Frag<true> {
   }
 };
 
+// The rows' scales of a stage: floats in LDS behind the stages, loaded with side B.  With
+// PING, whose stages fill LDS, each lane keeps those of its rows, loaded a stage ahead.
+template <class S>
+constexpr uint32_t f8_scales() {
+  return S::PING ? 0 : S::NB < 64 ? 64 : S::NB;
+}
+
 template <class S, class TO, bool EXACT, bool PART>
 __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   constexpr int TA = S::MA / 16, TB = S::MB / 16;
-  constexpr uint32_t SCALES = (S::NB < 64 ? 64 : S::NB), STAGE = (S::NA + S::NB) * 128u + SCALES * 4u;
+  constexpr uint32_t SCALES = f8_scales<S>();
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const uint32_t tid = threadIdx.x, l = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid / 64u);
-  const uint32_t lo = l & 15u, hi = l >> 4, wa = wave / S::WB, wb = wave % S::WB;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), wa = wave / S::WB, wb = wave % S::WB;
   uint32_t ia, ib;
   tile_place(blockIdx.x, gridDim.x, g.ta, g.tb, ia, ib);
   const uint32_t c0 = ia * S::NA;
@@ -133,75 +139,106 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   const uint32_t s0 = (uint32_t)((uint64_t)g.steps * blockIdx.y / g.splits);
   const uint32_t s1 = (uint32_t)((uint64_t)g.steps * (blockIdx.y + 1u) / g.splits);
 
-  Side<S, S::NA, false> sa;
-  Side<S, S::NB, false> sb;
-  sa.init((uint32_t)g.w_stride, [&](uint32_t r) { return min(r, g.q - 1u - c0); });
-  sb.init(g.kp, [&](uint32_t r) { return (uint32_t)min((uint64_t)r, g.rows - 1u - r0); });
+  typedef Side<S, S::NA, false> SideA;
+  typedef Side<S, S::NB, false> SideB;
+  const SideA sa{(uint32_t)g.w_stride, g.q - 1u - c0};
+  const SideB sb{g.kp, (uint32_t)min(g.rows - 1u - r0, (uint64_t)S::NB)};
+  auto a_first = [&](int p) { return p * SideA::STEP; };
+  auto b_first = [&](int p) { return p * SideB::STEP; };
   const uint8_t *a0 = g.w + (uint64_t)c0 * g.w_stride, *b0 = g.x + r0 * g.kp;
-  const uint32_t part = wave % (SCALES / 64u) * 64u;
-  const float *sx0 = g.scale + r0 + part;
   // the wave's block of channels (of 128: MA divides it)
   const float *sw0 = g.w_scale + (uint64_t)(min(c0 + wa * S::MA, g.q - 1u) / 128u) * g.steps;
-  const uint32_t lds0 = lds_address(lds);
-  auto fetch = [&](uint32_t s, uint32_t buffer) {
-    const uint32_t to = lds0 + buffer * STAGE, to_a = to + wave * 1024u, to_b = to_a + S::NA * 128u;
+  const uint32_t lds0 = lds_address(lds) + wave % (S::LOADERS / 64u) * 1024u;
+  auto a_base = [&](uint32_t s) { return [&, s](int) { return a0 + s * 128u; }; };
+  auto b_base = [&](uint32_t s) { return [&, s](int) { return b0 + s * 128u; }; };
+  auto fetch_a = [&](uint32_t s, uint32_t slot) {
     const uint32_t left = g.k - s * 128u;
-    auto a_base = [&](int) -> const void * { return a0 + s * 128u; };
-    auto b_base = [&](int) -> const void * { return b0 + s * 128u; };
     if (left >= 128u)
-      sa.fetch(a_base, to_a);
+      sa.fetch(a_base(s), a_first, lds0 + S::a_at(slot));
     else
-      sa.fetch_end(a_base, to_a, left);
-    sb.fetch(b_base, to_b);  // (rows of kp, zeros behind k)
-    word_to_lds(sx0 + s * g.scale_pitch, l * 4u, to + (S::NA + S::NB) * 128u + part * 4u);
+      sa.fetch_end(a_base(s), a_first, lds0 + S::a_at(slot), left);
+  };
+  auto fetch_b = [&](uint32_t s, uint32_t slot) {
+    if constexpr (!S::PING) {
+      const uint32_t part = wave % (SCALES / 64u) * 64u;
+      word_to_lds(g.scale + s * g.scale_pitch + r0 + part, (here(threadIdx.x) & 63u) * 4u,
+                  lds_address(lds) + S::BYTES + (slot * SCALES + part) * 4u);
+    }
+    sb.fetch(b_base(s), b_first, lds0 + S::b_at(slot));  // (rows of kp, zeros behind k)
   };
   F8Frag<EXACT> va[TA], vb[TB];
-  float sx[TB];
+  float sx[TB], next_sx[TB], next_sw = 0.0f;
   f32x4 acc[TA][TB] = {};
   uint32_t stage = s0;
-  auto take = [&](uint32_t base, uint32_t row, F8Frag<EXACT> &f) {
+  auto take = [&](uint32_t l, uint32_t base, F8Frag<EXACT> &f) {
     // (pieces hi and hi + 4 of the row: any order of the block's indices, the same on both sides)
-    const uint32_t at = base + (row + lo) * 128u + ((hi ^ (lo >> 1 & 7u)) * 16u);
+    const uint32_t lo = l & 15u, hi = l >> 4, at = base + lo * 128u + ((hi ^ tile_turn<S>(lo)) * 16u);
     f.set(*reinterpret_cast<const u32x4 *>(lds + at), *reinterpret_cast<const u32x4 *>(lds + (at ^ 64u)));
   };
-  auto read = [&](uint32_t buffer) {
-    const uint32_t base = buffer * STAGE, base_b = base + S::NA * 128u, base_s = base_b + S::NB * 128u;
-    const float sw = sw0[stage++];
+  // PING: the scales of stage s
+  auto scales = [&](uint32_t s) {
+    const float *p = g.scale + s * g.scale_pitch + r0 + wb * S::MB;
+    const uint32_t lo = here(threadIdx.x) & 15u;
 #pragma unroll
-    for (int j = 0; j < TB; ++j) take(base_b, wb * S::MB + 16u * j, vb[j]);
-#pragma unroll
-    for (int j = 0; j < TB; ++j) sx[j] = *reinterpret_cast<const float *>(lds + base_s + (wb * S::MB + 16u * j + lo) * 4u) * sw;
-#pragma unroll
-    for (int i = 0; i < TA; ++i) take(base, wa * S::MA + 16u * i, va[i]);
+    for (int j = 0; j < TB; ++j) next_sx[j] = p[16u * j + lo];
+    next_sw = sw0[s];
   };
-  // two products at a time, the results of the two before added meanwhile (the fences keep
-  // the compiler from holding more of them: operands and sums take 224 registers of a
-  // 256 x 256 tile's 256)
+  if (S::PING) scales(s0);
+  auto read = [&](uint32_t slot_a, uint32_t slot_b) {
+    const uint32_t l = here(threadIdx.x) & 63u;
+    if (S::PING) {
+      // (before this stage's loads into LDS are begun: the compiler waits for all loads)
+#pragma unroll
+      for (int j = 0; j < TB; ++j) sx[j] = next_sx[j] * next_sw;
+      scales(min(stage + 1u, s1 - 1u));
+    } else {
+      next_sw = sw0[stage];
+#pragma unroll
+      for (int j = 0; j < TB; ++j)
+        sx[j] = *reinterpret_cast<const float *>(lds + S::BYTES + (slot_b * SCALES + wb * S::MB + 16u * j + (l & 15u)) * 4u);
+    }
+    ++stage;
+#pragma unroll
+    for (int j = 0; j < TB; ++j) take(l, S::b_at(slot_b) + (wb * S::MB + 16u * j) * 128u, vb[j]);
+#pragma unroll
+    for (int i = 0; i < TA; ++i) take(l, S::a_at(slot_a) + (wa * S::MA + 16u * i) * 128u, va[i]);
+  };
+  // A product's result is added three products later, when the matrix unit has it.  (The
+  // fences keep the compiler from other orders: it would add each result at once, with a
+  // wait, or hold more of them than the 256 registers of a 256 x 256 tile have room for
+  // beside 224 of operands and sums.)
   auto multiply = [&]() {
-    constexpr int G = TA % 2 ? 1 : 2, GROUPS = TA / G * TB;
-    f32x4 t[2][G];
+    constexpr int LAG = 3;
+    f32x4 t[LAG + 1];
+    if (!S::PING) {
 #pragma unroll
-    for (int n = 0; n <= GROUPS; ++n) {
-      if (n < GROUPS) {
+      for (int j = 0; j < TB; ++j) sx[j] *= next_sw;
+    }
 #pragma unroll
-        for (int e = 0; e < G; ++e) t[n & 1][e] = F8Frag<EXACT>::mul(va[n * G % TA + e], vb[n * G / TA]);
-      }
-      if (n > 0) {
-        const int m = n - 1;
-        const float s = sx[m * G / TA];
-#pragma unroll
-        for (int e = 0; e < G; ++e)
-#pragma unroll
-          for (int h = 0; h < 4; ++h) acc[m * G % TA + e][m * G / TA][h] = __builtin_fmaf(t[m & 1][e][h], s, acc[m * G % TA + e][m * G / TA][h]);
-      }
+    for (int n = 0; n < TA * TB + LAG; ++n) {
+      if (n < TA * TB) t[n % (LAG + 1)] = F8Frag<EXACT>::mul(va[n % TA], vb[n / TA]);
       if (S::PING) __builtin_amdgcn_sched_barrier(0);
+      if (n >= LAG) {
+        const int m = n - LAG;
+        f32x4 &to = acc[m % TA][m / TA];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = __builtin_fmaf(t[m % (LAG + 1)][e], sx[m / TA], to[e]);
+        if (S::PING) asm volatile("" : "+v"(to));
+        if (S::PING) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
-  tile_loop<S, S::PA + S::PB + 1>(s0, s1, fetch, read, multiply);
+  tile_loop<S, S::PB + (S::PING ? 0 : 1)>(s0, s1, fetch_a, fetch_b, read, multiply);
 
   // The end: 16 rows x MA channels at a time through LDS, 8 neighbouring channels to a lane.
   constexpr uint32_t PITCH = S::MA + 4, LPR = S::MA / 8u;
+  const uint32_t l = here(threadIdx.x) & 63u, lo = l & 15u, hi = l >> 4;
   float *mine = reinterpret_cast<float *>(lds) + wave * 16u * PITCH;
+  static_assert(64u % LPR == 0, "a lane's channels are the same in every row");
+  const uint32_t cl = l % LPR * 8u, c = c0 + wa * S::MA + cl, m = c < g.q ? g.q - c : 0u;
+  float bias[8];
+#pragma unroll
+  for (uint32_t e = 0; e < 8; ++e) bias[e] = !PART && g.bias && e < m ? g.bias[c + e] : 0.0f;
 #pragma unroll
   for (int j = 0; j < TB; ++j) {
 #pragma unroll
@@ -210,10 +247,9 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
     wait_reads();
 #pragma unroll
     for (uint32_t t = 0; t < (16u * LPR + 63u) / 64u; ++t) {
-      const uint32_t rl = (t * 64u + l) / LPR, cl = (t * 64u + l) % LPR * 8u, c = c0 + wa * S::MA + cl;
+      const uint32_t rl = (t * 64u + l) / LPR;
       const uint64_t row = r0 + wb * S::MB + 16u * j + rl;
-      if (rl >= 16u || row >= g.rows || c >= g.q) continue;
-      const uint32_t m = g.q - c;
+      if (rl >= 16u || row >= g.rows || m == 0) continue;
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = mine[rl * PITCH + cl + e];
@@ -222,8 +258,7 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
       } else {
         if (g.bias) {
 #pragma unroll
-          for (uint32_t e = 0; e < 8; ++e)
-            if (e < m) v[e] += g.bias[c + e];
+          for (int e = 0; e < 8; ++e) v[e] += bias[e];
         }
         store8(reinterpret_cast<TO *>(g.y) + (int64_t)row * g.y_stride + c, m, v);
       }
@@ -279,12 +314,12 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const uint8_t *__restrict_
 
 // ---------------------------------------------------------------------------
 // Calls
-static constexpr TileKind f8_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
-static constexpr TileKind f8_exact_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.3f, 0.25f}, {128, 128, 0.8f, 0.7f}};
-typedef TileShape<16, 32, 4, 1, 1, 6, false> F8Tile32;
-typedef TileShape<32, 32, 2, 2, 1, 4, false> F8Tile64;
-typedef TileShape<64, 64, 2, 2, 1, 3, false> F8Tile128;
-typedef TileShape<128, 64, 2, 4, 1, 2, true> F8Tile256;
+static constexpr TileKind f8_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.25f, 0.2f}, {128, 128, 128, 0.5f, 0.45f}, {256, 256, 128, 1.0f, 1.0f}};
+static constexpr TileKind f8_exact_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.3f, 0.25f}, {128, 128, 128, 0.8f, 0.7f}};
+typedef TileShape<16, 32, 4, 1, 1, 128, 6, false> F8Tile32;
+typedef TileShape<32, 32, 2, 2, 1, 128, 4, false> F8Tile64;
+typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> F8Tile128;
+typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> F8Tile256;
 
 struct F8Plan {
   bool pack;
@@ -299,7 +334,7 @@ struct F8Plan {
     x_bytes = tile_bytes(a.rows * kp);
     w_bytes = pack ? tile_bytes((uint64_t)a.q * kp) : 0;
     const bool exact = out_dtype == THRML_DTYPE_F32;
-    tiles = plan_tiles(ctx, exact ? f8_exact_kinds : f8_kinds, exact ? 3 : 4, a.q, a.rows, false, kp / 128u, a.rows * a.q);
+    tiles = plan_tiles(ctx, exact ? f8_exact_kinds : f8_kinds, exact ? 3 : 4, a.q, a.rows, false, kp, a.rows * a.q);
   }
 };
 
@@ -310,8 +345,7 @@ uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int, int out_dtype) {
 
 template <class S, class TO, bool EXACT>
 static int launch_f8_kind(thrml_ctx *ctx, const F8Tiles &g) {
-  constexpr size_t stage = (S::NA + S::NB) * 128u + (S::NB < 64 ? 64 : S::NB) * 4u;
-  const size_t lds = std::max<size_t>(stage * S::STAGES, (size_t)S::WAVES * 16 * (S::MA + 4) * 4);
+  const size_t lds = std::max<size_t>(S::BYTES + S::STAGES_B * f8_scales<S>() * 4, (size_t)S::WAVES * 16 * (S::MA + 4) * 4);
   auto *f = g.splits > 1 ? &f8_tile_kernel<S, TO, EXACT, true> : &f8_tile_kernel<S, TO, EXACT, false>;
   return launch_tiles(ctx, f, g, S::THREADS, lds);
 }

@@ -35,7 +35,10 @@ struct Frag<f16_t> {
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == THRML_ACT_RELU) return z < 0.0f ? 0.0f : z;  // (NaN stays)
-  if constexpr (ACT == THRML_ACT_SILU) return z / (1.0f + expf(-z));
+  // (hardware exponential and reciprocal: within |z| 2^-24 and 2^-23 of the value, where its
+  // result is rounded to 16 bits; with expf and a division the end of a tile took 17 of 200
+  // thousand cycles)
+  if constexpr (ACT == THRML_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950f));
   return 0.5f * z * (1.0f + erff(z * 0.70710678f));
 }
 template <int ACT>
@@ -78,12 +81,11 @@ template <class S, int OP, class T, int ACT, bool PART>
 __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   constexpr bool A_CROSS = OP != G_FORWARD, B_CROSS = OP == G_WEIGHT;
   constexpr uint32_t HALF = OP == G_FORWARD ? S::NA / 2 : S::NA;  // channels of a tile
-  constexpr int TA = S::MA / 32, TB = S::MB / 32, SLICES = 4 / S::WK;
-  constexpr uint32_t STAGE = (S::NA + S::NB) * 128u;
+  constexpr int TA = S::MA / 32, TB = S::MB / 32, SLICES = S::KB / 32 / S::WK;
+  constexpr uint32_t ROWS = S::KB / 2;  // reduction indices of a stage
   typedef typename Frag<T>::type V;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const uint32_t tid = threadIdx.x, l = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid / 64u);
-  const uint32_t lo = l & 31u, hi = l >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
   const uint32_t wk = wave / (S::WA * S::WB), wa = wave % (S::WA * S::WB) / S::WB, wb = wave % S::WB;
   uint32_t ia, ib;
   tile_place(blockIdx.x, gridDim.x, g.ta, g.tb, ia, ib);
@@ -94,21 +96,15 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   const uint32_t s0 = (uint32_t)((uint64_t)g.steps * blockIdx.y / g.splits);
   const uint32_t s1 = (uint32_t)((uint64_t)g.steps * (blockIdx.y + 1u) / g.splits);
 
-  Side<S, S::NA, A_CROSS> sa;
-  Side<S, S::NB, B_CROSS> sb;
-  // the block of 32 rows of side A is one wave's and one weight's
-  auto is_up = [&](uint32_t r) { return OP == G_FORWARD && r % S::MA >= S::MA / 2u; };
-  sa.init((uint32_t)g.a_stride, [&](uint32_t r) -> uint32_t {
-    if (OP == G_FORWARD) {
-      const uint32_t c = r / S::MA * (S::MA / 2u) + r % (S::MA / 2u);
-      return min(c, g.n - 1u - c0);
-    }
-    return c0 + r < ((g.k + 7u) & ~7u) ? r : 0u;  // 8 columns of w or x
-  });
-  sb.init((uint32_t)g.b_stride, [&](uint32_t r) -> uint32_t {
-    if (OP == G_WEIGHT) return r0 + r < g.np ? r : 0u;  // 8 columns of dz or du
-    return (uint32_t)min((uint64_t)r, g.rows - 1u - r0);
-  });
+  // (across, rows come in eights: k is padded to them, np is a multiple of 64)
+  typedef Side<S, S::NA, A_CROSS> SideA;
+  typedef Side<S, S::NB, B_CROSS> SideB;
+  const SideA sa{(uint32_t)g.a_stride, OP == G_FORWARD ? g.n - 1u - c0 : ((g.k + 7u) & ~7u) - 1u - c0};
+  const SideB sb{(uint32_t)g.b_stride, OP == G_WEIGHT ? (uint32_t)(g.np - 1u - r0) : (uint32_t)min(g.rows - 1u - r0, (uint64_t)S::NB)};
+  // G_FORWARD: a wave's MA rows of side A are half w_gate's, half w_up's, the same channels
+  static_assert(OP != G_FORWARD || S::MA / 2 % SideA::STEP == 0, "a piece is one weight's");
+  auto a_first = [&](int p) { return OP == G_FORWARD ? (p * SideA::STEP) / S::MA * (S::MA / 2u) + p * SideA::STEP % (S::MA / 2u) : p * SideA::STEP; };
+  auto b_first = [&](int p) { return p * SideB::STEP; };
   const uint32_t half_steps = g.steps / 2u;  // G_INPUT: the stages of w_gate
   const uint8_t *a0 = reinterpret_cast<const uint8_t *>(g.a0), *a1 = reinterpret_cast<const uint8_t *>(g.a1);
   const uint8_t *b0 = reinterpret_cast<const uint8_t *>(g.b);
@@ -120,61 +116,66 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     a1 += (uint64_t)c0 * 2u;
   }
   b0 += OP == G_WEIGHT ? (r0 + (uint64_t)up * g.np) * 2u : r0 * g.b_stride;
-  const uint32_t lds0 = lds_address(lds);
-  auto fetch = [&](uint32_t s, uint32_t buffer) {
-    const uint32_t to = lds0 + buffer * STAGE + wave * 1024u, to_b = to + S::NA * 128u;
-    // what is left of the reduction: bytes of a row, or rows
-    const uint32_t sa_step = OP == G_INPUT && s >= half_steps ? s - half_steps : s;
-    const uint64_t left = OP == G_FORWARD ? (uint64_t)g.k * 2u - (uint64_t)s * 128u
-                          : OP == G_INPUT ? (uint64_t)g.n - (uint64_t)sa_step * 64u
-                                          : g.rows - (uint64_t)s * 64u;
-    const uint8_t *seg = OP == G_INPUT && s >= half_steps ? a1 : a0;
-    const uint64_t ao = A_CROSS ? (uint64_t)sa_step * 64u * g.a_stride : (uint64_t)s * 128u;
-    const uint64_t bo = B_CROSS ? (uint64_t)s * 64u * g.b_stride : (uint64_t)s * 128u;
-    auto a_base = [&](int p) -> const void * {
-      // (a wave's 8 rows of a piece are one weight's)
-      if (OP == G_FORWARD) return (is_up(((uint32_t)p * S::THREADS + wave * 64u) / 8u) ? a1 : a0) + ao;
-      return seg + ao;
+  // G_INPUT: the stage's number among its weight's
+  auto in_half = [&](uint32_t s) { return OP == G_INPUT && s >= half_steps ? s - half_steps : s; };
+  // what is left of the reduction: bytes of a row, or indices
+  auto left = [&](uint32_t s) -> uint64_t {
+    return OP == G_FORWARD ? (uint64_t)g.k * 2u - (uint64_t)s * S::KB
+           : OP == G_INPUT ? (uint64_t)g.n - min((uint64_t)in_half(s) * ROWS, (uint64_t)g.n)
+                           : g.rows - (uint64_t)s * ROWS;
+  };
+  auto whole = [&](uint32_t s) { return left(s) >= (OP == G_FORWARD ? S::KB : ROWS); };
+  auto a_base = [&](uint32_t s) {
+    return [&, s](int p) {
+      const uint64_t at = A_CROSS ? (uint64_t)in_half(s) * ROWS * g.a_stride : (uint64_t)s * S::KB;
+      if (OP == G_FORWARD) return (p * SideA::STEP % S::MA >= S::MA / 2u ? a1 : a0) + at;
+      return (OP == G_INPUT && s >= half_steps ? a1 : a0) + at;
     };
-    auto b_base = [&](int) -> const void * { return b0 + bo; };
-    const bool whole = left >= (OP == G_FORWARD ? 128u : 64u);
-    if (whole) {
-      sa.fetch(a_base, to);
-      sb.fetch(b_base, to_b);
-    } else {
-      sa.fetch_end(a_base, to, (uint32_t)left);
-      if (OP == G_INPUT)
-        sb.fetch(b_base, to_b);  // (dz and du have zeros behind their ends)
-      else
-        sb.fetch_end(b_base, to_b, (uint32_t)left);
-    }
+  };
+  auto b_base = [&](uint32_t s) {
+    return [&, s](int) { return b0 + (B_CROSS ? (uint64_t)s * ROWS * g.b_stride : (uint64_t)s * S::KB); };
+  };
+  const uint32_t lds0 = lds_address(lds) + wave % (S::LOADERS / 64u) * 1024u;
+  auto fetch_a = [&](uint32_t s, uint32_t slot) {
+    if (whole(s))
+      sa.fetch(a_base(s), a_first, lds0 + S::a_at(slot));
+    else
+      sa.fetch_end(a_base(s), a_first, lds0 + S::a_at(slot), (uint32_t)left(s));
+  };
+  auto fetch_b = [&](uint32_t s, uint32_t slot) {
+    if (OP == G_INPUT || whole(s))  // (dz and du have zeros behind their ends)
+      sb.fetch(b_base(s), b_first, lds0 + S::b_at(slot));
+    else
+      sb.fetch_end(b_base(s), b_first, lds0 + S::b_at(slot), (uint32_t)left(s));
   };
 
   V va[SLICES][TA], vb[SLICES][TB];
   f32x16 acc[TA][TB] = {};
-  // 8 reduction indices of a slice of 16 (the lane's half of it) for 32 rows of a side
-  auto take = [&](uint32_t base, uint32_t row, uint32_t ks) -> V {
-    return *reinterpret_cast<const V *>(lds + base + row * 128u + lo * 128u + (((2u * ks + hi) ^ (lo >> 1 & 7u)) * 16u));
+  // 8 reduction indices of a slice of 16 (the lane's half of it) for 32 rows of a side, of
+  // lane l
+  auto take = [&](uint32_t l, uint32_t base, uint32_t ks) -> V {
+    const uint32_t lo = l & 31u, hi = l >> 5;
+    return *reinterpret_cast<const V *>(lds + base + lo * S::KB + (((2u * ks + hi) ^ tile_turn<S>(lo)) * 16u));
   };
-  auto take_cross = [&](uint32_t base, uint32_t pitch, uint32_t chunks, uint32_t chunk, uint32_t ks) -> V {
+  auto take_cross = [&](uint32_t l, uint32_t base, uint32_t pitch, uint32_t chunks, uint32_t chunk, uint32_t ks) -> V {
     const uint32_t q = (l & 15u) / 4u, turn = chunks >= 4 ? q : chunks == 2 ? q >> 1 : 0u;
-    const uint32_t at = base + (16u * ks + 8u * hi + q) * pitch + ((chunk ^ turn) * 64u) + (l >> 4 & 1u) * 32u + (l & 3u) * 8u;
+    const uint32_t at = base + (16u * ks + 8u * (l >> 5) + q) * pitch + ((chunk ^ turn) * 64u) + (l >> 4 & 1u) * 32u + (l & 3u) * 8u;
     typedef __attribute__((address_space(3))) s16x4 *P;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at));
     const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at + 4u * pitch));
     return __builtin_bit_cast(V, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto read = [&](uint32_t buffer) {
-    const uint32_t base = buffer * STAGE, base_b = base + S::NA * 128u;
+  auto read = [&](uint32_t slot_a, uint32_t slot_b) {
+    const uint32_t base = S::a_at(slot_a), base_b = S::b_at(slot_b), l = here(threadIdx.x) & 63u;
 #pragma unroll
     for (int k = 0; k < SLICES; ++k) {
       const uint32_t ks = wk * SLICES + k;
 #pragma unroll
       for (int i = 0; i < TA; ++i)
-        va[k][i] = A_CROSS ? take_cross(base, S::NA * 2u, S::NA / 32, wa * TA + i, ks) : take(base, wa * S::MA + 32u * i, ks);
+        va[k][i] = A_CROSS ? take_cross(l, base, S::NA * 2u, S::NA / 32, wa * TA + i, ks) : take(l, base + (wa * S::MA + 32u * i) * S::KB, ks);
 #pragma unroll
       for (int j = 0; j < TB; ++j)
-        vb[k][j] = B_CROSS ? take_cross(base_b, S::NB * 2u, S::NB / 32, wb * TB + j, ks) : take(base_b, wb * S::MB + 32u * j, ks);
+        vb[k][j] = B_CROSS ? take_cross(l, base_b, S::NB * 2u, S::NB / 32, wb * TB + j, ks) : take(l, base_b + (wb * S::MB + 32u * j) * S::KB, ks);
     }
   };
   auto multiply = [&]() {
@@ -185,13 +186,14 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
 #pragma unroll
         for (int j = 0; j < TB; ++j) acc[i][j] = Frag<T>::mul(va[k][i], vb[k][j], acc[i][j]);
   };
-  tile_loop<S, S::PA + S::PB>(s0, s1, fetch, read, multiply);
+  tile_loop<S, S::PB>(s0, s1, fetch_a, fetch_b, read, multiply);
 
   // The end: a wave turns 32 rows x MA columns at a time through its part of LDS, so that
   // 8 neighbouring columns come to a lane (rows are padded by 16 bytes: 16 lanes that write
   // together fall on all banks).
   constexpr uint32_t PITCH = S::MA + 4, LPR = HALF / S::WA / 8u, RPI = 64u / LPR;  // floats; lanes per row, rows at a time
   constexpr uint32_t PARTS = S::WA * S::WB;
+  const uint32_t l = here(threadIdx.x) & 63u, lo = l & 31u, hi = l >> 5;
   float *mine = reinterpret_cast<float *>(lds) + (wave % PARTS) * 32u * PITCH;
   T *out = reinterpret_cast<T *>(up ? g.out1 : g.out);
   const uint64_t limit = OP == G_WEIGHT ? g.n : g.rows;  // rows of the output
@@ -367,11 +369,11 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
          (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
 }
 
-static constexpr TileKind gated_kinds[] = {{64, 32, 0.2f, 0.15f}, {64, 64, 0.25f, 0.2f}, {128, 128, 0.5f, 0.45f}, {256, 256, 1.0f, 1.0f}};
-typedef TileShape<64, 32, 1, 1, 4, 6, false> Tile32;
-typedef TileShape<64, 32, 1, 2, 2, 4, false> Tile64;
-typedef TileShape<64, 64, 2, 2, 1, 3, false> Tile128;
-typedef TileShape<128, 64, 2, 4, 1, 2, true> Tile256;
+static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.25f, 0.2f}, {128, 128, 128, 0.5f, 0.45f}, {256, 256, 128, 1.0f, 1.0f}};
+typedef TileShape<64, 32, 1, 1, 4, 128, 6, false> Tile32;
+typedef TileShape<64, 32, 1, 2, 2, 128, 4, false> Tile64;
+typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> Tile128;
+typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> Tile256;
 
 struct GatedPlan {
   bool pack_x, pack_w;
@@ -386,9 +388,9 @@ struct GatedPlan {
     x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;
     w_bytes = pack_w ? tile_bytes((uint64_t)g.n * kp * 2u) : 0;
     d_bytes = tile_bytes(g.rows * 2u * np * 2u);
-    forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, tile_cdiv(g.k, 64), g.rows * 2u * g.n);
-    input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, 2u * (np / 64u), g.rows * g.k);
-    weight = plan_tiles(ctx, gated_kinds, 4, g.k, g.n, true, tile_cdiv(g.rows, 64), 2ull * g.n * g.k);
+    forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, g.k * 2ull, g.rows * 2u * g.n);
+    input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, np * 4ull, g.rows * g.k);
+    weight = plan_tiles(ctx, gated_kinds, 4, g.k, g.n, true, g.rows * 2ull, 2ull * g.n * g.k);
   }
 };
 
@@ -407,8 +409,7 @@ static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t r
 
 template <class S, int OP, class T, int ACT>
 static int launch_kind(thrml_ctx *ctx, const GatedTiles &g) {
-  constexpr size_t stage = (S::NA + S::NB) * 128u;
-  const size_t lds = std::max<size_t>(stage * S::STAGES, (size_t)S::WA * S::WB * 32 * (S::MA + 4) * 4);
+  const size_t lds = std::max<size_t>(S::BYTES, (size_t)S::WA * S::WB * 32 * (S::MA + 4) * 4);
   auto *f = g.splits > 1 ? &gated_tile_kernel<S, OP, T, ACT, true> : &gated_tile_kernel<S, OP, T, ACT, false>;
   return launch_tiles(ctx, f, g, S::THREADS, lds);
 }

@@ -2,17 +2,18 @@
 // hidden block (k_gated.hip) and its 8-bit product (k_f8.hip).
 //
 // out[r][c] = sum over j of B[r][j] A[c][j]: side A are the output's columns (its
-// contiguous direction), side B its rows.  A stage is 128 bytes of the reduction of
-// every row of both sides.  An operand lies in memory either with the reduction
+// contiguous direction), side B its rows.  A stage is KB (64 or 128) bytes of the reduction
+// of every row of both sides.  An operand lies in memory either with the reduction
 // contiguous (a row of a side is a row in memory), or across (CROSS: a row in memory
 // holds one reduction index for all rows of the side), as a gradient's operands do.
 //
 // In LDS, 16-byte pieces:
-//   along   rows of 128 bytes, a row's 8 pieces permuted by (row >> 1) & 7.  A 16-byte
-//           read takes 16 lanes at a time, four quads of lanes: 0, 3, 5, 6 of a half wave,
-//           then 1, 2, 4, 7; two rows of 128 bytes fill the banks, and the rows of one
-//           parity that meet (0, 2, 12, 14, 20, 22, 24, 26 of 32) differ in those bits.
-//   across  64 rows, one for each reduction index, of the side's rows in chunks of 32
+//   along   rows of KB bytes, a row's pieces permuted by bits of the row: (row >> 1) & 7 for
+//           128 bytes, (row >> 3) & 3 for 64.  A 16-byte read takes 16 lanes at a time, four
+//           quads of lanes: 0, 3, 5, 6 of a half wave, then 1, 2, 4, 7; two rows of 128 bytes
+//           fill the banks, and the rows of one parity that meet (0, 2, 12, 14, 20, 22, 24, 26
+//           of 32) differ in those bits, as do four that meet of 64 bytes.
+//   across  KB / 2 rows, one for each reduction index, of the side's rows in chunks of 32
 //           (64 bytes), permuted so that the 4 neighbouring indices that the transposing
 //           read takes together fall on different banks.
 // Both permutations are made in the addresses that the loads into LDS read from: these
@@ -64,106 +65,157 @@ __device__ __forceinline__ void tile_barrier() {
 }
 
 // A workgroup of WA x WB x WK waves; a wave takes MA rows of side A by MB of side B
-// and, of each stage, one of WK parts of the reduction.
-template <int MA_, int MB_, int WA_, int WB_, int WK_, int STAGES_, bool PING_>
+// and, of each stage, one of WK parts of the reduction.  STAGES: those in LDS; PING (below)
+// has three of side A and two of side B.
+template <int MA_, int MB_, int WA_, int WB_, int WK_, int KB_, int STAGES_, bool PING_>
 struct TileShape {
-  static constexpr int MA = MA_, MB = MB_, WA = WA_, WB = WB_, WK = WK_, STAGES = STAGES_;
+  static constexpr int MA = MA_, MB = MB_, WA = WA_, WB = WB_, WK = WK_, KB = KB_;
+  static constexpr int STAGES_A = PING_ ? 3 : STAGES_, STAGES_B = PING_ ? 2 : STAGES_;
   static constexpr bool PING = PING_;
   static constexpr int NA = MA * WA, NB = MB * WB, WAVES = WA * WB * WK, THREADS = 64 * WAVES;
-  static constexpr int PA = NA * 8 / THREADS, PB = NB * 8 / THREADS;  // pieces per lane
-  static_assert(PA * THREADS == NA * 8 && PB * THREADS == NB * 8, "a stage is whole pieces of every lane");
-  static_assert(!PING || (WAVES == 8 && WK == 1 && STAGES == 2), "two waves of a SIMD take turns");
+  static constexpr int LOADERS = PING_ ? THREADS / 2 : THREADS;       // threads that load a side
+  static constexpr int PIECES = KB / 16;                              // of a row
+  static constexpr int PA = NA * PIECES / LOADERS, PB = NB * PIECES / LOADERS;  // for each of them
+  static constexpr int B_AT = STAGES_A * NA * KB, BYTES = B_AT + STAGES_B * NB * KB;  // in LDS: side A's stages, then B's
+  static_assert(PA * LOADERS == NA * PIECES && PB * LOADERS == NB * PIECES, "a stage is whole pieces of every lane");
+  static_assert(!PING || (WAVES == 8 && WK == 1), "two waves of a SIMD take turns");
+  __device__ static __forceinline__ uint32_t a_at(uint32_t slot) { return slot * (NA * KB); }
+  __device__ static __forceinline__ uint32_t b_at(uint32_t slot) { return B_AT + slot * (NB * KB); }
 };
 
-// What a lane loads of one side.
+// a row's permutation of its pieces
+template <class S>
+__device__ __forceinline__ uint32_t tile_turn(uint32_t row) {
+  return S::KB == 128 ? row >> 1 & 7u : row >> 3 & 3u;
+}
+
+// What a lane loads of one side, in P pieces.  Along, its pieces lie STEP rows apart, at
+// the same bytes of a row; across, STEP indices apart, at the same rows.  Where they lie in
+// memory is computed from the thread's number at each stage (here() keeps the compiler from
+// doing it once): kept, it was what did not fit into the registers of a 256 x 256 tile.
 template <class S, int N, bool CROSS>
 struct Side {
-  static constexpr int P = N * 8 / S::THREADS;
-  static constexpr int CHUNKS = N / 32;  // of a row in LDS, where CROSS
-  uint32_t off[P];                       // bytes from the stage's first
+  static constexpr int P = N * S::PIECES / S::LOADERS;
+  static constexpr int CHUNKS = N / 32;                              // of a row in LDS, where CROSS
+  static constexpr uint32_t STEP = CROSS ? S::LOADERS / (N / 8) : S::LOADERS / S::PIECES;
+  static_assert(CROSS ? STEP % 4 == 0 || P == 1 : STEP % (S::KB == 128 ? 16 : 32) == 0 || P == 1, "pieces are permuted alike");
+  uint32_t stride, last;    // bytes between rows in memory (below 2^24), the last valid row
 
-  __device__ static uint32_t turn(uint32_t kk) { return CHUNKS >= 4 ? kk & 3u : CHUNKS == 2 ? kk >> 1 & 1u : 0u; }
-  // piece p's place: (row, first byte in the row) along, (first row, reduction index) across
-  __device__ static uint32_t element(int p) { return (uint32_t)p * S::THREADS + threadIdx.x; }
-  __device__ static uint32_t row(int p) {
-    const uint32_t e = element(p);
-    if (!CROSS) return e / 8u;
-    const uint32_t pos = e % (N / 8u);
-    return ((pos / 4u ^ turn(index(p))) * 4u + pos % 4u) * 8u;
+  struct Place {            // of piece 0
+    uint32_t row, index;    // along: row and first byte in it; across: first row and index
+  };
+  __device__ __forceinline__ Place place() const {
+    const uint32_t e = here(threadIdx.x) % S::LOADERS;
+    Place a;
+    if (CROSS) {
+      const uint32_t pos = e % (N / 8u);
+      a.index = e / (N / 8u);
+      const uint32_t turn = CHUNKS >= 4 ? a.index & 3u : CHUNKS == 2 ? a.index >> 1 & 1u : 0u;
+      a.row = ((pos / 4u ^ turn) * 4u + pos % 4u) * 8u;
+      if (a.row > last) a.row = 0;  // (8 rows: last is 7 mod 8)
+    } else {
+      a.row = e / S::PIECES;
+      a.index = (e % S::PIECES ^ tile_turn<S>(a.row)) * 16u;
+    }
+    return a;
   }
-  __device__ static uint32_t index(int p) {  // bytes along, an index across
-    const uint32_t e = element(p);
-    return CROSS ? e / (N / 8u) : ((e & 7u) ^ (e / 8u >> 1 & 7u)) * 16u;
-  }
-  // src(row): a valid row of the operand, from the tile's first on
+  // piece p's bytes from base(p) on.  first(p): along, the row in memory of the side's row
+  // p STEP
   template <class F>
-  __device__ __forceinline__ void init(uint32_t stride, F src) {
-#pragma unroll
-    for (int p = 0; p < P; ++p) off[p] = CROSS ? index(p) * stride + src(row(p)) * 2u : src(row(p)) * stride + index(p);
+  __device__ __forceinline__ uint32_t offset(int p, Place a, F first) const {
+    if (CROSS) return __umul24(a.index, stride) + a.row * 2u;
+    return __umul24(min(a.row + first(p), last), stride) + a.index;
   }
-  // base(p): where the stage begins in memory, the wave's
-  template <class F>
-  __device__ __forceinline__ void fetch(F base, uint32_t lds) const {
+  template <class B, class F>
+  __device__ __forceinline__ void fetch(B base, F first, uint32_t lds) const {
+    const Place a = place();
 #pragma unroll
-    for (int p = 0; p < P; ++p) piece_to_lds(base(p), off[p], lds + (uint32_t)p * S::THREADS * 16u);
+    for (int p = 0; p < P; ++p)
+      piece_to_lds(base(p) + (CROSS ? (uint64_t)p * STEP * stride : 0u), offset(p, a, first), lds + (uint32_t)p * S::LOADERS * 16u);
   }
   // the same where only `left` of the stage's bytes (along) or indices (across) are left
-  template <class F>
-  __device__ __forceinline__ void fetch_end(F base, uint32_t lds, uint32_t left) const {
+  template <class B, class F>
+  __device__ __forceinline__ void fetch_end(B base, F first, uint32_t lds, uint32_t left) const {
+    const Place a = place();
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const uint8_t *at = reinterpret_cast<const uint8_t *>(base(p)) + off[p];
-      piece_to_lds(index(p) < left ? at : reinterpret_cast<const uint8_t *>(&zero_piece), lds + (uint32_t)p * S::THREADS * 16u);
+      const uint8_t *at = base(p) + (CROSS ? (uint64_t)p * STEP * stride : 0u) + offset(p, a, first);
+      const bool in = CROSS ? a.index + p * STEP < left : a.index < left;
+      piece_to_lds(in ? at : reinterpret_cast<const uint8_t *>(&zero_piece), lds + (uint32_t)p * S::LOADERS * 16u);
     }
   }
 };
 
-// The loop over the stages s0 .. s1 - 1.  fetch(s, buffer) begins the loads of stage s,
-// of LOADS instructions a wave, read(buffer) takes a wave's operands from LDS, multiply()
-// multiplies them.
+// The loop over the stages s0 .. s1 - 1.  fetch_a(s, slot) and fetch_b begin the loads of
+// a side's stage s, of S::PA and LOADS_B instructions a wave, read(slot of A, of B) takes a
+// wave's operands from LDS, multiply() multiplies them.
 //
 // PING: a SIMD's two waves take turns: one reads its operands of a stage while the other
 // multiplies, so that the matrix unit always has a wave that needs nothing but registers.
-// The second wave is one phase, half a stage, behind.  A stage's loads have two phases to
-// arrive.
-template <class S, int LOADS, class Fetch, class Read, class Multiply>
-__device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, Fetch fetch, Read read, Multiply multiply) {
+// The second wave is one phase, half a stage, behind.  Behind its reads, the first loads
+// the next stage of side B, the second the next but one of side A.  A load into LDS
+// holds its wave up for some 40 cycles, also between products: so each phase has half of
+// them, and none is among the products.  Cycles of a phase at 4096 x 4096 x 16384 in bf16:
+// 1055 multiply (of 1024 that the products take), 650 read, 400 load.  With all loads
+// from the first wave a stage took 2830 cycles, with all among the second's products 3350.
+template <class S, int LOADS_B, class FetchA, class FetchB, class Read, class Multiply>
+__device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch_a, FetchB fetch_b, Read read, Multiply multiply) {
   if constexpr (S::PING) {
     const bool second = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u) >= 4u;
-    fetch(s0, 0);
+    if (second) {
+      fetch_a(s0, 0);
+      if (s0 + 1 < s1) fetch_a(s0 + 1, 1);
+    } else {
+      fetch_b(s0, 0);
+    }
     wait_loads<0>();
     tile_barrier();
-    if (second) {
-      if (s0 + 1 < s1) fetch(s0 + 1, 1);
-      tile_barrier();
-    }
+    if (second) tile_barrier();
+    uint32_t a = 0, b = 0;
     for (uint32_t s = s0; s < s1; ++s) {
-      const uint32_t b = (s - s0) & 1u;
-      read(b);
-      if (!second && s + 1 < s1) fetch(s + 1, b ^ 1u);
+      read(a, b);
+      // (A's slot held stage s - 1, B's too, which everyone has read)
+      const bool more = s + (second ? 2u : 1u) < s1;
+      if (more) {
+        if (second)
+          fetch_a(s + 2, a == 0 ? 2u : a - 1u);
+        else
+          fetch_b(s + 1, b ^ 1u);
+      }
       wait_reads();
-      if (second) wait_loads<0>();
+      // side A's stage s + 1 has come
+      if (second) {
+        if (more)
+          wait_loads<S::PA>();
+        else
+          wait_loads<0>();
+      }
       tile_barrier();
-      if (second && s + 2 < s1) fetch(s + 2, b);
       __builtin_amdgcn_s_setprio(1);
       multiply();
       __builtin_amdgcn_s_setprio(0);
-      if (!second) wait_loads<0>();
+      if (!second) wait_loads<0>();  // side B's
       if (!second || s + 1 < s1) tile_barrier();
+      a = a == 2 ? 0 : a + 1u;
+      b ^= 1u;
     }
     tile_barrier();
   } else {
     // fetches past the end repeat the last stage, so that every wait counts alike
-    constexpr uint32_t AHEAD = S::STAGES - 1;
-    for (uint32_t i = 0; i < AHEAD; ++i) fetch(min(s0 + i, s1 - 1u), i);
+    constexpr uint32_t AHEAD = S::STAGES_A - 1;
+    for (uint32_t i = 0; i < AHEAD; ++i) {
+      fetch_a(min(s0 + i, s1 - 1u), i);
+      fetch_b(min(s0 + i, s1 - 1u), i);
+    }
     uint32_t b = 0;
     for (uint32_t s = s0; s < s1; ++s) {
       // (a wave's reads of the stage before have ended: its products have been issued)
-      wait_loads<(S::STAGES - 2) * LOADS>();
+      wait_loads<(S::STAGES_A - 2) * (S::PA + LOADS_B)>();
       tile_barrier();
       const uint32_t into = b == 0 ? AHEAD : b - 1u;
-      fetch(min(s + AHEAD, s1 - 1u), into);
-      read(b);
+      fetch_a(min(s + AHEAD, s1 - 1u), into);
+      fetch_b(min(s + AHEAD, s1 - 1u), into);
+      read(b, b);
       wait_reads();
       multiply();
       b = b == AHEAD ? 0 : b + 1u;
@@ -188,6 +240,7 @@ static inline uint64_t tile_bytes(uint64_t n) { return (n + 255u) & ~(uint64_t)2
 
 struct TileKind {
   uint32_t na, nb;
+  uint32_t kb;        // bytes of a row in a stage
   float alone, many;  // us a stage: of a tile alone on a compute unit, and of one of several
 };
 
@@ -199,15 +252,16 @@ struct TilePlan {
 
 // The kind of tile, and into how many parts the reduction goes, by an estimate of each
 // one's time: its stages, and about 6 more for beginning and end, at its time for one.
-// cols: the rows of side A; rows: those of side B, of two matrices where `halves`.
+// row_bytes: of the reduction, in a row; cols: the rows of side A; rows: those of side B, of two matrices where `halves`.
 static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, int n, uint64_t cols, uint64_t rows, bool halves,
-                                  uint32_t steps, uint64_t out_values) {
+                                  uint64_t row_bytes, uint64_t out_values) {
   TilePlan best;
   double best_t = 0.0;
   for (int i = 0; i < n; ++i) {
     const TileKind &kd = kinds[i];
     const uint32_t ta = tile_cdiv(cols, kd.na), tb = tile_cdiv(rows, kd.nb) * (halves ? 2u : 1u);
     const uint64_t tiles = (uint64_t)ta * tb;
+    const uint32_t steps = tile_cdiv(row_bytes, kd.kb);
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
       if (splits > 1 && (steps < 8 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
       const double one = std::max<double>(kd.alone, (double)kd.many * (double)tile_cdiv(tiles * splits, ctx->cu_count));
