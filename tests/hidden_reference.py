@@ -76,3 +76,39 @@ def close(got, want, bound, what):
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} off, the worst by "
                            f"{float((err / bound).nan_to_num(1e30).max()):.3g} times what is allowed, first at "
                            f"{bad.nonzero()[0].tolist()}")
+
+
+F8 = torch.float8_e4m3fn
+
+
+def quantised(x):
+    """(8-bit floats [rows, blocks, 128] and scales [rows, blocks] in 64 bits) of rows of
+    f32: s = max(2^-126, max |x| times 1 / 448), a = x / s, both in f32, on the CPU"""
+    rows, k = x.shape
+    wide = torch.zeros(rows, -(-k // 128) * 128)
+    wide[:, :k] = x.cpu().float()
+    blocks = wide.view(rows, -1, 128)
+    s = (blocks.abs().amax(2) * torch.tensor(1.0 / 448.0)).clamp(min=2.0**-126)
+    return (blocks / s[:, :, None]).to(F8).double(), s.double()
+
+
+def linear_f8(x, w, w_scale, bias, out):
+    """(y, error allowed) on the CPU in 64 bits.  f32: k + 4 roundings of sums, scales and bias.
+    16 bits: besides, in each block of 128 each product is off by at most 2^-16 of the
+    largest, and the result by half a step."""
+    (a, s), q, k = quantised(x), w.shape[0], x.shape[1]
+    rows, blocks = s.shape
+    ww = torch.zeros(q, blocks * 128, dtype=torch.float64)
+    ww[:, :k] = w.cpu().double()
+    ww = ww.view(q, blocks, 128)
+    ws = w_scale.cpu().double().repeat_interleave(128, 0)[:q]
+    left, right = (a * s[:, :, None]).flatten(1), (ww * ws[:, :, None]).flatten(1)
+    y, size = left @ right.T, left.abs() @ right.abs().T
+    if bias is not None:
+        y = y + bias.cpu().double()
+        size = size + bias.cpu().double().abs()
+    err = (k + 4) * U32 * size + tiny(torch.float32) * k
+    if out != torch.float32:
+        err = err + 128 * 2.0**-16 * (a.abs().amax(2) * s) @ (ww.abs().amax(2) * ws).T
+        err = err + half_step(out) * (y.abs() + err) + tiny(out)
+    return y, err

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
             c = 0;
             ++r;
           }
-          if (c < 0 || r >= (int64_t)a.rows) continue;
+          if (c < 0 || c >= (int64_t)a.cols || r >= (int64_t)a.rows) continue;  // (a group behind the end begins there)
           float f = bits >> e & 1u ? (float)x[r * a.x_stride + c] * a.scale : 0.0f;
           if (RESIDUAL) f = (float)res[r * a.residual_stride + c] + f;
           y[r * a.y_stride + c] = (T)f;
