@@ -82,6 +82,7 @@ struct F8Tiles {
   uint64_t w_stride, scale_pitch, rows;
   uint32_t k, kp, q;
   uint32_t ta, tb, splits, steps;
+  bool small_b;           // x stays in the caches
   void *y;
   int64_t y_stride;
   float *part;            // [split][row][column]
@@ -151,14 +152,18 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   const uint32_t lds0 = lds_address(lds) + wave % (S::LOADERS / 64u) * 1024u;
   auto a_base = [&](uint32_t s) { return [&, s](int) { return a0 + s * 128u; }; };
   auto b_base = [&](uint32_t s) { return [&, s](int) { return b0 + s * 128u; }; };
-  auto fetch_a = [&](uint32_t s, uint32_t slot) {
+  const uint32_t start = tile_start(ia, s1 - s0, g.small_b);
+  auto ring = [&](uint32_t s) { return s + start < s1 ? s + start : s + start - (s1 - s0); };
+  auto fetch_a = [&](uint32_t s_, uint32_t slot) {
+    const uint32_t s = ring(s_);
     const uint32_t left = g.k - s * 128u;
     if (left >= 128u)
       sa.fetch(a_base(s), a_first, lds0 + S::a_at(slot));
     else
       sa.fetch_end(a_base(s), a_first, lds0 + S::a_at(slot), left);
   };
-  auto fetch_b = [&](uint32_t s, uint32_t slot) {
+  auto fetch_b = [&](uint32_t s_, uint32_t slot) {
+    const uint32_t s = ring(s_);
     if constexpr (!S::PING) {
       const uint32_t part = wave % (SCALES / 64u) * 64u;
       word_to_lds(g.scale + s * g.scale_pitch + r0 + part, (here(threadIdx.x) & 63u) * 4u,
@@ -176,7 +181,8 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
     f.set(*reinterpret_cast<const u32x4 *>(lds + at), *reinterpret_cast<const u32x4 *>(lds + (at ^ 64u)));
   };
   // PING: the scales of stage s
-  auto scales = [&](uint32_t s) {
+  auto scales = [&](uint32_t s_) {
+    const uint32_t s = ring(s_);
     const float *p = g.scale + s * g.scale_pitch + r0 + wb * S::MB;
     const uint32_t lo = here(threadIdx.x) & 15u;
 #pragma unroll
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
       for (int j = 0; j < TB; ++j) sx[j] = next_sx[j] * next_sw;
       scales(min(stage + 1u, s1 - 1u));
     } else {
-      next_sw = sw0[stage];
+      next_sw = sw0[ring(stage)];
 #pragma unroll
       for (int j = 0; j < TB; ++j)
         sx[j] = *reinterpret_cast<const float *>(lds + S::BYTES + (slot_b * SCALES + wb * S::MB + 16u * j + (l & 15u)) * 4u);
@@ -394,6 +400,7 @@ int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, 
   g.tb = p.tiles.tb;
   g.splits = p.tiles.splits;
   g.steps = p.tiles.steps;
+  g.small_b = tile_small(a.rows, p.kp);
   return with_type(out_dtype, [&](auto t) -> int {
     typedef decltype(t) TO;
     constexpr bool EXACT = sizeof(TO) == 4;

@@ -71,6 +71,7 @@ struct GatedTiles {
   uint32_t np;          // columns from a row's dz to its du
   uint32_t ta, tb;      // tiles
   uint32_t splits, steps;  // of the reduction; stages in all
+  bool small_b;         // side B stays in the caches
   // G_FORWARD: h and, unless null, z and u; G_INPUT: dx; G_WEIGHT: dw_gate and dw_up
   void *out, *out1, *out2;
   int64_t out_stride;   // elements
@@ -136,13 +137,17 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     return [&, s](int) { return b0 + (B_CROSS ? (uint64_t)s * ROWS * g.b_stride : (uint64_t)s * S::KB); };
   };
   const uint32_t lds0 = lds_address(lds) + wave % (S::LOADERS / 64u) * 1024u;
-  auto fetch_a = [&](uint32_t s, uint32_t slot) {
+  const uint32_t start = tile_start(ia, s1 - s0, g.small_b);
+  auto ring = [&](uint32_t s) { return s + start < s1 ? s + start : s + start - (s1 - s0); };
+  auto fetch_a = [&](uint32_t s_, uint32_t slot) {
+    const uint32_t s = ring(s_);
     if (whole(s))
       sa.fetch(a_base(s), a_first, lds0 + S::a_at(slot));
     else
       sa.fetch_end(a_base(s), a_first, lds0 + S::a_at(slot), (uint32_t)left(s));
   };
-  auto fetch_b = [&](uint32_t s, uint32_t slot) {
+  auto fetch_b = [&](uint32_t s_, uint32_t slot) {
+    const uint32_t s = ring(s_);
     if (OP == G_INPUT || whole(s))  // (dz and du have zeros behind their ends)
       sb.fetch(b_base(s), b_first, lds0 + S::b_at(slot));
     else
@@ -370,7 +375,7 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
 }
 
 static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.25f, 0.2f}, {128, 128, 128, 0.5f, 0.45f}, {256, 256, 128, 1.0f, 1.0f}};
-typedef TileShape<64, 32, 1, 1, 4, 128, 6, false> Tile32;
+typedef TileShape<64, 32, 1, 1, 4, 128, 4, false> Tile32;
 typedef TileShape<64, 32, 1, 2, 2, 128, 4, false> Tile64;
 typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> Tile128;
 typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> Tile256;
@@ -420,6 +425,7 @@ static int launch_product(thrml_ctx *ctx, const TilePlan &p, GatedTiles g) {
   g.tb = p.tb;
   g.splits = p.splits;
   g.steps = p.steps;
+  g.small_b = OP == G_WEIGHT ? tile_small(g.rows, g.np * 4ull) : tile_small(g.rows, g.b_stride);
   int rc;
   switch (p.kind) {
     case 0: rc = launch_kind<Tile32, OP, T, ACT>(ctx, g); break;

@@ -86,7 +86,7 @@ struct TileShape {
 // a row's permutation of its pieces
 template <class S>
 __device__ __forceinline__ uint32_t tile_turn(uint32_t row) {
-  return S::KB == 128 ? row >> 1 & 7u : row >> 3 & 3u;
+  return S::KB >= 256 ? row & 15u : S::KB == 128 ? row >> 1 & 7u : row >> 3 & 3u;
 }
 
 // What a lane loads of one side, in P pieces.  Along, its pieces lie STEP rows apart, at
@@ -98,7 +98,7 @@ struct Side {
   static constexpr int P = N * S::PIECES / S::LOADERS;
   static constexpr int CHUNKS = N / 32;                              // of a row in LDS, where CROSS
   static constexpr uint32_t STEP = CROSS ? S::LOADERS / (N / 8) : S::LOADERS / S::PIECES;
-  static_assert(CROSS ? STEP % 4 == 0 || P == 1 : STEP % (S::KB == 128 ? 16 : 32) == 0 || P == 1, "pieces are permuted alike");
+  static_assert(CROSS ? STEP % 4 == 0 || P == 1 : STEP % (S::KB >= 128 ? 16 : 32) == 0 || P == 1, "pieces are permuted alike");
   uint32_t stride, last;    // bytes between rows in memory (below 2^24), the last valid row
 
   struct Place {            // of piece 0
@@ -234,6 +234,16 @@ __device__ __forceinline__ void tile_place(uint32_t index, uint32_t tiles, uint3
   a = j / n;
 }
 
+// Where a tile begins in its stages, of which it takes n in a ring.  Rows of a power of two
+// bytes have the same columns on few channels of memory, and tiles that all begin at the
+// first column ask those for everything.  Where side B is small enough to stay in the caches,
+// each tile of side A begins elsewhere (one row by 4096 x 32768 in bf16: 54 us, not 65; 49
+// either way at 4160); otherwise the tiles of an XCD, which share what they load, begin
+// together.
+__device__ __forceinline__ uint32_t tile_start(uint32_t ia, uint32_t n, bool small_b) {
+  return small_b ? ia * 5u % n : (blockIdx.x & 7u) * n / 8u;
+}
+
 // ---------------------------------------------------------------------------
 // On the host: which tiles a call takes
 static inline uint64_t tile_bytes(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
@@ -280,6 +290,8 @@ static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, i
   }
   return best;
 }
+
+static inline bool tile_small(uint64_t rows, uint64_t row_bytes) { return rows * row_bytes <= (2u << 20); }
 
 // One workgroup for each tile and split.
 template <class G>
