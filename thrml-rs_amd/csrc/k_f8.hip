@@ -23,7 +23,47 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 // rows of the scales of one block, so that any tile's 256 are there
 static uint64_t scale_rows(uint64_t rows) { return ((rows + 255u) & ~(uint64_t)255u) + 64u; }
 
-// A wave quantises 512 values of a row: 16 lanes have a block.
+// A wave quantises the 512 values of a row from part * 512 on, 8 in a lane, 16 lanes to a
+// block; a lane's 8 bytes, its block's scale (NaN where a value is not finite).
+template <class T>
+__device__ __forceinline__ uint2 f8_quantise(const T *row, uint32_t c, uint32_t k, float &scale) {
+  Raw8<T> r;
+  if (c + 8u <= k)
+    load8(row + c, r);
+  else
+    load8_part(row + c, c < k ? k - c : 0u, r);
+  float v[8], m = 0.0f;
+  int bad = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = value(r, j);
+    bad |= !(fabsf(v[j]) < INFINITY);
+    m = fmaxf(m, fabsf(v[j]));
+  }
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, s));
+    bad |= __shfl_xor(bad, s);
+  }
+  // 1 / 448 is rounded first, as a division by a number is on the device; a scale below
+  // 2^-126 would be rounded to so few bits that quotients leave e4m3's range
+  const float s = fmaxf(m * (1.0f / 448.0f), 0x1p-126f);
+  scale = bad ? __builtin_nanf("") : s;
+  uint32_t w[2] = {0, 0};
+  if (!bad) {
+    const Divisor d(s);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = d.plain ? d.fast(v[j]) : v[j] / s;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h], f[4 * h + 1], 0, false);
+      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h + 2], f[4 * h + 3], t, true);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void f8_quantise_kernel(const T *__restrict__ x, int64_t x_stride, uint64_t rows, uint32_t k,
                                                           uint32_t kp, float *__restrict__ scale, uint64_t scale_pitch,
@@ -33,43 +73,11 @@ __global__ __launch_bounds__(256) void f8_quantise_kernel(const T *__restrict__ 
   for (uint64_t i = (uint64_t)blockIdx.x * 4u + threadIdx.x / 64u; i < rows * parts; i += waves) {
     const uint64_t row = i / parts;
     const uint32_t c = (uint32_t)(i - row * parts) * 512u + l * 8u;
-    const T *p = x + (int64_t)row * x_stride + c;
-    Raw8<T> r;
-    if (c + 8u <= k)
-      load8(p, r);
-    else
-      load8_part(p, c < k ? k - c : 0u, r);
-    float v[8], m = 0.0f;
-    int bad = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = value(r, j);
-      bad |= !(fabsf(v[j]) < INFINITY);
-      m = fmaxf(m, fabsf(v[j]));
-    }
-#pragma unroll
-    for (int s = 8; s > 0; s >>= 1) {
-      m = fmaxf(m, __shfl_xor(m, s));
-      bad |= __shfl_xor(bad, s);
-    }
-    // 1 / 448 is rounded first, as a division by a number is on the device; a scale below
-    // 2^-126 would be rounded to so few bits that quotients leave e4m3's range
-    const float s = fmaxf(m * (1.0f / 448.0f), 0x1p-126f);
+    float s;
+    const uint2 w = f8_quantise(x + (int64_t)row * x_stride, c, k, s);
     if (c < kp) {
-      uint32_t w[2] = {0, 0};
-      if (!bad) {
-        const Divisor d(s);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = d.plain ? d.fast(v[j]) : v[j] / s;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          int t = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h], f[4 * h + 1], 0, false);
-          w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h + 2], f[4 * h + 3], t, true);
-        }
-      }
-      *reinterpret_cast<uint2 *>(xq + row * kp + c) = make_uint2(w[0], w[1]);
-      if ((l & 15u) == 0) scale[(uint64_t)(c / 128u) * scale_pitch + row] = bad ? __builtin_nanf("") : s;
+      *reinterpret_cast<uint2 *>(xq + row * kp + c) = w;
+      if ((l & 15u) == 0) scale[(uint64_t)(c / 128u) * scale_pitch + row] = s;
     }
   }
 }
@@ -86,6 +94,8 @@ struct F8Tiles {
   void *y;
   int64_t y_stride;
   float *part;            // [split][row][column]
+  const void *x_own;      // the rows themselves, where each workgroup quantises them
+  int64_t x_own_stride;
 };
 
 __device__ __forceinline__ bf16x8 widen8(uint32_t a, uint32_t b) {
@@ -121,14 +131,21 @@ struct F8Frag<true> {
 };
 
 // The rows' scales of a stage: floats in LDS behind the stages, loaded with side B.  With
-// PING, whose stages fill LDS, each lane keeps those of its rows, loaded a stage ahead.
+// PING, whose stages fill LDS, a wave keeps those of four stages in its four groups of 16
+// lanes and hands them around: the compiler waits for all loads under way before it uses
+// one of its own, so that these are loaded every fourth stage, four stages ahead.  The weights'
+// scales of 64 stages lie in a wave's 64 lanes (a scalar load in each stage: 25 of 306 us at
+// 4096 x 4096 x 16384).
 template <class S>
 constexpr uint32_t f8_scales() {
   return S::PING ? 0 : S::NB < 64 ? 64 : S::NB;
 }
 
-template <class S, class TO, bool EXACT, bool PART>
+// OWN (few values in all): each workgroup quantises the rows itself, of the type OWN, into
+// LDS behind the stages of side A, while its first weights load: one launch for a call.
+template <class S, class TO, bool EXACT, bool PART, class OWN = void>
 __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
+  constexpr bool IS_OWN = !std::is_void<OWN>::value;
   constexpr int TA = S::MA / 16, TB = S::MB / 16;
   constexpr uint32_t SCALES = f8_scales<S>();
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -164,6 +181,7 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   };
   auto fetch_b = [&](uint32_t s_, uint32_t slot) {
     const uint32_t s = ring(s_);
+    if constexpr (IS_OWN) return;
     if constexpr (!S::PING) {
       const uint32_t part = wave % (SCALES / 64u) * 64u;
       word_to_lds(g.scale + s * g.scale_pitch + r0 + part, (here(threadIdx.x) & 63u) * 4u,
@@ -172,40 +190,54 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
     sb.fetch(b_base(s), b_first, lds0 + S::b_at(slot));  // (rows of kp, zeros behind k)
   };
   F8Frag<EXACT> va[TA], vb[TB];
-  float sx[TB], next_sx[TB], next_sw = 0.0f;
+  float sx[TB], quad[S::PING ? TB : 1], next_quad[S::PING ? TB : 1], sw64 = 0.0f, sw = 0.0f;
   f32x4 acc[TA][TB] = {};
-  uint32_t stage = s0;
+  uint32_t turn = 0;  // stages read
+  auto scales = [&](uint32_t i) {  // PING: of turns i .. i + 3
+    const uint32_t l = here(threadIdx.x) & 63u;
+    const float *p = g.scale + (uint64_t)ring(min(s0 + i + (l >> 4), s1 - 1u)) * g.scale_pitch + r0 + wb * S::MB + (l & 15u);
+#pragma unroll
+    for (int j = 0; j < TB; ++j) next_quad[j] = p[16 * j];
+  };
+  if constexpr (S::PING) scales(0);
   auto take = [&](uint32_t l, uint32_t base, F8Frag<EXACT> &f) {
     // (pieces hi and hi + 4 of the row: any order of the block's indices, the same on both sides)
     const uint32_t lo = l & 15u, hi = l >> 4, at = base + lo * 128u + ((hi ^ tile_turn<S>(lo)) * 16u);
     f.set(*reinterpret_cast<const u32x4 *>(lds + at), *reinterpret_cast<const u32x4 *>(lds + (at ^ 64u)));
   };
-  // PING: the scales of stage s
-  auto scales = [&](uint32_t s_) {
-    const uint32_t s = ring(s_);
-    const float *p = g.scale + s * g.scale_pitch + r0 + wb * S::MB;
-    const uint32_t lo = here(threadIdx.x) & 15u;
-#pragma unroll
-    for (int j = 0; j < TB; ++j) next_sx[j] = p[16u * j + lo];
-    next_sw = sw0[s];
-  };
-  if (S::PING) scales(s0);
   auto read = [&](uint32_t slot_a, uint32_t slot_b) {
     const uint32_t l = here(threadIdx.x) & 63u;
-    if (S::PING) {
-      // (before this stage's loads into LDS are begun: the compiler waits for all loads)
+    const uint32_t stage_at = ring(s0 + turn), row = wb * S::MB + (l & 15u);
+    if (turn % 64u == 0) sw64 = sw0[ring(min(s0 + turn + l, s1 - 1u))];
+    sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sw64), turn % 64u));
+    if constexpr (IS_OWN) {
+      const float *own_s = reinterpret_cast<const float *>(lds + S::B_AT + (uint32_t)g.rows * g.kp);
 #pragma unroll
-      for (int j = 0; j < TB; ++j) sx[j] = next_sx[j] * next_sw;
-      scales(min(stage + 1u, s1 - 1u));
-    } else {
-      next_sw = sw0[ring(stage)];
+      for (int j = 0; j < TB; ++j) sx[j] = own_s[min(row + 16u * j, (uint32_t)g.rows - 1u) * g.steps + stage_at];
+    } else if constexpr (S::PING) {
+      if (turn % 4u == 0) {
+#pragma unroll
+        for (int j = 0; j < TB; ++j) quad[j] = next_quad[j];
+        scales(turn + 4u);
+      }
 #pragma unroll
       for (int j = 0; j < TB; ++j)
-        sx[j] = *reinterpret_cast<const float *>(lds + S::BYTES + (slot_b * SCALES + wb * S::MB + 16u * j + (l & 15u)) * 4u);
-    }
-    ++stage;
+        sx[j] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((int)((turn % 4u * 16u + (l & 15u)) * 4u), __builtin_bit_cast(int, quad[j])));
+    } else {
 #pragma unroll
-    for (int j = 0; j < TB; ++j) take(l, S::b_at(slot_b) + (wb * S::MB + 16u * j) * 128u, vb[j]);
+      for (int j = 0; j < TB; ++j)
+        sx[j] = *reinterpret_cast<const float *>(lds + S::BYTES + (slot_b * SCALES + row + 16u * j) * 4u);
+    }
+    ++turn;
+#pragma unroll
+    for (int j = 0; j < TB; ++j) {
+      if constexpr (IS_OWN) {
+        const uint8_t *at = lds + S::B_AT + min(row + 16u * j, (uint32_t)g.rows - 1u) * g.kp + stage_at * 128u + (l >> 4) * 16u;
+        vb[j].set(*reinterpret_cast<const u32x4 *>(at), *reinterpret_cast<const u32x4 *>(at + 64u));
+      } else {
+        take(l, S::b_at(slot_b) + (wb * S::MB + 16u * j) * 128u, vb[j]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < TA; ++i) take(l, S::a_at(slot_a) + (wa * S::MA + 16u * i) * 128u, va[i]);
   };
@@ -216,10 +248,8 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   auto multiply = [&]() {
     constexpr int LAG = 3;
     f32x4 t[LAG + 1];
-    if (!S::PING) {
 #pragma unroll
-      for (int j = 0; j < TB; ++j) sx[j] *= next_sw;
-    }
+    for (int j = 0; j < TB; ++j) sx[j] *= sw;
 #pragma unroll
     for (int n = 0; n < TA * TB + LAG; ++n) {
       if (n < TA * TB) t[n % (LAG + 1)] = F8Frag<EXACT>::mul(va[n % TA], vb[n / TA]);
@@ -234,7 +264,23 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
       }
     }
   };
-  tile_loop<S, S::PB + (S::PING ? 0 : 1)>(s0, s1, fetch_a, fetch_b, read, multiply);
+  auto begin = [&]() {
+    if constexpr (IS_OWN) {
+      const uint32_t parts = (g.kp + 511u) / 512u, l = threadIdx.x & 63u;
+      float *own_s = reinterpret_cast<float *>(lds + S::B_AT + (uint32_t)g.rows * g.kp);
+      for (uint32_t i = threadIdx.x / 64u; i < (uint32_t)g.rows * parts; i += S::WAVES) {
+        const uint32_t row = i / parts, c = (i - row * parts) * 512u + l * 8u;
+        float s;
+        const uint2 w = f8_quantise(reinterpret_cast<const OWN *>(g.x_own) + (int64_t)row * g.x_own_stride, c, g.k, s);
+        if (c < g.kp) {
+          *reinterpret_cast<uint2 *>(lds + S::B_AT + row * g.kp + c) = w;
+          if ((l & 15u) == 0) own_s[row * g.steps + c / 128u] = s;
+        }
+      }
+      __syncthreads();
+    }
+  };
+  tile_loop<S, IS_OWN ? 0 : S::PB + (S::PING ? 0 : 1)>(s0, s1, fetch_a, fetch_b, read, multiply, begin);
 
   // The end: 16 rows x MA channels at a time through LDS, 8 neighbouring channels to a lane.
   constexpr uint32_t PITCH = S::MA + 4, LPR = S::MA / 8u;
@@ -271,6 +317,55 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
     }
     __builtin_amdgcn_wave_barrier();
     wait_reads();
+  }
+}
+
+// Few rows, weights at any alignment (tile.hpp): a workgroup takes 16 channels and up to 64
+// rows; its four waves take turns in the blocks of 128, and their sums meet in LDS.
+template <class TO, bool EXACT, int ROWS16>
+__global__ __launch_bounds__(256) void f8_few_kernel(F8Tiles g) {
+  __shared__ f32x4 part[4][ROWS16][64];
+  const uint32_t l = threadIdx.x & 63u, wave = threadIdx.x / 64u, lo = l & 15u, hi = l >> 4;
+  const uint32_t c0 = blockIdx.x * 16u;
+  const uint8_t *w = g.w + (uint64_t)min(c0 + lo, g.q - 1u) * g.w_stride;
+  const float *sw = g.w_scale + (uint64_t)(c0 / 128u) * g.steps;
+  uint32_t row[ROWS16];
+#pragma unroll
+  for (int j = 0; j < ROWS16; ++j) row[j] = min(16u * j + lo, (uint32_t)g.rows - 1u);
+  f32x4 acc[ROWS16] = {};
+#pragma unroll 2
+  for (uint32_t s = wave; s < g.steps; s += 4u) {
+    const uint32_t at = s * 128u + hi * 16u;
+    F8Frag<EXACT> a, b[ROWS16];
+    const u32x4 a0 = row_piece(w, at, g.k), a1 = row_piece(w, at + 64u, g.k);
+    float sx[ROWS16];
+#pragma unroll
+    for (int j = 0; j < ROWS16; ++j) {
+      const uint8_t *p = g.x + (uint64_t)row[j] * g.kp + at;
+      b[j].set(*reinterpret_cast<const u32x4 *>(p), *reinterpret_cast<const u32x4 *>(p + 64));
+      sx[j] = g.scale[s * g.scale_pitch + row[j]] * sw[s];
+    }
+    a.set(a0, a1);
+#pragma unroll
+    for (int j = 0; j < ROWS16; ++j) {
+      const f32x4 t = F8Frag<EXACT>::mul(a, b[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = __builtin_fmaf(t[e], sx[j], acc[j][e]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS16; ++j) part[wave][j][l] = acc[j];
+  __syncthreads();
+  for (uint32_t j = wave; j < ROWS16; j += 4u) {
+    f32x4 v = part[0][j][l];
+#pragma unroll
+    for (int o = 1; o < 4; ++o) v += part[o][j][l];
+    const uint32_t r = 16u * j + lo, c = c0 + 4u * hi;
+    if (r >= g.rows || c >= g.q) continue;
+    float f[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) f[e] = v[e] + (g.bias && c + e < g.q ? g.bias[c + e] : 0.0f);
+    store4(reinterpret_cast<TO *>(g.y) + (int64_t)r * g.y_stride + c, g.q - c, f);
   }
 }
 
@@ -328,7 +423,7 @@ typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> F8Tile128;
 typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> F8Tile256;
 
 struct F8Plan {
-  bool pack;
+  bool few, pack, own;
   uint32_t kp;
   uint64_t scale_bytes, x_bytes, w_bytes;
   TilePlan tiles;
@@ -336,17 +431,30 @@ struct F8Plan {
     kp = (a.k + 127u) & ~127u;
     pack = a.k % 16u != 0 || reinterpret_cast<uintptr_t>(a.w) % 16u != 0 ||
            (a.q > 1 && (a.w_stride % 16 != 0 || a.w_stride >= (1 << 23)));
+    few = pack && a.rows <= 64;
+    pack = pack && !few;
     scale_bytes = tile_bytes(scale_rows(a.rows) * (kp / 128u) * 4u);
     x_bytes = tile_bytes(a.rows * kp);
     w_bytes = pack ? tile_bytes((uint64_t)a.q * kp) : 0;
     const bool exact = out_dtype == THRML_DTYPE_F32;
     tiles = plan_tiles(ctx, exact ? f8_exact_kinds : f8_kinds, exact ? 3 : 4, a.q, a.rows, false, kp, a.rows * a.q);
+    // (the quantisation's own launch: 4 us and the gap behind it)
+    own = !few && !pack && tiles.kind == 0 && tiles.tb == 1 && tiles.splits == 1 && a.rows * kp <= 16384;
+    if (own) scale_bytes = x_bytes = 0;
+    if (few) tiles.part = 0;
   }
 };
 
 uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int, int out_dtype) {
   const F8Plan p(ctx, a, out_dtype);
   return p.scale_bytes + p.x_bytes + p.w_bytes + p.tiles.part;
+}
+
+template <class TO, bool EXACT, class T>
+static int launch_f8_own(thrml_ctx *ctx, const F8Tiles &g) {
+  typedef F8Tile32 S;
+  const size_t lds = std::max<size_t>(S::B_AT + g.rows * (g.kp + g.steps * 4), (size_t)S::WAVES * 16 * (S::MA + 4) * 4);
+  return launch_tiles(ctx, &f8_tile_kernel<S, TO, EXACT, false, T>, g, S::THREADS, lds);
 }
 
 template <class S, class TO, bool EXACT>
@@ -370,7 +478,7 @@ int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, 
   at += p.scale_bytes;
   g.x = at;
   at += p.x_bytes;
-  const int rc = with_type(dtype, [&](auto t) -> int {
+  const int rc = p.own ? THRML_OK : with_type(dtype, [&](auto t) -> int {
     typedef decltype(t) T;
     const uint64_t n = a.rows * ((p.kp + 511u) / 512u);
     hipLaunchKernelGGL((f8_quantise_kernel<T>), dim3((uint32_t)std::min<uint64_t>((n + 3u) / 4u, 1u << 16)), dim3(256), 0, ctx->stream,
@@ -404,6 +512,19 @@ int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, 
   return with_type(out_dtype, [&](auto t) -> int {
     typedef decltype(t) TO;
     constexpr bool EXACT = sizeof(TO) == 4;
+    if (p.own) {
+      g.x_own = a.x;
+      g.x_own_stride = a.x_stride;
+      return with_type(dtype, [&](auto t) { return launch_f8_own<TO, EXACT, decltype(t)>(ctx, g); });
+    }
+    if (p.few) {
+      auto *f = a.rows <= 16 ? &f8_few_kernel<TO, EXACT, 1> : a.rows <= 32 ? &f8_few_kernel<TO, EXACT, 2> : a.rows <= 48 ? &f8_few_kernel<TO, EXACT, 3> : &f8_few_kernel<TO, EXACT, 4>;
+      g.splits = 1;
+      g.steps = p.kp / 128u;
+      hipLaunchKernelGGL(f, dim3(tile_cdiv(a.q, 16)), dim3(256), 0, ctx->stream, g);
+      THRML_HIP(hipGetLastError());
+      return THRML_OK;
+    }
     int rc = THRML_OK;
     switch (p.tiles.kind) {
       case 0: rc = launch_f8_kind<F8Tile32, TO, EXACT>(ctx, g); break;

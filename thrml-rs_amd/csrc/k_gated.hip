@@ -191,7 +191,7 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
 #pragma unroll
         for (int j = 0; j < TB; ++j) acc[i][j] = Frag<T>::mul(va[k][i], vb[k][j], acc[i][j]);
   };
-  tile_loop<S, S::PB>(s0, s1, fetch_a, fetch_b, read, multiply);
+  tile_loop<S, S::PB>(s0, s1, fetch_a, fetch_b, read, multiply, [] {});
 
   // The end: a wave turns 32 rows x MA columns at a time through its part of LDS, so that
   // 8 neighbouring columns come to a lane (rows are padded by 16 bytes: 16 lanes that write
@@ -261,6 +261,87 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     else
       __builtin_amdgcn_wave_barrier();
     wait_reads();
+  }
+}
+
+// Few rows, operands at any alignment (tile.hpp): a workgroup takes 16 units and up to 64
+// rows; its four waves take turns in the stages of 128 bytes, and their sums meet in LDS.
+template <class T>
+struct FewFrag;
+template <>
+struct FewFrag<bf16_t> {
+  __device__ static __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct FewFrag<f16_t> {
+  __device__ static __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+template <class T, int ACT, int ROWS16>
+__global__ __launch_bounds__(256) void gated_few_kernel(GatedTiles g, int64_t gate_stride, int64_t up_stride, int64_t x_stride) {
+  __shared__ f32x4 part[4][2][ROWS16][64];
+  const uint32_t l = threadIdx.x & 63u, wave = threadIdx.x / 64u, lo = l & 15u, hi = l >> 4;
+  const uint32_t c0 = blockIdx.x * 16u, c = min(c0 + lo, g.n - 1u), bytes = g.k * 2u, steps = (bytes + 127u) / 128u;
+  const uint64_t r0 = (uint64_t)blockIdx.y * (16u * ROWS16);
+  const uint8_t *wg = reinterpret_cast<const uint8_t *>(g.a0) + (int64_t)c * gate_stride * 2;
+  const uint8_t *wu = reinterpret_cast<const uint8_t *>(g.a1) + (int64_t)c * up_stride * 2;
+  const uint8_t *x[ROWS16];
+#pragma unroll
+  for (int j = 0; j < ROWS16; ++j)
+    x[j] = reinterpret_cast<const uint8_t *>(g.b) + (int64_t)min(r0 + 16u * j + lo, g.rows - 1u) * x_stride * 2;
+  f32x4 z[ROWS16] = {}, u[ROWS16] = {};
+#pragma unroll 2
+  for (uint32_t s = wave; s < steps; s += 4u) {
+    u32x4 a[2][2], b[ROWS16][2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t at = s * 128u + hi * 16u + h * 64u;
+      a[0][h] = row_piece(wg, at, bytes);
+      a[1][h] = row_piece(wu, at, bytes);
+#pragma unroll
+      for (int j = 0; j < ROWS16; ++j) b[j][h] = row_piece(x[j], at, bytes);
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < ROWS16; ++j) {
+        z[j] = FewFrag<T>::mul(a[0][h], b[j][h], z[j]);
+        u[j] = FewFrag<T>::mul(a[1][h], b[j][h], u[j]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS16; ++j) {
+    part[wave][0][j][l] = z[j];
+    part[wave][1][j][l] = u[j];
+  }
+  __syncthreads();
+  for (uint32_t j = wave; j < ROWS16; j += 4u) {
+    f32x4 zs = part[0][0][j][l], us = part[0][1][j][l];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      zs += part[w][0][j][l];
+      us += part[w][1][j][l];
+    }
+    const uint64_t row = r0 + 16u * j + lo;
+    const uint32_t cc = c0 + 4u * hi;
+    if (row >= g.rows || cc >= g.n) continue;
+    float v[4], w[4], h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = zs[e];
+      w[e] = us[e];
+      h[e] = act_value<ACT>(v[e]) * w[e];
+    }
+    const int64_t saved = (int64_t)row * g.n + cc;
+    if (g.out1) {
+      store4(reinterpret_cast<T *>(g.out1) + saved, g.n - cc, v);
+      store4(reinterpret_cast<T *>(g.out2) + saved, g.n - cc, w);
+    }
+    store4(reinterpret_cast<T *>(g.out) + (int64_t)row * g.out_stride + cc, g.n - cc, h);
   }
 }
 
@@ -381,6 +462,7 @@ typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> Tile128;
 typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> Tile256;
 
 struct GatedPlan {
+  bool few;  // the forward pass reads the operands as they lie
   bool pack_x, pack_w;
   uint32_t kp, np;
   uint64_t x_bytes, w_bytes, d_bytes;  // packed x, each packed weight, dz and du
@@ -393,6 +475,7 @@ struct GatedPlan {
     x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;
     w_bytes = pack_w ? tile_bytes((uint64_t)g.n * kp * 2u) : 0;
     d_bytes = tile_bytes(g.rows * 2u * np * 2u);
+    few = (pack_x || pack_w) && g.rows <= 32;
     forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, g.k * 2ull, g.rows * 2u * g.n);
     input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, np * 4ull, g.rows * g.k);
     weight = plan_tiles(ctx, gated_kinds, 4, g.k, g.n, true, g.rows * 2ull, 2ull * g.n * g.k);
@@ -401,6 +484,7 @@ struct GatedPlan {
 
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward) {
   const GatedPlan p(ctx, g);
+  if (p.few && !backward) return 0;
   return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
 }
 
@@ -486,6 +570,27 @@ int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride
   const GatedPlan p(ctx, g);
   uint8_t *w = reinterpret_cast<uint8_t *>(work);
   GatedTiles t;
+  if (p.few) {
+    t = GatedTiles{};
+    t.rows = g.rows;
+    t.k = g.k;
+    t.n = g.n;
+    t.a0 = g.w_gate;
+    t.a1 = g.w_up;
+    t.b = g.x;
+    t.out = h;
+    t.out_stride = h_stride;
+    t.out1 = gate;
+    t.out2 = up;
+    return with_gated(g, [&](auto e, auto act) -> int {
+      typedef decltype(e) T;
+      constexpr int ACT = decltype(act)::value;
+      auto *f = g.rows <= 16 ? &gated_few_kernel<T, ACT, 1> : &gated_few_kernel<T, ACT, 2>;
+      hipLaunchKernelGGL(f, dim3(tile_cdiv(g.n, 16), 1), dim3(256), 0, ctx->stream, t, g.gate_stride, g.up_stride, g.x_stride);
+      THRML_HIP(hipGetLastError());
+      return THRML_OK;
+    });
+  }
   const void *x;
   uint64_t x_stride;
   if (int rc = operands(ctx, g, p, w, t, x, x_stride)) return rc;

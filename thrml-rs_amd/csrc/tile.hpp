@@ -148,7 +148,8 @@ struct Side {
 
 // The loop over the stages s0 .. s1 - 1.  fetch_a(s, slot) and fetch_b begin the loads of
 // a side's stage s, of S::PA and LOADS_B instructions a wave, read(slot of A, of B) takes a
-// wave's operands from LDS, multiply() multiplies them.
+// wave's operands from LDS, multiply() multiplies them.  begin() is called when the loads
+// of the first stage are under way (not with PING; it may wait for all that are).
 //
 // PING: a SIMD's two waves take turns: one reads its operands of a stage while the other
 // multiplies, so that the matrix unit always has a wave that needs nothing but registers.
@@ -158,8 +159,8 @@ struct Side {
 // them, and none is among the products.  Cycles of a phase at 4096 x 4096 x 16384 in bf16:
 // 1055 multiply (of 1024 that the products take), 650 read, 400 load.  With all loads
 // from the first wave a stage took 2830 cycles, with all among the second's products 3350.
-template <class S, int LOADS_B, class FetchA, class FetchB, class Read, class Multiply>
-__device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch_a, FetchB fetch_b, Read read, Multiply multiply) {
+template <class S, int LOADS_B, class FetchA, class FetchB, class Read, class Multiply, class Begin>
+__device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch_a, FetchB fetch_b, Read read, Multiply multiply, Begin begin) {
   if constexpr (S::PING) {
     const bool second = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u) >= 4u;
     if (second) {
@@ -206,6 +207,7 @@ __device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch
     for (uint32_t i = 0; i < AHEAD; ++i) {
       fetch_a(min(s0 + i, s1 - 1u), i);
       fetch_b(min(s0 + i, s1 - 1u), i);
+      if (i == 0) begin();
     }
     uint32_t b = 0;
     for (uint32_t s = s0; s < s1; ++s) {
@@ -223,6 +225,24 @@ __device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch
     wait_loads<0>();
     tile_barrier();
   }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows whose operands do not start at 16 bytes: straight from memory into the operand
+// registers of 16 x 16 products, without a copy.  16 bytes of a row from byte c on, zeros
+// from byte n on; p at any address (such a load takes longer than one of whole pieces, but
+// a copy reads and writes all of it).
+typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ u32x4 row_piece(const uint8_t *p, uint32_t c, uint32_t n) {
+  if (c + 16u <= n) return *reinterpret_cast<const u32x4_a1 *>(p + c);
+  u32x4 v = {0, 0, 0, 0};
+  if (c < n) {
+    const uint32_t left = here(n - c);
+#pragma unroll
+    for (uint32_t j = 0; j < 15; ++j)
+      if (j < left) v[j / 4u] |= (uint32_t)p[c + j] << (8u * (j & 3u));
+  }
+  return v;
 }
 
 // Tiles in an order in which those that run together share operands: workgroups of one
