@@ -26,12 +26,14 @@ static uint64_t scale_rows(uint64_t rows) { return ((rows + 255u) & ~(uint64_t)2
 // A wave quantises the 512 values of a row from part * 512 on, 8 in a lane, 16 lanes to a
 // block; a lane's 8 bytes, its block's scale (NaN where a value is not finite).
 template <class T>
-__device__ __forceinline__ uint2 f8_quantise(const T *row, uint32_t c, uint32_t k, float &scale) {
-  Raw8<T> r;
+__device__ __forceinline__ void f8_load(const T *row, uint32_t c, uint32_t k, Raw8<T> &r) {
   if (c + 8u <= k)
     load8(row + c, r);
   else
     load8_part(row + c, c < k ? k - c : 0u, r);
+}
+template <class T>
+__device__ __forceinline__ uint2 f8_quantise(const Raw8<T> &r, float &scale) {
   float v[8], m = 0.0f;
   int bad = 0;
 #pragma unroll
@@ -73,8 +75,10 @@ __global__ __launch_bounds__(256) void f8_quantise_kernel(const T *__restrict__ 
   for (uint64_t i = (uint64_t)blockIdx.x * 4u + threadIdx.x / 64u; i < rows * parts; i += waves) {
     const uint64_t row = i / parts;
     const uint32_t c = (uint32_t)(i - row * parts) * 512u + l * 8u;
+    Raw8<T> r;
+    f8_load(x + (int64_t)row * x_stride, c, k, r);
     float s;
-    const uint2 w = f8_quantise(x + (int64_t)row * x_stride, c, k, s);
+    const uint2 w = f8_quantise(r, s);
     if (c < kp) {
       *reinterpret_cast<uint2 *>(xq + row * kp + c) = w;
       if ((l & 15u) == 0) scale[(uint64_t)(c / 128u) * scale_pitch + row] = s;
@@ -208,7 +212,10 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   auto read = [&](uint32_t slot_a, uint32_t slot_b) {
     const uint32_t l = here(threadIdx.x) & 63u;
     const uint32_t stage_at = ring(s0 + turn), row = wb * S::MB + (l & 15u);
-    if (turn % 64u == 0) sw64 = sw0[ring(min(s0 + turn + l, s1 - 1u))];
+    if (turn % 64u == 0) {
+      sw64 = sw0[ring(min(s0 + turn + l, s1 - 1u))];
+      asm volatile("" : "+v"(sw64));  // (waited for here, not in every stage)
+    }
     sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sw64), turn % 64u));
     if constexpr (IS_OWN) {
       const float *own_s = reinterpret_cast<const float *>(lds + S::B_AT + (uint32_t)g.rows * g.kp);
@@ -217,7 +224,10 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
     } else if constexpr (S::PING) {
       if (turn % 4u == 0) {
 #pragma unroll
-        for (int j = 0; j < TB; ++j) quad[j] = next_quad[j];
+        for (int j = 0; j < TB; ++j) {
+          quad[j] = next_quad[j];
+          asm volatile("" : "+v"(quad[j]));
+        }
         scales(turn + 4u);
       }
 #pragma unroll
@@ -266,15 +276,28 @@ __global__ __launch_bounds__(S::THREADS) void f8_tile_kernel(F8Tiles g) {
   };
   auto begin = [&]() {
     if constexpr (IS_OWN) {
-      const uint32_t parts = (g.kp + 511u) / 512u, l = threadIdx.x & 63u;
+      // (four parts of 512 values of a row at a time, their loads together)
+      constexpr uint32_t U = 4;
+      const uint32_t parts = (g.kp + 511u) / 512u, all = (uint32_t)g.rows * parts, l = threadIdx.x & 63u;
       float *own_s = reinterpret_cast<float *>(lds + S::B_AT + (uint32_t)g.rows * g.kp);
-      for (uint32_t i = threadIdx.x / 64u; i < (uint32_t)g.rows * parts; i += S::WAVES) {
-        const uint32_t row = i / parts, c = (i - row * parts) * 512u + l * 8u;
-        float s;
-        const uint2 w = f8_quantise(reinterpret_cast<const OWN *>(g.x_own) + (int64_t)row * g.x_own_stride, c, g.k, s);
-        if (c < g.kp) {
-          *reinterpret_cast<uint2 *>(lds + S::B_AT + row * g.kp + c) = w;
-          if ((l & 15u) == 0) own_s[row * g.steps + c / 128u] = s;
+      for (uint32_t i = threadIdx.x / 64u; i < all; i += S::WAVES * U) {
+        Raw8<OWN> r[U];
+#pragma unroll
+        for (uint32_t e = 0; e < U; ++e) {
+          const uint32_t n = min(i + e * S::WAVES, all - 1u), row = n / parts, c = (n - row * parts) * 512u + l * 8u;
+          f8_load(reinterpret_cast<const OWN *>(g.x_own) + (int64_t)row * g.x_own_stride, c, g.k, r[e]);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < U; ++e) {
+          const uint32_t n = i + e * S::WAVES;
+          if (n >= all) break;
+          const uint32_t row = n / parts, c = (n - row * parts) * 512u + l * 8u;
+          float s;
+          const uint2 w = f8_quantise(r[e], s);
+          if (c < g.kp) {
+            *reinterpret_cast<uint2 *>(lds + S::B_AT + row * g.kp + c) = w;
+            if ((l & 15u) == 0) own_s[row * g.steps + c / 128u] = s;
+          }
         }
       }
       __syncthreads();
