@@ -571,20 +571,20 @@ typedef struct {
   int64_t up_stride;
 } thrml_gated;
 /* h[row][c] rounded once to the type; gate and up, both or neither NULL, receive z and
- * u, [rows][n] contiguous, for thrml_gated_backward.  work: thrml_gated_work(in, 0)
+ * u in f32, [rows][n] contiguous, for thrml_gated_backward.  work: thrml_gated_work(in, 0)
  * bytes.  The operands are read as they lie where their rows are whole 16-byte pieces
  * (k a multiple of 8, pointers of 16 bytes, strides of 8 elements, those of the two
  * weights alike), else from a copy in work. */
 uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward);
-int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, void *gate,
-                        void *up, void *work, uint64_t work_bytes);
+int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, float *gate,
+                        float *up, void *work, uint64_t work_bytes);
 /* From grad = d loss / d h [rows][n] and the z and u that the forward call kept:
  *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
  *   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x
  * dx [rows][k] in rows of dx_stride (NULL: not computed), dw_gate and dw_up [n][k]
  * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes. */
 int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
-                         const void *gate, const void *up, void *dx, int64_t dx_stride, void *dw_gate,
+                         const float *gate, const float *up, void *dx, int64_t dx_stride, void *dw_gate,
                          void *dw_up, void *work, uint64_t work_bytes);
 /* Dropout from a key: with the half words b of the ChaCha8 stream of seed_from_u64(seed)
  * (the generator of thrml_rng_split; 32 half words in a block, the lower one of a word

@@ -44,7 +44,8 @@ def gated(x, wg, wu, name):
     eh = STEEPEST * ez * (u.abs() + eu) + (a.abs() + STEEPEST * ez) * eu + 16 * U32 * z.abs() * u.abs()
     out = {}
     for n, v, e in (("h", h, eh), ("gate", z, ez), ("up", u, eu)):
-        out[n] = v, e + half_step(dtype) * (v.abs() + e) + tiny(dtype)
+        step, least = (half_step(dtype), tiny(dtype)) if n == "h" else (U32, tiny(torch.float32))
+        out[n] = v, e + step * (v.abs() + e) + least
     return out
 
 

@@ -10,6 +10,7 @@ B = torch.bfloat16
 X = torch.zeros(3, 70, dtype=B)
 W = torch.zeros(40, 70, dtype=B)
 H = torch.zeros(3, 40, dtype=B)
+G = torch.zeros(3, 40)
 KEY = th.RngKey(1)
 W8 = torch.zeros(200, 70, dtype=torch.uint8).view(torch.float8_e4m3fn)
 S8 = torch.zeros(2, 1)
@@ -30,9 +31,9 @@ def test_gated(args, kw, msg):
 
 
 @pytest.mark.parametrize("args,msg", [
-    ((H.half(), X, W, W, H, H), "grad must be a bfloat16 tensor"), ((H[:2], X, W, W, H, H), "grad must have shape"),
-    ((H, X, W, W, H[:, :39], H), "gate must have shape"), ((H, X, W, W, H, None), "up must be a"),
-    ((H, X, W, W, H, H, "none"), "activation must be"), ((H, X, W, W, H, H), "x is on cpu"),
+    ((H.half(), X, W, W, G, G), "grad must be a bfloat16 tensor"), ((H[:2], X, W, W, G, G), "grad must have shape"),
+    ((H, X, W, W, G[:, :39], G), "gate must have shape"), ((H, X, W, W, H, G), "gate must be a float32 tensor"), ((H, X, W, W, G, None), "up must be a"),
+    ((H, X, W, W, G, G, "none"), "activation must be"), ((H, X, W, W, G, G), "x is on cpu"),
 ])
 def test_gated_grad(args, msg):
     with pytest.raises(th.ThrmlError, match=msg):

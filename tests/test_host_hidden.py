@@ -52,8 +52,8 @@ REFUSED = [
     (_forward(xs=-70), "x: stride -70 is negative"), (_forward(wg=None), "w_gate is NULL"), (_forward(wu=P + 1), "w_up is not aligned"),
     (_forward(us=-1), "w_up: stride -1"), (_forward(h=None), "h is NULL"), (_forward(hs=39), "h: stride 39 makes rows overlap"),
     (_forward(gate=None), "gate and up go together"), (_forward(up=None), "gate and up go together"),
-    (_forward(gate=P + 1), "gate is not aligned"), (_forward(work=None), "work holds 0 bytes"), (_forward(have=100), "work holds 100 bytes"),
-    (_forward(work=P + 8), "work is not aligned"),
+    (_forward(gate=P + 1), "gate is not aligned"), (_forward(rows=99, work=None), "work holds 0 bytes"), (_forward(rows=99, have=100), "work holds 100 bytes"),
+    (_forward(rows=99, work=P + 8), "work is not aligned"),
     (_backward(grad=None), "grad is NULL"), (_backward(gs=-1), "grad: stride -1"), (_backward(gate=None), "gate is NULL"),
     (_backward(up=None), "up is NULL"), (_backward(dx=P + 1), "dx is not aligned"), (_backward(dxs=69), "dx: stride 69"),
     (_backward(dwg=None), "dw_gate is NULL"), (_backward(dwu=P + 1), "dw_up is not aligned"), (_backward(have=5), "work holds 5 bytes"),
@@ -68,7 +68,7 @@ REFUSED = [
     (_f8(q=0), "q must be positive"), (_f8(rows=(1 << 30) + 1), "2\\^30 rows"), (_f8(dtype=0), "x must be"), (_f8(od=7), "output must be"),
     (_f8(x=None), "x is NULL"), (_f8(w=None), "w is NULL"), (_f8(ws=-70), "w: stride -70"), (_f8(sc=None), "w_scale is NULL"),
     (_f8(sc=P + 2), "w_scale is not aligned"), (_f8(b=P + 2), "bias is not aligned"), (_f8(y=None), "y is NULL"),
-    (_f8(ys=39), "rows overlap"), (_f8(work=None), "work holds 0 bytes"), (_f8(have=100), "bytes"), (_f8(work=P + 4), "not aligned to 16"),
+    (_f8(ys=39), "rows overlap"), (_f8(rows=99, work=None), "work holds 0 bytes"), (_f8(rows=99, have=100), "bytes"), (_f8(rows=99, work=P + 4), "not aligned to 16"),
 ]
 
 
@@ -102,10 +102,10 @@ def _names(calls):
 def test_aligned_operands_are_not_copied():
     for k, pad, shift, copied in ((64, 0, 0, False), (64, 8, 0, False), (64, 8, 16, False), (65, 0, 0, True), (64, 1, 0, True),
                                   (64, 0, 2, True), (63, 1, 0, True)):
-        names, = _names([_forward(k=k, xs=k + pad, gs=k + pad, us=k + pad, x=P + shift, wg=P + shift, wu=P + shift)])
+        names, = _names([_forward(rows=99, k=k, xs=k + pad, gs=k + pad, us=k + pad, x=P + shift, wg=P + shift, wu=P + shift)])
         assert ("gated_pack_kernel" in names) == copied, (k, pad, shift, names)
     for k, pad, shift, copied in ((64, 0, 0, False), (80, 16, 0, False), (64, 0, 16, False), (64, 8, 0, True), (72, 0, 0, True), (64, 0, 8, True)):
-        names, = _names([_f8(k=k, xs=k, ws=k + pad, w=P + shift)])
+        names, = _names([_f8(rows=99, k=k, xs=k, ws=k + pad, w=P + shift)])
         assert ("f8_pack_kernel" in names) == copied, (k, pad, shift, names)
 
 
@@ -127,6 +127,22 @@ def _work_calls():
             for have in (w, w - 1) if w else ():
                 out.append((f(dev.handle, d, *a, P, have), have == w))
         w = lib.thrml_linear_f8_work(dev.handle, 2, rows, k, P, n, k, 1)
-        for have in (w, w - 1):
+        for have in (w, w - 1) if w else ():
             out.append((lib.thrml_linear_f8(dev.handle, P, 2, rows, k, k, P, n, k, P, None, P, 1, n, P, have), have == w))
     return out
+
+
+def test_few_unaligned_rows_are_read_as_they_lie():
+    for call, kernel in ((_forward(rows=16, k=71), "gated_few_kernel"), (_forward(rows=32, k=71, work=None, have=0), "gated_few_kernel"),
+                         (_f8(rows=64, k=71, xs=71), "f8_few_kernel")):
+        names, = _names([call])
+        assert kernel in names and "pack" not in names and "tile" not in names, (call, names)
+
+
+def test_each_kind_of_tile():
+    """the shapes that the GPU tests name reach the tiles that they are meant for"""
+    names = _names([_forward(rows=r, k=k, n=n, xs=k, gs=k, us=k, hs=n) for r, k, n in ((1, 4096, 704), (64, 4096, 8192), (512, 1024, 4096), (2056, 1024, 2048))])
+    for shape, got in zip(("64,32,1,1,4", "64,32,1,2,2", "64,64,2,2,1", "128,64,2,4,1"), names):
+        mangled = "".join(f"Li{n}E" for n in shape.split(","))
+        assert shape in got or mangled in got, (shape, got)
+    assert "join" in names[0]

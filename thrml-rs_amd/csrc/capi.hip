@@ -2260,15 +2260,15 @@ extern "C" uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int 
              : 0;
 }
 
-extern "C" int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, void *gate,
-                                   void *up, void *work, uint64_t work_bytes) {
+extern "C" int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, float *gate,
+                                   float *up, void *work, uint64_t work_bytes) {
   if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
   if (int rc = check_gated(in)) return rc;
   if (int rc = check_rows("h", h, 2, in->rows, in->n, h_stride, true)) return rc;
   if (in->rows && !gate != !up) return fail(THRML_EINVAL, "gate and up go together");
   if (gate) {
-    if (int rc = check_rows("gate", gate, 2, in->rows, in->n, in->n, true)) return rc;
-    if (int rc = check_rows("up", up, 2, in->rows, in->n, in->n, true)) return rc;
+    if (int rc = check_rows("gate", gate, 4, in->rows, in->n, in->n, true)) return rc;
+    if (int rc = check_rows("up", up, 4, in->rows, in->n, in->n, true)) return rc;
   }
   if (int rc = check_work(work, work_bytes, thrml_gated_work(ctx, in, 0))) return rc;
   THRML_HIP(hipSetDevice(ctx->device));
@@ -2276,13 +2276,13 @@ extern "C" int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *
 }
 
 extern "C" int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
-                                    const void *gate, const void *up, void *dx, int64_t dx_stride, void *dw_gate,
+                                    const float *gate, const float *up, void *dx, int64_t dx_stride, void *dw_gate,
                                     void *dw_up, void *work, uint64_t work_bytes) {
   if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
   if (int rc = check_gated(in)) return rc;
   if (int rc = check_rows("grad", grad, 2, in->rows, in->n, grad_stride, false)) return rc;
-  if (int rc = check_rows("gate", gate, 2, in->rows, in->n, in->n, false)) return rc;
-  if (int rc = check_rows("up", up, 2, in->rows, in->n, in->n, false)) return rc;
+  if (int rc = check_rows("gate", gate, 4, in->rows, in->n, in->n, false)) return rc;
+  if (int rc = check_rows("up", up, 4, in->rows, in->n, in->n, false)) return rc;
   if (dx)
     if (int rc = check_rows("dx", dx, 2, in->rows, in->k, dx_stride, true)) return rc;
   if (int rc = check_rows("dw_gate", dw_gate, 2, in->n, in->k, in->k, true)) return rc;

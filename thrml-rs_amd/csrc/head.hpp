@@ -105,9 +105,9 @@ int launch_dropout(thrml_ctx *ctx, DropoutArgs a, int dtype);
 uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype);
 int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, void *work);
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward);
-int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, void *gate, void *up, void *work);
-int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const void *gate,
-                      const void *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work);
+int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, float *gate, float *up, void *work);
+int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const float *gate,
+                      const float *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work);
 
 // ---------------------------------------------------------------------------
 // Device helpers

@@ -399,13 +399,8 @@ __global__ __launch_bounds__(256) void f8_join_kernel(F8Tiles g) {
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < g.rows * groups; i += (uint64_t)gridDim.x * 256u) {
     const uint64_t row = i / groups;
     const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = g.q - c;
-    float v[8] = {};
-    for (uint32_t s = 0; s < g.splits; ++s) {
-      const float *p = g.part + (s * g.rows + row) * g.q + c;
-#pragma unroll
-      for (uint32_t e = 0; e < 8; ++e)
-        if (e < m) v[e] += p[e];
-    }
+    float v[8];
+    join8(g.part + row * g.q + c, g.rows * g.q, g.splits, m, v);
     if (g.bias) {
 #pragma unroll
       for (uint32_t e = 0; e < 8; ++e)

@@ -8,8 +8,9 @@
 // writes dz and du, rounded to 16 bits as operands of the two products behind it have to
 // be (half a step of 2^-8 or 2^-11, as is every operand), and those products, whose
 // operands lie across the reduction and are transposed on their way from LDS.
-// z and u are kept between the two in 16 bits: recomputing them in f32 would cost half
-// of the backward pass again.
+// z and u are kept between the two in f32 (rounded to 16 bits they would put as much error
+// again into the gradients as dz, du and the results' own rounding have together: 3.1e-3 of the
+// norm in bf16, not 2.4e-3; at 4096 x 8192 it would save 60 us of a step's 1450).
 #include "tile.hpp"
 
 namespace thrml {
@@ -245,8 +246,8 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
         } else if constexpr (OP == G_FORWARD) {
           const int64_t saved = (int64_t)row * g.n + c;
           if (g.out1) {
-            store8(reinterpret_cast<T *>(g.out1) + saved, m, v);
-            store8(reinterpret_cast<T *>(g.out2) + saved, m, w);
+            store8(reinterpret_cast<float *>(g.out1) + saved, m, v);
+            store8(reinterpret_cast<float *>(g.out2) + saved, m, w);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
@@ -338,8 +339,8 @@ __global__ __launch_bounds__(256) void gated_few_kernel(GatedTiles g, int64_t ga
     }
     const int64_t saved = (int64_t)row * g.n + cc;
     if (g.out1) {
-      store4(reinterpret_cast<T *>(g.out1) + saved, g.n - cc, v);
-      store4(reinterpret_cast<T *>(g.out2) + saved, g.n - cc, w);
+      store4(reinterpret_cast<float *>(g.out1) + saved, g.n - cc, v);
+      store4(reinterpret_cast<float *>(g.out2) + saved, g.n - cc, w);
     }
     store4(reinterpret_cast<T *>(g.out) + (int64_t)row * g.out_stride + cc, g.n - cc, h);
   }
@@ -353,21 +354,15 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
     const uint64_t row = i / groups;
     const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = cols - c;
-    float v[8] = {}, w[8] = {};
-    for (uint32_t s = 0; s < g.splits; ++s) {
-      const float *p = g.part + (s * rows + row) * pitch + c;
-#pragma unroll
-      for (uint32_t e = 0; e < 8; ++e)
-        if (e < m) {
-          v[e] += p[e];
-          if (OP == G_FORWARD) w[e] += p[g.n + e];
-        }
-    }
+    float v[8], w[8];
+    const float *p = g.part + row * pitch + c;
+    join8(p, rows * pitch, g.splits, m, v);
+    if (OP == G_FORWARD) join8(p + g.n, rows * pitch, g.splits, m, w);
     if constexpr (OP == G_FORWARD) {
       const int64_t saved = (int64_t)row * g.n + c;
       if (g.out1) {
-        store8(reinterpret_cast<T *>(g.out1) + saved, m, v);
-        store8(reinterpret_cast<T *>(g.out2) + saved, m, w);
+        store8(reinterpret_cast<float *>(g.out1) + saved, m, v);
+        store8(reinterpret_cast<float *>(g.out2) + saved, m, w);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
@@ -381,11 +376,11 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
   }
 }
 
-// dz and du from dh and the z and u that the forward pass kept: rows of 2 np elements,
+// dz and du from dh and the z and u that the forward pass kept (14 bytes a unit): rows of 2 np elements,
 // zeros behind the n of each half.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ grad, int64_t grad_stride,
-                                                          const T *__restrict__ z, const T *__restrict__ u, uint64_t rows,
+                                                          const float *__restrict__ z, const float *__restrict__ u, uint64_t rows,
                                                           uint32_t n, uint32_t np, T *__restrict__ d) {
   const uint32_t groups = np / 8u;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
@@ -393,8 +388,10 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
     const uint32_t c = (uint32_t)(i - row * groups) * 8u;
     float a[8], b[8];
     if (c < n) {
-      Raw8<T> rg, rz, ru;
-      const T *pg = grad + (int64_t)row * grad_stride + c, *pz = z + row * n + c, *pu = u + row * n + c;
+      Raw8<T> rg;
+      Raw8<float> rz, ru;
+      const T *pg = grad + (int64_t)row * grad_stride + c;
+      const float *pz = z + row * n + c, *pu = u + row * n + c;
       if (c + 8u <= n) {
         load8(pg, rg);
         load8(pz, rz);
@@ -455,7 +452,7 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
          (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
 }
 
-static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.25f, 0.2f}, {128, 128, 128, 0.5f, 0.45f}, {256, 256, 128, 1.0f, 1.0f}};
+static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.30f, 0.20f}, {64, 64, 128, 0.36f, 0.23f}, {128, 128, 128, 0.57f, 0.62f}, {256, 256, 128, 0.9f, 1.5f}};
 typedef TileShape<64, 32, 1, 1, 4, 128, 4, false> Tile32;
 typedef TileShape<64, 32, 1, 2, 2, 128, 4, false> Tile64;
 typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> Tile128;
@@ -565,7 +562,7 @@ static int operands(thrml_ctx *ctx, const thrml_gated &g, const GatedPlan &p, ui
   return THRML_OK;
 }
 
-int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, void *gate, void *up, void *work) {
+int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, float *gate, float *up, void *work) {
   if (g.rows == 0) return THRML_OK;
   const GatedPlan p(ctx, g);
   uint8_t *w = reinterpret_cast<uint8_t *>(work);
@@ -604,8 +601,8 @@ int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride
   return with_gated(g, [&](auto e, auto act) { return launch_product<G_FORWARD, decltype(e), decltype(act)::value>(ctx, p.forward, t); });
 }
 
-int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const void *gate,
-                      const void *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work) {
+int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, int64_t grad_stride, const float *gate,
+                      const float *up, void *dx, int64_t dx_stride, void *dw_gate, void *dw_up, void *work) {
   if (g.rows == 0) {
     const uint64_t n = (uint64_t)g.n * g.k;
     hipLaunchKernelGGL(gated_zero_kernel, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
@@ -628,8 +625,7 @@ int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, in
     const uint64_t n = g.rows * (p.np / 8u);
     auto *slope = &gated_slope_kernel<T, decltype(act)::value>;
     hipLaunchKernelGGL(slope, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
-                       reinterpret_cast<const T *>(grad), grad_stride, reinterpret_cast<const T *>(gate),
-                       reinterpret_cast<const T *>(up), g.rows, g.n, p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)));
+                       reinterpret_cast<const T *>(grad), grad_stride, gate, up, g.rows, g.n, p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)));
     THRML_HIP(hipGetLastError());
     // (the products do not use the activation)
     if (dx) {

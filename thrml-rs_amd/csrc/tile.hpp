@@ -264,6 +264,23 @@ __device__ __forceinline__ uint32_t tile_start(uint32_t ia, uint32_t n, bool sma
   return small_b ? ia * 5u % n : (blockIdx.x & 7u) * n / 8u;
 }
 
+// The sums of the splits for 8 neighbouring values (n of them, at most 8), added in their
+// order; several loads are under way together.
+__device__ __forceinline__ void join8(const float *p, uint64_t pitch, uint32_t splits, uint32_t n, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+#pragma unroll 4
+  for (uint32_t s = 0; s < splits; ++s) {
+    Raw8<float> r;
+    if (n >= 8u)
+      load8(p + s * pitch, r);
+    else
+      load8_part(p + s * pitch, n, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += value(r, e);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // On the host: which tiles a call takes
 static inline uint64_t tile_bytes(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
@@ -271,7 +288,7 @@ static inline uint64_t tile_bytes(uint64_t n) { return (n + 255u) & ~(uint64_t)2
 struct TileKind {
   uint32_t na, nb;
   uint32_t kb;        // bytes of a row in a stage
-  float alone, many;  // us a stage: of a tile alone on a compute unit, and of one of several
+  float alone, many;  // us a stage: of a tile where few compute units have one, and where each has one or several
 };
 
 struct TilePlan {
@@ -293,10 +310,12 @@ static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, i
     const uint64_t tiles = (uint64_t)ta * tb;
     const uint32_t steps = tile_cdiv(row_bytes, kd.kb);
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (steps < 8 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
-      const double one = std::max<double>(kd.alone, (double)kd.many * (double)tile_cdiv(tiles * splits, ctx->cu_count));
-      // a join reads what the splits wrote, 3 bytes a ps, and is a launch
-      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 5.0 + (double)out_values * 4 * 2 * splits / 3e6 : 0.0);
+      if (splits > 1 && (steps < 4 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
+      const uint64_t groups = tiles * splits, cus = (uint64_t)ctx->cu_count;
+      const double one = groups > cus ? (double)kd.many * (double)tile_cdiv(groups, cus)
+                                      : kd.alone + std::max(0.0f, kd.many - kd.alone) * (double)groups / (double)cus;
+      // a join reads what the splits wrote, together 4.5 bytes a ps, and is a launch
+      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 7.0 + (double)out_values * 4 * 2 * splits / 4.5e6 : 0.0);
       if (best_t == 0.0 || t < best_t) {
         best_t = t;
         best.kind = i;

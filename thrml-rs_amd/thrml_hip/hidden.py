@@ -51,8 +51,7 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
     """Hidden units h [rows, n] = act(x @ w_gate.T) * (x @ w_up.T) of features x [rows, k]
     and weights [n, k], all bfloat16 or all float16; sums, activation and product in
     float32, rounded once.  activation: "silu", "gelu" (of the error function) or "relu".
-    With save, (h, gate, up): also both products, rounded to the type, for
-    gated_linear_grad.  out: a tensor for h, other than x and the weights.
+    With save, (h, gate, up): also both products in float32, for gated_linear_grad.  out: a tensor for h, other than x and the weights.
 
     Rows that are not whole 16-byte pieces (k not a multiple of 8, a view that starts or
     steps elsewhere) are copied first; the weights of a model are better kept aligned."""
@@ -69,7 +68,7 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
     where = out.device
     gate = up = None
     if save:
-        gate, up = (head.torch.empty((rows, n), dtype=dtype, device=where) for _ in range(2))
+        gate, up = (head.torch.empty((rows, n), dtype=head.torch.float32, device=where) for _ in range(2))
     lib = load()
     size = lib.thrml_gated_work(device.handle, d, 0)
     work = head.torch.empty(size, dtype=head.torch.uint8, device=where) if size else None
@@ -80,8 +79,8 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
 
 def gated_linear_grad(device, grad, x, w_gate, w_up, gate, up, activation="silu", input_grad=True):
     """(dx, dw_gate, dw_up): the gradients of a loss in x [rows, k] and the weights [n, k],
-    in their type, from grad [rows, n], its gradient in gated_linear's result, and the
-    products gate and up that this kept.  With z = gate, u = up:
+    in their type, from grad [rows, n], its gradient in gated_linear's result in that type,
+    and the products gate and up [rows, n] float32 that this kept.  With z = gate, u = up:
       dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
       dx = dz @ w_gate + du @ w_up,  dw_gate = dz.T @ x,  dw_up = du.T @ x
     relu'(0) is 0.  Without rows the weights' gradients are 0.  input_grad False: dx is
@@ -89,8 +88,8 @@ def gated_linear_grad(device, grad, x, w_gate, w_up, gate, up, activation="silu"
     d, keep, rows, k, n = _gated(x, w_gate, w_up, activation)
     same = (keep[0].dtype,)
     grad, grad_stride = _matrix("grad", grad, same, rows, n)
-    gate, _ = _matrix("gate", gate, same, rows, n)
-    up, _ = _matrix("up", up, same, rows, n)
+    gate, _ = _matrix("gate", gate, head._FLOAT32, rows, n)
+    up, _ = _matrix("up", up, head._FLOAT32, rows, n)
     gate, up = gate.contiguous(), up.contiguous()
     _on_device(device, _NAMES + ("grad", "gate", "up"), keep + (grad, gate, up), False)
     torch, where = head.torch, keep[0].device
