@@ -265,8 +265,10 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   }
 }
 
-// Few rows, operands at any alignment (tile.hpp): a workgroup takes 16 units and up to 64
+// Few rows, operands at any alignment (tile.hpp): a workgroup takes 16 units and up to 32
 // rows; its four waves take turns in the stages of 128 bytes, and their sums meet in LDS.
+// One row of 4095 x 16384 in bf16: 75 us, by tiles from a copy 165 (50 at 4096); 32 of 4095 x
+// 8192: 64, from a copy 83.
 template <class T>
 struct FewFrag;
 template <>
@@ -297,21 +299,22 @@ __global__ __launch_bounds__(256) void gated_few_kernel(GatedTiles g, int64_t ga
   f32x4 z[ROWS16] = {}, u[ROWS16] = {};
 #pragma unroll 2
   for (uint32_t s = wave; s < steps; s += 4u) {
-    u32x4 a[2][2], b[ROWS16][2];
+    RowPiece a[2][2], b[ROWS16][2];
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
       const uint32_t at = s * 128u + hi * 16u + h * 64u;
-      a[0][h] = row_piece(wg, at, bytes);
-      a[1][h] = row_piece(wu, at, bytes);
+      a[0][h].load(wg, at, bytes);
+      a[1][h].load(wu, at, bytes);
 #pragma unroll
-      for (int j = 0; j < ROWS16; ++j) b[j][h] = row_piece(x[j], at, bytes);
+      for (int j = 0; j < ROWS16; ++j) b[j][h].load(x[j], at, bytes);
     }
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < ROWS16; ++j) {
-        z[j] = FewFrag<T>::mul(a[0][h], b[j][h], z[j]);
-        u[j] = FewFrag<T>::mul(a[1][h], b[j][h], u[j]);
+        const u32x4 xs = b[j][h].get();
+        z[j] = FewFrag<T>::mul(a[0][h].get(), xs, z[j]);
+        u[j] = FewFrag<T>::mul(a[1][h].get(), xs, u[j]);
       }
   }
 #pragma unroll

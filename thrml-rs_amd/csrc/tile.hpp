@@ -230,20 +230,34 @@ __device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch
 // ---------------------------------------------------------------------------
 // Few rows whose operands do not start at 16 bytes: straight from memory into the operand
 // registers of 16 x 16 products, without a copy.  16 bytes of a row from byte c on, zeros
-// from byte n on; p at any address (such a load takes longer than one of whole pieces, but
-// a copy reads and writes all of it).
-typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
-__device__ __forceinline__ u32x4 row_piece(const uint8_t *p, uint32_t c, uint32_t n) {
-  if (c + 16u <= n) return *reinterpret_cast<const u32x4_a1 *>(p + c);
+// from byte n on; p at any address.  The words that hold them are loaded and shifted: loads
+// from addresses within a word take longer.
+struct RowPiece {
   u32x4 v = {0, 0, 0, 0};
-  if (c < n) {
-    const uint32_t left = here(n - c);
+  uint32_t next = 0, shift = 0;
+  __device__ __forceinline__ void load(const uint8_t *p, uint32_t c, uint32_t n) {
+    typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (c + 20u <= n) {
+      shift = (uint32_t)(uintptr_t)p & 3u;
+      const uint8_t *at = p + c - shift;
+      v = *reinterpret_cast<const u32x4_a4 *>(at);
+      next = reinterpret_cast<const uint32_t *>(at)[shift ? 4 : 0];
+    } else {
+      v = u32x4{0, 0, 0, 0};
+      shift = 0;
+      if (c < n) {
+        const uint32_t left = here(n - c);
 #pragma unroll
-    for (uint32_t j = 0; j < 15; ++j)
-      if (j < left) v[j / 4u] |= (uint32_t)p[c + j] << (8u * (j & 3u));
+        for (uint32_t j = 0; j < 16; ++j)
+          if (j < left) v[j / 4u] |= (uint32_t)p[c + j] << (8u * (j & 3u));
+      }
+    }
   }
-  return v;
-}
+  __device__ __forceinline__ u32x4 get() const {
+    return u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], shift), __builtin_amdgcn_alignbyte(v[2], v[1], shift),
+                 __builtin_amdgcn_alignbyte(v[3], v[2], shift), __builtin_amdgcn_alignbyte(next, v[3], shift)};
+  }
+};
 
 // Tiles in an order in which those that run together share operands: workgroups of one
 // XCD take neighbouring tiles, 8 of side B at a time.
