@@ -570,7 +570,7 @@ typedef struct {
   const void *w_up;
   int64_t up_stride;
 } thrml_gated;
-/* h[row][c] rounded once to the type; gate and up, both or neither NULL, receive z and
+/* h[row][c] rounded once to the type (not x or a weight); gate and up, both or neither NULL, receive z and
  * u in f32, [rows][n] contiguous, for thrml_gated_backward.  work: thrml_gated_work(in, 0)
  * bytes.  The operands are read as they lie where their rows are whole 16-byte pieces
  * (k a multiple of 8, pointers of 16 bytes, strides of 8 elements, those of the two

@@ -194,3 +194,66 @@ def test_captured(device):
     del graphs
     torch.cuda.synchronize()
     dev.close()
+
+
+@pytest.mark.parametrize("stride", [(1 << 22) - 8, 1 << 22])
+def test_rows_far_apart(device, stride):
+    """offsets that pass 32 bits, at the largest stride that tiles read as it lies and at
+    the first that is copied"""
+    rows, k, n = 600, 64, 72
+    x, wg, wu, dh = _inputs(rows, k, n, BF16)
+    wide = torch.empty((rows - 1) * stride + k, dtype=BF16, device="cuda")
+    far = wide.as_strided((rows, k), (stride, 1))
+    far.copy_(x)
+    h, gate, up = th.gated_linear(device, x, wg, wu, save=True)
+    assert torch.equal(th.gated_linear(device, far, wg, wu), h)
+    for got, want in zip(th.gated_linear_grad(device, dh, far, wg, wu, gate, up), th.gated_linear_grad(device, dh, x, wg, wu, gate, up)):
+        assert torch.equal(got, want)
+
+
+def test_two_threads(device):
+    """two devices' calls at once, each on its own stream, give what each gives alone"""
+    import threading
+
+    cases = [(70, 200, 130), (300, 264, 512)]
+    ins = [_inputs(*c, BF16, seed=3) for c in cases]
+    want = [th.gated_linear(device, x, wg, wu) for x, wg, wu, _ in ins]
+    torch.cuda.synchronize()
+    wrong, errors = [0, 0], []
+
+    def work(i):
+        try:
+            dev, side = th.Device(0), torch.cuda.Stream()
+            dev.set_stream(side.cuda_stream)
+            with torch.cuda.stream(side):
+                for _ in range(20):
+                    x, wg, wu, _ = ins[i]
+                    wrong[i] += int(not torch.equal(th.gated_linear(dev, x, wg, wu), want[i]))
+            side.synchronize()
+            dev.close()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and wrong == [0, 0]
+
+
+def test_refuses_what_would_be_overwritten(device):
+    x, wg, wu, _ = _inputs(64, 64, 64, BF16)
+    for out in (x, wg, wu):
+        with pytest.raises(th.ThrmlError, match="h must not be x or a weight"):
+            th.gated_linear(device, x, wg, wu, out=out)
+
+
+def test_tensors_that_require_a_gradient(device):
+    x, wg, wu, dh = _inputs(9, 64, 64, BF16)
+    x.requires_grad_(True)
+    with pytest.raises(th.ThrmlError, match="x requires a gradient"):
+        th.gated_linear(device, x, wg, wu)
+    with torch.no_grad():
+        _, gate, up = th.gated_linear(device, x, wg, wu, save=True)
+    assert not any(t.requires_grad for t in th.gated_linear_grad(device, dh, x, wg, wu, gate, up))

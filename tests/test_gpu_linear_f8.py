@@ -155,3 +155,26 @@ def test_streams_and_graphs(device):
     del graphs
     torch.cuda.synchronize()
     dev.close()
+
+
+@pytest.mark.parametrize("stride", [(1 << 23) - 16, 1 << 23])
+def test_rows_far_apart(device, stride):
+    """weights whose offsets pass 32 bits, at the largest stride that tiles read as it lies and
+    at the first that is copied"""
+    rows, k, q = 100, 144, 600
+    x, w, ws, bias = _inputs(rows, k, q, BF16)
+    wide = torch.empty((q - 1) * stride + k, dtype=torch.uint8, device="cuda").view(F8)
+    far = wide.as_strided((q, k), (stride, 1))
+    far.view(torch.uint8).copy_(w.view(torch.uint8))
+    want = th.linear_f8(device, x, w, ws, bias=bias)
+    assert torch.equal(th.linear_f8(device, x, far, ws, bias=bias), want)
+    ref.close(th.linear_f8(device, x[:5], far, ws, bias=bias).cpu(), *ref.linear_f8(x[:5], w, ws, bias, BF16), "few rows")
+
+
+def test_few_rows_of_every_count(device):
+    """rows quantised by the workgroups themselves, or read by the kernel for unaligned weights"""
+    for k in (256, 257):
+        x, w, ws, bias = _inputs(65, k, 200, F16)
+        for rows in (1, 2, 15, 16, 17, 31, 32, 33, 48, 49, 64, 65):
+            got = th.linear_f8(device, x[:rows], w, ws, bias=bias)
+            ref.close(got.cpu(), *ref.linear_f8(x[:rows], w, ws, bias, F16), f"{rows} rows of {k}")

@@ -45,7 +45,7 @@ def test_gated_grad(args, msg):
     (X, 5, 0.5, {}, "key must be an RngKey or"), (X, None, 0.5, {}, "key must be"),
     (X, torch.zeros(2, dtype=torch.int64), 0.5, {}, "key must be"), (X, torch.zeros(1), 0.5, {}, "key must be"),
     (X, KEY, 0.5, dict(residual=X.half()), "residual must be a bfloat16 tensor"),
-    (X, KEY, 0.5, dict(residual=X[:2]), "residual must have shape"), (X, KEY, 0.5, dict(first_row=-1), "first_row must not"),
+    (X, KEY, 0.5, dict(residual=X[:2]), "residual must have shape"), (X, KEY, 0.5, dict(first_row=-1), "first_row must lie"), (X, KEY, 0.5, dict(first_row=1 << 64), "first_row must lie"),
     (X, KEY, 0.5, dict(out=X[:2]), "out must be"), (X, KEY, 0.5, {}, "x is on cpu"),
 ])
 def test_dropout(x, key, p, kw, msg):

@@ -7,6 +7,7 @@ import hostrun
 import thrml_hip as th
 from thrml_hip import _lib, hidden
 
+Q = 1 << 21
 P = 1 << 20  # an address that nothing reads: kernels do not run there
 WORK = 1 << 50
 
@@ -26,11 +27,11 @@ def _calls(calls):
     return out
 
 
-def _forward(h=P, hs=40, gate=P, up=P, work=P, have=WORK, ctx="ctx", **kw):
+def _forward(h=Q, hs=40, gate=P, up=P, work=P, have=WORK, ctx="ctx", **kw):
     return "thrml_gated_forward", [ctx, _desc(**kw), h, hs, gate, up, work, have]
 
 
-def _backward(grad=P, gs=40, gate=P, up=P, dx=P, dxs=70, dwg=P, dwu=P, work=P, have=WORK, **kw):
+def _backward(grad=P, gs=40, gate=P, up=P, dx=Q, dxs=70, dwg=Q, dwu=Q, work=P, have=WORK, **kw):
     wgs = kw.pop("wgs", 70)
     return "thrml_gated_backward", ["ctx", _desc(gs=wgs, **kw), grad, gs, gate, up, dx, dxs, dwg, dwu, work, have]
 
@@ -55,8 +56,10 @@ REFUSED = [
     (_forward(gate=P + 1), "gate is not aligned"), (_forward(rows=99, work=None), "work holds 0 bytes"), (_forward(rows=99, have=100), "work holds 100 bytes"),
     (_forward(rows=99, work=P + 8), "work is not aligned"),
     (_backward(grad=None), "grad is NULL"), (_backward(gs=-1), "grad: stride -1"), (_backward(gate=None), "gate is NULL"),
-    (_backward(up=None), "up is NULL"), (_backward(dx=P + 1), "dx is not aligned"), (_backward(dxs=69), "dx: stride 69"),
-    (_backward(dwg=None), "dw_gate is NULL"), (_backward(dwu=P + 1), "dw_up is not aligned"), (_backward(have=5), "work holds 5 bytes"),
+    (_backward(up=None), "up is NULL"), (_backward(dx=Q + 1), "dx is not aligned"), (_backward(dxs=69), "dx: stride 69"),
+    (_backward(dwg=None), "dw_gate is NULL"), (_backward(dwu=Q + 1), "dw_up is not aligned"), (_backward(have=5), "work holds 5 bytes"),
+    (_forward(h=P), "h must not be x or a weight"), (_backward(dx=P), "dx must not be"), (_backward(dwg=P), "dw_gate must not be"),
+    (_backward(dwu=P), "dw_up must not be"),
     (_dropout(ctx=None), "NULL argument"), (_dropout(dtype=0), "x must be"), (_dropout(p=-0.1), "p must lie in"),
     (_dropout(p=1.1), "p must lie in"), (_dropout(p=float("nan")), "p must lie in"), (_dropout(x=None), "x is NULL"),
     (_dropout(x=P + 1), "x is not aligned"), (_dropout(xs=-1), "x: stride -1"), (_dropout(res=P + 1), "residual is not aligned"),
@@ -123,7 +126,7 @@ def _work_calls():
         for back in (0, 1):
             w = lib.thrml_gated_work(dev.handle, d, back)
             f = lib.thrml_gated_backward if back else lib.thrml_gated_forward
-            a = (P, n, P, P, P, k, P, P) if back else (P, n, P, P)
+            a = (P, n, P, P, Q, k, Q, Q) if back else (Q, n, P, P)
             for have in (w, w - 1) if w else ():
                 out.append((f(dev.handle, d, *a, P, have), have == w))
         w = lib.thrml_linear_f8_work(dev.handle, 2, rows, k, P, n, k, 1)

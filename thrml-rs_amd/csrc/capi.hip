@@ -2252,6 +2252,13 @@ int check_gated(const thrml_gated *in) {
   return check_rows("w_up", in->w_up, 2, in->n, in->k, in->up_stride, false);
 }
 
+// An output that other workgroups still read as an operand
+int check_apart(const thrml_gated *in, const char *name, const void *p) {
+  if (in->rows && p && (p == in->x || p == in->w_gate || p == in->w_up))
+    return fail(THRML_EINVAL, std::string(name) + " must not be x or a weight");
+  return THRML_OK;
+}
+
 }  // namespace
 
 extern "C" uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward) {
@@ -2265,6 +2272,7 @@ extern "C" int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *
   if (!ctx || !in) return fail(THRML_EINVAL, "NULL argument");
   if (int rc = check_gated(in)) return rc;
   if (int rc = check_rows("h", h, 2, in->rows, in->n, h_stride, true)) return rc;
+  if (int rc = check_apart(in, "h", h)) return rc;
   if (in->rows && !gate != !up) return fail(THRML_EINVAL, "gate and up go together");
   if (gate) {
     if (int rc = check_rows("gate", gate, 4, in->rows, in->n, in->n, true)) return rc;
@@ -2285,6 +2293,9 @@ extern "C" int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const
   if (int rc = check_rows("up", up, 4, in->rows, in->n, in->n, false)) return rc;
   if (dx)
     if (int rc = check_rows("dx", dx, 2, in->rows, in->k, dx_stride, true)) return rc;
+  const std::pair<const char *, const void *> outs[] = {{"dx", dx}, {"dw_gate", dw_gate}, {"dw_up", dw_up}};
+  for (const auto &o : outs)
+    if (int rc = check_apart(in, o.first, o.second)) return rc;
   if (int rc = check_rows("dw_gate", dw_gate, 2, in->n, in->k, in->k, true)) return rc;
   if (int rc = check_rows("dw_up", dw_up, 2, in->n, in->k, in->k, true)) return rc;
   if (int rc = check_work(work, work_bytes, thrml_gated_work(ctx, in, 1))) return rc;

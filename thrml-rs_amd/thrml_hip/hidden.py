@@ -136,8 +136,8 @@ def dropout(device, x, key, p, residual=None, first_row=0, out=None):
         if seed is None:
             _refuse("key must be an RngKey or an int64 tensor of one element")
     first_row = int(first_row)
-    if first_row < 0:
-        _refuse("first_row must not be negative")
+    if not 0 <= first_row <= 1 << 37:
+        _refuse("first_row must lie in 0 .. 2^37")
     if out is not None:
         _out("out", out, rows, cols, x.dtype)
         if (out is x0 and x is not x0) or (out is residual0 and residual is not residual0):
