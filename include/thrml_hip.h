@@ -609,7 +609,7 @@ int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint6
  * or f16 the products of a block are added by the 8-bit matrix unit, which keeps 2^-16 of
  * the largest; for y in f32 exactly.  A row of x with an infinity or a NaN gives NaN.
  * work: thrml_linear_f8_work bytes, for the same arguments. */
-uint64_t thrml_linear_f8_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t k, const void *w, uint32_t q,
+uint64_t thrml_linear_f8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, const void *w, uint32_t q,
                               int64_t w_stride, int out_dtype);
 int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
                     const void *w, uint32_t q, int64_t w_stride, const float *w_scale, const float *bias,

@@ -129,7 +129,7 @@ def _work_calls():
             a = (P, n, P, P, Q, k, Q, Q) if back else (Q, n, P, P)
             for have in (w, w - 1) if w else ():
                 out.append((f(dev.handle, d, *a, P, have), have == w))
-        w = lib.thrml_linear_f8_work(dev.handle, 2, rows, k, P, n, k, 1)
+        w = lib.thrml_linear_f8_work(dev.handle, rows, k, P, n, k, 1)
         for have in (w, w - 1) if w else ():
             out.append((lib.thrml_linear_f8(dev.handle, P, 2, rows, k, k, P, n, k, P, None, P, 1, n, P, have), have == w))
     return out

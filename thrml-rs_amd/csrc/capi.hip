@@ -2331,7 +2331,7 @@ constexpr uint32_t F8_MAX_K = 1u << 20;  // a tile's rows lie within 32 bits
 
 }  // namespace
 
-extern "C" uint64_t thrml_linear_f8_work(thrml_ctx *ctx, int dtype, uint64_t rows, uint32_t k, const void *w, uint32_t q,
+extern "C" uint64_t thrml_linear_f8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, const void *w, uint32_t q,
                                          int64_t w_stride, int out_dtype) {
   if (!ctx || !rows || !k || !q || rows > HEAD_MAX_ROWS || q > HEAD_MAX_Q || k > F8_MAX_K) return 0;
   F8Args a{};
@@ -2340,7 +2340,7 @@ extern "C" uint64_t thrml_linear_f8_work(thrml_ctx *ctx, int dtype, uint64_t row
   a.q = q;
   a.w = reinterpret_cast<const uint8_t *>(w);
   a.w_stride = w_stride;
-  return linear_f8_work(ctx, a, dtype, out_dtype);
+  return linear_f8_work(ctx, a, out_dtype);
 }
 
 extern "C" int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,
@@ -2359,7 +2359,7 @@ extern "C" int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_
   if (int rc = check_vector("w_scale", w_scale)) return rc;
   if (int rc = check_vector("bias", bias)) return rc;
   if (int rc = check_rows("y", y, out_size, rows, q, y_stride, true)) return rc;
-  if (int rc = check_work(work, work_bytes, thrml_linear_f8_work(ctx, dtype, rows, k, w, q, w_stride, out_dtype))) return rc;
+  if (int rc = check_work(work, work_bytes, thrml_linear_f8_work(ctx, rows, k, w, q, w_stride, out_dtype))) return rc;
   THRML_HIP(hipSetDevice(ctx->device));
   const F8Args a{x, x_stride, rows, k, q, reinterpret_cast<const uint8_t *>(w), w_stride, w_scale, bias, y, y_stride};
   return launch_linear_f8(ctx, a, dtype, out_dtype, work);

@@ -102,7 +102,7 @@ int launch_distill(thrml_ctx *ctx, const DistillArgs &a, int dtype, void *work);
 uint64_t linear_i8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, uint32_t q);
 int launch_linear_i8(thrml_ctx *ctx, const LinearArgs &a, int dtype, int out_dtype, void *work);
 int launch_dropout(thrml_ctx *ctx, DropoutArgs a, int dtype);
-uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype);
+uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int out_dtype);
 int launch_linear_f8(thrml_ctx *ctx, const F8Args &a, int dtype, int out_dtype, void *work);
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward);
 int launch_gated(thrml_ctx *ctx, const thrml_gated &g, void *h, int64_t h_stride, float *gate, float *up, void *work);

@@ -436,8 +436,14 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const uint8_t *__restrict_
 
 // ---------------------------------------------------------------------------
 // Calls
-static constexpr TileKind f8_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.25f, 0.2f}, {128, 128, 128, 0.5f, 0.45f}, {256, 256, 128, 1.0f, 1.0f}};
-static constexpr TileKind f8_exact_kinds[] = {{64, 32, 128, 0.2f, 0.15f}, {64, 64, 128, 0.3f, 0.25f}, {128, 128, 128, 0.8f, 0.7f}};
+// Taken and next best (us a call):
+//     1 x 4096 x 4096   64 x 32 in 8 parts: 18.9  in one: 19.6      128 x 4096 x 16384  64 x 64: 28    128 x 128: 33
+//    16 x 8192 x 8192   64 x 32 in 4 parts: 23    in one: 32       1024 x 4096 x 8192  128 x 128: 67  256 x 256: 69
+//    64 x 4096 x 16384  64 x 64: 23.6  64 x 32: 24.0               2048 x 1024 x 2048  128 x 128: 19   64 x 64: 22
+// For results in f32 (the products at half the rate; 256 x 256 would need more registers):
+//   256 x 4096 x 4096   64 x 64: 30  64 x 32: 32                  1024 x 4096 x 8192  128 x 128: 104  64 x 64: 121
+static constexpr TileKind f8_kinds[] = {{64, 32, 128, 0.33f, 0.21f}, {64, 64, 128, 0.40f, 0.26f}, {128, 128, 128, 0.65f, 0.77f}, {256, 256, 128, 1.5f, 1.75f}};
+static constexpr TileKind f8_exact_kinds[] = {{64, 32, 128, 0.40f, 0.26f}, {64, 64, 128, 0.55f, 0.37f}, {128, 128, 128, 1.2f, 1.26f}};
 typedef TileShape<16, 32, 4, 1, 1, 128, 6, false> F8Tile32;
 typedef TileShape<32, 32, 2, 2, 1, 128, 4, false> F8Tile64;
 typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> F8Tile128;
@@ -466,7 +472,7 @@ struct F8Plan {
   }
 };
 
-uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int, int out_dtype) {
+uint64_t linear_f8_work(thrml_ctx *ctx, const F8Args &a, int out_dtype) {
   const F8Plan p(ctx, a, out_dtype);
   return p.scale_bytes + p.x_bytes + p.w_bytes + p.tiles.part;
 }

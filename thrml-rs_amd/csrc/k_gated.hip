@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(const uint16_t *__restr
     if (c + 8u <= k)
       load8(p, r);
     else
-      load8_part(p, k - c, r);
+      load8_part(p, c < k ? k - c : 0u, r);
     *reinterpret_cast<u32x4 *>(out + row * kp + c) = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
   }
 }
@@ -455,6 +455,12 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
          (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
 }
 
+// Taken and next best (us a call):
+//    16 x 4096 x 8192   64 x 32: 23.7  64 x 64: 24.0               512 x 4096 x 8192  256 x 256: 81  128 x 128: 93
+//    64 x 4096 x 8192   64 x 64: 25    64 x 32: 30                1024 x 2048 x 2048  128 x 128: 25   64 x 64: 33
+//   300 x 8192 x 256    64 x 64 in 8 parts: 20  in one: 38        1024 x 4096 x 8192  256 x 256: 114  128 x 128: 178
+// and of the gradient in x:
+//  1024 x 1024 x 4096   128 x 128 in 4 parts: 39  64 x 64: 57     2048 x 4096 x 4096  256 x 256 in 2 parts: 145  in one: 178
 static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.30f, 0.20f}, {64, 64, 128, 0.36f, 0.23f}, {128, 128, 128, 0.57f, 0.62f}, {256, 256, 128, 0.9f, 1.5f}};
 typedef TileShape<64, 32, 1, 1, 4, 128, 4, false> Tile32;
 typedef TileShape<64, 32, 1, 2, 2, 128, 4, false> Tile64;
@@ -468,7 +474,9 @@ struct GatedPlan {
   uint64_t x_bytes, w_bytes, d_bytes;  // packed x, each packed weight, dz and du
   TilePlan forward, input, weight;
   GatedPlan(const thrml_ctx *ctx, const thrml_gated &g) {
-    kp = padded(g.k, 8);
+    // (whole lines of memory: rows of 7088 bytes take 34 us where rows of 7168 take 26, at 121 x
+    // 3544 x 4952)
+    kp = padded(g.k, 64);
     np = padded(g.n, 64);
     pack_x = !tile_rows(g.x, g.x_stride, g.rows, g.k);
     pack_w = !tile_rows(g.w_gate, g.gate_stride, g.n, g.k) || !tile_rows(g.w_up, g.up_stride, g.n, g.k) || (g.n > 1 && g.gate_stride != g.up_stride);
@@ -499,7 +507,8 @@ static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t r
 template <class S, int OP, class T, int ACT>
 static int launch_kind(thrml_ctx *ctx, const GatedTiles &g) {
   const size_t lds = std::max<size_t>(S::BYTES, (size_t)S::WA * S::WB * 32 * (S::MA + 4) * 4);
-  auto *f = g.splits > 1 ? &gated_tile_kernel<S, OP, T, ACT, true> : &gated_tile_kernel<S, OP, T, ACT, false>;
+  // (the sums of splits do not use the activation)
+  auto *f = g.splits > 1 ? &gated_tile_kernel<S, OP, T, THRML_ACT_RELU, true> : &gated_tile_kernel<S, OP, T, ACT, false>;
   return launch_tiles(ctx, f, g, S::THREADS, lds);
 }
 

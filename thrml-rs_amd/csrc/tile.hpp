@@ -157,8 +157,9 @@ struct Side {
 // the next stage of side B, the second the next but one of side A.  A load into LDS
 // holds its wave up for some 40 cycles, also between products: so each phase has half of
 // them, and none is among the products.  Cycles of a phase at 4096 x 4096 x 16384 in bf16:
-// 1055 multiply (of 1024 that the products take), 650 read, 400 load.  With all loads
-// from the first wave a stage took 2830 cycles, with all among the second's products 3350.
+// 1055 multiply (of 1024 that the products take), 650 read, 400 load; a stage, two phases,
+// takes 2460.  With all loads from the first wave it took 2830, with all among the
+// second's products 3350.
 template <class S, int LOADS_B, class FetchA, class FetchB, class Read, class Multiply, class Begin>
 __device__ __forceinline__ void tile_loop(uint32_t s0, uint32_t s1, FetchA fetch_a, FetchB fetch_b, Read read, Multiply multiply, Begin begin) {
   if constexpr (S::PING) {

@@ -182,7 +182,7 @@ def linear_f8(device, x, w, w_scale, bias=None, out_dtype=None):
     y = torch.empty((rows, q), dtype=dtype, device=where)
     lib = load()
     wp, ws = w.data_ptr(), ws if q > 1 else k
-    n = lib.thrml_linear_f8_work(device.handle, in_code, rows, k, wp, q, ws, code)
+    n = lib.thrml_linear_f8_work(device.handle, rows, k, wp, q, ws, code)
     work = torch.empty(n, dtype=torch.uint8, device=where) if n else None
     _run(device, lib.thrml_linear_f8, x.data_ptr(), in_code, rows, k, xs if rows > 1 else k, wp, q, ws,
          w_scale.data_ptr(), bias.data_ptr() if bias is not None else 0, y.data_ptr(), code, q,
