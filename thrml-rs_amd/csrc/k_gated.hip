@@ -98,7 +98,7 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   const uint32_t s0 = (uint32_t)((uint64_t)g.steps * blockIdx.y / g.splits);
   const uint32_t s1 = (uint32_t)((uint64_t)g.steps * (blockIdx.y + 1u) / g.splits);
 
-  // (across, rows come in eights: k is padded to them, np is a multiple of 64)
+  // (across, rows come in eights: k is padded to them, np is a multiple of 128)
   typedef Side<S, S::NA, A_CROSS> SideA;
   typedef Side<S, S::NB, B_CROSS> SideB;
   const SideA sa{(uint32_t)g.a_stride, OP == G_FORWARD ? g.n - 1u - c0 : ((g.k + 7u) & ~7u) - 1u - c0};
@@ -461,8 +461,11 @@ static bool tile_rows(const void *p, int64_t stride, uint64_t rows, uint32_t k) 
 //   300 x 8192 x 256    64 x 64 in 8 parts: 20  in one: 38        1024 x 4096 x 8192  256 x 256: 114  128 x 128: 178
 // and of the gradient in x:
 //  1024 x 1024 x 4096   128 x 128 in 4 parts: 39  64 x 64: 57     2048 x 4096 x 4096  256 x 256 in 2 parts: 145  in one: 178
-static constexpr TileKind gated_kinds[] = {{64, 32, 128, 0.30f, 0.20f}, {64, 64, 128, 0.36f, 0.23f}, {128, 128, 128, 0.57f, 0.62f}, {256, 256, 128, 0.9f, 1.5f}};
-typedef TileShape<64, 32, 1, 1, 4, 128, 4, false> Tile32;
+static constexpr TileKind gated_kinds[] = {{64, 32, 256, 0.56f, 0.38f}, {64, 64, 128, 0.36f, 0.23f}, {128, 128, 128, 0.57f, 0.62f}, {256, 256, 128, 0.9f, 1.5f}};
+// (stages of 256 bytes for the fewest rows: with 128, rows that are no whole lines have each
+// line on two of them; one row of 4104 x 16384: 53 -> 49.5 us, of 4096 x 16384: 51.5 -> 47.  With 64
+// rows such stages take 34 us for 38 at 3544 x 8192, but 38 for 31 at 4096 x 8192)
+typedef TileShape<64, 32, 1, 1, 4, 256, 3, false> Tile32;
 typedef TileShape<64, 32, 1, 2, 2, 128, 4, false> Tile64;
 typedef TileShape<64, 64, 2, 2, 1, 128, 3, false> Tile128;
 typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> Tile256;
@@ -477,7 +480,7 @@ struct GatedPlan {
     // (whole lines of memory: rows of 7088 bytes take 34 us where rows of 7168 take 26, at 121 x
     // 3544 x 4952)
     kp = padded(g.k, 64);
-    np = padded(g.n, 64);
+    np = padded(g.n, 128);  // whole stages of each weight
     pack_x = !tile_rows(g.x, g.x_stride, g.rows, g.k);
     pack_w = !tile_rows(g.w_gate, g.gate_stride, g.n, g.k) || !tile_rows(g.w_up, g.up_stride, g.n, g.k) || (g.n > 1 && g.gate_stride != g.up_stride);
     x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;

@@ -2,14 +2,14 @@
 // hidden block (k_gated.hip) and its 8-bit product (k_f8.hip).
 //
 // out[r][c] = sum over j of B[r][j] A[c][j]: side A are the output's columns (its
-// contiguous direction), side B its rows.  A stage is KB (64 or 128) bytes of the reduction
+// contiguous direction), side B its rows.  A stage is KB (64, 128 or 256) bytes of the reduction
 // of every row of both sides.  An operand lies in memory either with the reduction
 // contiguous (a row of a side is a row in memory), or across (CROSS: a row in memory
 // holds one reduction index for all rows of the side), as a gradient's operands do.
 //
 // In LDS, 16-byte pieces:
 //   along   rows of KB bytes, a row's pieces permuted by bits of the row: (row >> 1) & 7 for
-//           128 bytes, (row >> 3) & 3 for 64.  A 16-byte read takes 16 lanes at a time, four
+//           128 bytes, row & 15 for 256 (among 16 pieces), (row >> 3) & 3 for 64.  A 16-byte read takes 16 lanes at a time, four
 //           quads of lanes: 0, 3, 5, 6 of a half wave, then 1, 2, 4, 7; two rows of 128 bytes
 //           fill the banks, and the rows of one parity that meet (0, 2, 12, 14, 20, 22, 24, 26
 //           of 32) differ in those bits, as do four that meet of 64 bytes.
@@ -313,7 +313,8 @@ struct TilePlan {
 };
 
 // The kind of tile, and into how many parts the reduction goes, by an estimate of each
-// one's time: its stages, and about 6 more for beginning and end, at its time for one.
+// one's time: its stages, and about 6 more of 128 bytes for beginning and end, at its time
+// for one.
 // row_bytes: of the reduction, in a row; cols: the rows of side A; rows: those of side B, of two matrices where `halves`.
 static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, int n, uint64_t cols, uint64_t rows, bool halves,
                                   uint64_t row_bytes, uint64_t out_values) {
@@ -324,13 +325,14 @@ static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, i
     const uint32_t ta = tile_cdiv(cols, kd.na), tb = tile_cdiv(rows, kd.nb) * (halves ? 2u : 1u);
     const uint64_t tiles = (uint64_t)ta * tb;
     const uint32_t steps = tile_cdiv(row_bytes, kd.kb);
+    // (a split has two stages or more: an empty one would have no last stage to repeat)
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (steps < 4 * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
+      if (splits > 1 && (steps * (uint64_t)kd.kb < 512u * splits || tiles * splits > 2u * (uint32_t)ctx->cu_count)) break;
       const uint64_t groups = tiles * splits, cus = (uint64_t)ctx->cu_count;
       const double one = groups > cus ? (double)kd.many * (double)tile_cdiv(groups, cus)
                                       : kd.alone + std::max(0.0f, kd.many - kd.alone) * (double)groups / (double)cus;
       // a join reads what the splits wrote, together 4.5 bytes a ps, and is a launch
-      const double t = one * (tile_cdiv(steps, splits) + 6) + (splits > 1 ? 7.0 + (double)out_values * 4 * 2 * splits / 4.5e6 : 0.0);
+      const double t = one * (tile_cdiv(steps, splits) + 768.0 / kd.kb) + (splits > 1 ? 7.0 + (double)out_values * 4 * 2 * splits / 4.5e6 : 0.0);
       if (best_t == 0.0 || t < best_t) {
         best_t = t;
         best.kind = i;
