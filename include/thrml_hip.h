@@ -579,7 +579,8 @@ uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward);
 int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, float *gate,
                         float *up, void *work, uint64_t work_bytes);
 /* From grad = d loss / d h [rows][n] and the z and u that the forward call kept:
- *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
+ *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type; f16: all divided by a
+ *                                             power of two where one would pass 65504)
  *   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x
  * dx [rows][k] in rows of dx_stride (NULL: not computed), dw_gate and dw_up [n][k]
  * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes. */

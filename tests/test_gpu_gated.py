@@ -257,3 +257,29 @@ def test_tensors_that_require_a_gradient(device):
     with torch.no_grad():
         _, gate, up = th.gated_linear(device, x, wg, wu, save=True)
     assert not any(t.requires_grad for t in th.gated_linear_grad(device, dh, x, wg, wu, gate, up))
+
+
+@pytest.mark.parametrize("rows,k,n", [(5, 72, 90), (5, 70, 1000), (300, 264, 520)])
+def test_large_f16_gradients(device, rows, k, n):
+    """a loss scale that takes dz and du past 65504: results that are within it come out as
+    exactly as ever, the others infinite, none NaN"""
+    x, wg, wu, dh = _inputs(rows, k, n, F16)
+    dh = (dh.float() * 13000).clamp(-60000, 60000).to(F16)
+    x = x * 0.02  # (dw within the range)
+    wg, wu = wg * 50, wu * 50
+    _, gate, up = th.gated_linear(device, x, wg, wu, save=True)
+    a, slope = ref.act(gate.double(), "silu")
+    largest = max(float((dh.double() * up.double() * slope).abs().max()), float((dh.double() * a).abs().max()))
+    assert largest > 65504
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up)
+    # what is divided by 2^down is rounded in steps of at least 2^-24 times that
+    step = ref.tiny(F16) * 2.0**(math.floor(math.log2(largest)) - 14)
+    more = {"dx": step * (wg.double().abs() + wu.double().abs()).sum(0), "dw_gate": step * x.double().abs().sum(0)}
+    more["dw_up"] = more["dw_gate"]
+    for (name, (want, bound)), got in zip(ref.gated_grad(dh, x, wg, wu, gate, up, "silu").items(), grads):
+        bound = bound + more[name] * 1.01
+        assert not got.isnan().any()
+        inside, outside = want.abs() + bound < 65504, want.abs() - bound > 65520
+        assert inside.any()
+        ref.close(got[inside], want[inside], bound[inside], name)
+        assert got[outside].isinf().all()

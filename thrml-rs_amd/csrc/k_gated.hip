@@ -77,6 +77,7 @@ struct GatedTiles {
   void *out, *out1, *out2;
   int64_t out_stride;   // elements
   float *part;          // sums of the splits, [split][row][column], in place of the above
+  const float *factor;  // of the results, or null
 };
 
 template <class S, int OP, class T, int ACT, bool PART>
@@ -253,6 +254,10 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
           for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
           store8(out + (int64_t)row * g.out_stride + c, m, v);
         } else {
+          if (g.factor) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
+          }
           store8(out + (int64_t)row * g.out_stride + c, m, v);
         }
       }
@@ -361,6 +366,10 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
     const float *p = g.part + row * pitch + c;
     join8(p, rows * pitch, g.splits, m, v);
     if (OP == G_FORWARD) join8(p + g.n, rows * pitch, g.splits, m, w);
+    if (OP != G_FORWARD && g.factor) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
+    }
     if constexpr (OP == G_FORWARD) {
       const int64_t saved = (int64_t)row * g.n + c;
       if (g.out1) {
@@ -379,12 +388,39 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
   }
 }
 
-// dz and du from dh and the z and u that the forward pass kept (14 bytes a unit): rows of 2 np elements,
-// zeros behind the n of each half.
-template <class T, int ACT>
+// dz and du from dh and the z and u that the forward pass kept (14 bytes a unit): rows of 2
+// np elements, zeros behind the n of each half.
+//
+// f16 (gradients that carry a loss scale may pass its 65504 here, where neither dh nor the
+// results do): each workgroup leaves the largest finite magnitude that it wrote, and a
+// second launch, AGAIN, writes them once more divided by a power of two if that was too
+// large, and otherwise ends at once.  The products' results are multiplied by it.
+constexpr uint32_t SLOPE_GROUPS = 2048;  // workgroups, with f16; the factor lies behind their maxima
+
+__device__ __forceinline__ float slope_max(float m, float *shared) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  if ((threadIdx.x & 63u) == 0) shared[threadIdx.x / 64u] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+}
+
+template <class T, int ACT, bool AGAIN>
 __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ grad, int64_t grad_stride,
                                                           const float *__restrict__ z, const float *__restrict__ u, uint64_t rows,
-                                                          uint32_t n, uint32_t np, T *__restrict__ d) {
+                                                          uint32_t n, uint32_t np, T *__restrict__ d, float *maxima) {
+  constexpr bool SCALED = __is_same(T, f16_t);
+  __shared__ float shared[4];
+  float factor = 1.0f, most = 0.0f;
+  if constexpr (AGAIN) {
+    float m = 0.0f;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += 256u) m = fmaxf(m, maxima[i]);
+    m = slope_max(m, shared);
+    const int down = m > 65504.0f ? ilogbf(m) - 14 : 0;  // m 2^-down < 2^15
+    if (blockIdx.x == 0 && threadIdx.x == 0) maxima[SLOPE_GROUPS] = ldexpf(1.0f, down);
+    if (down == 0) return;
+    factor = ldexpf(1.0f, -down);
+  }
   const uint32_t groups = np / 8u;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
     const uint64_t row = i / groups;
@@ -412,6 +448,13 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
         // (behind the end: zeros)
         a[e] = c + e < n ? dh * value(ru, e) * slope : 0.0f;
         b[e] = c + e < n ? dh * value_ : 0.0f;
+        if constexpr (AGAIN) {
+          a[e] *= factor;
+          b[e] *= factor;
+        } else if constexpr (SCALED) {
+          const float m = fmaxf(fabsf(a[e]), fabsf(b[e]));  // (of a NaN and a number: the number)
+          most = m < INFINITY ? fmaxf(most, m) : most;
+        }
       }
     } else {
 #pragma unroll
@@ -420,6 +463,10 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
     T *o = d + row * 2u * np + c;
     store8(o, 8, a);
     store8(o + np, 8, b);
+  }
+  if constexpr (SCALED && !AGAIN) {
+    most = slope_max(most, shared);
+    if (threadIdx.x == 0) maxima[blockIdx.x] = most;
   }
 }
 
@@ -474,7 +521,7 @@ struct GatedPlan {
   bool few;  // the forward pass reads the operands as they lie
   bool pack_x, pack_w;
   uint32_t kp, np;
-  uint64_t x_bytes, w_bytes, d_bytes;  // packed x, each packed weight, dz and du
+  uint64_t x_bytes, w_bytes, d_bytes, m_bytes;  // packed x, each packed weight, dz and du, their maxima
   TilePlan forward, input, weight;
   GatedPlan(const thrml_ctx *ctx, const thrml_gated &g) {
     // (whole lines of memory: rows of 7088 bytes take 34 us where rows of 7168 take 26, at 121 x
@@ -486,6 +533,7 @@ struct GatedPlan {
     x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;
     w_bytes = pack_w ? tile_bytes((uint64_t)g.n * kp * 2u) : 0;
     d_bytes = tile_bytes(g.rows * 2u * np * 2u);
+    m_bytes = g.dtype == THRML_DTYPE_F16 ? tile_bytes((SLOPE_GROUPS + 1) * 4) : 0;
     few = (pack_x || pack_w) && g.rows <= 32;
     forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, g.k * 2ull, g.rows * 2u * g.n);
     input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, np * 4ull, g.rows * g.k);
@@ -496,7 +544,7 @@ struct GatedPlan {
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward) {
   const GatedPlan p(ctx, g);
   if (p.few && !backward) return 0;
-  return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
+  return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes + p.m_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
 }
 
 static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t rows, uint32_t k, uint32_t kp, void *out) {
@@ -634,14 +682,24 @@ int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, in
   t.b = w;
   t.b_stride = (uint64_t)p.np * 4u;
   w += p.d_bytes;
+  float *maxima = p.m_bytes ? reinterpret_cast<float *>(w) : nullptr;
+  t.factor = maxima ? maxima + SLOPE_GROUPS : nullptr;
+  w += p.m_bytes;
   t.part = reinterpret_cast<float *>(w);
   return with_gated(g, [&](auto e, auto act) -> int {
     typedef decltype(e) T;
+    constexpr int ACT = decltype(act)::value;
     const uint64_t n = g.rows * (p.np / 8u);
-    auto *slope = &gated_slope_kernel<T, decltype(act)::value>;
-    hipLaunchKernelGGL(slope, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream,
-                       reinterpret_cast<const T *>(grad), grad_stride, gate, up, g.rows, g.n, p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)));
-    THRML_HIP(hipGetLastError());
+    const dim3 grid((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), maxima ? SLOPE_GROUPS : 1u << 16));
+    auto slope = [&](auto *f) -> int {
+      hipLaunchKernelGGL(f, grid, dim3(256), 0, ctx->stream, reinterpret_cast<const T *>(grad), grad_stride, gate, up, g.rows, g.n,
+                         p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)), maxima);
+      THRML_HIP(hipGetLastError());
+      return THRML_OK;
+    };
+    if (int rc = slope(&gated_slope_kernel<T, ACT, false>)) return rc;
+    if constexpr (__is_same(T, f16_t))
+      if (int rc = slope(&gated_slope_kernel<T, ACT, true>)) return rc;
     // (the products do not use the activation)
     if (dx) {
       GatedTiles i = t;

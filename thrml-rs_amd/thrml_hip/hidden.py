@@ -81,7 +81,8 @@ def gated_linear_grad(device, grad, x, w_gate, w_up, gate, up, activation="silu"
     """(dx, dw_gate, dw_up): the gradients of a loss in x [rows, k] and the weights [n, k],
     in their type, from grad [rows, n], its gradient in gated_linear's result in that type,
     and the products gate and up [rows, n] float32 that this kept.  With z = gate, u = up:
-      dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
+      dz = grad u act'(z),  du = grad act(z)   (rounded to the type; float16: all divided
+                                      by a power of two where one would pass 65504)
       dx = dz @ w_gate + du @ w_up,  dw_gate = dz.T @ x,  dw_up = du.T @ x
     relu'(0) is 0.  Without rows the weights' gradients are 0.  input_grad False: dx is
     not computed, and None."""
