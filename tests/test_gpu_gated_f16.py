@@ -1,0 +1,66 @@
+"""Gradients of the gated block in f16 at the edge of the type's range: which results are
+infinite, next to 65520 too, and rows and units of very different size, against the
+definition in 64 bits (hidden_reference.py) from the z and u that the forward call kept."""
+import math
+
+import hidden_reference as ref
+import pytest
+import torch
+from conftest import log_case
+
+import thrml_hip as th
+
+pytestmark = pytest.mark.gpu
+
+F16 = torch.float16
+BORDER = 65520.0  # what is rounded to f16 from here on is infinite
+
+
+def _inputs(rows, k, n, seed=0):
+    g = torch.Generator("cuda").manual_seed(seed + 7 * rows + k * 31 + n)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x = rand(rows, k).to(F16)
+    wg, wu = ((rand(n, k) / math.sqrt(k)).to(F16) for _ in range(2))
+    return x, wg, wu, rand(rows, n)
+
+
+def _exact(dh, x, wg, wu, z, u, act):
+    """{name: (value, error of f32)}: what an f32 computation of dz and du (16 roundings of
+    its factors, as in hidden_reference.gated_grad) leaves of each result, sums in 64 bits"""
+    dh, x, wg, wu, z, u = (t.double() for t in (dh, x, wg, wu, z, u))
+    a, slope = ref.act(z, act)
+    dz, du = dh * u * slope, dh * a
+    ez, eu = 16 * ref.U32 * (dh * u).abs() * (1 + z.abs()), 16 * ref.U32 * (dh * z).abs()
+    dzt, dut, ezt, eut = (t.t().contiguous() for t in (dz, du, ez, eu))
+    return {"dx": (torch.mm(dz, wg) + torch.mm(du, wu), torch.mm(ez, wg.abs()) + torch.mm(eu, wu.abs())),
+            "dw_gate": (torch.mm(dzt, x), torch.mm(ezt, x.abs())), "dw_up": (torch.mm(dut, x), torch.mm(eut, x.abs()))}
+
+
+# rows, k, n, what the gradients are multiplied by: in each some per cent of the results of dx,
+# of the weights' gradients or of both pass the range; every kind of tile, with a split
+# reduction and without, operands that are copied, and few rows
+STEPS = [
+    (5, 7040, 2000, 13107.0), (1, 264, 4104, 40000.0), (13, 2000, 1003, 20000.0), (40, 264, 392, 9000.0),
+    (300, 264, 520, 5000.0), (600, 1032, 600, 2000.0), (65, 136, 6000, 8000.0), (520, 1032, 2056, 2500.0), (2050, 136, 136, 4000.0),
+]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows,k,n,size", STEPS)
+def test_what_passes_the_range(device, rows, k, n, size, act):
+    """infinite exactly where the definition is, but for what f32 cannot tell from 65520"""
+    log_case(f"f16 range {rows} {k} {n} {size} {act}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    dh = (dh * size).clamp(-65504, 65504).to(F16)
+    _, gate, up = th.gated_linear(device, x, wg, wu, act, save=True)
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, act)
+    near = passed = 0
+    for (name, (want, err)), got in zip(_exact(dh, x, wg, wu, gate, up, act).items(), grads):
+        assert not got.isnan().any(), name
+        told = (want.abs() - BORDER).abs() > err
+        wrong = told & (got.isinf() != (want.abs() >= BORDER))
+        assert not wrong.any(), (name, int(wrong.sum()), want[wrong][:5].tolist(), got[wrong][:5].tolist())
+        assert ((got > 0) == (want > 0))[got.isinf()].all(), name
+        near += int(((want.abs() - BORDER).abs() < 32.0).sum())
+        passed += int((want.abs() >= BORDER).sum())
+    assert near > 0 and passed > 0, "the case does not come near the border"

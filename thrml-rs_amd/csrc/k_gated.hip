@@ -78,7 +78,116 @@ struct GatedTiles {
   int64_t out_stride;   // elements
   float *part;          // sums of the splits, [split][row][column], in place of the above
   const float *factor;  // of the results, or null
+  // f16 gradients: what dz and du are computed from
+  const f16_t *grad;
+  int64_t grad_stride;
+  const float *z, *u;
+  int32_t act;
 };
+
+// dz and du of one unit
+template <int ACT>
+__device__ __forceinline__ void slopes(float dh, float z, float u, float &dz, float &du) {
+  float value, slope;
+  act_both<ACT>(z, value, slope);
+  dz = dh * u * slope;
+  du = dh * value;
+}
+
+// A gradient that comes out near f16's border (65520: what is rounded from there on is
+// infinite) says nothing of which side it is on: the rounding of dz and du to 11 bits moved
+// it by a rms of 0.29 2^-11 of a term times the root of the terms' number, 2e-4 of what is a
+// typical result of its row.  Such results are summed again by a wave, dz and du in f32 and
+// the sum in 64 bits.  Near is within 2^-9 of the largest of 64 results of the row (at least
+// twice a typical one, and those at the border are among them), a quarter of the border at
+// most.  Results far from the border pay comparisons: a step of 1021 x 2001 x 5003 takes 266 us
+// with them and 264 without.  One of 5 x 7040 x 8000 takes 253 where 1.5 % of the weights' gradients
+// pass the border and 35 thousand are near it, 193 without.
+//
+// One result, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c
+template <int OP>
+__device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row, uint32_t c) {
+  const uint32_t l = here(threadIdx.x) & 63u;
+  auto pair = [&](uint64_t r, uint32_t unit, float &dz, float &du) {
+    const float dh = (float)g.grad[(int64_t)r * g.grad_stride + unit], z = g.z[r * g.n + unit], u = g.u[r * g.n + unit];
+    if (g.act == THRML_ACT_RELU)
+      slopes<THRML_ACT_RELU>(dh, z, u, dz, du);
+    else if (g.act == THRML_ACT_GELU)
+      slopes<THRML_ACT_GELU>(dh, z, u, dz, du);
+    else
+      slopes<THRML_ACT_SILU>(dh, z, u, dz, du);
+  };
+  auto operand = [&](const void *p, uint64_t r) {
+    return (double)(float)*reinterpret_cast<const f16_t *>(reinterpret_cast<const uint8_t *>(p) + r * g.a_stride + c * 2ull);
+  };
+  double sum = 0.0;
+  float dz, du;
+  if constexpr (OP == G_WEIGHT) {
+    const bool up = row >= g.n;
+    for (uint64_t r = l; r < g.rows; r += 64u) {
+      pair(r, up ? row - g.n : row, dz, du);
+      sum += (double)(up ? du : dz) * operand(g.a0, r);
+    }
+  } else {
+    for (uint32_t unit = l; unit < g.n; unit += 64u) {
+      pair(row, unit, dz, du);
+      sum += (double)dz * operand(g.a0, unit) + (double)du * operand(g.a1, unit);
+    }
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  return sum;
+}
+
+constexpr float BORDER = 65520.0f;
+
+// what a lane has seen of results: the largest, and how near one came to the border
+struct Border {
+  float most = 0.0f, nearest = INFINITY;
+  __device__ __forceinline__ void see(const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      most = fmaxf(most, fabsf(v[e]));
+      nearest = fminf(nearest, fabsf(fabsf(v[e]) - BORDER));
+    }
+  }
+  // whether a lane of the wave has seen one that is near; band: the distance that is, from
+  // what 8 lanes have seen
+  __device__ __forceinline__ bool any_near(float &band) const {
+    if (!__any(most >= 0.75f * BORDER)) return false;
+    float m = most;
+#pragma unroll
+    for (int s = 1; s < 8; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
+    band = fminf(0x1p-9f * m, 0.25f * BORDER);
+    return __any(nearest <= band);
+  }
+};
+
+// The results v of row `row` from column c on, of which m count (0 in a lane that has none:
+// all lanes of the wave come here); whether this lane's were summed again.
+template <int OP>
+__device__ __forceinline__ bool settle_border(const GatedTiles &g, float (&v)[8], uint32_t m, uint32_t row, uint32_t c) {
+  Border b;
+  if (m) b.see(v);
+  float band;
+  if (!b.any_near(band)) return false;
+  uint32_t bits = 0;
+#pragma unroll
+  for (uint32_t e = 0; e < 8; ++e) bits |= (uint32_t)(e < m && fabsf(fabsf(v[e]) - BORDER) <= band) << e;
+  const bool some = bits != 0;
+  for (uint64_t any = __ballot(bits != 0); any; any = __ballot(bits != 0)) {
+    const int lane = __builtin_ctzll(any);
+    const uint32_t of = (uint32_t)__builtin_amdgcn_readlane((int)bits, lane), at = (uint32_t)__builtin_ctz(of);
+    const float sum = (float)gated_again<OP>(g, (uint32_t)__builtin_amdgcn_readlane((int)row, lane),
+                                             (uint32_t)__builtin_amdgcn_readlane((int)c, lane) + at);
+    if ((here(threadIdx.x) & 63u) == (uint32_t)lane) {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) v[e] = e == at ? sum : v[e];
+      bits &= bits - 1u;
+    }
+  }
+  return some;
+}
 
 template <class S, int OP, class T, int ACT, bool PART>
 __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
@@ -226,12 +335,15 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     __builtin_amdgcn_wave_barrier();
     wait_reads();
     if (S::WK == 1 || wk == 0) {
-#pragma unroll
-      for (uint32_t t = 0; t < 32u / RPI; ++t) {
+      constexpr bool SETTLE = !PART && OP != G_FORWARD && __is_same(T, f16_t);
+      Border seen;
+      // 8 columns of one of RPI rows; with AGAIN, those near the border are settled
+      auto end = [&](uint32_t t, auto again) {
+        constexpr bool AGAIN = decltype(again)::value;
         const uint32_t rl = t * RPI + l / LPR;
         const uint64_t row = r0 + wb * S::MB + 32u * j + rl;
-        if (row >= limit || c >= cols) continue;
-        const uint32_t m = cols - c;
+        const uint32_t m = row < limit && c < cols ? cols - c : 0u;
+        if (!AGAIN && m == 0) return;
         float v[8], w[8];
         const float *at = mine + rl * PITCH + cl;
 #pragma unroll
@@ -258,7 +370,21 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
           }
+          if constexpr (AGAIN) {
+            if (!settle_border<OP>(g, v, m, (uint32_t)row + up * g.n, c)) return;
+          } else if constexpr (SETTLE) {
+            seen.see(v);
+          }
           store8(out + (int64_t)row * g.out_stride + c, m, v);
+        }
+      };
+#pragma unroll
+      for (uint32_t t = 0; t < 32u / RPI; ++t) end(t, std::false_type{});
+      if constexpr (SETTLE) {
+        float band;
+        if (seen.any_near(band)) {
+#pragma unroll 1
+          for (uint32_t t = 0; t < 32u / RPI; ++t) end(t, std::true_type{});
         }
       }
     }
@@ -359,7 +485,10 @@ template <int OP, class T, int ACT>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
   const uint32_t cols = OP == G_FORWARD ? g.n : g.k, groups = (cols + 7u) / 8u;
   const uint64_t rows = OP == G_WEIGHT ? 2ull * g.n : g.rows, pitch = OP == G_FORWARD ? 2ull * g.n : g.k;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
+  constexpr bool SETTLE = OP != G_FORWARD && __is_same(T, f16_t);
+  // (SETTLE: whole waves; lanes behind the end repeat the last group and store nothing)
+  for (uint64_t i_ = (uint64_t)blockIdx.x * 256u + threadIdx.x; (SETTLE ? i_ & ~(uint64_t)63u : i_) < rows * groups; i_ += (uint64_t)gridDim.x * 256u) {
+    const uint64_t i = SETTLE ? min(i_, rows * groups - 1u) : i_;
     const uint64_t row = i / groups;
     const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = cols - c;
     float v[8], w[8];
@@ -369,6 +498,10 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
     if (OP != G_FORWARD && g.factor) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
+    }
+    if constexpr (SETTLE) {
+      settle_border<OP>(g, v, i == i_ ? m : 0u, (uint32_t)row, c);
+      if (i != i_) continue;
     }
     if constexpr (OP == G_FORWARD) {
       const int64_t saved = (int64_t)row * g.n + c;
@@ -442,12 +575,11 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float value_, slope;
-        act_both<ACT>(value(rz, e), value_, slope);
-        const float dh = value(rg, e);
+        float dz, du;
+        slopes<ACT>(value(rg, e), value(rz, e), value(ru, e), dz, du);
         // (behind the end: zeros)
-        a[e] = c + e < n ? dh * value(ru, e) * slope : 0.0f;
-        b[e] = c + e < n ? dh * value_ : 0.0f;
+        a[e] = c + e < n ? dz : 0.0f;
+        b[e] = c + e < n ? du : 0.0f;
         if constexpr (AGAIN) {
           a[e] *= factor;
           b[e] *= factor;
@@ -684,6 +816,11 @@ int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, in
   w += p.d_bytes;
   float *maxima = p.m_bytes ? reinterpret_cast<float *>(w) : nullptr;
   t.factor = maxima ? maxima + SLOPE_GROUPS : nullptr;
+  t.grad = reinterpret_cast<const f16_t *>(grad);
+  t.grad_stride = grad_stride;
+  t.z = gate;
+  t.u = up;
+  t.act = g.act;
   w += p.m_bytes;
   t.part = reinterpret_cast<float *>(w);
   return with_gated(g, [&](auto e, auto act) -> int {
