@@ -98,10 +98,12 @@ __device__ __forceinline__ void slopes(float dh, float z, float u, float &dz, fl
 // infinite) says nothing of which side it is on: the rounding of dz and du to 11 bits moved
 // it by a rms of 0.29 2^-11 of a term times the root of the terms' number, 2e-4 of what is a
 // typical result of its row.  Such results are summed again by a wave, dz and du in f32 and
-// the sum in 64 bits.  Near is within 2^-9 of the largest of 64 results of the row (at least
-// twice a typical one, and those at the border are among them), a quarter of the border at
-// most.  Results far from the border pay comparisons: a step of 1021 x 2001 x 5003 takes 266 us
-// with them and 264 without.  One of 5 x 7040 x 8000 takes 253 where 1.5 % of the weights' gradients
+// the sum in 64 bits.  Near is within 2^-9 of the border, or 2^-8 of a large result of the
+// row's 64 columns here, which is about 1.2 typical ones: 25 times the rms or more.  (Among 8 lanes'
+// largest, the smaller one of pairs, the larger one of two pairs, the smaller one of those: a
+// column that is far larger than the others does not make these near.)  Results far from
+// the border pay comparisons: a step of 1021 x 2001 x 5003 takes 266 us with them and 264
+// without.  One of 5 x 7040 x 8000 takes 252 where 1.5 % of the weights' gradients
 // pass the border and 35 thousand are near it, 193 without.
 //
 // One result, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c
@@ -154,11 +156,11 @@ struct Border {
   // whether a lane of the wave has seen one that is near; band: the distance that is, from
   // what 8 lanes have seen
   __device__ __forceinline__ bool any_near(float &band) const {
-    if (!__any(most >= 0.75f * BORDER)) return false;
-    float m = most;
-#pragma unroll
-    for (int s = 1; s < 8; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
-    band = fminf(0x1p-9f * m, 0.25f * BORDER);
+    if (!__any(most >= 0.99f * BORDER)) return false;  // (a band over 0.01 of the border comes from one beyond it)
+    float m = fminf(most, __shfl_xor(most, 1));
+    m = fmaxf(m, __shfl_xor(m, 2));
+    m = fminf(m, __shfl_xor(m, 4));
+    band = fmaxf(0x1p-8f * m, 0x1p-9f * BORDER);
     return __any(nearest <= band);
   }
 };
@@ -168,7 +170,7 @@ struct Border {
 template <int OP>
 __device__ __forceinline__ bool settle_border(const GatedTiles &g, float (&v)[8], uint32_t m, uint32_t row, uint32_t c) {
   Border b;
-  if (m) b.see(v);
+  b.see(v);  // (those of no column or row are as large as the others)
   float band;
   if (!b.any_near(band)) return false;
   uint32_t bits = 0;
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
         const uint32_t rl = t * RPI + l / LPR;
         const uint64_t row = r0 + wb * S::MB + 32u * j + rl;
         const uint32_t m = row < limit && c < cols ? cols - c : 0u;
-        if (!AGAIN && m == 0) return;
+        if (!SETTLE && m == 0) return;
         float v[8], w[8];
         const float *at = mine + rl * PITCH + cl;
 #pragma unroll
@@ -373,7 +375,8 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
           if constexpr (AGAIN) {
             if (!settle_border<OP>(g, v, m, (uint32_t)row + up * g.n, c)) return;
           } else if constexpr (SETTLE) {
-            seen.see(v);
+            seen.see(v);  // (those of no column, too: they repeat others)
+            if (m == 0) return;
           }
           store8(out + (int64_t)row * g.out_stride + c, m, v);
         }
