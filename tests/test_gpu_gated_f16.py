@@ -83,3 +83,84 @@ def test_what_is_within_the_range_among_results_far_beyond_it(device, rows, k, n
         assert not got.isnan().any() and not wrong.any(), (name, int(wrong.sum()), want[wrong][:5].tolist(), got[wrong][:5].tolist())
         within += int((told & (want.abs() < BORDER)).sum())
     assert within > 0
+
+
+def _down(largest):
+    """by what power of two dz and du are divided whose largest magnitude is this"""
+    return torch.where(largest > 65504, torch.floor(torch.log2(largest.clamp(min=1))) - 14, torch.zeros_like(largest))
+
+
+def _compare(device, dh, x, wg, wu, act):
+    """every result within what its own row's and unit's rounding of dz and du allows"""
+    _, gate, up = th.gated_linear(device, x, wg, wu, act, save=True)
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, act)
+    a, slope = ref.act(gate.double(), act)
+    dz, du = (dh.double() * t for t in (up.double() * slope, a))
+    # (a value next to a power of two may be rounded to it)
+    scales = {"dx": torch.maximum(dz.abs().amax(1), du.abs().amax(1)), "dw_gate": dz.abs().amax(0), "dw_up": du.abs().amax(0)}
+    least = {n: (ref.tiny(F16) * 2.0**_down(s * (1 + 2.0**-20)))[:, None] for n, s in scales.items()}
+    assert max(float(s.max()) for s in scales.values()) > 65504 * 64
+    other = {"dx": wg.double().abs().sum(0) + wu.double().abs().sum(0), "dw_gate": x.double().abs().sum(0)}
+    other["dw_up"] = other["dw_gate"]
+    exact = _exact(dh, x, wg, wu, gate, up, act)
+    finite = 0
+    for (name, (want, bound)), got in zip(ref.gated_grad(dh, x, wg, wu, gate, up, act).items(), grads):
+        bound = bound + least[name] * other[name]
+        assert not got.isnan().any(), name
+        told = (want.abs() - BORDER).abs() > exact[name][1]
+        assert not (told & (got.isinf() != (want.abs() >= BORDER))).any(), name
+        fine = got.isfinite()
+        finite += int(fine.sum())
+        if fine.any():
+            ref.close(got[fine], want[fine], bound[fine], name)
+    assert finite
+
+
+SHAPES = [(5, 72, 90), (24, 72, 392), (40, 264, 392), (300, 264, 520), (600, 1032, 600), (65, 136, 6000), (129, 4104, 24), (1, 264, 4104)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_rows_of_different_size(device, rows, k, n, act):
+    """a row whose dz and du pass the range does not take the bits of the others, whose
+    gradients are 2^20 and 2^30 times smaller"""
+    log_case(f"f16 rows {rows} {k} {n} {act}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    size = torch.full((rows,), 2.0**-6, device="cuda")
+    size[1::3] = 2.0**-15
+    size[::7] = 2.0**14
+    dh = (dh * size[:, None]).clamp(-65504, 65504)
+    _compare(device, dh.to(F16), x * 16, wg * 8, wu * 64, act)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_units_of_different_size(device, rows, k, n, act):
+    """a unit whose dz and du pass the range does not take the bits of the others"""
+    log_case(f"f16 units {rows} {k} {n} {act}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    dh = dh * 2.0**-10
+    dh[:, ::5] *= 2.0**20
+    dh[:, 1::5] *= 2.0**-4
+    large = torch.ones(n, 1, device="cuda", dtype=F16)
+    large[::5] = 512
+    _compare(device, dh.to(F16), x * 16, wg * 8, wu * large * 8, act)
+
+
+def test_an_infinite_unit_beside_one_that_passes_the_range(device):
+    """dz = inf of one unit (x and the weights at the type's end) does not hide from the
+    choice of the power of two that du of the same unit passes the range"""
+    x = torch.full((3, 64), 60000.0, device="cuda", dtype=F16)
+    wg = torch.full((8, 64), 1e-3, device="cuda", dtype=F16)
+    wu = torch.full((8, 64), 1e-3, device="cuda", dtype=F16)
+    dh = torch.full((3, 8), 64.0, device="cuda", dtype=F16)
+    h, gate, up = th.gated_linear(device, x, wg, wu, "relu", save=True)
+    gate[:, [0, 1, 3, 4, 5, 6, 7]] = 1.0
+    up[:, 2] = math.inf  # (only there du passes the range, and dz beside it is infinite)
+    dx, dwg, dwu = th.gated_linear_grad(device, dh, x * 2.0**-24, wg, wu, gate, up, "relu")
+    du = dh.double() * gate.double()
+    want = torch.mm(du.t().contiguous(), (x * 2.0**-24).double())
+    assert float(du.abs().max()) > 65504 and float(want.abs().max()) < 65504
+    assert dwg[2].isinf().all() and not dwg[2].isnan().any()
+    err = (dwu.double() - want).abs()
+    assert (err <= 8 * 2.0**-11 * want.abs()).all()

@@ -66,6 +66,7 @@ enum { G_FORWARD = 0, G_INPUT = 1, G_WEIGHT = 2 };  // h; dx; dw_gate and dw_up
 struct GatedTiles {
   const void *a0, *a1;  // G_FORWARD, G_INPUT: w_gate, w_up; G_WEIGHT: x
   const void *b;        // G_FORWARD: x; else dz and du, a row's du behind its dz
+  const void *b_units;  // G_WEIGHT in f16: the same, where some passed the type's range
   uint64_t a_stride, b_stride;  // bytes
   uint64_t rows;        // of x
   uint32_t k, n;
@@ -77,8 +78,11 @@ struct GatedTiles {
   void *out, *out1, *out2;
   int64_t out_stride;   // elements
   float *part;          // sums of the splits, [split][row][column], in place of the above
-  const float *factor;  // of the results, or null
-  // f16 gradients: what dz and du are computed from
+  // f16 gradients: whether dz or du passed the type's range, and then the factors of dx's rows,
+  // or of dw_gate's and, from np on, dw_up's
+  const uint32_t *passed;
+  const float *factor;
+  // and what dz and du are computed from
   const f16_t *grad;
   int64_t grad_stride;
   const float *z, *u;
@@ -96,14 +100,14 @@ __device__ __forceinline__ void slopes(float dh, float z, float u, float &dz, fl
 
 // A gradient that comes out near f16's border (65520: what is rounded from there on is
 // infinite) says nothing of which side it is on: the rounding of dz and du to 11 bits moved
-// it by a rms of 0.29 2^-11 of a term times the root of the terms' number, 2e-4 of what is a
+// it by a rms of 0.4 2^-11 of a term times the root of the terms' number, 2e-4 of what is a
 // typical result of its row.  Such results are summed again by a wave, dz and du in f32 and
 // the sum in 64 bits.  Near is within 2^-9 of the border, or 2^-8 of a large result of the
 // row's 64 columns here, which is about 1.2 typical ones: 25 times the rms or more.  (Among 8 lanes'
 // largest, the smaller one of pairs, the larger one of two pairs, the smaller one of those: a
 // column that is far larger than the others does not make these near.)  Results far from
 // the border pay comparisons: a step of 1021 x 2001 x 5003 takes 266 us with them and 264
-// without.  One of 5 x 7040 x 8000 takes 252 where 1.5 % of the weights' gradients
+// without.  One of 5 x 7040 x 8000 takes 264 where 1.5 % of the weights' gradients
 // pass the border and 35 thousand are near it, 193 without.
 //
 // One result, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c
@@ -222,6 +226,8 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   const uint32_t half_steps = g.steps / 2u;  // G_INPUT: the stages of w_gate
   const uint8_t *a0 = reinterpret_cast<const uint8_t *>(g.a0), *a1 = reinterpret_cast<const uint8_t *>(g.a1);
   const uint8_t *b0 = reinterpret_cast<const uint8_t *>(g.b);
+  if constexpr (OP == G_WEIGHT && __is_same(T, f16_t))
+    if (*g.passed) b0 = reinterpret_cast<const uint8_t *>(g.b_units);
   if (OP == G_FORWARD) {
     a0 += (uint64_t)c0 * g.a_stride;
     a1 += (uint64_t)c0 * g.a_stride;
@@ -317,6 +323,9 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
   const uint64_t limit = OP == G_WEIGHT ? g.n : g.rows;  // rows of the output
   const uint32_t cols = OP == G_FORWARD ? g.n : g.k;
   const uint32_t cl = (l % LPR) * 8u, c = c0 + wa * (HALF / S::WA) + cl;
+  constexpr bool SETTLE = !PART && OP != G_FORWARD && __is_same(T, f16_t);
+  uint32_t passed = 0;
+  if constexpr (SETTLE) passed = *g.passed;
 #pragma unroll
   for (int j = 0; j < TB; ++j) {
     // (the waves that share a tile add their sums one after another)
@@ -337,7 +346,6 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     __builtin_amdgcn_wave_barrier();
     wait_reads();
     if (S::WK == 1 || wk == 0) {
-      constexpr bool SETTLE = !PART && OP != G_FORWARD && __is_same(T, f16_t);
       Border seen;
       // 8 columns of one of RPI rows; with AGAIN, those near the border are settled
       auto end = [&](uint32_t t, auto again) {
@@ -368,9 +376,10 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
           for (int e = 0; e < 8; ++e) v[e] = act_value<ACT>(v[e]) * w[e];
           store8(out + (int64_t)row * g.out_stride + c, m, v);
         } else {
-          if (g.factor) {
+          if (SETTLE && passed) {
+            const float f = row < limit ? g.factor[row + up * g.np] : 1.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
+            for (int e = 0; e < 8; ++e) v[e] *= f;
           }
           if constexpr (AGAIN) {
             if (!settle_border<OP>(g, v, m, (uint32_t)row + up * g.n, c)) return;
@@ -498,11 +507,10 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
     const float *p = g.part + row * pitch + c;
     join8(p, rows * pitch, g.splits, m, v);
     if (OP == G_FORWARD) join8(p + g.n, rows * pitch, g.splits, m, w);
-    if (OP != G_FORWARD && g.factor) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= *g.factor;
-    }
     if constexpr (SETTLE) {
+      const float f = *g.passed ? g.factor[OP == G_WEIGHT && row >= g.n ? row - g.n + g.np : row] : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= f;
       settle_border<OP>(g, v, i == i_ ? m : 0u, (uint32_t)row, c);
       if (i != i_) continue;
     }
@@ -525,38 +533,31 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
 }
 
 // dz and du from dh and the z and u that the forward pass kept (14 bytes a unit): rows of 2
-// np elements, zeros behind the n of each half.
-//
-// f16 (gradients that carry a loss scale may pass its 65504 here, where neither dh nor the
-// results do): each workgroup leaves the largest finite magnitude that it wrote, and a
-// second launch, AGAIN, writes them once more divided by a power of two if that was too
-// large, and otherwise ends at once.  The products' results are multiplied by it.
-constexpr uint32_t SLOPE_GROUPS = 2048;  // workgroups, with f16; the factor lies behind their maxima
+// np elements, zeros behind the n of each half.  f16: each workgroup leaves the largest
+// finite magnitude that it wrote.
+constexpr uint32_t SLOPE_GROUPS = 2048;  // workgroups, with f16
 
+__device__ __forceinline__ float larger_finite(float m, float v) {
+  v = fabsf(v);
+  return v < INFINITY ? fmaxf(m, v) : m;
+}
+// of the workgroup
 __device__ __forceinline__ float slope_max(float m, float *shared) {
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  __syncthreads();
   if ((threadIdx.x & 63u) == 0) shared[threadIdx.x / 64u] = m;
   __syncthreads();
   return fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
 }
 
-template <class T, int ACT, bool AGAIN>
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ grad, int64_t grad_stride,
                                                           const float *__restrict__ z, const float *__restrict__ u, uint64_t rows,
                                                           uint32_t n, uint32_t np, T *__restrict__ d, float *maxima) {
   constexpr bool SCALED = __is_same(T, f16_t);
   __shared__ float shared[4];
-  float factor = 1.0f, most = 0.0f;
-  if constexpr (AGAIN) {
-    float m = 0.0f;
-    for (uint32_t i = threadIdx.x; i < gridDim.x; i += 256u) m = fmaxf(m, maxima[i]);
-    m = slope_max(m, shared);
-    const int down = m > 65504.0f ? ilogbf(m) - 14 : 0;  // m 2^-down < 2^15
-    if (blockIdx.x == 0 && threadIdx.x == 0) maxima[SLOPE_GROUPS] = ldexpf(1.0f, down);
-    if (down == 0) return;
-    factor = ldexpf(1.0f, -down);
-  }
+  float most = 0.0f;
   const uint32_t groups = np / 8u;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * groups; i += (uint64_t)gridDim.x * 256u) {
     const uint64_t row = i / groups;
@@ -583,13 +584,7 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
         // (behind the end: zeros)
         a[e] = c + e < n ? dz : 0.0f;
         b[e] = c + e < n ? du : 0.0f;
-        if constexpr (AGAIN) {
-          a[e] *= factor;
-          b[e] *= factor;
-        } else if constexpr (SCALED) {
-          const float m = fmaxf(fabsf(a[e]), fabsf(b[e]));  // (of a NaN and a number: the number)
-          most = m < INFINITY ? fmaxf(most, m) : most;
-        }
+        if constexpr (SCALED) most = larger_finite(larger_finite(most, a[e]), b[e]);
       }
     } else {
 #pragma unroll
@@ -599,9 +594,92 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(const T *__restrict__ 
     store8(o, 8, a);
     store8(o + np, 8, b);
   }
-  if constexpr (SCALED && !AGAIN) {
+  if constexpr (SCALED) {
     most = slope_max(most, shared);
     if (threadIdx.x == 0) maxima[blockIdx.x] = most;
+  }
+}
+
+// f16 gradients that carry a loss scale may pass its 65504 in dz and du, where neither dh nor
+// the results do.  Where one did (else this launch ends at once, 4.7 us), they are
+// written once more, for dx with each row divided by a power of two that takes its
+// largest below 2^15, and for dw_gate and dw_up, into d_units, with each unit's dz and du
+// so: a result depends on its own row, or unit, and the others' sizes take none of its
+// bits.  The products' results are multiplied by the powers.
+__device__ __forceinline__ int passed_by(float largest) { return largest > 65504.0f ? ilogbf(largest) - 14 : 0; }
+
+template <int ACT>
+__global__ __launch_bounds__(256) void gated_rescale_kernel(const f16_t *__restrict__ grad, int64_t grad_stride,
+                                                            const float *__restrict__ z, const float *__restrict__ u, uint64_t rows,
+                                                            uint32_t n, uint32_t np, f16_t *__restrict__ d, f16_t *__restrict__ d_units,
+                                                            const float *__restrict__ maxima, uint32_t groups, uint32_t *passed,
+                                                            float *__restrict__ row_factor, float *__restrict__ unit_factor) {
+  constexpr uint32_t COLS = 32, DEEP = 256 / COLS;  // units of a workgroup, rows at a time
+  __shared__ float shared[4], tall[2][DEEP][COLS];
+  float m = 0.0f;
+  for (uint32_t i = threadIdx.x; i < groups; i += 256u) m = fmaxf(m, maxima[i]);
+  m = slope_max(m, shared);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *passed = m > 65504.0f;
+  if (!(m > 65504.0f)) return;
+  auto pair = [&](uint64_t row, uint32_t c, float &dz, float &du) {
+    slopes<ACT>((float)grad[(int64_t)row * grad_stride + c], z[row * n + c], u[row * n + c], dz, du);
+  };
+  float dz, du;
+  // rows first, then units
+  for (uint64_t item = blockIdx.x; item < rows + np / COLS; item += gridDim.x) {
+    if (item < rows) {
+      float most = 0.0f;
+#pragma unroll 4
+      for (uint32_t c = threadIdx.x; c < n; c += 256u) {
+        pair(item, c, dz, du);
+        most = larger_finite(larger_finite(most, dz), du);
+      }
+      const int down = passed_by(slope_max(most, shared));
+      if (threadIdx.x == 0) row_factor[item] = ldexpf(1.0f, down);
+      if (down == 0) continue;  // (written so already)
+      const float f = ldexpf(1.0f, -down);
+#pragma unroll 4
+      for (uint32_t c = threadIdx.x; c < n; c += 256u) {
+        pair(item, c, dz, du);
+        f16_t *o = d + item * 2u * np + c;
+        o[0] = (f16_t)(dz * f);
+        o[np] = (f16_t)(du * f);
+      }
+    } else {
+      const uint32_t lo = threadIdx.x % COLS, hi = threadIdx.x / COLS, c = (uint32_t)(item - rows) * COLS + lo;
+      float za = 0.0f, ua = 0.0f;
+      if (c < n) {
+#pragma unroll 4
+        for (uint64_t row = hi; row < rows; row += DEEP) {
+          pair(row, c, dz, du);
+          za = larger_finite(za, dz);
+          ua = larger_finite(ua, du);
+        }
+      }
+      __syncthreads();
+      tall[0][hi][lo] = za;
+      tall[1][hi][lo] = ua;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t i = 0; i < DEEP; ++i) {
+        za = fmaxf(za, tall[0][i][lo]);
+        ua = fmaxf(ua, tall[1][i][lo]);
+      }
+      const int zd = passed_by(za), ud = passed_by(ua);
+      if (hi == 0) {
+        unit_factor[c] = ldexpf(1.0f, zd);
+        unit_factor[np + c] = ldexpf(1.0f, ud);
+      }
+      const float zf = ldexpf(1.0f, -zd), uf = ldexpf(1.0f, -ud);
+#pragma unroll 4
+      for (uint64_t row = hi; row < rows; row += DEEP) {
+        dz = du = 0.0f;
+        if (c < n) pair(row, c, dz, du);
+        f16_t *o = d_units + row * 2u * np + c;
+        o[0] = (f16_t)(dz * zf);
+        o[np] = (f16_t)(du * uf);
+      }
+    }
   }
 }
 
@@ -655,8 +733,10 @@ typedef TileShape<128, 64, 2, 4, 1, 128, 2, true> Tile256;
 struct GatedPlan {
   bool few;  // the forward pass reads the operands as they lie
   bool pack_x, pack_w;
+  bool scaled;  // dz and du may pass the type's range
   uint32_t kp, np;
-  uint64_t x_bytes, w_bytes, d_bytes, m_bytes;  // packed x, each packed weight, dz and du, their maxima
+  // packed x, each packed weight, dz and du; f16: their maxima, whether one passed, and factors
+  uint64_t x_bytes, w_bytes, d_bytes, m_bytes;
   TilePlan forward, input, weight;
   GatedPlan(const thrml_ctx *ctx, const thrml_gated &g) {
     // (whole lines of memory: rows of 7088 bytes take 34 us where rows of 7168 take 26, at 121 x
@@ -668,7 +748,8 @@ struct GatedPlan {
     x_bytes = pack_x ? tile_bytes(g.rows * kp * 2u) : 0;
     w_bytes = pack_w ? tile_bytes((uint64_t)g.n * kp * 2u) : 0;
     d_bytes = tile_bytes(g.rows * 2u * np * 2u);
-    m_bytes = g.dtype == THRML_DTYPE_F16 ? tile_bytes((SLOPE_GROUPS + 1) * 4) : 0;
+    scaled = g.dtype == THRML_DTYPE_F16;
+    m_bytes = scaled ? tile_bytes((SLOPE_GROUPS + 1 + g.rows + 2ull * np) * 4) : 0;
     few = (pack_x || pack_w) && g.rows <= 32;
     forward = plan_tiles(ctx, gated_kinds, 4, 2ull * g.n, g.rows, false, g.k * 2ull, g.rows * 2u * g.n);
     input = plan_tiles(ctx, gated_kinds, 4, g.k, g.rows, false, np * 4ull, g.rows * g.k);
@@ -679,7 +760,7 @@ struct GatedPlan {
 uint64_t gated_work(thrml_ctx *ctx, const thrml_gated &g, bool backward) {
   const GatedPlan p(ctx, g);
   if (p.few && !backward) return 0;
-  return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes + p.m_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
+  return p.x_bytes + 2 * p.w_bytes + (backward ? p.d_bytes * (p.scaled ? 2 : 1) + p.m_bytes + std::max(p.input.part, p.weight.part) : p.forward.part);
 }
 
 static int launch_pack(thrml_ctx *ctx, const void *x, int64_t stride, uint64_t rows, uint32_t k, uint32_t kp, void *out) {
@@ -817,8 +898,11 @@ int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, in
   t.b = w;
   t.b_stride = (uint64_t)p.np * 4u;
   w += p.d_bytes;
-  float *maxima = p.m_bytes ? reinterpret_cast<float *>(w) : nullptr;
-  t.factor = maxima ? maxima + SLOPE_GROUPS : nullptr;
+  t.b_units = w;
+  if (p.scaled) w += p.d_bytes;
+  float *maxima = reinterpret_cast<float *>(w), *row_factor = maxima + SLOPE_GROUPS + 1, *unit_factor = row_factor + g.rows;
+  uint32_t *passed = reinterpret_cast<uint32_t *>(maxima + SLOPE_GROUPS);
+  t.passed = passed;
   t.grad = reinterpret_cast<const f16_t *>(grad);
   t.grad_stride = grad_stride;
   t.z = gate;
@@ -830,24 +914,28 @@ int launch_gated_grad(thrml_ctx *ctx, const thrml_gated &g, const void *grad, in
     typedef decltype(e) T;
     constexpr int ACT = decltype(act)::value;
     const uint64_t n = g.rows * (p.np / 8u);
-    const dim3 grid((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), maxima ? SLOPE_GROUPS : 1u << 16));
-    auto slope = [&](auto *f) -> int {
-      hipLaunchKernelGGL(f, grid, dim3(256), 0, ctx->stream, reinterpret_cast<const T *>(grad), grad_stride, gate, up, g.rows, g.n,
-                         p.np, reinterpret_cast<T *>(const_cast<void *>(t.b)), maxima);
+    const dim3 grid((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), p.scaled ? SLOPE_GROUPS : 1u << 16));
+    const T *dh = reinterpret_cast<const T *>(grad);
+    T *d = reinterpret_cast<T *>(const_cast<void *>(t.b)), *d_units = reinterpret_cast<T *>(const_cast<void *>(t.b_units));
+    hipLaunchKernelGGL((gated_slope_kernel<T, ACT>), grid, dim3(256), 0, ctx->stream, dh, grad_stride, gate, up, g.rows, g.n, p.np, d,
+                       p.scaled ? maxima : nullptr);
+    THRML_HIP(hipGetLastError());
+    if constexpr (__is_same(T, f16_t)) {
+      const dim3 items((uint32_t)std::min<uint64_t>(g.rows + p.np / 32u, SLOPE_GROUPS));
+      hipLaunchKernelGGL((gated_rescale_kernel<ACT>), items, dim3(256), 0, ctx->stream, dh, grad_stride, gate, up, g.rows, g.n, p.np, d,
+                         d_units, maxima, grid.x, passed, row_factor, unit_factor);
       THRML_HIP(hipGetLastError());
-      return THRML_OK;
-    };
-    if (int rc = slope(&gated_slope_kernel<T, ACT, false>)) return rc;
-    if constexpr (__is_same(T, f16_t))
-      if (int rc = slope(&gated_slope_kernel<T, ACT, true>)) return rc;
+    }
     // (the products do not use the activation)
     if (dx) {
       GatedTiles i = t;
+      i.factor = row_factor;
       i.out = dx;
       i.out_stride = dx_stride;
       if (int rc = launch_product<G_INPUT, T, THRML_ACT_RELU>(ctx, p.input, i)) return rc;
     }
     GatedTiles i = t;
+    i.factor = unit_factor;
     i.a0 = i.a1 = x;
     i.a_stride = x_stride;
     i.out = dw_gate;
