@@ -164,3 +164,47 @@ def test_an_infinite_unit_beside_one_that_passes_the_range(device):
     assert dwg[2].isinf().all() and not dwg[2].isnan().any()
     err = (dwu.double() - want).abs()
     assert (err <= 8 * 2.0**-11 * want.abs()).all()
+
+
+def test_captured(device):
+    """a captured step, replayed on gradients that pass the range and that do not, in turn"""
+    dev = th.Device(0)
+    side = torch.cuda.Stream()
+    dev.set_stream(side.cuda_stream)
+    cases = [(300, 264, 520), (13, 1000, 1003)]
+    ins = [[*_inputs(*c)] for c in cases]
+    for i in ins:
+        i[3] = i[3].to(F16)
+    step = lambda x, wg, wu, dh: (lambda h, a, b: th.gated_linear_grad(dev, dh, x, wg, wu, a, b))(  # noqa: E731
+        *th.gated_linear(dev, x, wg, wu, save=True))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for i in ins:
+            step(*i)
+    side.synchronize()
+    graphs, outs = [], []
+    for i in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step(*i))
+        graphs.append(graph)
+    infinite = []
+    for turn in range(4):
+        for c, i in zip(cases, ins):
+            for t, new in zip(i, _inputs(*c, seed=turn + 1)):
+                t.copy_((new * 9000).clamp(-65504, 65504) if t is i[3] and turn % 2 else new)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for graph in graphs:
+                graph.replay()
+            eager = [step(*i) for i in ins]
+            for graph in reversed(graphs):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, eager):
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+        infinite.append(any(bool(t.isinf().any()) for want in eager for t in want))
+    assert infinite == [False, True, False, True]
+    del graphs
+    torch.cuda.synchronize()
+    dev.close()

@@ -101,43 +101,55 @@ __device__ __forceinline__ void slopes(float dh, float z, float u, float &dz, fl
 // A gradient that comes out near f16's border (65520: what is rounded from there on is
 // infinite) says nothing of which side it is on: the rounding of dz and du to 11 bits moved
 // it by a rms of 0.4 2^-11 of a term times the root of the terms' number, 2e-4 of what is a
-// typical result of its row.  Such results are summed again by a wave, dz and du in f32 and
-// the sum in 64 bits.  Near is within 2^-9 of the border, or 2^-8 of a large result of the
-// row's 64 columns here, which is about 1.2 typical ones: 25 times the rms or more.  (Among 8 lanes'
+// typical result of its row.  Such results are summed again, dz and du in f32 and the sum in
+// 64 bits.  Near is within 2^-10 of the border, or 2^-9 of a large result of the row's 64
+// columns here, which is about 1.2 typical ones: 12 times the rms.  (Among 8 lanes'
 // largest, the smaller one of pairs, the larger one of two pairs, the smaller one of those: a
 // column that is far larger than the others does not make these near.)  Results far from
-// the border pay comparisons: a step of 1021 x 2001 x 5003 takes 266 us with them and 264
-// without.  One of 5 x 7040 x 8000 takes 264 where 1.5 % of the weights' gradients
-// pass the border and 35 thousand are near it, 193 without.
-//
-// One result, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c
+// the border pay comparisons: a step of 1021 x 2001 x 5003 takes 261 us with them
+// and without.  One of 5 x 7040 x 8000 takes 273 where 1.5 % of the weights' gradients pass the
+// border and 17 thousand are near it, 193 without these sums.
+__device__ __forceinline__ void slopes_of(const GatedTiles &g, float dh, float z, float u, float &dz, float &du) {
+  if (g.act == THRML_ACT_RELU)
+    slopes<THRML_ACT_RELU>(dh, z, u, dz, du);
+  else if (g.act == THRML_ACT_GELU)
+    slopes<THRML_ACT_GELU>(dh, z, u, dz, du);
+  else
+    slopes<THRML_ACT_SILU>(dh, z, u, dz, du);
+}
+
+// One result by a wave, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c;
+// the loads of U turns are under way together
 template <int OP>
 __device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row, uint32_t c) {
-  const uint32_t l = here(threadIdx.x) & 63u;
-  auto pair = [&](uint64_t r, uint32_t unit, float &dz, float &du) {
-    const float dh = (float)g.grad[(int64_t)r * g.grad_stride + unit], z = g.z[r * g.n + unit], u = g.u[r * g.n + unit];
-    if (g.act == THRML_ACT_RELU)
-      slopes<THRML_ACT_RELU>(dh, z, u, dz, du);
-    else if (g.act == THRML_ACT_GELU)
-      slopes<THRML_ACT_GELU>(dh, z, u, dz, du);
-    else
-      slopes<THRML_ACT_SILU>(dh, z, u, dz, du);
-  };
-  auto operand = [&](const void *p, uint64_t r) {
-    return (double)(float)*reinterpret_cast<const f16_t *>(reinterpret_cast<const uint8_t *>(p) + r * g.a_stride + c * 2ull);
-  };
+  constexpr uint32_t U = 8;
+  const bool up = OP == G_WEIGHT && row >= g.n;
+  const uint64_t all = OP == G_WEIGHT ? g.rows : g.n;
   double sum = 0.0;
-  float dz, du;
-  if constexpr (OP == G_WEIGHT) {
-    const bool up = row >= g.n;
-    for (uint64_t r = l; r < g.rows; r += 64u) {
-      pair(r, up ? row - g.n : row, dz, du);
-      sum += (double)(up ? du : dz) * operand(g.a0, r);
+  for (uint64_t i0 = here(threadIdx.x) & 63u; i0 < all; i0 += 64u * U) {
+    float dh[U], z[U], u[U], a0[U], a1[U];
+#pragma unroll
+    for (uint32_t e = 0; e < U; ++e) {
+      const uint64_t i = min(i0 + 64u * e, all - 1u), r = OP == G_WEIGHT ? i : row;
+      const uint32_t unit = OP == G_WEIGHT ? (up ? row - g.n : row) : (uint32_t)i;
+      auto operand = [&](const void *p) {
+        return (float)*reinterpret_cast<const f16_t *>(reinterpret_cast<const uint8_t *>(p) + i * g.a_stride + c * 2ull);
+      };
+      dh[e] = (float)g.grad[(int64_t)r * g.grad_stride + unit];
+      z[e] = g.z[r * g.n + unit];
+      u[e] = g.u[r * g.n + unit];
+      a0[e] = operand(g.a0);
+      if (OP == G_INPUT) a1[e] = operand(g.a1);
     }
-  } else {
-    for (uint32_t unit = l; unit < g.n; unit += 64u) {
-      pair(row, unit, dz, du);
-      sum += (double)dz * operand(g.a0, unit) + (double)du * operand(g.a1, unit);
+#pragma unroll
+    for (uint32_t e = 0; e < U; ++e) {
+      if (i0 + 64u * e >= all) break;
+      float dz, du;
+      slopes_of(g, dh[e], z[e], u[e], dz, du);
+      if (OP == G_WEIGHT)
+        sum += (double)(up ? du : dz) * (double)a0[e];
+      else
+        sum += (double)dz * (double)a0[e] + (double)du * (double)a1[e];
     }
   }
 #pragma unroll
@@ -164,23 +176,28 @@ struct Border {
     float m = fminf(most, __shfl_xor(most, 1));
     m = fmaxf(m, __shfl_xor(m, 2));
     m = fminf(m, __shfl_xor(m, 4));
-    band = fmaxf(0x1p-8f * m, 0x1p-9f * BORDER);
+    band = fmaxf(0x1p-9f * m, 0x1p-10f * BORDER);
     return __any(nearest <= band);
   }
 };
 
-// The results v of row `row` from column c on, of which m count (0 in a lane that has none:
-// all lanes of the wave come here); whether this lane's were summed again.
-template <int OP>
-__device__ __forceinline__ bool settle_border(const GatedTiles &g, float (&v)[8], uint32_t m, uint32_t row, uint32_t c) {
+// which of 8 results are near, m of them that count (all lanes of the wave come here)
+__device__ __forceinline__ uint32_t border_bits(const float (&v)[8], uint32_t m) {
   Border b;
   b.see(v);  // (those of no column or row are as large as the others)
   float band;
-  if (!b.any_near(band)) return false;
+  if (!b.any_near(band)) return 0;
   uint32_t bits = 0;
 #pragma unroll
   for (uint32_t e = 0; e < 8; ++e) bits |= (uint32_t)(e < m && fabsf(fabsf(v[e]) - BORDER) <= band) << e;
-  const bool some = bits != 0;
+  return bits;
+}
+
+// The results v of row `row` from column c on, of which m count (0 in a lane that has none), one
+// after another: the few of a join.
+template <int OP>
+__device__ __forceinline__ void settle_each(const GatedTiles &g, float (&v)[8], uint32_t m, uint32_t row, uint32_t c) {
+  uint32_t bits = border_bits(v, m);
   for (uint64_t any = __ballot(bits != 0); any; any = __ballot(bits != 0)) {
     const int lane = __builtin_ctzll(any);
     const uint32_t of = (uint32_t)__builtin_amdgcn_readlane((int)bits, lane), at = (uint32_t)__builtin_ctz(of);
@@ -192,7 +209,109 @@ __device__ __forceinline__ bool settle_border(const GatedTiles &g, float (&v)[8]
       bits &= bits - 1u;
     }
   }
-  return some;
+}
+
+// Those of a wave's 32 rows (from row0 on, of `limit`) x MA columns (from c0 on) at the end of
+// a tile, which lie in `mine` before their factors and have been stored: each lane sums one, 64
+// at a time, of operands that come through LDS, DEEP of the reduction at a time: 32 rows' dz
+// or du (dx: both) and MA columns of the other side.  In a step of 4096 x 4096 x 8192 with 87 %
+// of the weights' gradients infinite, the
+// gradient takes 7.6 ms (1.06 where none is near); each by the wave (gated_again) it took 122.
+template <int OP, int MA, uint32_t LPR>
+__device__ __forceinline__ void settle_slab(const GatedTiles &g, bool passed, float *mine, uint64_t row0, uint32_t up, uint64_t limit,
+                                            uint32_t c0, uint32_t cols, f16_t *out) {
+  constexpr uint32_t PITCH = MA + 4, RPI = 64u / LPR, DEEP = 16, DP = 33, SIDES = OP == G_INPUT ? 2 : 1;
+  static_assert(256u + SIDES * DEEP * (DP * 4u + MA * 2u) <= 32u * PITCH * 4u, "fits where the results were");
+  const uint32_t l = here(threadIdx.x) & 63u;
+  uint64_t marks = 0;
+#pragma unroll 1
+  for (uint32_t t = 0; t < 32u / RPI; ++t) {
+    const uint32_t rl = t * RPI + l / LPR, cl = l % LPR * 8u;
+    const uint64_t row = row0 + rl;
+    const float f = passed && row < limit ? g.factor[row + up * g.np] : 1.0f;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = mine[rl * PITCH + cl + e] * f;
+    marks |= (uint64_t)border_bits(v, row < limit && c0 + cl < cols ? cols - c0 - cl : 0u) << (8u * t);
+  }
+  wait_loads<0>();  // (the stores of these results have ended)
+  uint32_t *list = reinterpret_cast<uint32_t *>(mine);
+  float *d = mine + 64;
+  uint32_t *a = reinterpret_cast<uint32_t *>(d + SIDES * DEEP * DP);
+  auto fence = [] {
+    __builtin_amdgcn_wave_barrier();
+    wait_reads();
+  };
+  while (__ballot(marks != 0)) {
+    // the next 64 of the wave's
+    uint32_t scan = (uint32_t)__popcll(marks);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const uint32_t o = (uint32_t)__shfl_up((int)scan, s);
+      if (l >= (uint32_t)s) scan += o;
+    }
+    const uint32_t total = min((uint32_t)__builtin_amdgcn_readlane((int)scan, 63), 64u);
+    uint32_t at = scan - (uint32_t)__popcll(marks);
+    fence();
+    while (marks && at < 64u) {
+      const uint32_t bit = (uint32_t)__builtin_ctzll(marks);
+      marks &= marks - 1u;
+      list[at++] = (bit / 8u * RPI + l / LPR) << 16 | (l % LPR * 8u + bit % 8u);
+    }
+    fence();
+    const uint32_t code = list[min(l, total - 1u)], rl = code >> 16, cl = code & 0xffffu;
+    const uint64_t all = OP == G_WEIGHT ? g.rows : g.n;
+    double sum = 0.0;
+    for (uint64_t i0 = 0; i0 < all; i0 += DEEP) {
+      constexpr uint32_t D_TURNS = DEEP / 2, A_ROWS = 128 / MA, A_TURNS = DEEP / A_ROWS;
+      float dh[D_TURNS], z[D_TURNS], u[D_TURNS];
+      uint32_t w[SIDES][A_TURNS];
+      // lanes along what is contiguous: units
+      auto place = [&](uint32_t e, uint32_t &i, uint32_t &r) {  // of the reduction, of the rows
+        i = OP == G_WEIGHT ? 2u * e + l / 32u : l % DEEP;
+        r = OP == G_WEIGHT ? l % 32u : 4u * e + l / DEEP;
+      };
+#pragma unroll
+      for (uint32_t e = 0; e < D_TURNS; ++e) {
+        uint32_t i, r;
+        place(e, i, r);
+        const uint64_t red = min(i0 + i, all - 1u), own = min(row0 + r, limit - 1u);
+        const uint64_t row = OP == G_WEIGHT ? red : own, unit = OP == G_WEIGHT ? own : red;
+        dh[e] = (float)g.grad[(int64_t)row * g.grad_stride + (int64_t)unit];
+        z[e] = g.z[row * g.n + unit];
+        u[e] = g.u[row * g.n + unit];
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < A_TURNS; ++e) {
+        const uint64_t red = min(i0 + e * A_ROWS + l / (MA / 2u), all - 1u);
+        const uint32_t c = min(c0 + l % (MA / 2u) * 2u, ((g.k + 7u) & ~7u) - 2u);
+        w[0][e] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(g.a0) + red * g.a_stride + c * 2ull);
+        if (SIDES == 2) w[1][e] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(g.a1) + red * g.a_stride + c * 2ull);
+      }
+      fence();
+#pragma unroll
+      for (uint32_t e = 0; e < D_TURNS; ++e) {
+        uint32_t i, r;
+        place(e, i, r);
+        float dz, du;
+        slopes_of(g, dh[e], z[e], u[e], dz, du);
+        d[i * DP + r] = OP == G_WEIGHT && up ? du : dz;
+        if (SIDES == 2) d[(DEEP + i) * DP + r] = du;
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < A_TURNS; ++e)
+#pragma unroll
+        for (uint32_t o = 0; o < SIDES; ++o) a[(o * DEEP + e * A_ROWS) * (MA / 2u) + l] = w[o][e];
+      fence();
+      const uint32_t left = (uint32_t)min((uint64_t)DEEP, all - i0);
+#pragma unroll
+      for (uint32_t o = 0; o < SIDES; ++o)
+#pragma unroll 4
+        for (uint32_t i = 0; i < left; ++i)
+          sum += (double)d[(o * DEEP + i) * DP + rl] * (double)(float)reinterpret_cast<const f16_t *>(a)[(o * DEEP + i) * MA + cl];
+    }
+    if (l < total) out[(int64_t)(row0 + rl) * g.out_stride + c0 + cl] = (f16_t)(float)sum;
+  }
 }
 
 template <class S, int OP, class T, int ACT, bool PART>
@@ -347,13 +466,12 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
     wait_reads();
     if (S::WK == 1 || wk == 0) {
       Border seen;
-      // 8 columns of one of RPI rows; with AGAIN, those near the border are settled
-      auto end = [&](uint32_t t, auto again) {
-        constexpr bool AGAIN = decltype(again)::value;
+#pragma unroll
+      for (uint32_t t = 0; t < 32u / RPI; ++t) {
         const uint32_t rl = t * RPI + l / LPR;
         const uint64_t row = r0 + wb * S::MB + 32u * j + rl;
         const uint32_t m = row < limit && c < cols ? cols - c : 0u;
-        if (!SETTLE && m == 0) return;
+        if (!SETTLE && m == 0) continue;
         float v[8], w[8];
         const float *at = mine + rl * PITCH + cl;
 #pragma unroll
@@ -381,23 +499,17 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= f;
           }
-          if constexpr (AGAIN) {
-            if (!settle_border<OP>(g, v, m, (uint32_t)row + up * g.n, c)) return;
-          } else if constexpr (SETTLE) {
+          if constexpr (SETTLE) {
             seen.see(v);  // (those of no column, too: they repeat others)
-            if (m == 0) return;
+            if (m == 0) continue;
           }
           store8(out + (int64_t)row * g.out_stride + c, m, v);
         }
-      };
-#pragma unroll
-      for (uint32_t t = 0; t < 32u / RPI; ++t) end(t, std::false_type{});
+      }
       if constexpr (SETTLE) {
         float band;
-        if (seen.any_near(band)) {
-#pragma unroll 1
-          for (uint32_t t = 0; t < 32u / RPI; ++t) end(t, std::true_type{});
-        }
+        if (seen.any_near(band))
+          settle_slab<OP, S::MA, LPR>(g, passed != 0, mine, r0 + wb * S::MB + 32u * j, up, limit, c0 + wa * (HALF / S::WA), cols, out);
       }
     }
     if (S::WK > 1)
@@ -511,7 +623,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
       const float f = *g.passed ? g.factor[OP == G_WEIGHT && row >= g.n ? row - g.n + g.np : row] : 1.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= f;
-      settle_border<OP>(g, v, i == i_ ? m : 0u, (uint32_t)row, c);
+      settle_each<OP>(g, v, i == i_ ? m : 0u, (uint32_t)row, c);
       if (i != i_) continue;
     }
     if constexpr (OP == G_FORWARD) {
