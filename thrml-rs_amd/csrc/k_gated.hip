@@ -33,14 +33,39 @@ struct Frag<f16_t> {
 
 // ---------------------------------------------------------------------------
 // The activation and its derivative
+
+// The normal distribution function at z, and e = exp(-z^2 / 2), for gelu: below 0, where 1 +
+// erf(z / sqrt 2) loses its bits, it is e Q(t) t with t = 1 / (1 + 0.345 |z|), and above 1 less
+// that.  Q is the polynomial of degree 8 of least relative error over |z| up to 13.5 (2e-8;
+// weighted least squares).  In all within (8 + 2 z^2) 2^-24 of its value, the second part from
+// the rounded exponent; 0 from about z = -13.2 down.  A forward product of 4096 x 4096 x 8192
+// takes 427 us with it, 435 with erff and 438 with erfcf.
+__device__ __forceinline__ float normal_cdf(float z, float &e) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.345f, 1.0f));
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  float q = -0.028427219f;
+  q = __builtin_fmaf(q, t, 0.14548801f);
+  q = __builtin_fmaf(q, t, -0.27156994f);
+  q = __builtin_fmaf(q, t, 0.18761782f);
+  q = __builtin_fmaf(q, t, -0.037870139f);
+  q = __builtin_fmaf(q, t, 0.11190453f);
+  q = __builtin_fmaf(q, t, 0.11721380f);
+  q = __builtin_fmaf(q, t, 0.13802400f);
+  q = __builtin_fmaf(q, t, 0.13761912f);
+  q *= t * e;
+  return z < 0.0f ? q : 1.0f - q;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == THRML_ACT_RELU) return z < 0.0f ? 0.0f : z;  // (NaN stays)
-  // (hardware exponential and reciprocal: within |z| 2^-24 and 2^-23 of the value, where its
-  // result is rounded to 16 bits; with expf and a division the end of a tile took 17 of 200
-  // thousand cycles)
+  // (hardware exponential and reciprocal: the exponent is rounded, and its factor's 2^-26, so
+  // that the value is off by (1.3 |z| + 8) 2^-24 of it at most, where it is rounded to 16
+  // bits; with expf and a division the end of a tile took 17 of 200 thousand cycles.  0 from
+  // about z = -88 down)
   if constexpr (ACT == THRML_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950f));
-  return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+  float e;
+  return z * normal_cdf(z, e);
 }
 template <int ACT>
 __device__ __forceinline__ void act_both(float z, float &value, float &slope) {
@@ -53,9 +78,10 @@ __device__ __forceinline__ void act_both(float z, float &value, float &slope) {
     value = z * sig;
     slope = sig * (1.0f + z * other);
   } else {
-    const float cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
+    float e;
+    const float cdf = normal_cdf(z, e);
     value = z * cdf;
-    slope = cdf + z * expf(-0.5f * z * z) * 0.39894228f;
+    slope = cdf + z * e * 0.39894228f;
   }
 }
 
