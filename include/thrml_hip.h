@@ -570,8 +570,9 @@ typedef struct {
   const void *w_up;
   int64_t up_stride;
 } thrml_gated;
-/* h[row][c] rounded once to the type (not x or a weight); gate and up, both or neither NULL, receive z and
- * u in f32, [rows][n] contiguous, for thrml_gated_backward.  work: thrml_gated_work(in, 0)
+/* h[row][c] rounded once to the type; gate and up, both or neither NULL, receive z and
+ * u in f32, [rows][n] contiguous, for thrml_gated_backward.  Outputs share no memory with
+ * x, the weights, work or each other (their pointers are compared, their ranges are the caller's).  work: thrml_gated_work(in, 0)
  * bytes.  The operands are read as they lie where their rows are whole 16-byte pieces
  * (k a multiple of 8, pointers of 16 bytes, strides of 8 elements, those of the two
  * weights alike), else from a copy in work. */
@@ -583,7 +584,8 @@ int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t 
  *                                             power of two where one would pass 65504)
  *   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x
  * dx [rows][k] in rows of dx_stride (NULL: not computed), dw_gate and dw_up [n][k]
- * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes. */
+ * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes.  Outputs
+ * share no memory with an input, work or each other. */
 int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad, int64_t grad_stride,
                          const float *gate, const float *up, void *dx, int64_t dx_stride, void *dw_gate,
                          void *dw_up, void *work, uint64_t work_bytes);
@@ -595,7 +597,7 @@ int thrml_gated_backward(thrml_ctx *ctx, const thrml_gated *in, const void *grad
  * is kept), product and sum in f32, rounded once to the type.  A dropped unit counts as 0
  * whatever it holds.  seed_at, unless NULL, is device memory with the seed, read when
  * the kernel runs, in place of seed.  residual may be NULL.  y may be x or residual (with
- * its stride).  With x the gradient in y and no residual it gives the gradient in x.
+ * its stride), and shares no other memory with them or seed_at.  With x the gradient in y and no residual it gives the gradient in x.
  * (first_row + rows) cols is at most 2^37. */
 int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint64_t cols, int64_t x_stride,
                   const void *residual, int64_t residual_stride, uint64_t seed, const int64_t *seed_at,
@@ -609,7 +611,8 @@ int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint6
  * w_scale [ceil(q / 128)][ceil(k / 128)], bias may be NULL.  Sums are f32.  For y in bf16
  * or f16 the products of a block are added by the 8-bit matrix unit, which keeps 2^-16 of
  * the largest; for y in f32 exactly.  A row of x with an infinity or a NaN gives NaN.
- * work: thrml_linear_f8_work bytes, for the same arguments. */
+ * work: thrml_linear_f8_work bytes, for the same arguments.  y shares no memory with an input
+ * or work. */
 uint64_t thrml_linear_f8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, const void *w, uint32_t q,
                               int64_t w_stride, int out_dtype);
 int thrml_linear_f8(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint32_t k, int64_t x_stride,

@@ -12,6 +12,8 @@ do not go through them (gated_linear_grad gives the gradients).
 """
 import struct
 
+import numpy as np
+
 from . import _lib, head
 from ._lib import load
 from .head import _matrix, _on_device, _out, _refuse, _run
@@ -26,6 +28,28 @@ def _halves():
     if head.torch is None:
         head._setup()
     return head._FLOATS[1:]
+
+
+def _layout(t):
+    """(rows, bytes from one row to the next, bytes of a row) of a matrix with contiguous rows"""
+    rows, cols = t.shape
+    size = t.element_size()
+    return (rows, t.stride(0) * size, cols * size) if rows > 1 and t.stride(0) else (min(rows, 1), cols * size, cols * size)
+
+
+def _overlap(a, b):
+    """Whether two matrices with contiguous rows share memory: rows of one may lie between
+    those of the other."""
+    (ra, sa, la), (rb, sb, lb) = _layout(a), _layout(b)
+    d = b.data_ptr() - a.data_ptr()
+    if not (ra and rb and la and lb) or d >= (ra - 1) * sa + la or -d >= (rb - 1) * sb + lb:
+        return False
+    if ra > rb:
+        ra, sa, la, rb, sb, lb, d = rb, sb, lb, ra, sa, la, -d
+    # row i of a and j of b share bytes where i sa - d - lb < j sb < i sa - d + la
+    at = np.arange(ra, dtype=np.int64) * sa - d
+    first = np.maximum((at - lb) // sb + 1, 0)
+    return bool(((first < rb) & (first * sb < at + la)).any())
 
 
 def _gated(x, w_gate, w_up, activation):
@@ -51,7 +75,8 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
     """Hidden units h [rows, n] = act(x @ w_gate.T) * (x @ w_up.T) of features x [rows, k]
     and weights [n, k], all bfloat16 or all float16; sums, activation and product in
     float32, rounded once.  activation: "silu", "gelu" (of the error function) or "relu".
-    With save, (h, gate, up): also both products in float32, for gated_linear_grad.  out: a tensor for h, other than x and the weights.
+    With save, (h, gate, up): also both products in float32, for gated_linear_grad.  out: a
+    tensor for h, which shares no memory with x and the weights.
 
     Rows that are not whole 16-byte pieces (k not a multiple of 8, a view that starts or
     steps elsewhere) are copied first; the weights of a model are better kept aligned."""
@@ -62,7 +87,10 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
         _on_device(device, _NAMES, keep)
         out = head.torch.empty((rows, n), dtype=dtype, device=keep[0].device)
     else:
-        _on_device(device, _NAMES + ("out",), keep + (_out("out", out, rows, n, dtype),))
+        _out("out", out, rows, n, dtype)
+        if any(_overlap(out, t) for t in keep):
+            _refuse("h must not be x or a weight, nor lie in their memory")
+        _on_device(device, _NAMES + ("out",), keep + (out,))
         if rows > 1:
             stride = out.stride(0)
     where = out.device
@@ -115,11 +143,11 @@ def dropout(device, x, key, p, residual=None, first_row=0, out=None):
     key: an RngKey, used for nothing else, or its seed in an int64 tensor of one element
     on the device, which is read when the kernel runs: a captured call draws other bits
     when it changes.  first_row: where x is a part of a larger batch, its first row
-    there.  out: a tensor for the result; it may be x or residual."""
+    there.  out: a tensor for the result; it may be x or residual (the same rows), and share
+    no other memory with them."""
     if head.torch is None:
         head._setup()
     torch = head.torch
-    x0, residual0 = x, residual
     x, xs = _matrix("x", x, head._FLOATS)
     rows, cols = x.shape
     rs = rp = 0
@@ -141,8 +169,12 @@ def dropout(device, x, key, p, residual=None, first_row=0, out=None):
         _refuse("first_row must lie in 0 .. 2^37")
     if out is not None:
         _out("out", out, rows, cols, x.dtype)
-        if (out is x0 and x is not x0) or (out is residual0 and residual is not residual0):
-            _refuse("out may be x or residual only where their rows are contiguous")
+        for t in (x, residual):
+            same = t is not None and t.data_ptr() == out.data_ptr() and _layout(t) == _layout(out)
+            if t is not None and not same and _overlap(out, t):
+                _refuse("out may be x or residual, or other memory, not a part of theirs")
+        if seed_at is not None and _overlap(out, seed_at.reshape(1, 1)):
+            _refuse("out must not hold the key")
     _on_device(device, ("x", "residual", "key", "out"), (x, residual, seed_at, out))
     if out is None:
         out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
