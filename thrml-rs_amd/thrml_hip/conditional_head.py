@@ -114,14 +114,14 @@ class GatedHead:
         self.b = torch.zeros(q, device=where)
 
     def quantised(self):
-        """(8-bit weights, scales): the largest of a block becomes 448"""
+        """(8-bit weights, scales): the largest of a block becomes 448, but for blocks so small
+        that the scale is its least, 2^-126, as for linear_f8's activations"""
         import torch
 
         q, k = self.w.shape
         wide = torch.nn.functional.pad(self.w, (0, -k % 128, 0, -q % 128))
         blocks = wide.view(wide.shape[0] // 128, 128, wide.shape[1] // 128, 128)
-        scale = blocks.abs().amax((1, 3)) / 448.0
-        scale = scale.masked_fill(scale == 0.0, 1.0)
+        scale = (blocks.abs().amax((1, 3)) / 448.0).clamp(min=2.0**-126)
         w = (blocks / scale[:, None, :, None]).to(torch.float8_e4m3fn)
         return w.view(wide.shape)[:q, :k].contiguous(), scale
 
