@@ -349,11 +349,16 @@ static inline TilePlan plan_tiles(const thrml_ctx *ctx, const TileKind *kinds, i
 
 static inline bool tile_small(uint64_t rows, uint64_t row_bytes) { return rows * row_bytes <= (2u << 20); }
 
-// One workgroup for each tile and split.
+// One workgroup for each tile and split, which all have a stage or more: one without would repeat
+// stage -1.
 template <class G>
 static int launch_tiles(thrml_ctx *ctx, void (*f)(G), const G &g, uint32_t threads, size_t lds) {
   if ((uint64_t)g.ta * g.tb * threads >> 32) {
     set_error("more tiles than a launch takes");
+    return THRML_EUNSUPPORTED;
+  }
+  if (g.splits == 0 || g.splits > g.steps) {
+    set_error("a split of the reduction without a stage");
     return THRML_EUNSUPPORTED;
   }
   if (lds > 65536)
