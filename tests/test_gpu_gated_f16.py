@@ -5,6 +5,7 @@ import math
 
 import hidden_reference as ref
 import pytest
+import test_gpu_hidden_tiles as tiles
 import torch
 from conftest import log_case
 
@@ -208,3 +209,26 @@ def test_captured(device):
     del graphs
     torch.cuda.synchronize()
     dev.close()
+
+
+@pytest.mark.parametrize("which,tile", [*(("dx", t) for t in tiles.INPUT), *(("dw", t) for t in tiles.WEIGHT)])
+def test_every_kind_of_tile_at_the_border(device, which, tile):
+    """the border lies at about two typical results of the product that reaches the tile"""
+    rows, k, n = (tiles.INPUT if which == "dx" else tiles.WEIGHT)[tile]
+    log_case(f"f16 border {which} {tile}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    wg, wu = wg * 16, wu * 16
+    # dz and du are about 8 times dh
+    typical = 8 * (16 * math.sqrt(2 * n / k) if which == "dx" else math.sqrt(rows))
+    dh = (dh * (BORDER / 2 / typical)).clamp(-65504, 65504).to(F16)
+    _, gate, up = th.gated_linear(device, x, wg, wu, "silu", save=True)
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, "silu")
+    exact = _exact(dh, x, wg, wu, gate, up, "silu")
+    for (name, (want, err)), got in zip(exact.items(), grads):
+        told = (want.abs() - BORDER).abs() > err
+        wrong = told & (got.isinf() != (want.abs() >= BORDER))
+        assert not got.isnan().any() and not wrong.any(), (name, int(wrong.sum()), want[wrong][:5].tolist(), got[wrong][:5].tolist())
+    for name in ("dx",) if which == "dx" else ("dw_gate", "dw_up"):
+        want = exact[name][0]
+        # (0.9 % of them are within 2 % of the border, of 1353 and more)
+        assert (want.abs() >= BORDER).any() and ((want.abs() - BORDER).abs() < 0.02 * BORDER).any(), name
