@@ -572,17 +572,20 @@ typedef struct {
 } thrml_gated;
 /* h[row][c] rounded once to the type; gate and up, both or neither NULL, receive z and
  * u in f32, [rows][n] contiguous, for thrml_gated_backward.  Outputs share no memory with
- * x, the weights, work or each other (their pointers are compared, their ranges are the caller's).  work: thrml_gated_work(in, 0)
- * bytes.  The operands are read as they lie where their rows are whole 16-byte pieces
- * (k a multiple of 8, pointers of 16 bytes, strides of 8 elements, those of the two
- * weights alike), else from a copy in work. */
+ * x, the weights, work or each other: h equal to one of these is refused, the rest is the
+ * caller's to see to.  work: thrml_gated_work(in, 0) bytes.  The operands are read as they
+ * lie where their rows are whole 16-byte pieces (k a multiple of 8, pointers of 16 bytes,
+ * strides of 8 elements, those of the two weights alike) or x has at most 32 rows, else from
+ * a copy in work. */
 uint64_t thrml_gated_work(thrml_ctx *ctx, const thrml_gated *in, int backward);
 int thrml_gated_forward(thrml_ctx *ctx, const thrml_gated *in, void *h, int64_t h_stride, float *gate,
                         float *up, void *work, uint64_t work_bytes);
 /* From grad = d loss / d h [rows][n] and the z and u that the forward call kept:
- *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type; f16: all divided by a
- *                                             power of two where one would pass 65504)
+ *   dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
  *   dx = dz w_gate + du w_up,  dw_gate = dz^T x,  dw_up = du^T x
+ * f16: where dz or du of a row (for dx) or of a unit (for dw_gate, dw_up) would pass 65504,
+ * they are divided by a power of two of that row or unit; results near 65520, from where on
+ * they are infinite, are summed again from dz and du in f32.
  * dx [rows][k] in rows of dx_stride (NULL: not computed), dw_gate and dw_up [n][k]
  * contiguous, all in the type.  relu'(0) is 0.  work: thrml_gated_work(in, 1) bytes.  Outputs
  * share no memory with an input, work or each other. */
@@ -611,6 +614,8 @@ int thrml_dropout(thrml_ctx *ctx, const void *x, int dtype, uint64_t rows, uint6
  * w_scale [ceil(q / 128)][ceil(k / 128)], bias may be NULL.  Sums are f32.  For y in bf16
  * or f16 the products of a block are added by the 8-bit matrix unit, which keeps 2^-16 of
  * the largest; for y in f32 exactly.  A row of x with an infinity or a NaN gives NaN.
+ * Weights whose rows are not whole 16-byte pieces are read from a copy in work where there
+ * are more than 64 rows.
  * work: thrml_linear_f8_work bytes, for the same arguments.  y shares no memory with an input
  * or work. */
 uint64_t thrml_linear_f8_work(thrml_ctx *ctx, uint64_t rows, uint32_t k, const void *w, uint32_t q,

@@ -2,17 +2,17 @@
 // hidden block (k_gated.hip) and its 8-bit product (k_f8.hip).
 //
 // out[r][c] = sum over j of B[r][j] A[c][j]: side A are the output's columns (its
-// contiguous direction), side B its rows.  A stage is KB (64, 128 or 256) bytes of the reduction
-// of every row of both sides.  An operand lies in memory either with the reduction
+// contiguous direction), side B its rows.  A stage is KB (128 or 256) bytes of the reduction of
+// every row of both sides.  An operand lies in memory either with the reduction
 // contiguous (a row of a side is a row in memory), or across (CROSS: a row in memory
 // holds one reduction index for all rows of the side), as a gradient's operands do.
 //
 // In LDS, 16-byte pieces:
 //   along   rows of KB bytes, a row's pieces permuted by bits of the row: (row >> 1) & 7 for
-//           128 bytes, row & 15 for 256 (among 16 pieces), (row >> 3) & 3 for 64.  A 16-byte read takes 16 lanes at a time, four
-//           quads of lanes: 0, 3, 5, 6 of a half wave, then 1, 2, 4, 7; two rows of 128 bytes
-//           fill the banks, and the rows of one parity that meet (0, 2, 12, 14, 20, 22, 24, 26
-//           of 32) differ in those bits, as do four that meet of 64 bytes.
+//           128 bytes, row & 15 for 256 (among 16 pieces).  A 16-byte read takes 16 lanes at a
+//           time, four quads of lanes: 0, 3, 5, 6 of a half wave, then 1, 2, 4, 7; two rows of 128
+//           bytes fill the banks, and the rows of one parity that meet (0, 2, 12, 14, 20, 22, 24,
+//           26 of 32) differ in those bits.
 //   across  KB / 2 rows, one for each reduction index, of the side's rows in chunks of 32
 //           (64 bytes), permuted so that the 4 neighbouring indices that the transposing
 //           read takes together fall on different banks.
@@ -86,7 +86,8 @@ struct TileShape {
 // a row's permutation of its pieces
 template <class S>
 __device__ __forceinline__ uint32_t tile_turn(uint32_t row) {
-  return S::KB >= 256 ? row & 15u : S::KB == 128 ? row >> 1 & 7u : row >> 3 & 3u;
+  static_assert(S::KB == 128 || S::KB == 256, "8 or 16 pieces");
+  return S::KB == 256 ? row & 15u : row >> 1 & 7u;
 }
 
 // What a lane loads of one side, in P pieces.  Along, its pieces lie STEP rows apart, at
@@ -98,7 +99,7 @@ struct Side {
   static constexpr int P = N * S::PIECES / S::LOADERS;
   static constexpr int CHUNKS = N / 32;                              // of a row in LDS, where CROSS
   static constexpr uint32_t STEP = CROSS ? S::LOADERS / (N / 8) : S::LOADERS / S::PIECES;
-  static_assert(CROSS ? STEP % 4 == 0 || P == 1 : STEP % (S::KB >= 128 ? 16 : 32) == 0 || P == 1, "pieces are permuted alike");
+  static_assert(CROSS ? STEP % 4 == 0 || P == 1 : STEP % 16 == 0 || P == 1, "pieces are permuted alike");
   uint32_t stride, last;    // bytes between rows in memory (below 2^24), the last valid row
 
   struct Place {            // of piece 0

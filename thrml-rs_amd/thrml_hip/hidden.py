@@ -78,8 +78,10 @@ def gated_linear(device, x, w_gate, w_up, activation="silu", save=False, out=Non
     With save, (h, gate, up): also both products in float32, for gated_linear_grad.  out: a
     tensor for h, which shares no memory with x and the weights.
 
-    Rows that are not whole 16-byte pieces (k not a multiple of 8, a view that starts or
-    steps elsewhere) are copied first; the weights of a model are better kept aligned."""
+    Operands whose rows are not whole 16-byte pieces (k not a multiple of 8, a view that starts
+    or steps elsewhere, weights of different strides) are copied first where x has more than 32
+    rows, and else read as they lie, more slowly; gated_linear_grad always copies them.  The
+    weights of a model are better kept aligned."""
     d, keep, rows, k, n = _gated(x, w_gate, w_up, activation)
     dtype = keep[0].dtype
     stride = n
@@ -109,11 +111,13 @@ def gated_linear_grad(device, grad, x, w_gate, w_up, gate, up, activation="silu"
     """(dx, dw_gate, dw_up): the gradients of a loss in x [rows, k] and the weights [n, k],
     in their type, from grad [rows, n], its gradient in gated_linear's result in that type,
     and the products gate and up [rows, n] float32 that this kept.  With z = gate, u = up:
-      dz = grad u act'(z),  du = grad act(z)   (rounded to the type; float16: all divided
-                                      by a power of two where one would pass 65504)
+      dz = grad u act'(z),  du = grad act(z)   (rounded to the type)
       dx = dz @ w_gate + du @ w_up,  dw_gate = dz.T @ x,  dw_up = du.T @ x
-    relu'(0) is 0.  Without rows the weights' gradients are 0.  input_grad False: dx is
-    not computed, and None."""
+    float16: where dz or du of a row (for dx) or of a unit (for dw_gate, dw_up) would pass 65504,
+    they are divided by a power of two of that row or unit; results at the border of the type's
+    range are summed again without the rounding of dz and du, so that they are infinite where
+    the gradient is.  relu'(0) is 0.  Without rows the weights' gradients are 0.  input_grad
+    False: dx is not computed, and None."""
     d, keep, rows, k, n = _gated(x, w_gate, w_up, activation)
     same = (keep[0].dtype,)
     grad, grad_stride = _matrix("grad", grad, same, rows, n)
@@ -192,8 +196,8 @@ def linear_f8(device, x, w, w_scale, bias=None, out_dtype=None):
     float32.  For results in 16 bits the sum within a block keeps 2^-16 of its largest
     product, for float32 all.  A row of x with an infinity or a NaN gives NaN.
 
-    k is at most 2^20.  Weights whose rows are not whole 16-byte pieces are copied
-    first."""
+    k is at most 2^20.  Weights whose rows are not whole 16-byte pieces are copied first where
+    x has more than 64 rows, and else read as they lie, more slowly."""
     if head.torch is None:
         head._setup()
     torch = head.torch
