@@ -232,3 +232,23 @@ def test_every_kind_of_tile_at_the_border(device, which, tile):
         want = exact[name][0]
         # (0.9 % of them are within 2 % of the border, of 1353 and more)
         assert (want.abs() >= BORDER).any() and ((want.abs() - BORDER).abs() < 0.02 * BORDER).any(), name
+
+
+@pytest.mark.parametrize("rows,k,n,size", [(4, 4096, 1000, 9000.0), (40, 264, 392, 9000.0), (600, 1032, 600, 2000.0)])
+def test_infinite_gradients_stay_in_their_rows_and_units(device, rows, k, n, size):
+    """and do not make the finite results beside them near the border, nor far from it"""
+    log_case(f"f16 infinite dh {rows} {k} {n}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    dh = (dh * size).clamp(-65504, 65504).to(F16)
+    dh[1, 5] = math.inf
+    _, gate, up = th.gated_linear(device, x, wg, wu, "silu", save=True)
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, "silu")
+    dh[1, 5] = 0.0
+    clean = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, "silu")
+    for (name, (want, err)), got, without in zip(_exact(dh, x, wg, wu, gate, up, "silu").items(), grads, clean):
+        bad = 1 if name == "dx" else 5
+        assert not got[bad].isfinite().any(), name
+        rest = torch.arange(len(got), device="cuda") != bad
+        told = ((want.abs() - BORDER).abs() > err) & rest[:, None]
+        assert not (told & (got.isinf() != (want.abs() >= BORDER))).any(), name
+        assert torch.equal(got[rest], without[rest]), name

@@ -132,8 +132,8 @@ __device__ __forceinline__ void slopes(float dh, float z, float u, float &dz, fl
 // columns here, which is about 1.2 typical ones: 12 times the rms.  (Among 8 lanes'
 // largest, the smaller one of pairs, the larger one of two pairs, the smaller one of those: a
 // column that is far larger than the others does not make these near.)  Results far from
-// the border pay comparisons: a step of 1021 x 2001 x 5003 takes 261 us with them
-// and without.  One of 5 x 7040 x 8000 takes 273 where 1.5 % of the weights' gradients pass the
+// the border pay comparisons: a step of 1021 x 2001 x 5003 takes 257 us with them
+// and without.  One of 5 x 7040 x 8000 takes 280 where 1.5 % of the weights' gradients pass the
 // border and 17 thousand are near it, 193 without these sums.
 __device__ __forceinline__ void slopes_of(const GatedTiles &g, float dh, float z, float u, float &dz, float &du) {
   if (g.act == THRML_ACT_RELU)
@@ -144,19 +144,19 @@ __device__ __forceinline__ void slopes_of(const GatedTiles &g, float dh, float z
     slopes<THRML_ACT_SILU>(dh, z, u, dz, du);
 }
 
-// One result by a wave, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and column c;
-// the loads of U turns are under way together
+// One result by a workgroup of 256, of row `row` (G_WEIGHT: dw_up's come behind dw_gate's) and
+// column c; the loads of U turns are under way together
 template <int OP>
-__device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row, uint32_t c) {
+__device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row, uint32_t c, double *part) {
   constexpr uint32_t U = 8;
   const bool up = OP == G_WEIGHT && row >= g.n;
   const uint64_t all = OP == G_WEIGHT ? g.rows : g.n;
   double sum = 0.0;
-  for (uint64_t i0 = here(threadIdx.x) & 63u; i0 < all; i0 += 64u * U) {
+  for (uint64_t i0 = threadIdx.x; i0 < all; i0 += 256u * U) {
     float dh[U], z[U], u[U], a0[U], a1[U];
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
-      const uint64_t i = min(i0 + 64u * e, all - 1u), r = OP == G_WEIGHT ? i : row;
+      const uint64_t i = min(i0 + 256u * e, all - 1u), r = OP == G_WEIGHT ? i : row;
       const uint32_t unit = OP == G_WEIGHT ? (up ? row - g.n : row) : (uint32_t)i;
       auto operand = [&](const void *p) {
         return (float)*reinterpret_cast<const f16_t *>(reinterpret_cast<const uint8_t *>(p) + i * g.a_stride + c * 2ull);
@@ -169,7 +169,7 @@ __device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row,
     }
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
-      if (i0 + 64u * e >= all) break;
+      if (i0 + 256u * e >= all) break;
       float dz, du;
       slopes_of(g, dh[e], z[e], u[e], dz, du);
       if (OP == G_WEIGHT)
@@ -180,7 +180,14 @@ __device__ __forceinline__ double gated_again(const GatedTiles &g, uint32_t row,
   }
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-  return sum;
+  if ((threadIdx.x & 63u) == 0) part[threadIdx.x / 64u] = sum;
+  __syncthreads();
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__device__ __forceinline__ float larger_finite(float m, float v) {
+  v = fabsf(v);
+  return v < INFINITY ? fmaxf(m, v) : m;
 }
 
 constexpr float BORDER = 65520.0f;
@@ -188,53 +195,69 @@ constexpr float BORDER = 65520.0f;
 // what a lane has seen of results: the largest, and how near one came to the border
 struct Border {
   float most = 0.0f, nearest = INFINITY;
+  template <bool FINITE>  // whether infinite ones do not count as large
   __device__ __forceinline__ void see(const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      most = fmaxf(most, fabsf(v[e]));
+      most = FINITE ? larger_finite(most, v[e]) : fmaxf(most, fabsf(v[e]));
       nearest = fminf(nearest, fabsf(fabsf(v[e]) - BORDER));
     }
   }
   // whether a lane of the wave has seen one that is near; band: the distance that is, from
-  // what 8 lanes have seen
+  // what 8 lanes have seen.  MIXED (in a join, where they may be of two rows): and half as far
+  // from what this one has
+  template <bool MIXED>
   __device__ __forceinline__ bool any_near(float &band) const {
     if (!__any(most >= 0.99f * BORDER)) return false;  // (a band over 0.01 of the border comes from one beyond it)
     float m = fminf(most, __shfl_xor(most, 1));
     m = fmaxf(m, __shfl_xor(m, 2));
     m = fminf(m, __shfl_xor(m, 4));
     band = fmaxf(0x1p-9f * m, 0x1p-10f * BORDER);
+    if (MIXED) band = fmaxf(band, 0x1p-10f * most);
     return __any(nearest <= band);
   }
 };
 
 // which of 8 results are near, m of them that count (all lanes of the wave come here)
+template <bool MIXED>
 __device__ __forceinline__ uint32_t border_bits(const float (&v)[8], uint32_t m) {
   Border b;
-  b.see(v);  // (those of no column or row are as large as the others)
+  b.see<true>(v);  // (those of no column or row are as large as the others)
   float band;
-  if (!b.any_near(band)) return 0;
+  if (!b.any_near<MIXED>(band)) return 0;
   uint32_t bits = 0;
 #pragma unroll
   for (uint32_t e = 0; e < 8; ++e) bits |= (uint32_t)(e < m && fabsf(fabsf(v[e]) - BORDER) <= band) << e;
   return bits;
 }
 
-// The results v of row `row` from column c on, of which m count (0 in a lane that has none), one
-// after another: the few of a join.
+// The results v of row `row` from column c on, of which m count (0 in a thread that has none),
+// one after another: the few of a join.  All threads of the workgroup come here.
 template <int OP>
 __device__ __forceinline__ void settle_each(const GatedTiles &g, float (&v)[8], uint32_t m, uint32_t row, uint32_t c) {
-  uint32_t bits = border_bits(v, m);
-  for (uint64_t any = __ballot(bits != 0); any; any = __ballot(bits != 0)) {
-    const int lane = __builtin_ctzll(any);
-    const uint32_t of = (uint32_t)__builtin_amdgcn_readlane((int)bits, lane), at = (uint32_t)__builtin_ctz(of);
-    const float sum = (float)gated_again<OP>(g, (uint32_t)__builtin_amdgcn_readlane((int)row, lane),
-                                             (uint32_t)__builtin_amdgcn_readlane((int)c, lane) + at);
-    if ((here(threadIdx.x) & 63u) == (uint32_t)lane) {
+  __shared__ double part[4];
+  __shared__ uint32_t first, first_row, first_c;
+  uint32_t bits = border_bits<true>(v, m);
+  if (!__syncthreads_or(bits != 0)) return;
+  do {
+    if (threadIdx.x == 0) first = 256;
+    __syncthreads();
+    if (bits) atomicMin(&first, threadIdx.x);  // (which comes first does not change a sum)
+    __syncthreads();
+    const bool mine = first == threadIdx.x;
+    const uint32_t at = mine ? (uint32_t)__builtin_ctz(bits) : 0u;
+    if (mine) {
+      first_row = row;
+      first_c = c + at;
+    }
+    __syncthreads();
+    const float sum = (float)gated_again<OP>(g, first_row, first_c, part);
+    if (mine) {
 #pragma unroll
       for (uint32_t e = 0; e < 8; ++e) v[e] = e == at ? sum : v[e];
       bits &= bits - 1u;
     }
-  }
+  } while (__syncthreads_or(bits != 0));
 }
 
 // Those of a wave's 32 rows (from row0 on, of `limit`) x MA columns (from c0 on) at the end of
@@ -258,7 +281,7 @@ __device__ __forceinline__ void settle_slab(const GatedTiles &g, bool passed, fl
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = mine[rl * PITCH + cl + e] * f;
-    marks |= (uint64_t)border_bits(v, row < limit && c0 + cl < cols ? cols - c0 - cl : 0u) << (8u * t);
+    marks |= (uint64_t)border_bits<false>(v, row < limit && c0 + cl < cols ? cols - c0 - cl : 0u) << (8u * t);
   }
   wait_loads<0>();  // (the stores of these results have ended)
   uint32_t *list = reinterpret_cast<uint32_t *>(mine);
@@ -526,7 +549,7 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
             for (int e = 0; e < 8; ++e) v[e] *= f;
           }
           if constexpr (SETTLE) {
-            seen.see(v);  // (those of no column, too: they repeat others)
+            seen.see<false>(v);  // (those of no column, too: they repeat others)
             if (m == 0) continue;
           }
           store8(out + (int64_t)row * g.out_stride + c, m, v);
@@ -534,7 +557,7 @@ __global__ __launch_bounds__(S::THREADS) void gated_tile_kernel(GatedTiles g) {
       }
       if constexpr (SETTLE) {
         float band;
-        if (seen.any_near(band))
+        if (seen.template any_near<false>(band))
           settle_slab<OP, S::MA, LPR>(g, passed != 0, mine, r0 + wb * S::MB + 32u * j, up, limit, c0 + wa * (HALF / S::WA), cols, out);
       }
     }
@@ -630,14 +653,20 @@ __global__ __launch_bounds__(256) void gated_few_kernel(GatedTiles g, int64_t ga
 }
 
 // The sums of the splits, added in their order.
+__host__ __device__ static inline uint32_t join_groups(uint64_t all) { return all < 65536u ? 32u : 256u; }
+
 template <int OP, class T, int ACT>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
   const uint32_t cols = OP == G_FORWARD ? g.n : g.k, groups = (cols + 7u) / 8u;
   const uint64_t rows = OP == G_WEIGHT ? 2ull * g.n : g.rows, pitch = OP == G_FORWARD ? 2ull * g.n : g.k;
   constexpr bool SETTLE = OP != G_FORWARD && __is_same(T, f16_t);
-  // (SETTLE: whole waves; lanes behind the end repeat the last group and store nothing)
-  for (uint64_t i_ = (uint64_t)blockIdx.x * 256u + threadIdx.x; (SETTLE ? i_ & ~(uint64_t)63u : i_) < rows * groups; i_ += (uint64_t)gridDim.x * 256u) {
-    const uint64_t i = SETTLE ? min(i_, rows * groups - 1u) : i_;
+  // SETTLE: whole workgroups, of few groups each where there are few, so that their long sums are
+  // in many; threads behind the end repeat the last group and store nothing
+  const uint64_t all = rows * groups;
+  const uint32_t own = SETTLE ? join_groups(all) : 256u;
+  for (uint64_t at = (uint64_t)blockIdx.x * own; at < all; at += (uint64_t)gridDim.x * own) {
+    const uint64_t i_ = at + threadIdx.x, i = SETTLE ? min(i_, min(at + own, all) - 1u) : i_;
+    if (!SETTLE && i >= all) break;
     const uint64_t row = i / groups;
     const uint32_t c = (uint32_t)(i - row * groups) * 8u, m = cols - c;
     float v[8], w[8];
@@ -674,10 +703,6 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedTiles g) {
 // finite magnitude that it wrote.
 constexpr uint32_t SLOPE_GROUPS = 2048;  // workgroups, with f16
 
-__device__ __forceinline__ float larger_finite(float m, float v) {
-  v = fabsf(v);
-  return v < INFINITY ? fmaxf(m, v) : m;
-}
 // of the workgroup
 __device__ __forceinline__ float slope_max(float m, float *shared) {
 #pragma unroll
@@ -766,21 +791,46 @@ __global__ __launch_bounds__(256) void gated_rescale_kernel(const f16_t *__restr
   for (uint64_t item = blockIdx.x; item < rows + np / COLS; item += gridDim.x) {
     if (item < rows) {
       float most = 0.0f;
-#pragma unroll 4
-      for (uint32_t c = threadIdx.x; c < n; c += 256u) {
-        pair(item, c, dz, du);
-        most = larger_finite(larger_finite(most, dz), du);
+      auto units = [&](uint32_t c, float (&a)[8], float (&b)[8]) {
+        Raw8<f16_t> rg;
+        Raw8<float> rz, ru;
+        const f16_t *pg = grad + (int64_t)item * grad_stride + c;
+        const float *pz = z + item * n + c, *pu = u + item * n + c;
+        if (c + 8u <= n) {
+          load8(pg, rg);
+          load8(pz, rz);
+          load8(pu, ru);
+        } else {
+          load8_part(pg, n - c, rg);
+          load8_part(pz, n - c, rz);
+          load8_part(pu, n - c, ru);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          slopes<ACT>(value(rg, e), value(rz, e), value(ru, e), a[e], b[e]);
+          if (c + e >= n) a[e] = b[e] = 0.0f;
+        }
+      };
+      float a[8], b[8];
+      for (uint32_t c = threadIdx.x * 8u; c < n; c += 2048u) {
+        units(c, a, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = larger_finite(larger_finite(most, a[e]), b[e]);
       }
       const int down = passed_by(slope_max(most, shared));
       if (threadIdx.x == 0) row_factor[item] = ldexpf(1.0f, down);
       if (down == 0) continue;  // (written so already)
       const float f = ldexpf(1.0f, -down);
-#pragma unroll 4
-      for (uint32_t c = threadIdx.x; c < n; c += 256u) {
-        pair(item, c, dz, du);
+      for (uint32_t c = threadIdx.x * 8u; c < n; c += 2048u) {
+        units(c, a, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          a[e] *= f;
+          b[e] *= f;
+        }
         f16_t *o = d + item * 2u * np + c;
-        o[0] = (f16_t)(dz * f);
-        o[np] = (f16_t)(du * f);
+        store8(o, 8, a);
+        store8(o + np, 8, b);
       }
     } else {
       const uint32_t lo = threadIdx.x % COLS, hi = threadIdx.x / COLS, c = (uint32_t)(item - rows) * COLS + lo;
@@ -933,7 +983,8 @@ static int launch_product(thrml_ctx *ctx, const TilePlan &p, GatedTiles g) {
   if (rc || p.splits == 1) return rc;
   const uint64_t n = (OP == G_WEIGHT ? 2ull * g.n : g.rows) * tile_cdiv(OP == G_FORWARD ? g.n : g.k, 8);
   auto *f = &gated_join_kernel<OP, T, ACT>;
-  hipLaunchKernelGGL(f, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, 256), 1u << 16)), dim3(256), 0, ctx->stream, g);
+  const uint32_t own = OP != G_FORWARD && __is_same(T, f16_t) ? join_groups(n) : 256u;
+  hipLaunchKernelGGL(f, dim3((uint32_t)std::min<uint64_t>(tile_cdiv(n, own), 1u << 16)), dim3(256), 0, ctx->stream, g);
   THRML_HIP(hipGetLastError());
   return THRML_OK;
 }
