@@ -263,9 +263,9 @@ __device__ __forceinline__ void settle_each(const GatedTiles &g, float (&v)[8], 
 // Those of a wave's 32 rows (from row0 on, of `limit`) x MA columns (from c0 on) at the end of
 // a tile, which lie in `mine` before their factors and have been stored: each lane sums one, 64
 // at a time, of operands that come through LDS, DEEP of the reduction at a time: 32 rows' dz
-// or du (dx: both) and MA columns of the other side.  In a step of 4096 x 4096 x 8192 with 87 %
-// of the weights' gradients infinite, the
-// gradient takes 7.6 ms (1.06 where none is near); each by the wave (gated_again) it took 122.
+// or du (dx: both) and MA columns of the other side.  The gradient of 4096 x 4096 x 8192 with 87 %
+// of the weights' results infinite takes 7.7 ms (1.06 where none is near); each by the wave, it
+// took 122.
 template <int OP, int MA, uint32_t LPR>
 __device__ __forceinline__ void settle_slab(const GatedTiles &g, bool passed, float *mine, uint64_t row0, uint32_t up, uint64_t limit,
                                             uint32_t c0, uint32_t cols, f16_t *out) {
