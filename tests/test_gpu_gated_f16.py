@@ -252,3 +252,27 @@ def test_infinite_gradients_stay_in_their_rows_and_units(device, rows, k, n, siz
         told = ((want.abs() - BORDER).abs() > err) & rest[:, None]
         assert not (told & (got.isinf() != (want.abs() >= BORDER))).any(), name
         assert torch.equal(got[rest], without[rest]), name
+
+
+@pytest.mark.parametrize("rows,k,n,size", [(2, 3, 4000, 25000.0), (3, 1, 3000, 20000.0), (40, 7, 2500, 8000.0), (300, 9, 1003, 3000.0), (4000, 5, 70, 900.0)])
+def test_few_features_at_the_border(device, rows, k, n, size):
+    """rows of fewer columns than a wave takes together, in wider buffers of NaN"""
+    log_case(f"f16 few features {rows} {k} {n}")
+    x, wg, wu, dh = _inputs(rows, k, n)
+    dh = (dh * size).clamp(-65504, 65504).to(F16)
+
+    def wide(t):
+        t, keep = torch.full((t.shape[0], t.shape[1] + 3), math.nan, device="cuda", dtype=F16), t
+        t[:, 2:-1] = keep
+        return t[:, 2:-1]
+
+    x, wg, wu, dh = (wide(t) for t in (x, wg, wu, dh))
+    _, gate, up = th.gated_linear(device, x, wg, wu, "gelu", save=True)
+    grads = th.gated_linear_grad(device, dh, x, wg, wu, gate, up, "gelu")
+    passed = 0
+    for (name, (want, err)), got in zip(_exact(dh, x, wg, wu, gate, up, "gelu").items(), grads):
+        told = (want.abs() - BORDER).abs() > err
+        wrong = told & (got.isinf() != (want.abs() >= BORDER))
+        assert not got.isnan().any() and not wrong.any(), (name, int(wrong.sum()), want[wrong][:5].tolist(), got[wrong][:5].tolist())
+        passed += int((want.abs() >= BORDER).sum())
+    assert passed > 0

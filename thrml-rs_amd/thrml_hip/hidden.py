@@ -44,6 +44,10 @@ def _overlap(a, b):
     d = b.data_ptr() - a.data_ptr()
     if not (ra and rb and la and lb) or d >= (ra - 1) * sa + la or -d >= (rb - 1) * sb + lb:
         return False
+    if sa == sb or ra == 1 or rb == 1:  # rows i of a and j of b: d - la < (i - j) s < d + lb
+        s = sb if ra == 1 else sa
+        least = max((d - la) // s + 1, 1 - rb)
+        return least < ra and least * s < d + lb
     if ra > rb:
         ra, sa, la, rb, sb, lb, d = rb, sb, lb, ra, sa, la, -d
     # row i of a and j of b share bytes where i sa - d - lb < j sb < i sa - d + la
